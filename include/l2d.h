@@ -362,6 +362,101 @@ L2D_API int l2d_pool_side(int device, const uint64_t *granules, size_t count, in
 /* Unmaps and frees the whole pool (every granule must be free). */
 L2D_API int l2d_pool_release(int device);
 
+/* ---- decoding operators (no counterpart in the reference): what one new token of a language model
+ *      reads around the GEMV -- 4-bit weights, and the paged cache of earlier keys and values ----
+ * All three are stream-ordered, allocate nothing when called and may be captured into a graph.
+ * Arguments the host can see are checked before anything is launched; what only the device can see
+ * (lengths, positions, page numbers) is checked by the kernels, which leave the access out and set a
+ * bit of *status, a device word of the caller's that only ever gains bits (NULL: not reported). */
+enum {
+    L2D_KV_BAD_PAGE = 1,    /* a page number outside [0, num_pages), a position or length past the page
+                               table, or a sequence outside it */
+    L2D_KV_BAD_POSITION = 2 /* a position past the rotation tables */
+};
+
+/* Matrix-vector products with 4-bit weights and group scales.
+ *   y[b][i] = sum_j s[i][j / group] * (q[i][j] - z[i][j / group]) * x[b][j]
+ * W holds q as rows of packed bytes, column 2j in the low half of byte j.  z is the low four bits of
+ * one byte per scale; without zeros every z is 8.  The difference q - z is exact in every dtype_x,
+ * products and sums are fp32, y is rounded once. */
+typedef struct {
+    int64_t M, N;
+    int64_t ldw;          /* bytes between rows of W (0 = ceil(N / 2)) */
+    int64_t lds;          /* elements between rows of scales and of zeros (0 = ceil(N / group)) */
+    int group;            /* columns per scale: 32, 64 or a multiple of 128 (the last group may be short) */
+    int dtype_x;          /* L2D_F32 / L2D_F16 / L2D_BF16 */
+    int dtype_y;
+    int dtype_s;          /* scales */
+    const void *W;
+    const void *scales;   /* [M][ceil(N / group)] */
+    const void *zeros;    /* uint8 [M][ceil(N / group)], or NULL */
+    int device;
+} l2d_q4_desc;
+/* y = W.x for `vectors` vectors, stride_x / stride_y elements apart (0 = N / M).  y must not overlap
+ * x or the weights.  Rows on 16-byte boundaries (W and ldw) are read fastest; any are read. */
+L2D_API int l2d_q4_gemv(const l2d_q4_desc *desc, const void *x, int64_t stride_x, void *y, int64_t stride_y,
+                        int64_t vectors, void *stream);
+
+/* A paged cache of keys and values: pages of page_size slots, each slot `heads` rows of head_dim
+ * elements (contiguous), any strides between rows.  k and v may be one buffer or two. */
+typedef struct {
+    void *k, *v;
+    int dtype;                                    /* of keys, values, queries and outputs */
+    int heads, head_dim;                          /* key-value heads; head_dim 1..256 */
+    int page_size;
+    int64_t num_pages;
+    int64_t k_page, k_slot, k_head;               /* elements between pages, slots, heads (0 = dense: */
+    int64_t v_page, v_slot, v_head;               /*  [page][slot][head][dim]) */
+    const int32_t *table;                         /* [num_seqs][table_stride]: the pages of each sequence in order */
+    int64_t table_stride;                         /* entries between sequences (0 = table_width) */
+    int num_seqs, table_width;
+    uint32_t *status;                             /* L2D_KV_BAD_* bits, or NULL */
+    int device;
+} l2d_kv_cache;
+
+/* Appending: rotates the keys of `tokens` new tokens by their positions and stores them, with the
+ * values as they are, into the cache; rotates the queries of the same tokens on the way.
+ * The pair (a, b) of a head becomes (a cos - b sin, b cos + a sin), computed in fp32 and rounded once;
+ * the first rot_dim elements of a head are rotated, the others kept.  Scaled or extended rotations are
+ * tables of another kind. */
+typedef struct {
+    int heads_q;                       /* query heads (0: keys and values only) */
+    const float *cos, *sin;            /* [max_pos][rot_dim / 2], dense; unused when rot_dim is 0 */
+    int64_t max_pos;
+    int rot_dim;                       /* even, 0..head_dim */
+    int interleaved;                   /* 0: pairs (i, i + rot_dim / 2); 1: pairs (2i, 2i + 1) */
+    int64_t k_token, v_token, q_token, q_out_token;  /* elements between tokens (0 = heads * head_dim) */
+} l2d_append_desc;
+/* pos[t]: the position of token t, both in its sequence's cache and for the rotation; a negative one
+ * marks padding, for which nothing is written.  seq[t]: its row of the page table (NULL: t).  q_out may
+ * be q.  Two tokens of one call must not share a slot.  A token with a bad page or position (status) is
+ * left out whole. */
+L2D_API int l2d_kv_append(const l2d_kv_cache *cache, const l2d_append_desc *desc, const void *k, const void *v,
+                          const void *q, void *q_out, const int32_t *pos, const int32_t *seq, int64_t tokens,
+                          void *stream);
+
+/* Attention of one new token per sequence over the cache:
+ *   out[b][h] = sum_p w_p v_p,  w = softmax over positions p of scale * (q[b][h] . k_p)
+ * over positions max(0, lens[b] - window) .. lens[b] - 1 (window 0: all), with key-value head
+ * h / (heads_q / heads).  A row with no position, or none whose score is above -inf, gives 0 and -inf in
+ * lse.  Slots outside those positions are never used, whatever they hold; a position on a bad page
+ * counts as absent.  Scores, softmax and sums are fp32. */
+typedef struct l2d_attn_plan l2d_attn_plan;
+typedef struct {
+    int heads_q;              /* a multiple of the cache's heads */
+    int window;
+    float scale;              /* 0 = 1 / sqrt(head_dim) */
+    int max_batch;            /* 0 = the cache's num_seqs */
+    int64_t q_token, out_token;  /* elements between sequences (0 = heads_q * head_dim) */
+} l2d_attn_desc;
+/* The plan owns its device scratch (allocated here, never during l2d_attn_decode) and keeps the cache's
+ * description; calls of one plan must not overlap on the GPU. */
+L2D_API int l2d_attn_plan_create(const l2d_kv_cache *cache, const l2d_attn_desc *desc, l2d_attn_plan **plan);
+/* Row b of q, out, lse (fp32 [batch][heads_q], or NULL) and lens belongs to row b of the page table. */
+L2D_API int l2d_attn_decode(l2d_attn_plan *plan, const void *q, void *out, float *lse, const int32_t *lens, int batch,
+                            void *stream);
+L2D_API int l2d_attn_plan_destroy(l2d_attn_plan *plan);
+
 /* ---- helpers used by the benchmark and the CLI ---- */
 /* Reference-mode inputs (init_data): A/x from mix32 of the flat index (stream 0 = A, 1 = x). */
 L2D_API int l2d_fill_ref(void *dst, int dtype, uint64_t first, uint64_t n, uint32_t seed, int stream,

@@ -10,6 +10,9 @@ Python mirror of the reference's probe/GEMV interface over the C ABI of ``lib/li
 * :func:`partition_rows`             -- same file :261-273
 * :class:`GemvPlan`                  -- build_side_info + the kernel launches (:73-103, :163-231, :301-334)
 
+The operators of a decoding step beside the GEMV (no counterpart in the reference): :class:`Q4Matrix`
+(products with 4-bit weights), :class:`KvCache` with :class:`KvAppend` and :class:`PagedAttention`.
+
 Errors raise :class:`L2DError` (the reference aborts the process instead).  There is no CPU
 fallback: importing this package without the built library raises immediately.
 """
@@ -89,6 +92,31 @@ class PlanStats(C.Structure):
                 ("placement", C.c_int), ("row_domain_bytes", C.c_int64 * 2)]
 
 
+class Q4Desc(C.Structure):
+    _fields_ = [("M", C.c_int64), ("N", C.c_int64), ("ldw", C.c_int64), ("lds", C.c_int64), ("group", C.c_int),
+                ("dtype_x", C.c_int), ("dtype_y", C.c_int), ("dtype_s", C.c_int), ("W", C.c_void_p),
+                ("scales", C.c_void_p), ("zeros", C.c_void_p), ("device", C.c_int)]
+
+
+class KvCacheDesc(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int), ("heads", C.c_int), ("head_dim", C.c_int),
+                ("page_size", C.c_int), ("num_pages", C.c_int64), ("k_page", C.c_int64), ("k_slot", C.c_int64),
+                ("k_head", C.c_int64), ("v_page", C.c_int64), ("v_slot", C.c_int64), ("v_head", C.c_int64),
+                ("table", C.c_void_p), ("table_stride", C.c_int64), ("num_seqs", C.c_int), ("table_width", C.c_int),
+                ("status", C.c_void_p), ("device", C.c_int)]
+
+
+class AppendDesc(C.Structure):
+    _fields_ = [("heads_q", C.c_int), ("cos", C.c_void_p), ("sin", C.c_void_p), ("max_pos", C.c_int64),
+                ("rot_dim", C.c_int), ("interleaved", C.c_int), ("k_token", C.c_int64), ("v_token", C.c_int64),
+                ("q_token", C.c_int64), ("q_out_token", C.c_int64)]
+
+
+class AttnDesc(C.Structure):
+    _fields_ = [("heads_q", C.c_int), ("window", C.c_int), ("scale", C.c_float), ("max_batch", C.c_int),
+                ("q_token", C.c_int64), ("out_token", C.c_int64)]
+
+
 # Every symbol include/l2d.h declares, with its ctypes signature.
 _vp, _i, _u32, _u64, _i64, _sz = C.c_void_p, C.c_int, C.c_uint32, C.c_uint64, C.c_int64, C.c_size_t
 _pi, _pu32, _pu64, _psz = C.POINTER(C.c_int), C.POINTER(C.c_uint32), C.POINTER(C.c_uint64), C.POINTER(C.c_size_t)
@@ -146,6 +174,11 @@ SIGNATURES = {
     "l2d_pool_info": (_i, [_i, _pu64, _pu64, _pu32]),
     "l2d_pool_side": (_i, [_i, _pu64, _sz, _pi]),
     "l2d_pool_release": (_i, [_i]),
+    "l2d_q4_gemv": (_i, [C.POINTER(Q4Desc), _vp, _i64, _vp, _i64, _i64, _vp]),
+    "l2d_kv_append": (_i, [C.POINTER(KvCacheDesc), C.POINTER(AppendDesc), _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "l2d_attn_plan_create": (_i, [C.POINTER(KvCacheDesc), C.POINTER(AttnDesc), C.POINTER(_vp)]),
+    "l2d_attn_decode": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _vp]),
+    "l2d_attn_plan_destroy": (_i, [_vp]),
     "l2d_fill_ref": (_i, [_vp, _i, _u64, _u64, _u32, _i, _i, _vp]),
     "l2d_fill_cfg": (_i, [_vp, _i, _u64, _u64, _u64, _u64, _i, C.c_float, C.c_float, _vp]),
     "l2d_l2_flush": (_i, [_i, _vp]),
@@ -545,6 +578,121 @@ class PeerShard:
             self.close()
         except Exception:
             pass
+
+
+# --------------------------------------------------------------------------------------------
+# Decoding operators: 4-bit weights, the paged cache, attention over it
+# --------------------------------------------------------------------------------------------
+
+KV_BAD_PAGE, KV_BAD_POSITION = 1, 2
+
+
+class Q4Matrix:
+    """An M x N matrix of 4-bit weights with group scales: ``y = W.x`` for one or a few vectors.
+
+    ``weights`` are rows of packed bytes (column 2j in the low half of byte j, ``ldw`` bytes between
+    rows, 0 = ceil(N / 2)); ``scales`` [M][ceil(N / group)] of ``dtype_s`` and, where given, ``zeros`` of
+    the same shape in uint8 (their low four bits; 8 everywhere otherwise), ``lds`` elements between
+    rows.  W[i, j] = scales[i, j // group] * (q[i, j] - zeros[i, j // group])."""
+
+    def __init__(self, weights, scales, M: int, N: int, group: int, zeros=None, dtype_x: int = F16,
+                 dtype_y: Optional[int] = None, dtype_s: int = F16, ldw: int = 0, lds: int = 0, device: int = 0):
+        self.M, self.N, self.device = M, N, device
+        self._hold = (weights, scales, zeros)
+        self.desc = Q4Desc(M=M, N=N, ldw=ldw, lds=lds, group=group, dtype_x=dtype_x,
+                           dtype_y=dtype_x if dtype_y is None else dtype_y, dtype_s=dtype_s, W=_ptr(weights),
+                           scales=_ptr(scales), zeros=_ptr(zeros), device=device)
+        self._ref = C.byref(self.desc)
+        self._call = lib().l2d_q4_gemv
+
+    def gemv(self, x, y, vectors: int = 1, stride_x: int = 0, stride_y: int = 0, stream=None) -> None:
+        """y[b] = W.x[b]; stride_x / stride_y: elements between vectors (0 = N / M)."""
+        check(self._call(self._ref, _ptr(x), stride_x, _ptr(y), stride_y, vectors, _stream_handle(stream)))
+
+
+class KvCache:
+    """A paged cache of keys and values in memory of the caller's: ``num_pages`` pages of ``page_size``
+    slots of ``heads`` rows of ``head_dim`` elements.  ``k_strides`` / ``v_strides``: elements between
+    pages, slots and heads (None = dense [page][slot][head][dim])."""
+
+    def __init__(self, k, v, dtype: int, num_pages: int, page_size: int, heads: int, head_dim: int,
+                 k_strides: Optional[Sequence[int]] = None, v_strides: Optional[Sequence[int]] = None, device: int = 0):
+        self._hold = (k, v)
+        ks, vs = k_strides or (0, 0, 0), v_strides or (0, 0, 0)
+        self.fields = dict(k=_ptr(k), v=_ptr(v), dtype=dtype, heads=heads, head_dim=head_dim, page_size=page_size,
+                           num_pages=num_pages, k_page=ks[0], k_slot=ks[1], k_head=ks[2], v_page=vs[0], v_slot=vs[1],
+                           v_head=vs[2], device=device)
+
+    def desc(self, table, num_seqs: int, table_width: int, table_stride: int = 0, status=None) -> KvCacheDesc:
+        """The C description of this cache with a page table (int32, on the device)."""
+        return KvCacheDesc(table=_ptr(table), num_seqs=num_seqs, table_width=table_width, table_stride=table_stride,
+                           status=_ptr(status), **self.fields)
+
+
+class KvAppend:
+    """Appends new tokens' keys and values to a :class:`KvCache`, rotating keys (and queries) by their
+    positions on the way.  ``cos`` / ``sin``: fp32 [max_pos][rot_dim / 2], see :func:`rotation_tables`;
+    ``interleaved`` pairs elements (2i, 2i + 1) instead of (i, i + rot_dim / 2).  ``status``: a uint32 on the device that
+    collects KV_BAD_* bits."""
+
+    def __init__(self, cache: KvCache, table, num_seqs: int, table_width: int, heads_q: int = 0, cos=None, sin=None,
+                 max_pos: int = 0, rot_dim: int = 0, interleaved: bool = False, table_stride: int = 0, k_token: int = 0,
+                 v_token: int = 0, q_token: int = 0, q_out_token: int = 0, status=None):
+        self._hold = (cache, table, cos, sin, status)
+        self._cache = cache.desc(table, num_seqs, table_width, table_stride, status)
+        self._desc = AppendDesc(heads_q=heads_q, cos=_ptr(cos), sin=_ptr(sin), max_pos=max_pos, rot_dim=rot_dim,
+                                interleaved=int(interleaved), k_token=k_token, v_token=v_token, q_token=q_token,
+                                q_out_token=q_out_token)
+        self._refs = (C.byref(self._cache), C.byref(self._desc))
+        self._call = lib().l2d_kv_append
+
+    def append(self, k, v, pos, tokens: int, seq=None, q=None, q_out=None, stream=None) -> None:
+        """``pos`` (int32): each token's position, negative for padding; ``seq`` (int32): its row of the
+        page table (None: token t belongs to row t); ``q_out`` may be ``q``."""
+        check(self._call(self._refs[0], self._refs[1], _ptr(k), _ptr(v), _ptr(q), _ptr(q_out), _ptr(pos), _ptr(seq),
+                         tokens, _stream_handle(stream)))
+
+
+class PagedAttention:
+    """Attention of one new token per sequence over a :class:`KvCache`.  The plan owns its scratch; calls
+    of one plan must not overlap on the GPU.  ``scale`` 0 means 1 / sqrt(head_dim), ``window`` 0 all keys."""
+
+    def __init__(self, cache: KvCache, table, num_seqs: int, table_width: int, heads_q: int, scale: float = 0.0,
+                 window: int = 0, max_batch: int = 0, table_stride: int = 0, q_token: int = 0, out_token: int = 0,
+                 status=None):
+        self._plan = C.c_void_p(0)
+        self._hold = (cache, table, status)
+        cd = cache.desc(table, num_seqs, table_width, table_stride, status)
+        ad = AttnDesc(heads_q=heads_q, window=window, scale=scale, max_batch=max_batch, q_token=q_token,
+                      out_token=out_token)
+        check(lib().l2d_attn_plan_create(C.byref(cd), C.byref(ad), C.byref(self._plan)))
+        self._call = lib().l2d_attn_decode
+
+    def decode(self, q, out, lens, batch: int, lse=None, stream=None) -> None:
+        """out[b] = attention of q[b] over the first lens[b] (int32, on the device) positions of row b."""
+        check(self._call(self._plan, _ptr(q), _ptr(out), _ptr(lse), _ptr(lens), batch, _stream_handle(stream)))
+
+    def close(self) -> None:
+        if self._plan and self._plan.value:
+            check(lib().l2d_attn_plan_destroy(self._plan))
+            self._plan = C.c_void_p(0)
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def rotation_tables(max_pos: int, rot_dim: int, theta: float = 10000.0, stretch: float = 1.0, device=None):
+    """(cos, sin) fp32 [max_pos][rot_dim / 2] of position * theta^(-2i / rot_dim) / stretch, the angles in
+    64 bits (``stretch`` > 1 spreads a trained range over a longer context)."""
+    import torch
+
+    pos = torch.arange(max_pos, dtype=torch.float64, device=device)
+    freq = theta ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64, device=device) / max(rot_dim, 1)) / stretch
+    angle = pos[:, None] * freq[None, :]
+    return angle.cos().float(), angle.sin().float()
 
 
 # --------------------------------------------------------------------------------------------
