@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstring>
 #include <new>
 
 namespace l2d {
@@ -98,74 +99,665 @@ __global__ void __launch_bounds__(256) k_append(AppendArgs a) {
     }
 }
 
-// One block of four warps per sequence and query head; a warp takes every fourth key, a lane every 32nd
-// element of the head; the warps' parts meet in shared memory.
+// ---------------------------------------------------------------------------------------------
+// Attention of one token over the cache.
+//
+// Memory bound: each key and value is read once, for all query heads of its group.  A block of four
+// warps works on one key-value head of one sequence at a time; each warp streams its own 16 keys of
+// every 64 through a ring of shared memory of its own (asynchronous copies, no block-wide barrier in
+// the loop) and keeps a running maximum and sum per query head, so the data is passed over once.
+// 16-bit caches feed matrix instructions with the query heads as the 16 rows; 32-bit caches use fp32
+// fused multiply-adds.
+//
+// The tiles of all sequences and heads form one line that is cut into equal pieces, one per resident
+// block, whatever the lengths are: a long sequence is split over many blocks and a block may take
+// several short ones.  A piece that ends inside a sequence leaves its unnormalised sums in the plan's
+// scratch, and the last piece of that sequence to arrive adds them in piece order, so the result does
+// not depend on which block came last.
+// ---------------------------------------------------------------------------------------------
+
+constexpr int kAttnWarps = 4;
+constexpr int kAttnThreads = kAttnWarps * 32;
+constexpr int kMaxRows = 16;  // query heads a block works on
+
+struct AttnScratch {
+    float *part;         // [grid][2][kMaxRows][head_dim padded] unnormalised sums
+    float *ml;           // [grid][2][2][kMaxRows] their maxima (log2) and sums of weights
+    unsigned *arrived;   // [max_batch * heads * m_tiles], zero between calls
+};
+
+__device__ __forceinline__ uint32_t smem_addr(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+// 16 bytes to shared memory; none are read, and zeros stored, where `real` is false.
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool real) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+
 template <typename T>
-__global__ void __launch_bounds__(128) k_attn(AttnArgs a) {
-    dev::wait_for_previous();
-    const int D = a.c.head_dim, h = blockIdx.x % a.heads_q, b = blockIdx.x / a.heads_q;
-    const int hk = h / (a.heads_q / a.c.heads), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    constexpr int E = kMaxHeadDim / 32;
-    float q[E], o[E];
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(T lo, T hi) {
+    static_assert(sizeof(T) == 2, "16-bit types");
+    uint16_t a, b;
+    memcpy(&a, &lo, 2);
+    memcpy(&b, &hi, 2);
+    return static_cast<uint32_t>(a) | static_cast<uint32_t>(b) << 16;
+}
+
+// A running softmax's maximum, and what exponents are taken relative to: never -inf.
+__device__ __forceinline__ float finite_base(float m) { return m == -INFINITY ? 0.0f : m; }
+
+// One warp's part of one head group of a 16-bit cache: KS steps of 16 elements of the head, the query
+// heads as the rows of m16n8k16.  Groups of up to eight heads (SPLIT) use the other eight rows for the
+// low halves of the weights: p = hi + lo in two 16-bit numbers, so rounding p costs nothing there.
+// Larger groups round p once to the cache's type, 2^-9 (bf16) or 2^-12 (fp16) of each term.
+template <typename T, int KS, bool SPLIT>
+struct MmaCore {
+    using Elem = T;
+    static constexpr int kKeys = 16;                       // keys of a warp's tile
+    static constexpr int kRows = SPLIT ? 8 : 16;           // query heads
+    static constexpr int kDim = KS * 16;                   // head_dim, padded
+    static constexpr int kChunks = KS * 2;                 // 16-byte chunks of a row
+    static constexpr int kPitch = (kChunks + 1) * 16;      // an odd number of chunks: eight rows meet all banks
+    static constexpr bool kQueryInSmem = !SPLIT && KS > 8; // registers would not hold queries and sums
+    static constexpr int kQueryBytes = kQueryInSmem ? 16 * kPitch : 0;
+    static constexpr int kWarpBytes = 0;
+    uint32_t qa[kQueryInSmem ? 1 : KS][SPLIT ? 2 : 4];
+    float o[2 * KS][4], m[2], l[2];
+    uint32_t query;
+
+    // q: this group's first head; `heads` rows are real.  All threads of the block call it.
+    __device__ __forceinline__ void begin(const T *q, int heads, int D, char *smem_q, char *) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+        const T zero = dev::narrow<T>(0.0f);
+        if constexpr (kQueryInSmem) {
+            query = smem_addr(smem_q);
+            for (int e = threadIdx.x; e < 16 * kDim; e += kAttnThreads) {
+                const int r = e / kDim, i = e - r * kDim;
+                reinterpret_cast<T *>(smem_q + r * kPitch)[i] = r < heads && i < D ? q[int64_t(r) * D + i] : zero;
+            }
+            __syncthreads();
+        } else {
+            auto pair = [&](int r, int i) {
+                const T *p = q + int64_t(r) * D + i;
+                return pack2(r < heads && i < D ? p[0] : zero, r < heads && i + 1 < D ? p[1] : zero);
+            };
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int i = lane + 32 * e;
-        q[e] = i < D ? dev::widen(static_cast<const T *>(a.q)[b * a.q_token + int64_t(h) * D + i]) * a.scale : 0.0f;
-        o[e] = 0.0f;
+            for (int k = 0; k < KS; ++k) {
+                qa[k][0] = pair(g, 16 * k + 2 * t);
+                qa[k][SPLIT ? 1 : 2] = pair(g, 16 * k + 8 + 2 * t);
+                if constexpr (!SPLIT) {
+                    qa[k][1] = pair(g + 8, 16 * k + 2 * t);
+                    qa[k][3] = pair(g + 8, 16 * k + 8 + 2 * t);
+                }
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < 2 * KS; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n][e] = 0.0f;
+        m[0] = m[1] = -INFINITY;
+        l[0] = l[1] = 0.0f;
     }
-    float m = -INFINITY, l = 0.0f;
-    int64_t len = a.lens[b];
+
+    // One tile: keys at ks, values at vs (shared memory), bit j of live: key j counts.
+    __device__ __forceinline__ void step(const char *ks, const char *vs, uint32_t live, float scale2) {
+        const int lane = threadIdx.x & 31, t = lane & 3;
+        const uint32_t ka = smem_addr(ks) + ((lane >> 4) * 8 + (lane & 7)) * kPitch + ((lane >> 3) & 1) * 16;
+        const uint32_t va = smem_addr(vs) + (((lane >> 3) & 1) * 8 + (lane & 7)) * kPitch + (lane >> 4) * 16;
+        float s[2][4] = {};
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            uint32_t a[4], b[4];
+            if constexpr (kQueryInSmem) {
+                ldmatrix4(a, query + (((lane >> 3) & 1) * 8 + (lane & 7)) * kPitch + (lane >> 4) * 16 + k * 32);
+            } else if constexpr (SPLIT) {
+                a[0] = qa[k][0];
+                a[1] = 0;
+                a[2] = qa[k][1];
+                a[3] = 0;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) a[e] = qa[k][e];
+            }
+            ldmatrix4(b, ka + k * 32);
+            mma16816<T>(s[0], a, b[0], b[1]);
+            mma16816<T>(s[1], a, b[2], b[3]);
+        }
+        uint32_t p[4];
+#pragma unroll
+        for (int r = 0; r < (SPLIT ? 1 : 2); ++r) {
+            float x[4], top = -INFINITY;
+            bool ok[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                ok[e] = live >> ((e >> 1) * 8 + 2 * t + (e & 1)) & 1;
+                x[e] = s[e >> 1][2 * r + (e & 1)];
+                top = fmaxf(top, ok[e] ? x[e] * scale2 : -INFINITY);
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const float m2 = fmaxf(m[r], top), base = finite_base(m2);
+            if (__any_sync(0xffffffffu, m2 != m[r])) {
+                const float f = exp2_approx(m[r] - base);
+                l[r] *= f;
+#pragma unroll
+                for (int n = 0; n < 2 * KS; ++n) {
+                    o[n][2 * r] *= f;
+                    o[n][2 * r + 1] *= f;
+                    if constexpr (SPLIT) {
+                        o[n][2] *= f;
+                        o[n][3] *= f;
+                    }
+                }
+                m[r] = m2;
+            }
+            T hi[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[e] = ok[e] ? exp2_approx(fmaf(x[e], scale2, -base)) : 0.0f;
+                l[r] += x[e];
+                hi[e] = dev::narrow<T>(x[e]);
+            }
+            p[r] = pack2(hi[0], hi[1]);
+            p[r + 2] = pack2(hi[2], hi[3]);
+            if constexpr (SPLIT) {
+                p[1] = pack2(dev::narrow<T>(x[0] - dev::widen(hi[0])), dev::narrow<T>(x[1] - dev::widen(hi[1])));
+                p[3] = pack2(dev::narrow<T>(x[2] - dev::widen(hi[2])), dev::narrow<T>(x[3] - dev::widen(hi[3])));
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < KS; ++n) {
+            uint32_t b[4];
+            ldmatrix4_trans(b, va + n * 32);
+            mma16816<T>(o[2 * n], p, b[0], b[1]);
+            mma16816<T>(o[2 * n + 1], p, b[2], b[3]);
+        }
+    }
+
+    // This warp's sums [kRows][kDim], maxima and sums of weights [kRows] to shared memory.
+    __device__ __forceinline__ void end(float *so, float *sm, float *sl) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+        for (int r = 0; r < (SPLIT ? 1 : 2); ++r) {
+            float sum = l[r] + __shfl_xor_sync(0xffffffffu, l[r], 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            if (t == 0) {
+                sm[g + 8 * r] = m[r];
+                sl[g + 8 * r] = sum;
+            }
+#pragma unroll
+            for (int n = 0; n < 2 * KS; ++n) {
+                float2 v = make_float2(o[n][2 * r], o[n][2 * r + 1]);
+                if constexpr (SPLIT) v = make_float2(v.x + o[n][2], v.y + o[n][3]);
+                *reinterpret_cast<float2 *>(so + (g + 8 * r) * kDim + 8 * n + 2 * t) = v;
+            }
+        }
+    }
+};
+
+// The same for a 32-bit cache: GT query heads, DV x 128 elements of the head.  Scores: a lane per key
+// (two or four lanes share one, each every second or fourth chunk of the row), values: a lane per four
+// elements of the head, the weights passed through shared memory.
+template <int GT, int DV>
+struct SimdCore {
+    using Elem = float;
+    static constexpr int kKeys = DV == 1 ? 16 : 8;
+    static constexpr int kRows = GT;
+    static constexpr int kDim = DV * 128;
+    static constexpr int kChunks = kDim / 4;
+    static constexpr int kPitch = (kChunks + 1) * 16;
+    static constexpr int kQueryBytes = GT * kDim * 4;
+    static constexpr int kWarpBytes = GT * kKeys * 4;  // weights of the warp's tile
+    static constexpr int kParts = 32 / kKeys;
+    float o[GT][DV][4], m[GT], l[GT];
+    const float *query;
+    float *weights;
+    int chunks;
+
+    __device__ __forceinline__ void begin(const float *q, int heads, int D, char *smem_q, char *warp_smem) {
+        float *sq = reinterpret_cast<float *>(smem_q);
+        query = sq;
+        weights = reinterpret_cast<float *>(warp_smem);
+        chunks = (D + 3) / 4;
+        for (int e = threadIdx.x; e < GT * kDim; e += kAttnThreads) {
+            const int r = e / kDim, i = e - r * kDim;
+            sq[e] = r < heads && i < D ? q[int64_t(r) * D + i] : 0.0f;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int g = 0; g < GT; ++g) {
+            m[g] = -INFINITY;
+            l[g] = 0.0f;
+#pragma unroll
+            for (int v = 0; v < DV; ++v)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[g][v][e] = 0.0f;
+        }
+    }
+
+    __device__ __forceinline__ void step(const char *ks, const char *vs, uint32_t live, float scale2) {
+        const int lane = threadIdx.x & 31, key = lane % kKeys, sub = lane / kKeys;
+        float s[GT] = {};
+        const float4 *row = reinterpret_cast<const float4 *>(ks + key * kPitch);
+        for (int c = sub; c < chunks; c += kParts) {
+            const float4 k = row[c];
+#pragma unroll
+            for (int g = 0; g < GT; ++g) {
+                const float4 q = reinterpret_cast<const float4 *>(query + g * kDim)[c];
+                s[g] = fmaf(q.x, k.x, s[g]);
+                s[g] = fmaf(q.y, k.y, s[g]);
+                s[g] = fmaf(q.z, k.z, s[g]);
+                s[g] = fmaf(q.w, k.w, s[g]);
+            }
+        }
+        const bool ok = live >> key & 1;
+#pragma unroll
+        for (int g = 0; g < GT; ++g) {
+#pragma unroll
+            for (int d = kKeys; d < 32; d <<= 1) s[g] += __shfl_xor_sync(0xffffffffu, s[g], d);
+            float top = ok ? s[g] * scale2 : -INFINITY;
+#pragma unroll
+            for (int d = 1; d < kKeys; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            const float m2 = fmaxf(m[g], top), base = finite_base(m2), f = exp2_approx(m[g] - base);
+            const float w = ok ? exp2_approx(fmaf(s[g], scale2, -base)) : 0.0f;
+            l[g] = fmaf(l[g], f, w);
+            m[g] = m2;
+            if (sub == 0) weights[g * kKeys + key] = w;
+#pragma unroll
+            for (int v = 0; v < DV; ++v)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[g][v][e] *= f;
+        }
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < kKeys; j += 4) {
+#pragma unroll
+            for (int v = 0; v < DV; ++v) {
+                if (lane + 32 * v >= chunks) continue;
+                float4 x[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4 *>(vs + (j + i) * kPitch + (lane + 32 * v) * 16);
+#pragma unroll
+                for (int g = 0; g < GT; ++g) {
+                    const float4 w = *reinterpret_cast<const float4 *>(weights + g * kKeys + j);
+                    const float ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        o[g][v][0] = fmaf(ww[i], x[i].x, o[g][v][0]);
+                        o[g][v][1] = fmaf(ww[i], x[i].y, o[g][v][1]);
+                        o[g][v][2] = fmaf(ww[i], x[i].z, o[g][v][2]);
+                        o[g][v][3] = fmaf(ww[i], x[i].w, o[g][v][3]);
+                    }
+                }
+            }
+        }
+        __syncwarp();
+    }
+
+    __device__ __forceinline__ void end(float *so, float *sm, float *sl) {
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int g = 0; g < GT; ++g) {
+            float sum = l[g];
+#pragma unroll
+            for (int d = 1; d < kKeys; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+            if (lane == 0) {
+                sm[g] = m[g];
+                sl[g] = sum;
+            }
+#pragma unroll
+            for (int v = 0; v < DV; ++v)
+                *reinterpret_cast<float4 *>(so + g * kDim + 4 * (lane + 32 * v)) = make_float4(o[g][v][0], o[g][v][1], o[g][v][2], o[g][v][3]);
+        }
+    }
+};
+
+// Shared memory of a block: the rings (reused for the warps' sums at the end of a piece), queries, the
+// cores' own words, live bits per stage, maxima and sums.
+template <typename Core, int STAGES>
+struct AttnSmem {
+    static constexpr int kStage = 2 * Core::kKeys * Core::kPitch;
+    static constexpr int kRing = kAttnWarps * STAGES * kStage;
+    static constexpr int kSums = kAttnWarps * Core::kRows * Core::kDim * 4;
+    static constexpr int kQuery = kRing > kSums ? kRing : kSums;
+    static constexpr int kWarp = kQuery + Core::kQueryBytes;
+    static constexpr int kLive = kWarp + kAttnWarps * Core::kWarpBytes;
+    static constexpr int kMl = kLive + kAttnWarps * STAGES * 4;
+    static constexpr int kScan = kMl + kAttnWarps * 2 * kMaxRows * 4;
+    static constexpr int kBytes = kScan + 16 * 8;
+};
+
+// A warp's view of the keys of one sequence and head: page lookups run one tile ahead of the copies.
+template <typename Core, int STAGES>
+struct Stream {
+    using T = typename Core::Elem;
+    const Cache &c;
+    const char *k, *v;  // this head's rows
+    const int32_t *table;
+    char *ring;
+    uint32_t *live;
+    int64_t next;       // the key of lane 0 in the tile whose pages are in `page`
+    int len, step;      // keys of the sequence; keys between this warp's tiles
+    int slot, page;
+    bool aligned;
+
+    __device__ __forceinline__ Stream(const Cache &cache, char *r, uint32_t *lv, bool al) : c(cache), ring(r), live(lv), aligned(al) {}
+
+    __device__ __forceinline__ void lookup() {
+        const int lane = threadIdx.x & 31;
+        const int64_t key = next + lane;
+        page = -2;  // no such key
+        if (lane < Core::kKeys && key < len) {
+            const unsigned i = static_cast<unsigned>(key) / static_cast<unsigned>(c.page_size);
+            slot = static_cast<int>(static_cast<unsigned>(key) - i * static_cast<unsigned>(c.page_size));
+            page = max(table[i], -1);
+        }
+    }
+
+    // Starts the copies of the next tile into a stage of the ring.
+    __device__ __forceinline__ void issue(int stage) {
+        const int lane = threadIdx.x & 31;
+        const bool real = page >= 0 && page < c.num_pages;
+        if (!real && page != -2) report(c.status, L2D_KV_BAD_PAGE);
+        const uint32_t bits = __ballot_sync(0xffffffffu, real);
+        if (lane == 0) live[stage] = bits;
+        if (bits) {
+            const int64_t at = real ? page : 0;
+            const int64_t ko = real ? at * c.k_page + slot * c.k_slot : 0, vo = real ? at * c.v_page + slot * c.v_slot : 0;
+            char *dst = ring + stage * AttnSmem<Core, STAGES>::kStage;
+            const int row_bytes = c.head_dim * static_cast<int>(sizeof(T));
+            if (aligned) {
+                const uint32_t to = smem_addr(dst);
+#pragma unroll 4
+                for (int e = lane; e < Core::kKeys * Core::kChunks; e += 32) {
+                    const int r = e / Core::kChunks, ch = e - r * Core::kChunks;
+                    const int64_t kr = __shfl_sync(0xffffffffu, ko, r), vr = __shfl_sync(0xffffffffu, vo, r);
+                    const bool in = (bits >> r & 1) && ch * 16 < row_bytes;
+                    const int64_t off = in ? ch * 16 : 0;
+                    copy16(to + r * Core::kPitch + ch * 16, k + kr * static_cast<int>(sizeof(T)) + off, in);
+                    copy16(to + (Core::kKeys + r) * Core::kPitch + ch * 16, v + vr * static_cast<int>(sizeof(T)) + off, in);
+                }
+            } else {
+                for (int r = 0; r < Core::kKeys; ++r) {
+                    const int64_t kr = __shfl_sync(0xffffffffu, ko, r), vr = __shfl_sync(0xffffffffu, vo, r);
+                    T *kd = reinterpret_cast<T *>(dst + r * Core::kPitch), *vd = reinterpret_cast<T *>(dst + (Core::kKeys + r) * Core::kPitch);
+                    for (int i = lane; i < Core::kDim; i += 32) {
+                        const bool in = (bits >> r & 1) && i < c.head_dim;
+                        kd[i] = in ? reinterpret_cast<const T *>(k)[kr + i] : dev::narrow<T>(0.0f);
+                        vd[i] = in ? reinterpret_cast<const T *>(v)[vr + i] : dev::narrow<T>(0.0f);
+                    }
+                }
+            }
+        }
+        copies_commit();
+        next += step;
+        lookup();
+    }
+};
+
+struct Span {
+    int lo, len;
+    int64_t tiles;
+};
+
+template <int TILE>
+__device__ __forceinline__ Span span_of(const AttnArgs &a, int b) {
+    Span s;
     const int64_t room = int64_t(a.c.table_width) * a.c.page_size;
-    if (len > room) {
-        len = room;
-        if (threadIdx.x == 0) report(a.c.status, L2D_KV_BAD_PAGE);
+    s.len = static_cast<int>(min(static_cast<int64_t>(max(a.lens[b], 0)), room));
+    s.lo = a.window && s.len > a.window ? s.len - a.window : 0;
+    s.tiles = (int64_t(s.len) - s.lo + TILE - 1) / TILE;
+    return s;
+}
+
+template <typename Core, int STAGES>
+__global__ void __launch_bounds__(kAttnThreads) k_attn(AttnArgs a, AttnScratch sc, int m_tiles, int least, bool aligned) {
+    using T = typename Core::Elem;
+    using Sm = AttnSmem<Core, STAGES>;
+    constexpr int TILE = kAttnWarps * Core::kKeys;
+    extern __shared__ __align__(16) char smem[];
+    int64_t *scan = reinterpret_cast<int64_t *>(smem + Sm::kScan);
+    float *sm_m = reinterpret_cast<float *>(smem + Sm::kMl), *sm_l = sm_m + kAttnWarps * kMaxRows;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int D = a.c.head_dim, G = a.heads_q / a.c.heads, items = a.c.heads * m_tiles;
+    dev::wait_for_previous();
+
+    // Rows without a position.
+    for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
+        if (a.lens[b] > static_cast<int64_t>(a.c.table_width) * a.c.page_size && tid == 0) report(a.c.status, L2D_KV_BAD_PAGE);
+        if (span_of<TILE>(a, b).tiles) continue;
+        for (int i = tid; i < a.heads_q * D; i += kAttnThreads) static_cast<T *>(a.out)[b * a.out_token + i] = dev::narrow<T>(0.0f);
+        if (a.lse)
+            for (int h = tid; h < a.heads_q; h += kAttnThreads) a.lse[int64_t(b) * a.heads_q + h] = -INFINITY;
     }
-    for (int64_t p = (a.window && len > a.window ? len - a.window : 0) + warp; p < len; p += 4) {
-        const int64_t page = page_of(a.c, b, static_cast<int>(p));
-        if (page < 0) {
-            if (lane == 0) report(a.c.status, L2D_KV_BAD_PAGE);
+
+    // This block's piece of the line of tiles: where it starts.
+    int64_t mine = 0;
+    for (int b = tid; b < a.batch; b += kAttnThreads) mine += span_of<TILE>(a, b).tiles;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
+    if (lane == 0) scan[warp] = mine;
+    __syncthreads();
+    int64_t total = 0;
+#pragma unroll
+    for (int w = 0; w < kAttnWarps; ++w) total += scan[w];
+    total *= items;
+    const int64_t per = max((total + gridDim.x - 1) / gridDim.x, static_cast<int64_t>(least));
+    int64_t u = blockIdx.x * per;
+    const int64_t stop = min(total, u + per);
+    if (u >= stop) return;
+    int64_t before = 0;  // tiles of one head in the sequences before b
+    for (int first = 0;; first += kAttnThreads) {
+        const int64_t n = first + tid < a.batch ? span_of<TILE>(a, first + tid).tiles : 0;
+        int64_t upto = n;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int64_t x = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += x;
+        }
+        __syncthreads();
+        if (lane == 31) scan[warp] = upto;
+        if (tid == 0) scan[8] = -1;
+        __syncthreads();
+        int64_t base = before, all = before;
+#pragma unroll
+        for (int w = 0; w < kAttnWarps; ++w) {
+            if (w < warp) base += scan[w];
+            all += scan[w];
+        }
+        upto += base;
+        if (n && (upto - n) * items <= u && u < upto * items) {
+            scan[8] = first + tid;
+            scan[9] = upto - n;
+        }
+        __syncthreads();
+        before = all;
+        if (scan[8] >= 0) break;
+    }
+    int b = static_cast<int>(scan[8]);
+    before = scan[9];
+
+    const float scale2 = a.scale * 1.4426950408889634f;
+    Stream<Core, STAGES> in(a.c, smem + warp * STAGES * Sm::kStage, reinterpret_cast<uint32_t *>(smem + Sm::kLive) + warp * STAGES, aligned);
+    Core core;
+    const int64_t first_unit = u;
+    while (u < stop) {
+        const Span s = span_of<TILE>(a, b);
+        if (!s.tiles) {
+            ++b;
             continue;
         }
-        const int slot = static_cast<int>(p % a.c.page_size);
-        const T *k = reinterpret_cast<const T *>(a.c.k) + page * a.c.k_page + slot * a.c.k_slot + hk * a.c.k_head;
-        const T *v = reinterpret_cast<const T *>(a.c.v) + page * a.c.v_page + slot * a.c.v_slot + hk * a.c.v_head;
-        float s = 0.0f;
+        const int64_t at = u - before * items;
+        const int item = static_cast<int>(at / s.tiles);
+        if (item >= items) {
+            before += s.tiles;
+            ++b;
+            continue;
+        }
+        const int64_t t0 = at - item * s.tiles, t1 = min(s.tiles, t0 + (stop - u));
+        const int hk = item / m_tiles, row0 = (item - hk * m_tiles) * Core::kRows, rows = min(G - row0, Core::kRows);
+        const int head0 = hk * G + row0;
+
+        in.k = a.c.k + static_cast<int64_t>(hk) * a.c.k_head * static_cast<int64_t>(sizeof(T));
+        in.v = a.c.v + static_cast<int64_t>(hk) * a.c.v_head * static_cast<int64_t>(sizeof(T));
+        in.table = a.c.table + b * a.c.table_stride;
+        in.len = static_cast<int>(min(static_cast<int64_t>(s.len), s.lo + t1 * TILE));
+        in.next = s.lo + t0 * TILE + warp * Core::kKeys;
+        in.step = TILE;
+        const int n = static_cast<int>(t1 - t0);
+        in.lookup();
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (lane + 32 * e < D) s = fmaf(q[e], dev::widen(k[lane + 32 * e]), s);
+        for (int i = 0; i < STAGES - 1; ++i) in.issue(i);
+        core.begin(static_cast<const T *>(a.q) + b * a.q_token + static_cast<int64_t>(head0) * D, rows, D, smem + Sm::kQuery,
+                   smem + Sm::kWarp + warp * Core::kWarpBytes);
+        int stage = 0;
+        for (int i = 0; i < n; ++i) {
+            copies_wait<STAGES - 2>();
+            __syncwarp();
+            in.issue(stage == 0 ? STAGES - 1 : stage - 1);
+            const uint32_t live = in.live[stage];
+            const char *ks = in.ring + stage * Sm::kStage;
+            if (live) core.step(ks, ks + Core::kKeys * Core::kPitch, live, scale2);
+            stage = stage + 1 == STAGES ? 0 : stage + 1;
+        }
+        copies_wait<0>();
+        __syncthreads();
+
+        // The warps' sums meet.
+        float *sums = reinterpret_cast<float *>(smem);
+        core.end(sums + warp * Core::kRows * Core::kDim, sm_m + warp * kMaxRows, sm_l + warp * kMaxRows);
+        __syncthreads();
+        const bool whole = t0 == 0 && t1 == s.tiles;
+        const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + (u != first_unit);
+        for (int e = tid; e < rows * D; e += kAttnThreads) {
+            const int r = e / D, i = e - r * D;
+            float top = sm_m[r];
 #pragma unroll
-        for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-        const float m2 = fmaxf(m, s), base = m2 == -INFINITY ? 0.0f : m2;
-        const float f = expf(m - base), w = expf(s - base);
-        l = l * f + w;
+            for (int w = 1; w < kAttnWarps; ++w) top = fmaxf(top, sm_m[w * kMaxRows + r]);
+            const float base = finite_base(top);
+            float x = 0.0f, sum = 0.0f;
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (lane + 32 * e < D) o[e] = fmaf(w, dev::widen(v[lane + 32 * e]), o[e] * f);
-        m = m2;
+            for (int w = 0; w < kAttnWarps; ++w) {
+                const float f = exp2_approx(sm_m[w * kMaxRows + r] - base);
+                x = fmaf(f, sums[(w * Core::kRows + r) * Core::kDim + i], x);
+                sum = fmaf(f, sm_l[w * kMaxRows + r], sum);
+            }
+            if (whole) {
+                static_cast<T *>(a.out)[b * a.out_token + static_cast<int64_t>(head0 + r) * D + i] = dev::narrow<T>(sum == 0.0f ? 0.0f : x / sum);
+                if (i == 0 && a.lse)
+                    a.lse[static_cast<int64_t>(b) * a.heads_q + head0 + r] = sum == 0.0f ? -INFINITY : (base + log2f(sum)) * 0.6931471805599453f;
+            } else {
+                sc.part[(slot * kMaxRows + r) * Core::kDim + i] = x;
+                if (i == 0) {
+                    sc.ml[(slot * 2) * kMaxRows + r] = top;
+                    sc.ml[(slot * 2 + 1) * kMaxRows + r] = sum;
+                }
+            }
+        }
+        if (!whole) {
+            const int64_t u0 = u - t0, c0 = u0 / per, c1 = (u0 + s.tiles - 1) / per;
+            unsigned *count = sc.arrived + static_cast<int64_t>(b) * items + item;
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) {
+                const unsigned old = atomicAdd(count, 1u);
+                const bool last = old == static_cast<unsigned>(c1 - c0);
+                if (last) *count = 0;
+                scan[8] = last;
+            }
+            __syncthreads();
+            if (scan[8]) {
+                __threadfence();
+                for (int e = tid; e < rows * D; e += kAttnThreads) {
+                    const int r = e / D, i = e - r * D;
+                    float top = -INFINITY, x = 0.0f, sum = 0.0f;
+                    for (int64_t q = c0; q <= c1; ++q) {
+                        const int64_t ps = q * 2 + (q == c0 && u0 != c0 * per);
+                        const float pm = __ldcg(sc.ml + (ps * 2) * kMaxRows + r), pl = __ldcg(sc.ml + (ps * 2 + 1) * kMaxRows + r);
+                        const float px = __ldcg(sc.part + (ps * kMaxRows + r) * Core::kDim + i);
+                        const float m2 = fmaxf(top, pm), base = finite_base(m2), f0 = exp2_approx(top - base), f1 = exp2_approx(pm - base);
+                        x = fmaf(x, f0, px * f1);
+                        sum = fmaf(sum, f0, pl * f1);
+                        top = m2;
+                    }
+                    static_cast<T *>(a.out)[b * a.out_token + static_cast<int64_t>(head0 + r) * D + i] = dev::narrow<T>(sum == 0.0f ? 0.0f : x / sum);
+                    if (i == 0 && a.lse)
+                        a.lse[static_cast<int64_t>(b) * a.heads_q + head0 + r] =
+                            sum == 0.0f ? -INFINITY : (finite_base(top) + log2f(sum)) * 0.6931471805599453f;
+                }
+            }
+        }
+        u += t1 - t0;
+        __syncthreads();  // the rings hold sums until here
     }
-    __shared__ float part[4][kMaxHeadDim], pm[4], pl[4];
-#pragma unroll
-    for (int e = 0; e < E; ++e) part[warp][lane + 32 * e] = o[e];
-    if (lane == 0) {
-        pm[warp] = m;
-        pl[warp] = l;
+}
+
+struct AttnKernel {
+    void (*run)(AttnArgs, AttnScratch, int, int, bool);
+    int smem, rows, dim;
+};
+
+template <typename Core, int STAGES>
+AttnKernel attn_kernel() {
+    return {k_attn<Core, STAGES>, AttnSmem<Core, STAGES>::kBytes, Core::kRows, Core::kDim};
+}
+
+template <typename T, bool SPLIT>
+AttnKernel pick_mma(int D) {
+    if (D <= 64) return attn_kernel<MmaCore<T, 4, SPLIT>, 4>();
+    if (D <= 80) return attn_kernel<MmaCore<T, 5, SPLIT>, 4>();
+    if (D <= 96) return attn_kernel<MmaCore<T, 6, SPLIT>, 4>();
+    if (D <= 128) return attn_kernel<MmaCore<T, 8, SPLIT>, 3>();
+    if (D <= 192) return attn_kernel<MmaCore<T, 12, SPLIT>, 3>();
+    return attn_kernel<MmaCore<T, 16, SPLIT>, 3>();
+}
+
+AttnKernel pick_attn(int dtype, int D, int G) {
+    if (dtype == L2D_F16) return G <= 8 ? pick_mma<__half, true>(D) : pick_mma<__half, false>(D);
+    if (dtype == L2D_BF16) return G <= 8 ? pick_mma<__nv_bfloat16, true>(D) : pick_mma<__nv_bfloat16, false>(D);
+    if (D <= 128) {
+        if (G == 1) return attn_kernel<SimdCore<1, 1>, 3>();
+        if (G <= 4) return attn_kernel<SimdCore<4, 1>, 3>();
+        if (G <= 8) return attn_kernel<SimdCore<8, 1>, 3>();
+        return attn_kernel<SimdCore<16, 1>, 3>();
     }
-    __syncthreads();
-    const float top = fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])), base = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f, f[4];
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        f[w] = expf(pm[w] - base);
-        sum += f[w] * pl[w];
-    }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    for (int i = threadIdx.x; i < D; i += 128) {
-        float r = 0.0f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) r = fmaf(f[w], part[w][i], r);
-        static_cast<T *>(a.out)[b * a.out_token + int64_t(h) * D + i] = dev::narrow<T>(r * inv);
-    }
-    if (threadIdx.x == 0 && a.lse) a.lse[int64_t(b) * a.heads_q + h] = sum == 0.0f ? -INFINITY : base + logf(sum);
+    if (G == 1) return attn_kernel<SimdCore<1, 2>, 3>();
+    if (G <= 4) return attn_kernel<SimdCore<4, 2>, 3>();
+    return attn_kernel<SimdCore<8, 2>, 3>();
 }
 
 // Checks a cache description and fills in its strides.
@@ -222,7 +814,11 @@ using namespace l2d;
 struct l2d_attn_plan {
     Cache cache;
     l2d_attn_desc desc;
-    int dtype, device, sms;
+    int dtype, device, grid, m_tiles;
+    bool aligned;
+    AttnKernel kernel;
+    AttnScratch scratch;
+    void *memory;
 };
 
 extern "C" {
@@ -307,13 +903,45 @@ int l2d_attn_plan_create(const l2d_kv_cache *cache, const l2d_attn_desc *desc, l
     int sms = 0;
     st = device_sms(cache->device, &sms);
     if (st != L2D_OK) return st;
+    OnDevice on(cache->device);
+    L2D_CUDA_TRY(on.err);
+    const int G = d.heads_q / cache->heads;
+    const AttnKernel k = pick_attn(cache->dtype, cache->head_dim, G);
+    const int m_tiles = (G + k.rows - 1) / k.rows;
+    int blocks = 0;
+    L2D_CUDA_TRY(cudaFuncSetAttribute(k.run, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem));
+    L2D_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, k.run, kAttnThreads, k.smem));
+    if (blocks < 1) return set_error(L2D_ERR_CUDA, "the attention kernel does not fit an SM");
+    const int grid = sms * blocks;
+    const size_t part = size_t(grid) * 2 * kMaxRows * k.dim * 4, ml = size_t(grid) * 4 * kMaxRows * 4;
+    const size_t arrived = size_t(d.max_batch) * cache->heads * m_tiles * 4;
+    void *memory = nullptr;
+    L2D_CUDA_TRY(cudaMalloc(&memory, part + ml + arrived + 4));
+    cudaError_t e = cudaMemset(memory, 0, part + ml + arrived + 4);
+    if (e == cudaSuccess) e = cudaDeviceSynchronize();
+    if (e != cudaSuccess) {
+        cudaFree(memory);
+        return set_error(L2D_ERR_CUDA, "attention scratch: %s", cudaGetErrorString(e));
+    }
     l2d_attn_plan *p = new (std::nothrow) l2d_attn_plan();
-    if (!p) return set_error(L2D_ERR_INVALID, "out of host memory");
+    if (!p) {
+        cudaFree(memory);
+        return set_error(L2D_ERR_INVALID, "out of host memory");
+    }
+    char *base = static_cast<char *>(memory);
     p->cache = c;
     p->desc = d;
     p->dtype = cache->dtype;
     p->device = cache->device;
-    p->sms = sms;
+    p->grid = grid;
+    p->m_tiles = m_tiles;
+    p->kernel = k;
+    p->scratch = {reinterpret_cast<float *>(base), reinterpret_cast<float *>(base + part), reinterpret_cast<unsigned *>(base + part + ml)};
+    p->memory = memory;
+    // Asynchronous copies of 16 bytes need rows of whole 16-byte chunks on 16-byte boundaries.
+    const int64_t eb = elem_bytes(cache->dtype);
+    const int64_t any = cache->head_dim | c.k_page | c.k_slot | c.k_head | c.v_page | c.v_slot | c.v_head;
+    p->aligned = (any * eb) % 16 == 0 && !misaligned(c.k, 16) && !misaligned(c.v, 16);
     *plan = p;
     return L2D_OK;
 }
@@ -329,14 +957,16 @@ int l2d_attn_decode(l2d_attn_plan *p, const void *q, void *out, float *lse, cons
     OnDevice on(p->device);
     L2D_CUDA_TRY(on.err);
     AttnArgs a = {p->cache, q, out, lse, lens, p->desc.q_token, p->desc.out_token, p->desc.heads_q, p->desc.window, batch, p->desc.scale};
-    const dim3 grid(static_cast<unsigned>(batch) * p->desc.heads_q);
-    auto kernel = p->dtype == L2D_F32 ? k_attn<float> : p->dtype == L2D_F16 ? k_attn<__half> : k_attn<__nv_bfloat16>;
-    L2D_CUDA_TRY(launch(kernel, grid, 128, 0, stream, a));
+    L2D_CUDA_TRY(launch(p->kernel.run, dim3(p->grid), kAttnThreads, p->kernel.smem, stream, a, p->scratch, p->m_tiles, 4, p->aligned));
     return L2D_OK;
 }
 
 int l2d_attn_plan_destroy(l2d_attn_plan *p) {
+    if (!p) return L2D_OK;
+    OnDevice on(p->device);
+    cudaError_t e = cudaFree(p->memory);  // waits for the device
     delete p;
+    if (e != cudaSuccess) return set_error(L2D_ERR_CUDA, "attn_plan_destroy: %s", cudaGetErrorString(e));
     return L2D_OK;
 }
 
