@@ -118,7 +118,8 @@ __global__ void __launch_bounds__(256) k_append(AppendArgs a) {
 
 constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = kAttnWarps * 32;
-constexpr int kMaxRows = 16;  // query heads a block works on
+constexpr int kMaxRows = 16;    // query heads a block works on
+constexpr int kLeastTiles = 4;  // tiles of a block's piece, at least
 
 struct AttnScratch {
     float *part;         // [grid][2][kMaxRows][head_dim padded] unnormalised sums
@@ -193,37 +194,45 @@ struct MmaCore {
     static constexpr int kChunks = KS * 2;                 // 16-byte chunks of a row
     static constexpr int kPitch = (kChunks + 1) * 16;      // an odd number of chunks: eight rows meet all banks
     static constexpr bool kQueryInSmem = !SPLIT && KS > 8; // registers would not hold queries and sums
-    static constexpr int kQueryBytes = kQueryInSmem ? 16 * kPitch : 0;
+    static constexpr int kQueryBytes = kRows * kPitch;
     static constexpr int kWarpBytes = 0;
     uint32_t qa[kQueryInSmem ? 1 : KS][SPLIT ? 2 : 4];
     float o[2 * KS][4], m[2], l[2];
     uint32_t query;
 
     // q: this group's first head; `heads` rows are real.  All threads of the block call it.
-    __device__ __forceinline__ void begin(const T *q, int heads, int D, char *smem_q, char *) {
-        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-        const T zero = dev::narrow<T>(0.0f);
-        if constexpr (kQueryInSmem) {
-            query = smem_addr(smem_q);
-            for (int e = threadIdx.x; e < 16 * kDim; e += kAttnThreads) {
-                const int r = e / kDim, i = e - r * kDim;
-                reinterpret_cast<T *>(smem_q + r * kPitch)[i] = r < heads && i < D ? q[int64_t(r) * D + i] : zero;
+    __device__ __forceinline__ void begin(const T *q, int heads, int D, bool aligned, char *smem_q, char *) {
+        const int lane = threadIdx.x & 31;
+        if (aligned) {
+            for (int e = threadIdx.x; e < kRows * kChunks; e += kAttnThreads) {
+                const int r = e / kChunks, ch = e - r * kChunks;
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (r < heads && ch * 8 < D) x = *reinterpret_cast<const uint4 *>(q + r * D + ch * 8);
+                *reinterpret_cast<uint4 *>(smem_q + r * kPitch + ch * 16) = x;
             }
-            __syncthreads();
         } else {
-            auto pair = [&](int r, int i) {
-                const T *p = q + int64_t(r) * D + i;
-                return pack2(r < heads && i < D ? p[0] : zero, r < heads && i + 1 < D ? p[1] : zero);
-            };
+            for (int e = threadIdx.x; e < kRows * kDim; e += kAttnThreads) {
+                const int r = e / kDim, i = e - r * kDim;
+                reinterpret_cast<T *>(smem_q + r * kPitch)[i] = r < heads && i < D ? q[r * D + i] : dev::narrow<T>(0.0f);
+            }
+        }
+        __syncthreads();
+        query = smem_addr(smem_q);
+        if constexpr (SPLIT) {  // matrices of 8 heads x 8 elements, two steps of 16 at once
+            uint32_t r[4];
 #pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                qa[k][0] = pair(g, 16 * k + 2 * t);
-                qa[k][SPLIT ? 1 : 2] = pair(g, 16 * k + 8 + 2 * t);
-                if constexpr (!SPLIT) {
-                    qa[k][1] = pair(g + 8, 16 * k + 2 * t);
-                    qa[k][3] = pair(g + 8, 16 * k + 8 + 2 * t);
+            for (int k = 0; k < KS; k += 2) {
+                ldmatrix4(r, query + (lane & 7) * kPitch + min(2 * k + (lane >> 3), kChunks - 1) * 16);
+                qa[k][0] = r[0];
+                qa[k][1] = r[1];
+                if (k + 1 < KS) {
+                    qa[k + 1][0] = r[2];
+                    qa[k + 1][1] = r[3];
                 }
             }
+        } else if constexpr (!kQueryInSmem) {
+#pragma unroll
+            for (int k = 0; k < KS; ++k) load_query(qa[k], k);
         }
 #pragma unroll
         for (int n = 0; n < 2 * KS; ++n)
@@ -231,6 +240,11 @@ struct MmaCore {
             for (int e = 0; e < 4; ++e) o[n][e] = 0.0f;
         m[0] = m[1] = -INFINITY;
         l[0] = l[1] = 0.0f;
+    }
+
+    __device__ __forceinline__ void load_query(uint32_t (&a)[4], int k) const {
+        const int lane = threadIdx.x & 31;
+        ldmatrix4(a, query + (((lane >> 3) & 1) * 8 + (lane & 7)) * kPitch + (lane >> 4) * 16 + k * 32);
     }
 
     // One tile: keys at ks, values at vs (shared memory), bit j of live: key j counts.
@@ -243,7 +257,7 @@ struct MmaCore {
         for (int k = 0; k < KS; ++k) {
             uint32_t a[4], b[4];
             if constexpr (kQueryInSmem) {
-                ldmatrix4(a, query + (((lane >> 3) & 1) * 8 + (lane & 7)) * kPitch + (lane >> 4) * 16 + k * 32);
+                load_query(a, k);
             } else if constexpr (SPLIT) {
                 a[0] = qa[k][0];
                 a[1] = 0;
@@ -348,14 +362,14 @@ struct SimdCore {
     float *weights;
     int chunks;
 
-    __device__ __forceinline__ void begin(const float *q, int heads, int D, char *smem_q, char *warp_smem) {
+    __device__ __forceinline__ void begin(const float *q, int heads, int D, bool, char *smem_q, char *warp_smem) {
         float *sq = reinterpret_cast<float *>(smem_q);
         query = sq;
         weights = reinterpret_cast<float *>(warp_smem);
         chunks = (D + 3) / 4;
         for (int e = threadIdx.x; e < GT * kDim; e += kAttnThreads) {
             const int r = e / kDim, i = e - r * kDim;
-            sq[e] = r < heads && i < D ? q[int64_t(r) * D + i] : 0.0f;
+            sq[e] = r < heads && i < D ? q[r * D + i] : 0.0f;
         }
         __syncthreads();
 #pragma unroll
@@ -447,18 +461,22 @@ struct SimdCore {
 };
 
 // Shared memory of a block: the rings (reused for the warps' sums at the end of a piece), queries, the
-// cores' own words, live bits per stage, maxima and sums.
+// cores' own words, row offsets and live bits per stage, maxima and sums.
+constexpr int kJoin = 128;  // pieces whose factors are held at a time when a sequence's pieces are joined
 template <typename Core, int STAGES>
 struct AttnSmem {
     static constexpr int kStage = 2 * Core::kKeys * Core::kPitch;
     static constexpr int kRing = kAttnWarps * STAGES * kStage;
     static constexpr int kSums = kAttnWarps * Core::kRows * Core::kDim * 4;
-    static constexpr int kQuery = kRing > kSums ? kRing : kSums;
+    static constexpr int kFactors = kSums;  // behind the sums
+    static constexpr int kEnd = kFactors + kJoin * kMaxRows * 4;
+    static constexpr int kQuery = kRing > kEnd ? kRing : kEnd;
     static constexpr int kWarp = kQuery + Core::kQueryBytes;
-    static constexpr int kLive = kWarp + kAttnWarps * Core::kWarpBytes;
+    static constexpr int kRowAt = kWarp + kAttnWarps * Core::kWarpBytes;
+    static constexpr int kLive = kRowAt + kAttnWarps * Core::kKeys * 16;
     static constexpr int kMl = kLive + kAttnWarps * STAGES * 4;
-    static constexpr int kScan = kMl + kAttnWarps * 2 * kMaxRows * 4;
-    static constexpr int kBytes = kScan + 16 * 8;
+    static constexpr int kFlag = kMl + kAttnWarps * 2 * kMaxRows * 4;
+    static constexpr int kBytes = kFlag + 16;
 };
 
 // A warp's view of the keys of one sequence and head: page lookups run one tile ahead of the copies.
@@ -469,13 +487,15 @@ struct Stream {
     const char *k, *v;  // this head's rows
     const int32_t *table;
     char *ring;
+    longlong2 *row_at;  // where the rows of the tile being started are, in bytes from k and v
     uint32_t *live;
     int64_t next;       // the key of lane 0 in the tile whose pages are in `page`
     int len, step;      // keys of the sequence; keys between this warp's tiles
     int slot, page;
     bool aligned;
 
-    __device__ __forceinline__ Stream(const Cache &cache, char *r, uint32_t *lv, bool al) : c(cache), ring(r), live(lv), aligned(al) {}
+    __device__ __forceinline__ Stream(const Cache &cache, char *r, longlong2 *ra, uint32_t *lv, bool al)
+        : c(cache), ring(r), row_at(ra), live(lv), aligned(al) {}
 
     __device__ __forceinline__ void lookup() {
         const int lane = threadIdx.x & 31;
@@ -496,29 +516,33 @@ struct Stream {
         const uint32_t bits = __ballot_sync(0xffffffffu, real);
         if (lane == 0) live[stage] = bits;
         if (bits) {
-            const int64_t at = real ? page : 0;
-            const int64_t ko = real ? at * c.k_page + slot * c.k_slot : 0, vo = real ? at * c.v_page + slot * c.v_slot : 0;
+            constexpr int64_t eb = sizeof(T);
+            __syncwarp();  // the rows of the tile before have been read
+            if (lane < Core::kKeys)
+                row_at[lane] = real ? make_longlong2((page * c.k_page + slot * c.k_slot) * eb, (page * c.v_page + slot * c.v_slot) * eb)
+                                    : make_longlong2(0, 0);
+            __syncwarp();
             char *dst = ring + stage * AttnSmem<Core, STAGES>::kStage;
-            const int row_bytes = c.head_dim * static_cast<int>(sizeof(T));
             if (aligned) {
                 const uint32_t to = smem_addr(dst);
-#pragma unroll 4
+                const int row_bytes = c.head_dim * static_cast<int>(eb);
+#pragma unroll 8
                 for (int e = lane; e < Core::kKeys * Core::kChunks; e += 32) {
                     const int r = e / Core::kChunks, ch = e - r * Core::kChunks;
-                    const int64_t kr = __shfl_sync(0xffffffffu, ko, r), vr = __shfl_sync(0xffffffffu, vo, r);
+                    const longlong2 at = row_at[r];
                     const bool in = (bits >> r & 1) && ch * 16 < row_bytes;
-                    const int64_t off = in ? ch * 16 : 0;
-                    copy16(to + r * Core::kPitch + ch * 16, k + kr * static_cast<int>(sizeof(T)) + off, in);
-                    copy16(to + (Core::kKeys + r) * Core::kPitch + ch * 16, v + vr * static_cast<int>(sizeof(T)) + off, in);
+                    const int off = in ? ch * 16 : 0;
+                    copy16(to + r * Core::kPitch + ch * 16, k + at.x + off, in);
+                    copy16(to + (Core::kKeys + r) * Core::kPitch + ch * 16, v + at.y + off, in);
                 }
             } else {
                 for (int r = 0; r < Core::kKeys; ++r) {
-                    const int64_t kr = __shfl_sync(0xffffffffu, ko, r), vr = __shfl_sync(0xffffffffu, vo, r);
+                    const longlong2 at = row_at[r];
                     T *kd = reinterpret_cast<T *>(dst + r * Core::kPitch), *vd = reinterpret_cast<T *>(dst + (Core::kKeys + r) * Core::kPitch);
                     for (int i = lane; i < Core::kDim; i += 32) {
                         const bool in = (bits >> r & 1) && i < c.head_dim;
-                        kd[i] = in ? reinterpret_cast<const T *>(k)[kr + i] : dev::narrow<T>(0.0f);
-                        vd[i] = in ? reinterpret_cast<const T *>(v)[vr + i] : dev::narrow<T>(0.0f);
+                        kd[i] = in ? reinterpret_cast<const T *>(k + at.x)[i] : dev::narrow<T>(0.0f);
+                        vd[i] = in ? reinterpret_cast<const T *>(v + at.y)[i] : dev::narrow<T>(0.0f);
                     }
                 }
             }
@@ -530,121 +554,191 @@ struct Stream {
 };
 
 struct Span {
-    int lo, len;
-    int64_t tiles;
+    int lo, len, tiles;
 };
 
 template <int TILE>
 __device__ __forceinline__ Span span_of(const AttnArgs &a, int b) {
     Span s;
-    const int64_t room = int64_t(a.c.table_width) * a.c.page_size;
-    s.len = static_cast<int>(min(static_cast<int64_t>(max(a.lens[b], 0)), room));
+    const int room = a.c.table_width * a.c.page_size;  // below 2^31
+    s.len = min(max(a.lens[b], 0), room);
     s.lo = a.window && s.len > a.window ? s.len - a.window : 0;
-    s.tiles = (int64_t(s.len) - s.lo + TILE - 1) / TILE;
+    s.tiles = (s.len - s.lo) / TILE + ((s.len - s.lo) % TILE != 0);
     return s;
 }
 
+// a / b of two non-negative numbers, mostly below 2^32.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+    if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+    return a / b;
+}
+
+// Where a head's row of the output and its log-sum-exp go.
+template <typename T>
+__device__ __forceinline__ void store_row4(const AttnArgs &a, int b, int h, int i, int D, float4 x, float base, float sum) {
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float v[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
+    T *out = static_cast<T *>(a.out) + b * a.out_token + static_cast<int64_t>(h) * D + i;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (i + e < D) out[e] = dev::narrow<T>(sum == 0.0f ? 0.0f : v[e]);
+    if (i == 0 && a.lse) a.lse[static_cast<int64_t>(b) * a.heads_q + h] = sum == 0.0f ? -INFINITY : (base + log2f(sum)) * 0.6931471805599453f;
+}
+
+// Joins the pieces c0..c1 of one item: piece q's sums are in slot 2q, the first one's in slot 2 c0 + odd.
+template <typename Core>
+__device__ __forceinline__ void join(const AttnArgs &a, const AttnScratch &sc, int c0, int c1, int odd, int b, int head0, int rows,
+                                     float *sums, float *factors, float *sm_m, float *sm_l) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, D = a.c.head_dim, n = c1 - c0 + 1;
+    auto slot = [&](int j) { return static_cast<int64_t>(c0 + j) * 2 + (j == 0 ? odd : 0); };
+    // Each row's maximum and sum of weights, lanes over the pieces.
+    for (int r = warp; r < rows; r += kAttnWarps) {
+        float top = -INFINITY, sum = 0.0f;
+        for (int j = lane; j < n; j += 32) top = fmaxf(top, __ldcg(sc.ml + slot(j) * 2 * kMaxRows + r));
+#pragma unroll
+        for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        for (int j = lane; j < n; j += 32) {
+            const float *ml = sc.ml + slot(j) * 2 * kMaxRows + r;
+            sum = fmaf(exp2_approx(__ldcg(ml) - finite_base(top)), __ldcg(ml + kMaxRows), sum);
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if (lane == 0) {
+            sm_m[r] = finite_base(top);
+            sm_l[r] = sum;
+        }
+    }
+    __syncthreads();
+    // The sums, warps over the pieces, up to 1024 elements (of whole rows' float4s) at a time.
+    constexpr int kQuads = Core::kRows * Core::kDim / 4, kEach = kQuads < 256 ? kQuads / 32 : 8, kRowQuads = Core::kDim / 4;
+    static_assert(kQuads % 32 == 0, "a warp covers whole rows");
+    for (int first = 0; first < kQuads; first += 32 * kEach) {
+        float4 acc[kEach];
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) acc[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int p0 = 0; p0 < n; p0 += kJoin) {
+            const int pn = min(n - p0, kJoin);
+            __syncthreads();
+            for (int e = tid; e < pn * kMaxRows; e += kAttnThreads) {
+                const int j = e / kMaxRows, r = e % kMaxRows;
+                factors[e] = r < rows ? exp2_approx(__ldcg(sc.ml + slot(p0 + j) * 2 * kMaxRows + r) - sm_m[r]) : 0.0f;
+            }
+            __syncthreads();
+#pragma unroll 2
+            for (int j = warp; j < pn; j += kAttnWarps) {
+                const float4 *part = reinterpret_cast<const float4 *>(sc.part + slot(p0 + j) * kMaxRows * Core::kDim);
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) {
+                    const int q = first + lane + 32 * i, r = q / kRowQuads;
+                    if (q < kQuads && r < rows) {
+                        const float f = factors[j * kMaxRows + r];
+                        const float4 x = __ldcg(part + q);
+                        acc[i] = make_float4(fmaf(f, x.x, acc[i].x), fmaf(f, x.y, acc[i].y), fmaf(f, x.z, acc[i].z), fmaf(f, x.w, acc[i].w));
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            if (first + lane + 32 * i < kQuads) reinterpret_cast<float4 *>(sums)[warp * kQuads + first + lane + 32 * i] = acc[i];
+    }
+    __syncthreads();
+    for (int q = tid; q < rows * kRowQuads; q += kAttnThreads) {
+        const int r = q / kRowQuads, i = (q - r * kRowQuads) * 4;
+        if (i >= D) continue;
+        float4 x = reinterpret_cast<const float4 *>(sums)[q];
+#pragma unroll
+        for (int w = 1; w < kAttnWarps; ++w) {
+            const float4 y = reinterpret_cast<const float4 *>(sums)[w * kQuads + q];
+            x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+        }
+        store_row4<typename Core::Elem>(a, b, head0 + r, i, D, x, sm_m[r], sm_l[r]);
+    }
+}
+
 template <typename Core, int STAGES>
-__global__ void __launch_bounds__(kAttnThreads) k_attn(AttnArgs a, AttnScratch sc, int m_tiles, int least, bool aligned) {
+__global__ void __launch_bounds__(kAttnThreads) k_attn(AttnArgs a, AttnScratch sc, int m_tiles, int least, bool aligned, bool q_aligned) {
     using T = typename Core::Elem;
     using Sm = AttnSmem<Core, STAGES>;
     constexpr int TILE = kAttnWarps * Core::kKeys;
     extern __shared__ __align__(16) char smem[];
-    int64_t *scan = reinterpret_cast<int64_t *>(smem + Sm::kScan);
     float *sm_m = reinterpret_cast<float *>(smem + Sm::kMl), *sm_l = sm_m + kAttnWarps * kMaxRows;
+    int *flag = reinterpret_cast<int *>(smem + Sm::kFlag);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int D = a.c.head_dim, G = a.heads_q / a.c.heads, items = a.c.heads * m_tiles;
     dev::wait_for_previous();
 
-    // Rows without a position.
+    // All tiles of one head, and rows without a position.
+    int64_t total = 0;
+    for (int b = lane; b < a.batch; b += 32) total += span_of<TILE>(a, b).tiles;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
     for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
-        if (a.lens[b] > static_cast<int64_t>(a.c.table_width) * a.c.page_size && tid == 0) report(a.c.status, L2D_KV_BAD_PAGE);
+        if (tid == 0 && a.lens[b] > a.c.table_width * a.c.page_size) report(a.c.status, L2D_KV_BAD_PAGE);
         if (span_of<TILE>(a, b).tiles) continue;
         for (int i = tid; i < a.heads_q * D; i += kAttnThreads) static_cast<T *>(a.out)[b * a.out_token + i] = dev::narrow<T>(0.0f);
         if (a.lse)
-            for (int h = tid; h < a.heads_q; h += kAttnThreads) a.lse[int64_t(b) * a.heads_q + h] = -INFINITY;
+            for (int h = tid; h < a.heads_q; h += kAttnThreads) a.lse[static_cast<int64_t>(b) * a.heads_q + h] = -INFINITY;
     }
 
-    // This block's piece of the line of tiles: where it starts.
-    int64_t mine = 0;
-    for (int b = tid; b < a.batch; b += kAttnThreads) mine += span_of<TILE>(a, b).tiles;
-#pragma unroll
-    for (int d = 16; d; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
-    if (lane == 0) scan[warp] = mine;
-    __syncthreads();
-    int64_t total = 0;
-#pragma unroll
-    for (int w = 0; w < kAttnWarps; ++w) total += scan[w];
+    // This block's piece of the line of tiles, and the sequence it starts in (every warp looks for itself).
     total *= items;
-    const int64_t per = max((total + gridDim.x - 1) / gridDim.x, static_cast<int64_t>(least));
+    const int64_t per = max(quotient(total + gridDim.x - 1, gridDim.x), static_cast<int64_t>(least));
     int64_t u = blockIdx.x * per;
-    const int64_t stop = min(total, u + per);
+    const int64_t first_unit = u, stop = min(total, u + per);
     if (u >= stop) return;
     int64_t before = 0;  // tiles of one head in the sequences before b
-    for (int first = 0;; first += kAttnThreads) {
-        const int64_t n = first + tid < a.batch ? span_of<TILE>(a, first + tid).tiles : 0;
+    int b = 0;
+    for (;; b += 32) {
+        const int64_t n = b + lane < a.batch ? span_of<TILE>(a, b + lane).tiles : 0;
         int64_t upto = n;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
             const int64_t x = __shfl_up_sync(0xffffffffu, upto, d);
             if (lane >= d) upto += x;
         }
-        __syncthreads();
-        if (lane == 31) scan[warp] = upto;
-        if (tid == 0) scan[8] = -1;
-        __syncthreads();
-        int64_t base = before, all = before;
-#pragma unroll
-        for (int w = 0; w < kAttnWarps; ++w) {
-            if (w < warp) base += scan[w];
-            all += scan[w];
+        upto += before;
+        const unsigned found = __ballot_sync(0xffffffffu, n && u < upto * items);
+        if (found) {
+            const int l = __ffs(found) - 1;
+            before = __shfl_sync(0xffffffffu, upto - n, l);
+            b += l;
+            break;
         }
-        upto += base;
-        if (n && (upto - n) * items <= u && u < upto * items) {
-            scan[8] = first + tid;
-            scan[9] = upto - n;
-        }
-        __syncthreads();
-        before = all;
-        if (scan[8] >= 0) break;
+        before = __shfl_sync(0xffffffffu, upto, 31);
     }
-    int b = static_cast<int>(scan[8]);
-    before = scan[9];
 
     const float scale2 = a.scale * 1.4426950408889634f;
-    Stream<Core, STAGES> in(a.c, smem + warp * STAGES * Sm::kStage, reinterpret_cast<uint32_t *>(smem + Sm::kLive) + warp * STAGES, aligned);
+    Stream<Core, STAGES> in(a.c, smem + warp * STAGES * Sm::kStage, reinterpret_cast<longlong2 *>(smem + Sm::kRowAt) + warp * Core::kKeys,
+                            reinterpret_cast<uint32_t *>(smem + Sm::kLive) + warp * STAGES, aligned);
     Core core;
-    const int64_t first_unit = u;
     while (u < stop) {
         const Span s = span_of<TILE>(a, b);
-        if (!s.tiles) {
-            ++b;
-            continue;
-        }
         const int64_t at = u - before * items;
-        const int item = static_cast<int>(at / s.tiles);
-        if (item >= items) {
+        if (!s.tiles || at >= static_cast<int64_t>(s.tiles) * items) {
             before += s.tiles;
             ++b;
             continue;
         }
-        const int64_t t0 = at - item * s.tiles, t1 = min(s.tiles, t0 + (stop - u));
+        const int item = static_cast<int>(quotient(at, s.tiles));
+        const int t0 = static_cast<int>(at - static_cast<int64_t>(item) * s.tiles);
+        const int n = static_cast<int>(min(static_cast<int64_t>(s.tiles - t0), stop - u));
         const int hk = item / m_tiles, row0 = (item - hk * m_tiles) * Core::kRows, rows = min(G - row0, Core::kRows);
         const int head0 = hk * G + row0;
 
-        in.k = a.c.k + static_cast<int64_t>(hk) * a.c.k_head * static_cast<int64_t>(sizeof(T));
-        in.v = a.c.v + static_cast<int64_t>(hk) * a.c.v_head * static_cast<int64_t>(sizeof(T));
+        in.k = a.c.k + hk * a.c.k_head * static_cast<int64_t>(sizeof(T));
+        in.v = a.c.v + hk * a.c.v_head * static_cast<int64_t>(sizeof(T));
         in.table = a.c.table + b * a.c.table_stride;
-        in.len = static_cast<int>(min(static_cast<int64_t>(s.len), s.lo + t1 * TILE));
-        in.next = s.lo + t0 * TILE + warp * Core::kKeys;
+        in.len = static_cast<int>(min(static_cast<int64_t>(s.len), s.lo + static_cast<int64_t>(t0 + n) * TILE));
+        in.next = s.lo + static_cast<int64_t>(t0) * TILE + warp * Core::kKeys;
         in.step = TILE;
-        const int n = static_cast<int>(t1 - t0);
         in.lookup();
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < STAGES - 1; ++i) in.issue(i);
-        core.begin(static_cast<const T *>(a.q) + b * a.q_token + static_cast<int64_t>(head0) * D, rows, D, smem + Sm::kQuery,
+        core.begin(static_cast<const T *>(a.q) + b * a.q_token + static_cast<int64_t>(head0) * D, rows, D, q_aligned, smem + Sm::kQuery,
                    smem + Sm::kWarp + warp * Core::kWarpBytes);
         int stage = 0;
+#pragma unroll 1
         for (int i = 0; i < n; ++i) {
             copies_wait<STAGES - 2>();
             __syncwarp();
@@ -661,79 +755,65 @@ __global__ void __launch_bounds__(kAttnThreads) k_attn(AttnArgs a, AttnScratch s
         float *sums = reinterpret_cast<float *>(smem);
         core.end(sums + warp * Core::kRows * Core::kDim, sm_m + warp * kMaxRows, sm_l + warp * kMaxRows);
         __syncthreads();
-        const bool whole = t0 == 0 && t1 == s.tiles;
+        const bool whole = n == s.tiles;
         const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + (u != first_unit);
-        for (int e = tid; e < rows * D; e += kAttnThreads) {
-            const int r = e / D, i = e - r * D;
+        constexpr int kRowQuads = Core::kDim / 4;
+        for (int q = tid; q < rows * kRowQuads; q += kAttnThreads) {
+            const int r = q / kRowQuads, i = (q - r * kRowQuads) * 4;
+            if (i >= D) continue;
             float top = sm_m[r];
 #pragma unroll
             for (int w = 1; w < kAttnWarps; ++w) top = fmaxf(top, sm_m[w * kMaxRows + r]);
             const float base = finite_base(top);
-            float x = 0.0f, sum = 0.0f;
+            float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            float sum = 0.0f;
 #pragma unroll
             for (int w = 0; w < kAttnWarps; ++w) {
                 const float f = exp2_approx(sm_m[w * kMaxRows + r] - base);
-                x = fmaf(f, sums[(w * Core::kRows + r) * Core::kDim + i], x);
+                const float4 y = *reinterpret_cast<const float4 *>(sums + (w * Core::kRows + r) * Core::kDim + i);
+                x = make_float4(fmaf(f, y.x, x.x), fmaf(f, y.y, x.y), fmaf(f, y.z, x.z), fmaf(f, y.w, x.w));
                 sum = fmaf(f, sm_l[w * kMaxRows + r], sum);
             }
             if (whole) {
-                static_cast<T *>(a.out)[b * a.out_token + static_cast<int64_t>(head0 + r) * D + i] = dev::narrow<T>(sum == 0.0f ? 0.0f : x / sum);
-                if (i == 0 && a.lse)
-                    a.lse[static_cast<int64_t>(b) * a.heads_q + head0 + r] = sum == 0.0f ? -INFINITY : (base + log2f(sum)) * 0.6931471805599453f;
+                store_row4<T>(a, b, head0 + r, i, D, x, base, sum);
             } else {
-                sc.part[(slot * kMaxRows + r) * Core::kDim + i] = x;
+                *reinterpret_cast<float4 *>(sc.part + (slot * kMaxRows + r) * Core::kDim + i) = x;
                 if (i == 0) {
-                    sc.ml[(slot * 2) * kMaxRows + r] = top;
+                    sc.ml[slot * 2 * kMaxRows + r] = top;
                     sc.ml[(slot * 2 + 1) * kMaxRows + r] = sum;
                 }
             }
         }
         if (!whole) {
-            const int64_t u0 = u - t0, c0 = u0 / per, c1 = (u0 + s.tiles - 1) / per;
-            unsigned *count = sc.arrived + static_cast<int64_t>(b) * items + item;
+            const int64_t u0 = u - t0;
+            const int c0 = static_cast<int>(quotient(u0, per)), c1 = static_cast<int>(quotient(u0 + s.tiles - 1, per));
             __threadfence();
             __syncthreads();
             if (tid == 0) {
-                const unsigned old = atomicAdd(count, 1u);
-                const bool last = old == static_cast<unsigned>(c1 - c0);
+                unsigned *count = sc.arrived + static_cast<int64_t>(b) * items + item;
+                const bool last = atomicAdd(count, 1u) == static_cast<unsigned>(c1 - c0);
                 if (last) *count = 0;
-                scan[8] = last;
+                *flag = last;
             }
             __syncthreads();
-            if (scan[8]) {
+            if (*flag) {
                 __threadfence();
-                for (int e = tid; e < rows * D; e += kAttnThreads) {
-                    const int r = e / D, i = e - r * D;
-                    float top = -INFINITY, x = 0.0f, sum = 0.0f;
-                    for (int64_t q = c0; q <= c1; ++q) {
-                        const int64_t ps = q * 2 + (q == c0 && u0 != c0 * per);
-                        const float pm = __ldcg(sc.ml + (ps * 2) * kMaxRows + r), pl = __ldcg(sc.ml + (ps * 2 + 1) * kMaxRows + r);
-                        const float px = __ldcg(sc.part + (ps * kMaxRows + r) * Core::kDim + i);
-                        const float m2 = fmaxf(top, pm), base = finite_base(m2), f0 = exp2_approx(top - base), f1 = exp2_approx(pm - base);
-                        x = fmaf(x, f0, px * f1);
-                        sum = fmaf(sum, f0, pl * f1);
-                        top = m2;
-                    }
-                    static_cast<T *>(a.out)[b * a.out_token + static_cast<int64_t>(head0 + r) * D + i] = dev::narrow<T>(sum == 0.0f ? 0.0f : x / sum);
-                    if (i == 0 && a.lse)
-                        a.lse[static_cast<int64_t>(b) * a.heads_q + head0 + r] =
-                            sum == 0.0f ? -INFINITY : (finite_base(top) + log2f(sum)) * 0.6931471805599453f;
-                }
+                join<Core>(a, sc, c0, c1, u0 != c0 * per, b, head0, rows, sums, reinterpret_cast<float *>(smem + Sm::kFactors), sm_m, sm_l);
             }
         }
-        u += t1 - t0;
+        u += n;
         __syncthreads();  // the rings hold sums until here
     }
 }
 
 struct AttnKernel {
-    void (*run)(AttnArgs, AttnScratch, int, int, bool);
-    int smem, rows, dim;
+    void (*run)(AttnArgs, AttnScratch, int, int, bool, bool);
+    int smem, rows, dim, tile;
 };
 
 template <typename Core, int STAGES>
 AttnKernel attn_kernel() {
-    return {k_attn<Core, STAGES>, AttnSmem<Core, STAGES>::kBytes, Core::kRows, Core::kDim};
+    return {k_attn<Core, STAGES>, AttnSmem<Core, STAGES>::kBytes, Core::kRows, Core::kDim, kAttnWarps * Core::kKeys};
 }
 
 template <typename T, bool SPLIT>
@@ -956,8 +1036,13 @@ int l2d_attn_decode(l2d_attn_plan *p, const void *q, void *out, float *lse, cons
         return set_error(L2D_ERR_INVALID, "pointers must be aligned to their elements");
     OnDevice on(p->device);
     L2D_CUDA_TRY(on.err);
+    const bool q_aligned = !misaligned(q, 16) && (p->desc.q_token * eb) % 16 == 0 && (p->cache.head_dim * eb) % 16 == 0;
+    // No more blocks than pieces the page table leaves room for.
+    const int64_t room = int64_t(p->cache.table_width) * p->cache.page_size, tiles = (room + p->kernel.tile - 1) / p->kernel.tile;
+    const int64_t most = std::max<int64_t>(1, (tiles * batch * p->cache.heads * p->m_tiles + kLeastTiles - 1) / kLeastTiles);
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(p->grid, most)));
     AttnArgs a = {p->cache, q, out, lse, lens, p->desc.q_token, p->desc.out_token, p->desc.heads_q, p->desc.window, batch, p->desc.scale};
-    L2D_CUDA_TRY(launch(p->kernel.run, dim3(p->grid), kAttnThreads, p->kernel.smem, stream, a, p->scratch, p->m_tiles, 4, p->aligned));
+    L2D_CUDA_TRY(launch(p->kernel.run, grid, kAttnThreads, p->kernel.smem, stream, a, p->scratch, p->m_tiles, kLeastTiles, p->aligned, q_aligned));
     return L2D_OK;
 }
 
