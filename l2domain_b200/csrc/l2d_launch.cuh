@@ -54,18 +54,26 @@ struct OnDevice {
 // resident while that kernel drains, and wait for all of it with wait_for_previous() before their first
 // access to global memory; after any other kernel this is an ordinary stream-ordered launch.
 template <typename... P, typename... A>
-cudaError_t launch(void (*k)(P...), dim3 grid, int block, size_t smem, void *stream, A... args) {
+cudaError_t launch_clusters(void (*k)(P...), dim3 grid, int cluster, int block, size_t smem, void *stream, A... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(static_cast<unsigned>(block));
     cfg.dynamicSmemBytes = smem;
     cfg.stream = static_cast<cudaStream_t>(stream);
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, k, static_cast<P>(args)...);
+}
+
+template <typename... P, typename... A>
+cudaError_t launch(void (*k)(P...), dim3 grid, int block, size_t smem, void *stream, A... args) {
+    return launch_clusters(k, grid, 1, block, smem, stream, args...);
 }
 
 // Raises a kernel's dynamic shared memory limit on the current device, once per device.  `done` is the

@@ -3,23 +3,36 @@
 //   y[b][i] = sum_j s[i][j / g] * (q[i][j] - z[i][j / g]) * x[b][j]
 //
 // Memory bound: a weight is half a byte and is used once per vector.  At the bandwidth of HBM an SM
-// gets about 52 weights a cycle and has 128 lanes to treat them, so a weight may cost two instructions;
-// a fused multiply-add in fp32 alone would be one, with its conversion three.  So the products run on
-// matrix instructions (m16n8k16, fp32 sums): 16 rows of weights are the A operand, turned from nibbles
-// into exact 16-bit integers q - z in about 1.2 instructions a weight, the vectors are the columns of B,
-// and the scales are applied to the fp32 sums of each group, so nothing is rounded before the end.
+// gets about 52 weights a cycle and has 128 lanes to treat them, so a weight may cost little over two
+// instructions; a fused multiply-add in fp32 with its conversion would be three or four.  So the products
+// run on matrix instructions (m16n8k16, fp32 sums), 16 rows of weights as the A operand and the vectors
+// as columns of B, and everything else is arranged to spend next to nothing per weight:
 //
+//  * A nibble masked into the low mantissa bits of a 16-bit float is the subnormal q 2^-24, one higher up
+//    16 q 2^-24: both exact, and no instruction but the mask.  x of the columns that end up higher is a
+//    sixteenth of itself.  What the zero point takes away is z times the group's sum of x, which is
+//    computed once per block: sum (q - z) x = sum q x - z sum x, in fp32.
+//  * x is held in shared memory as fp16, each 128 columns of a vector scaled by a power of two to a
+//    largest value just under 2^15, in one part (fp16 and bf16) or two (fp32: 11 bits, and the next 11 as a
+//    column of their own).  That keeps fp16 and bf16 exact and fp32 to one rounding of 2^-24 for values
+//    down to 2^-28 of the largest among its 128 columns; smaller ones are off by up to 2^-36 of the largest.
+//  * Infinities and NaNs do not survive sum q x - z sum x.  They are staged as zeros, and the threads that
+//    store a vector's results add the terms of its infinities and NaNs at the end, one by one.
+//  * The scales are applied to the fp32 sums of each group.  One instruction sums over the four lanes of a
+//    row, 128 columns; where groups are shorter, x of the different groups goes to different columns of B
+//    (zeros elsewhere), so that each group still has a sum of its own: S = 128 / group columns per part.
 //  * A lane's 16 bytes (32 columns of one row) are loaded straight into registers from the row-major
-//    weights.  A product's order of columns is free, so the lane's nibbles are used in the order in
-//    which masks deliver them, and x is put into that order when it is staged in shared memory.
-//  * One instruction sums over the four lanes of a row, 128 columns.  Where groups are shorter, x of
-//    the different groups goes to different columns of B (zeros elsewhere), so that each group still has
-//    a sum of its own: S = 128 / group columns per vector.
-//  * fp32 vectors are split into three bf16 parts, 8 bits each, which hold all 24 bits: three columns.
+//    weights, a chunk ahead.  A product's order of columns is free, so nibbles are used in the order in
+//    which masks deliver them, and x is put into that order when it is staged.
 //  * A block's rows are its even share of M, in tiles of at most 16 rows of nearly equal size, so that
-//    blocks finish together whatever M is; its warps split the columns of a tile (or, where rows are
-//    short, several tiles) and meet in shared memory once per tile, in a fixed order.
+//    blocks finish together whatever M is; groups of its warps take a tile each, split its columns and
+//    meet in shared memory at its end, in a fixed order.  Where a block has
+//    few rows, staging all of x for them would cost as much as their weights: a cluster of blocks then
+//    takes more rows together, each block a share of the columns, and adds its sums over distributed
+//    shared memory, in rank order.
 #include "l2d_launch.cuh"
+
+#include <cooperative_groups.h>
 
 #include <algorithm>
 #include <cstring>
@@ -34,98 +47,57 @@ struct Q4Args {
     void *y;
     int64_t M, ldw, lds, stride_x, stride_y;
     int N, vectors, group, dtype_x, dtype_y, dtype_s;
-    int aligned;     // rows of W on 16-byte boundaries
-    int sub_shift;   // log2 of S, columns of B per vector part
-    int parts;       // columns of B per vector for its precision: 3 for fp32, else 1
+    int parts;       // columns of x per vector: 2 for fp32, else 1
     int warps_k;     // warps that split a tile's columns
-    int block_k;     // columns of x staged at a time
-    int blocks_k;    // how many times
-    int y_rows;      // rows of the block's sums kept over several stagings (0: one staging)
+    int ranks;       // blocks of a cluster, which split the columns
+    int stage_h;     // halves of 128 columns of x staged at a time
+    int y_rows;      // rows of the block's sums kept (0: one staging and no cluster)
+    uint64_t per_group;  // ceil(2^40 / (group / 128)): a half's group without a division
 };
 
-constexpr int kQ4Warps = 8;
+constexpr int kQ4Warps = 16;
 constexpr int kQ4Threads = kQ4Warps * 32;
-constexpr int kQ4Chunk = 256;      // columns a warp takes at a time: 128 bytes of each row
+constexpr int kQ4Half = 128;       // columns of one sum: 64 bytes of each row
+constexpr int kQ4Deep = 4;         // of them in a step, which a warp has in registers or on their way
 constexpr int kQ4Rows = 16;
-constexpr int kQ4MaxRows = 512;    // rows of a block, at most
+constexpr int kQ4MaxRows = 896;    // rows of a block, at most
+constexpr int kQ4Column = 320;     // bytes between columns of x in shared memory: 256 used, so that two lie in other banks
 
-// Byte offsets in dynamic shared memory.
+// Byte offsets in dynamic shared memory: x, zeros, its sums and factors, offsets of scales, the warps' sums, y.
 struct Q4Smem {
-    int red, y, bytes;
+    int zero, sums, offsets, red, y, bytes;
 };
-__host__ __device__ inline Q4Smem q4_smem(int tiles_n, int columns, int block_k, int y_rows) {
+__host__ __device__ inline Q4Smem q4_smem(int tiles_n, int columns, int stage_h, int y_floats) {
     Q4Smem s;
-    s.red = columns * block_k * 2;
-    s.y = s.red + 2 * kQ4Warps * kQ4Rows * 8 * tiles_n * 4;
-    s.bytes = s.y + y_rows * columns * 4;
+    s.zero = columns * stage_h * kQ4Column;
+    s.sums = s.zero + 256;
+    s.offsets = s.sums + stage_h * 8 * tiles_n * 8;
+    s.red = s.offsets + (stage_h + 3) / 4 * 16;
+    s.y = s.red + (tiles_n == 1 ? 2 : 1) * kQ4Warps * kQ4Rows * 8 * tiles_n * 4;
+    s.bytes = s.y + y_floats * 4;
     return s;
 }
 
-template <typename T>
-struct MmaType { using type = T; };
-template <>
-struct MmaType<float> { using type = __nv_bfloat16; };
-
-template <typename T>
+// c = a b, and c += a b.
+__device__ __forceinline__ void q4_mma_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ void q4_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <typename H2>
-__device__ __forceinline__ uint32_t bits_of(H2 v) {
-    uint32_t r;
-    memcpy(&r, &v, 4);
-    return r;
+// Eight nibbles as fp16 numbers, p[i] nibbles i and i + 4: q 2^-24, and 16 q 2^-24 in p[1] and p[3].
+__device__ __forceinline__ void unpack(uint32_t w, uint32_t (&p)[4]) {
+    p[0] = w & 0x000F000F;
+    p[1] = w & 0x00F000F0;
+    w >>= 8;
+    p[2] = w & 0x000F000F;
+    p[3] = w & 0x00F000F0;
 }
-template <typename H2>
-__device__ __forceinline__ H2 from_bits(uint32_t r) {
-    H2 v;
-    memcpy(&v, &r, 4);
-    return v;
-}
-
-__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t set) {
-    uint32_t d;
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(mask), "r"(set));
-    return d;
-}
-
-// Eight nibbles to q - z: p[i] holds nibbles i and i + 4.  A nibble or-ed into the low mantissa bits of
-// 2^n is 2^n + q; subtracting 2^n + z is exact.  z: that subtrahend, one per type (see zero_of).
-template <typename T>
-struct Nibbles;
-template <>
-struct Nibbles<__half> {
-    // 1024 + q from bits 0-3; 1024 + 16 q from bits 4-7, a sixteenth of which is 64 + q.
-    static __device__ __forceinline__ void unpack(uint32_t w, uint32_t z, uint32_t (&p)[4]) {
-        const __half2 lo = from_bits<__half2>(z);  // 1024 + z
-        const __half2 hi = __hsub2(__half2half2(__ushort_as_half(0x6380)), lo);  // 960 - (1024 + z) = -(64 + z)
-        const __half2 r16 = __half2half2(__ushort_as_half(0x2c00));              // 1 / 16
-        p[0] = bits_of(__hsub2(from_bits<__half2>(and_or(w, 0x000F000F, 0x64006400)), lo));
-        p[1] = bits_of(__hfma2(from_bits<__half2>(and_or(w, 0x00F000F0, 0x64006400)), r16, hi));
-        w >>= 8;
-        p[2] = bits_of(__hsub2(from_bits<__half2>(and_or(w, 0x000F000F, 0x64006400)), lo));
-        p[3] = bits_of(__hfma2(from_bits<__half2>(and_or(w, 0x00F000F0, 0x64006400)), r16, hi));
-    }
-    static __device__ __forceinline__ uint32_t zero_of(uint32_t z) { return (0x6400 | z) * 0x10001u; }
-};
-template <>
-struct Nibbles<__nv_bfloat16> {
-    // Seven mantissa bits: 128 + q, one nibble position at a time.
-    static __device__ __forceinline__ void unpack(uint32_t w, uint32_t z, uint32_t (&p)[4]) {
-        const __nv_bfloat162 lo = from_bits<__nv_bfloat162>(z);  // 128 + z
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[i] = bits_of(__hsub2(from_bits<__nv_bfloat162>(and_or(w >> (4 * i), 0x000F000F, 0x43004300)), lo));
-    }
-    static __device__ __forceinline__ uint32_t zero_of(uint32_t z) { return (0x4300 | z) * 0x10001u; }
-};
 
 __device__ __forceinline__ uint4 load_weights(const uint8_t *p) {
     uint4 v;
@@ -133,229 +105,286 @@ __device__ __forceinline__ uint4 load_weights(const uint8_t *p) {
     return v;
 }
 
-// The first n (0..16) bytes at p, zeros after them.
-__device__ __noinline__ uint4 load_bytes(const uint8_t *p, int n) {
+// 16 bytes at any address, of which `left` belong to the row (zeros after them), inside [begin, end): from the
+// two aligned ones around them where those are inside too, else byte by byte.
+__device__ __forceinline__ uint4 load_any(const uint8_t *p, int left, const uint8_t *begin, const uint8_t *end) {
+    if (left >= 16 && p >= begin + 16 && p + 32 <= end) {
+        const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 15;
+        const uint4 *q = reinterpret_cast<const uint4 *>(p - off);
+        const uint4 a = __ldg(q), b = off ? __ldg(q + 1) : a;
+        uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        if (off & 8) {
+#pragma unroll
+            for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+        }
+        if (off & 4) {
+#pragma unroll
+            for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+        }
+        const uint32_t s = (off & 3) * 8;
+        return make_uint4(__funnelshift_r(w[0], w[1], s), __funnelshift_r(w[1], w[2], s), __funnelshift_r(w[2], w[3], s),
+                          __funnelshift_r(w[3], w[4], s));
+    }
     uint32_t v[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-        if (i < n) v[i >> 2] |= static_cast<uint32_t>(p[i]) << (8 * (i & 3));
+        if (i < left) v[i >> 2] |= static_cast<uint32_t>(p[i]) << (8 * (i & 3));
     return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-// 16 bytes at any address, from the two aligned ones around them.
-__device__ __forceinline__ uint4 load_unaligned(const uint8_t *p) {
-    const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 15;
-    const uint4 *q = reinterpret_cast<const uint4 *>(p - off);
-    const uint4 a = __ldg(q);
-    const uint4 b = off ? __ldg(q + 1) : a;
-    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-    if (off & 8) {
-#pragma unroll
-        for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
-    }
-    if (off & 4) {
-#pragma unroll
-        for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
-    }
-    const uint32_t s = (off & 3) * 8;
-    return make_uint4(__funnelshift_r(w[0], w[1], s), __funnelshift_r(w[1], w[2], s), __funnelshift_r(w[2], w[3], s),
-                      __funnelshift_r(w[3], w[4], s));
-}
-
-// What a warp holds of one chunk (two halves of 128 columns) of a tile: this lane's 16 bytes of rows g
-// and g + 8, the scales of those rows' sums and the zeros of its columns.
-template <bool SUB, bool ZEROS>
-struct Q4Chunk {
-    uint4 w[2][2];                          // [half][row]
-    uint32_t s[2][2][SUB ? 2 : 1];          // [half][row][column of C], as stored
-    uint32_t z[2][ZEROS ? 2 : 1];
+// What a warp holds of 128 columns of a tile: this lane's 16 bytes of rows g and g + 8, the scales of those
+// rows' sums and the zeros of the same groups.
+template <int E, bool ZEROS>
+struct Q4Part {
+    uint4 w[2];
+    uint32_t s[2][E];              // [row][column of C], as stored
+    uint32_t z[2][ZEROS ? E : 1];
 };
 
-template <typename X, int NT, bool SUB, bool ZEROS>
-__global__ void __launch_bounds__(kQ4Threads, 2) k_q4_gemv(Q4Args a) {
-    using T = typename MmaType<X>::type;
+// S: columns of B per part of a vector (4, 2, 1 for groups of 32, 64, 128 columns), 0 for longer groups.
+// WORDS: every row of W is whole 16-byte words on 16-byte boundaries, and scales have 16 bits.
+template <int NT, int S, bool ZEROS, bool WORDS>
+__global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
+    constexpr int SUB = S > 1 ? S : 1, kShift = S == 4 ? 2 : S == 2 ? 1 : 0, E = S > 1 ? 2 : 1;
     extern __shared__ __align__(16) char smem[];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int columns = a.vectors * a.parts;  // columns of x in shared memory
-    const Q4Smem lay = q4_smem(NT, columns, a.block_k, a.y_rows);
+    const int tid = threadIdx.x, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // known to be the same in all lanes
+    const int columns = a.vectors * a.parts;                 // of x in shared memory
+    const Q4Smem lay = q4_smem(NT, columns, a.stage_h, a.y_rows * a.vectors);
+    float2 *sums = reinterpret_cast<float2 *>(smem + lay.sums);
+    int *offsets = reinterpret_cast<int *>(smem + lay.offsets);
     float *red = reinterpret_cast<float *>(smem + lay.red), *ysum = reinterpret_cast<float *>(smem + lay.y);
-    const int64_t r0 = a.M * blockIdx.x / gridDim.x;
-    const int rows = static_cast<int>(a.M * (blockIdx.x + 1) / gridDim.x - r0), tiles = (rows + kQ4Rows - 1) / kQ4Rows;
-    const int wk = warp % a.warps_k, wm = warp / a.warps_k, warps_m = kQ4Warps / a.warps_k;
-    const int rounds = (tiles + warps_m - 1) / warps_m;  // of one tile for each group of warps
+    // This block's rows, and its halves of 128 columns.
+    const int shares = gridDim.x / a.ranks, share = blockIdx.x / a.ranks, rank = blockIdx.x % a.ranks;
+    const int64_t r0 = a.M * share / shares;
+    const int rows = static_cast<int>(a.M * (share + 1) / shares - r0);
+    const int all_h = (a.N + kQ4Half - 1) / kQ4Half, all_steps = (all_h + kQ4Deep - 1) / kQ4Deep;
+    const int h_lo = static_cast<int>(static_cast<int64_t>(all_steps) * rank / a.ranks) * kQ4Deep;
+    const int h_hi = min(all_h, static_cast<int>(static_cast<int64_t>(all_steps) * (rank + 1) / a.ranks) * kQ4Deep);
+    // This warp's group: its rows, in tiles of q or q + 1 rows.
+    const int wk = warp & (a.warps_k - 1), wm = warp / a.warps_k, warps_m = kQ4Warps / a.warps_k;
+    const int g0 = rows * wm / warps_m, g_rows = rows * (wm + 1) / warps_m - g0;
+    const int tiles = (g_rows + kQ4Rows - 1) / kQ4Rows, tile_q = tiles ? g_rows / tiles : 0, tile_rest = g_rows - tiles * tile_q;
+    auto first_row = [&](int tile) { return g0 + tile * tile_q + min(tile, tile_rest); };
     const int row_bytes = (a.N + 1) / 2;
     const uint8_t *w_end = a.W + (a.M - 1) * a.ldw + row_bytes;
-    const int S = 1 << a.sub_shift;
+    // The group of a column: group / 128 is 1 or more, or groups are 32 or 64 columns.
+    auto group_of = [&](int col) {
+        return S > 1 ? col >> (7 - kShift) : static_cast<int>(static_cast<uint64_t>(col >> 7) * a.per_group >> 40);
+    };
+    const int s_size = WORDS ? 2 : a.dtype_s == L2D_F32 ? 4 : 2;
     dev::wait_for_previous();
 
-    auto chunks_in = [&](int kb) {  // chunks of a staging that fall to each warp
-        const int n = min(a.N - kb * a.block_k, a.block_k);
-        return ((n + kQ4Chunk - 1) / kQ4Chunk + a.warps_k - 1) / a.warps_k;
-    };
-    struct At {
-        int kb, round, i, n;
-    };
-    auto advance = [&](At &at) {
-        if (++at.i == at.n) {
-            at.i = 0;
-            if (++at.round == rounds) {
-                at.round = 0;
-                if (++at.kb < a.blocks_k) at.n = chunks_in(at.kb);
-            }
-        }
-    };
-    auto first_row = [&](int tile) { return tile * rows / tiles; };
-
-    auto load = [&](Q4Chunk<SUB, ZEROS> &c, const At &at) {
-        const int tile = at.round * warps_m + wm;
-        const int col = at.kb * a.block_k + (at.i * a.warps_k + wk) * kQ4Chunk;
-        if (at.kb >= a.blocks_k || tile >= tiles || col >= min(a.N, (at.kb + 1) * a.block_k)) return;
-        const int lo = first_row(tile), hi = first_row(tile + 1);
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const int row = lo + g + 8 * r;
-            const bool real = row < hi;
-            const uint8_t *base = a.W + (r0 + row) * a.ldw;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int at_byte = col / 2 + 64 * h + 16 * t, left = row_bytes - at_byte;
-                const uint8_t *p = base + at_byte;
-                c.w[h][r] = make_uint4(0, 0, 0, 0);
-                if (real && left > 0) {
-                    if (a.aligned && left >= 16) c.w[h][r] = load_weights(p);
-                    else if (left >= 16 && p >= a.W + 16 && p + 32 <= w_end) c.w[h][r] = load_unaligned(p);
-                    else c.w[h][r] = load_bytes(p, min(left, 16));
-                }
-                // Scales: of the columns 2t, 2t + 1 of C, which belong to the subgroups (2t) % S and (2t + 1) % S.
-                const int half = col + 128 * h;
-                const int64_t s_row = (r0 + row) * a.lds;
-#pragma unroll
-                for (int e = 0; e < (SUB ? 2 : 1); ++e) {
-                    const int at_col = half + ((2 * t + e) & (S - 1)) * a.group;
-                    c.s[h][r][e] = 0;
-                    if (real && at_col < a.N) {
-                        const int64_t i = s_row + (SUB ? at_col / 32 >> (2 - a.sub_shift) : at_col / a.group);
-                        c.s[h][r][e] = a.dtype_s == L2D_F32 ? reinterpret_cast<const uint32_t *>(a.scales)[i]
-                                                            : reinterpret_cast<const uint16_t *>(a.scales)[i];
-                    }
-                }
-                if constexpr (ZEROS) {
-                    const int mine = half + 32 * t;
-                    c.z[h][r] = 0;
-                    if (real && mine < a.N) c.z[h][r] = a.zeros[s_row + (SUB ? mine / 32 >> (2 - a.sub_shift) : mine / a.group)];
-                }
-            }
-        }
-    };
-
-    auto scale = [&](uint32_t v) {
-        if (a.dtype_s == L2D_F32) return __uint_as_float(v);
-        if (a.dtype_s == L2D_BF16) return __uint_as_float(v << 16);
-        return __half2float(__ushort_as_half(static_cast<unsigned short>(v)));
-    };
-
-    // The column of x that this lane feeds into column g of each n-tile: vector part (8 n + g) / S, if its
-    // own columns of W belong to that column's subgroup.
-    const bool feeds = (g & (S - 1)) == (t * S >> 2);
+    // The column of x that this lane feeds into column g of each n-tile: part (8 n + g) / S, if the lane's columns
+    // of W belong to that column's subgroup; else zeros, from a place that does not move.
+    const char *x_at[NT];
+    int x_half[NT];
     float acc[NT][4];
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n) {
+        const int column = (8 * n + g) >> kShift;
+        const bool feeds = (g & (SUB - 1)) == (t * SUB >> 2) && column < columns;
+        x_at[n] = feeds ? smem + column * kQ4Column + t * 16 : smem + lay.zero;
+        x_half[n] = feeds ? columns * kQ4Column : 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[n][e] = 0.0f;
+    }
 
-    auto consume = [&](const Q4Chunk<SUB, ZEROS> &c, const At &at) {
-        const int tile = at.round * warps_m + wm;
-        const int k = (at.i * a.warps_k + wk) * kQ4Chunk;  // in the staged columns
-        if (tile >= tiles || at.kb * a.block_k + k >= min(a.N, (at.kb + 1) * a.block_k)) return;
+    // Adds the products of half `half` of the staging.
+    auto multiply = [&](const Q4Part<E, ZEROS> &c, int half) {
+        const uint32_t w0[4] = {c.w[0].x, c.w[0].y, c.w[0].z, c.w[0].w}, w1[4] = {c.w[1].x, c.w[1].y, c.w[1].z, c.w[1].w};
+        float sum[NT][4];
+        const char *x[NT];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            float sum[NT][4] = {};
-            const uint4 *x = reinterpret_cast<const uint4 *>(smem) + static_cast<int64_t>(k / 128 + h) * columns * 16 + t;
-            const uint32_t z0 = Nibbles<T>::zero_of(ZEROS ? c.z[h][0] & 15 : 8), z1 = Nibbles<T>::zero_of(ZEROS ? c.z[h][ZEROS ? 1 : 0] & 15 : 8);
-            const uint32_t w0[4] = {c.w[h][0].x, c.w[h][0].y, c.w[h][0].z, c.w[h][0].w};
-            const uint32_t w1[4] = {c.w[h][1].x, c.w[h][1].y, c.w[h][1].z, c.w[h][1].w};
+        for (int n = 0; n < NT; ++n) x[n] = x_at[n] + half * x_half[n];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint32_t p0[4], p1[4];
-                Nibbles<T>::unpack(w0[j], z0, p0);
-                Nibbles<T>::unpack(w1[j], z1, p1);
-                const uint32_t a0[4] = {p0[0], p1[0], p0[1], p1[1]}, a1[4] = {p0[2], p1[2], p0[3], p1[3]};
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const int column = (8 * n + g) >> a.sub_shift;
-                    uint4 b = make_uint4(0, 0, 0, 0);
-                    if (feeds && column < columns) b = x[(j * columns + column) * 4];
-                    q4_mma<T>(sum[n], a0, b.x, b.y);
-                    q4_mma<T>(sum[n], a1, b.z, b.w);
-                }
-            }
-            const float s00 = scale(c.s[h][0][0]), s10 = scale(c.s[h][1][0]);
-            const float s01 = SUB ? scale(c.s[h][0][SUB ? 1 : 0]) : s00, s11 = SUB ? scale(c.s[h][1][SUB ? 1 : 0]) : s10;
+        for (int j = 0; j < 4; ++j) {
+            uint32_t p0[4], p1[4];
+            unpack(w0[j], p0);
+            unpack(w1[j], p1);
+            const uint32_t a0[4] = {p0[0], p1[0], p0[1], p1[1]}, a1[4] = {p0[2], p1[2], p0[3], p1[3]};
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                acc[n][0] = fmaf(s00, sum[n][0], acc[n][0]);
-                acc[n][1] = fmaf(s01, sum[n][1], acc[n][1]);
-                acc[n][2] = fmaf(s10, sum[n][2], acc[n][2]);
-                acc[n][3] = fmaf(s11, sum[n][3], acc[n][3]);
+                const uint4 b = *reinterpret_cast<const uint4 *>(x[n] + j * 64);
+                if (j == 0) q4_mma_first(sum[n], a0, b.x, b.y);
+                else q4_mma(sum[n], a0, b.x, b.y);
+                q4_mma(sum[n], a1, b.z, b.w);
+            }
+        }
+        float s[2][E], z[2][E];
+#pragma unroll
+        for (int e = 0; e < 2 * E; ++e) {
+            const uint32_t v = c.s[e / E][e % E];
+            const float wide = __uint_as_float(WORDS || s_size == 2 ? v << 16 : v);
+            s[e / E][e % E] = a.dtype_s == L2D_F16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(v))) : wide;
+            z[e / E][e % E] = ZEROS ? static_cast<float>(c.z[e / E][ZEROS ? e % E : 0] & 15) : 8.0f;
+        }
+        const float4 *xs = reinterpret_cast<const float4 *>(sums + half * 8 * NT) + t;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const float4 f = xs[4 * n];  // sum and factor of columns 2t and 2t + 1
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float v = fmaf(-z[e >> 1][(e & 1) % E], e & 1 ? f.z : f.x, sum[n][e]);
+                acc[n][e] = fmaf(s[e >> 1][(e & 1) % E], v * fabsf(e & 1 ? f.w : f.y), acc[n][e]);
             }
         }
     };
 
-    // x of one staging, in the order of the nibbles: 16 bytes hold columns (0, 4) (1, 5) (2, 6) (3, 7) of eight;
-    // [128 columns][word j][column of B][lane t].
+    // Where this lane reads: rows g and g + 8 of a tile, or the tile's last row where it has fewer (their sums are
+    // dropped), from half `half` of all on.
+    struct Rows {
+        const uint8_t *w[2], *s[2], *z[2];
+    };
+    // Scales of the columns 2t, 2t + 1 of C, which belong to the subgroups (2t) % S and (2t + 1) % S.
+    const int sub = S > 1 ? (2 * t) & (SUB - 1) : 0;
+    auto rows_of = [&](int tile, int half) {
+        Rows at;
+        const int last = first_row(tile + 1) - 1, lo = first_row(tile);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int64_t row = r0 + min(lo + g + 8 * r, last), first = S ? half * SUB + sub : 0;
+            at.w[r] = a.W + row * a.ldw + half * 64 + 16 * t;
+            at.s[r] = a.scales + (row * a.lds + first) * s_size;
+            at.z[r] = ZEROS ? a.zeros + row * a.lds + first : nullptr;
+        }
+        return at;
+    };
+    // Loads half h after those, which is half `half` of the staging.  `last`: the last one of a row that is not
+    // whole, where there may be fewer bytes and groups; scales past the last column belong to sums that are zero.
+    auto load = [&](Q4Part<E, ZEROS> &c, const Rows &at, int h, int half, int kb, bool last) {
+        const int col = (h_lo + kb * a.stage_h + half) * kQ4Half, left = row_bytes - (col >> 1) - 16 * t;
+        const int more = S > 1 && last && sub + 1 > group_of(a.N - 1) - group_of(col) ? 0 : 1, skip = S > 1 && last ? min(0, group_of(a.N - 1) - group_of(col) - sub) : 0;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const uint8_t *p = at.w[r] + h * 64;
+            if constexpr (!WORDS) c.w[r] = load_any(p, left, a.W, w_end);
+            else if (!last) c.w[r] = load_weights(p);
+            else c.w[r] = left > 0 ? load_weights(p) : make_uint4(0, 0, 0, 0);
+            const int first = S ? h * SUB + skip : offsets[half];
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int i = first + (e ? more : 0);
+                if (WORDS || s_size == 2) c.s[r][e] = __ldg(reinterpret_cast<const uint16_t *>(at.s[r]) + i);
+                else c.s[r][e] = __ldg(reinterpret_cast<const uint32_t *>(at.s[r]) + i);
+                if constexpr (ZEROS) c.z[r][e] = a.zeros ? __ldg(at.z[r] + i) : 8;
+            }
+        }
+    };
+
+    // x of one staging: 16 lanes take 128 columns of one vector, eight columns each.  16 bytes hold columns
+    // (0, 4) (1, 5) (2, 6) (3, 7) of eight; [half][column of x][word j][lane t].
     auto stage = [&](int kb) {
-        const int k0 = kb * a.block_k, n = (min(a.N - k0, a.block_k) + kQ4Chunk - 1) / kQ4Chunk * (kQ4Chunk / 8);
-        for (int e = tid; e < n * a.vectors; e += kQ4Threads) {
-            const int v = e / n, u = e - v * n, col = k0 + 8 * u;  // eight columns from col
-            const X *src = static_cast<const X *>(a.x) + v * a.stride_x + col;
-            const int half = u >> 4, tt = (u >> 2) & 3, j = u & 3;
-            uint4 *dst = reinterpret_cast<uint4 *>(smem) + (static_cast<int64_t>(half) * columns * 16 + (j * columns + v * a.parts) * 4 + tt);
-            if constexpr (sizeof(X) == 2) {
-                uint32_t h[8];
-                if (col + 8 <= a.N && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-                    const uint4 q = *reinterpret_cast<const uint4 *>(src);
+        bool any_odd = false;
+        const int first = h_lo + kb * a.stage_h, halves = min(h_hi - first, a.stage_h);
+        const int u = lane & 15;
+        for (int e = warp * 2 + (lane >> 4); e - (lane >> 4) < halves * a.vectors; e += kQ4Warps * 2) {
+            const bool real = e < halves * a.vectors;
+            const int v = real ? e / halves : 0, half = real ? e - v * halves : 0, col = (first + half) * kQ4Half + 8 * u;
+            float f[8];
+            const int eb = a.dtype_x == L2D_F32 ? 4 : 2;
+            const char *src = static_cast<const char *>(a.x) + (v * a.stride_x + col) * eb;
+            uint32_t raw[8];
+            if (col + 8 <= a.N && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+                const uint4 q = *reinterpret_cast<const uint4 *>(src);
+                if (a.dtype_x == L2D_F32) {
+                    const uint4 r = *reinterpret_cast<const uint4 *>(src + 16);
+                    raw[0] = q.x, raw[1] = q.y, raw[2] = q.z, raw[3] = q.w, raw[4] = r.x, raw[5] = r.y, raw[6] = r.z, raw[7] = r.w;
+                } else {
                     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) h[i] = w[i >> 1] >> (16 * (i & 1)) & 0xffff;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) h[i] = col + i < a.N ? reinterpret_cast<const uint16_t *>(src)[i] : 0;
+                    for (int i = 0; i < 8; ++i) raw[i] = w[i >> 1] >> (16 * (i & 1)) & 0xffff;
                 }
-                *dst = make_uint4(h[0] | h[4] << 16, h[1] | h[5] << 16, h[2] | h[6] << 16, h[3] | h[7] << 16);
             } else {
-                // fp32 into three bf16 parts by truncation: each takes the next 8 bits, so the three add up exactly.
-                // Infinities and NaNs stay whole in the first part.
-                uint32_t f[8];
-                if (col + 8 <= a.N && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-                    const uint4 q = *reinterpret_cast<const uint4 *>(src), r = *reinterpret_cast<const uint4 *>(src + 4);
-                    f[0] = q.x, f[1] = q.y, f[2] = q.z, f[3] = q.w, f[4] = r.x, f[5] = r.y, f[6] = r.z, f[7] = r.w;
-                } else {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) f[i] = col + i < a.N ? reinterpret_cast<const uint32_t *>(src)[i] : 0;
-                }
-                uint32_t part[3][8];
+                for (int i = 0; i < 8; ++i)
+                    raw[i] = col + i >= a.N ? 0
+                             : a.dtype_x == L2D_F32 ? reinterpret_cast<const uint32_t *>(src)[i] : reinterpret_cast<const uint16_t *>(src)[i];
+            }
+            uint32_t top = 0;
+            bool odd_ones = false;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                f[i] = a.dtype_x == L2D_F16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(raw[i])))
+                                            : __uint_as_float(a.dtype_x == L2D_F32 ? raw[i] : raw[i] << 16);
+                const uint32_t m = __float_as_uint(f[i]) & 0x7fffffffu;
+                if (m < 0x7f800000u) top = max(top, m);
+                else f[i] = 0.0f, odd_ones = true;
+            }
+#pragma unroll
+            for (int d = 1; d < 16; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+            // 2^(p - 127) takes the largest to [2^14, 2^15); the factor back is short of 2^12, which the end makes good.
+            const uint32_t p = min(268u - (top >> 23), 254u);
+            const float up = __uint_as_float(p << 23), back = __uint_as_float((266u - p) << 23);
+            uint32_t lo[8] = {}, hi[8];
+            float total_lo = 0.0f, total_hi = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                f[i] *= i & 1 ? up * 0.0625f : up;
+                const __half h = __float2half_rn(f[i]);
+                hi[i] = __half_as_ushort(h);
+                total_hi = fmaf(i & 1 ? 16.0f : 1.0f, __half2float(h), total_hi);
+            }
+            if (a.parts == 2) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const bool finite = (f[i] & 0x7f800000u) != 0x7f800000u;
-                    if (!finite && (f[i] & 0x007fffffu)) f[i] |= 0x00400000u;
-                    const float rest = finite ? __uint_as_float(f[i]) - __uint_as_float(f[i] & 0xffff0000u) : 0.0f;
-                    const uint32_t m = __float_as_uint(rest);
-                    const float last = rest - __uint_as_float(m & 0xffff0000u);
-                    part[0][i] = f[i] >> 16;
-                    part[1][i] = m >> 16;
-                    part[2][i] = __float_as_uint(last) >> 16;
+                    const __half h = __float2half_rn((f[i] - __half2float(__ushort_as_half(static_cast<unsigned short>(hi[i])))) * 2048.0f);
+                    lo[i] = __half_as_ushort(h);
+                    total_lo = fmaf(i & 1 ? 16.0f : 1.0f, __half2float(h), total_lo);
                 }
+            }
 #pragma unroll
-                for (int q = 0; q < 3; ++q)
-                    dst[4 * q] = make_uint4(part[q][0] | part[q][4] << 16, part[q][1] | part[q][5] << 16, part[q][2] | part[q][6] << 16,
-                                            part[q][3] | part[q][7] << 16);
+            for (int d = 1; d < 16 / SUB; d <<= 1) {
+                total_hi += __shfl_xor_sync(0xffffffffu, total_hi, d);
+                total_lo += __shfl_xor_sync(0xffffffffu, total_lo, d);
+            }
+            const bool odd = __ballot_sync(0xffffffffu, odd_ones) >> (lane & 16) & 0xffff;  // in these 128 columns
+            any_odd = any_odd || (real && odd);
+            if (real) {
+                const int column = v * a.parts, tt = u >> 2, j = u & 3;
+                uint4 *dst = reinterpret_cast<uint4 *>(smem + (half * columns + column) * kQ4Column) + j * 4 + tt;
+                dst[0] = make_uint4(hi[0] | hi[4] << 16, hi[1] | hi[5] << 16, hi[2] | hi[6] << 16, hi[3] | hi[7] << 16);
+                if (a.parts == 2)
+                    dst[kQ4Column / 16] = make_uint4(lo[0] | lo[4] << 16, lo[1] | lo[5] << 16, lo[2] | lo[6] << 16, lo[3] | lo[7] << 16);
+                if (u % (16 / SUB) == 0) {
+                    float2 *to = sums + half * 8 * NT + (column << kShift) + u / (16 / SUB);
+                    to[0] = make_float2(total_hi * 0x1p-24f, odd ? -back : back);  // the sign: see add_odd_ones()
+                    if (a.parts == 2) to[SUB] = make_float2(total_lo * 0x1p-24f, back * 0x1p-11f);
+                }
             }
         }
+        // Columns of B without a vector: their sums are dropped, but stay finite.
+        const int used = columns << kShift, unused = 8 * NT - used;
+        for (int e = tid; e < halves * unused; e += kQ4Threads) sums[e / unused * 8 * NT + used + e % unused] = make_float2(0.0f, 0.0f);
+        if (tid < 16) reinterpret_cast<uint4 *>(smem + lay.zero)[tid] = make_uint4(0, 0, 0, 0);
+        return any_odd;
     };
 
-    // One tile for each group of warps is done: their sums meet, in warp order.
+    bool odd_vectors = false;
+    // The terms of infinities and NaNs of x in this staging, for one result: row of the block, vector v.
+    auto add_odd_ones = [&](float sum, int kb, int row, int v) {
+        const int first = h_lo + kb * a.stage_h, halves = min(h_hi - first, a.stage_h);
+        for (int half = 0; half < halves; ++half) {
+            if (!(sums[half * 8 * NT + ((v * a.parts) << kShift)].y < 0.0f)) continue;
+            for (int col = (first + half) * kQ4Half; col < min(a.N, (first + half + 1) * kQ4Half); ++col) {
+                const float x = dev::load_as_float(a.x, a.dtype_x, v * a.stride_x + col);
+                if (isfinite(x)) continue;
+                const int64_t i = (r0 + row) * a.lds + group_of(col);
+                const int q = a.W[(r0 + row) * a.ldw + col / 2] >> (4 * (col & 1)) & 15, z = a.zeros ? a.zeros[i] & 15 : 8;
+                sum += dev::load_as_float(a.scales, a.dtype_s, i) * (static_cast<float>(q - z) * x);
+            }
+        }
+        return sum;
+    };
+
+    // A tile is done: its warps' sums meet, in warp order.
     int buffer = 0;
-    auto finish = [&](const At &at) {
+    auto meet = [&] {
+        if (a.warps_k == 1) __syncwarp();
+        else asm volatile("bar.sync %0, %1;" ::"r"(wm + 1), "r"(a.warps_k * 32) : "memory");
+    };
+    auto finish = [&](int kb, int tile) {
+        if (NT > 1) meet();  // the sums before have been read
         float *mine = red + (buffer * kQ4Warps + warp) * kQ4Rows * 8 * NT;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -364,48 +393,99 @@ __global__ void __launch_bounds__(kQ4Threads, 2) k_q4_gemv(Q4Args a) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[n][e] = 0.0f;
         }
-        __syncthreads();
-        const int per_vector = a.parts << a.sub_shift;
-        for (int e = tid; e < warps_m * kQ4Rows * a.vectors; e += kQ4Threads) {
-            const int v = e / (warps_m * kQ4Rows), rest = e - v * warps_m * kQ4Rows, m = rest / kQ4Rows, r = rest % kQ4Rows;
-            const int tile = at.round * warps_m + m;
-            if (tile >= tiles) continue;
-            const int row = first_row(tile) + r;
-            if (row >= first_row(tile + 1)) continue;
-            const float *p = red + ((buffer * kQ4Warps + m * a.warps_k) * kQ4Rows + r) * 8 * NT + v * per_vector;
+        meet();
+        const int lo = first_row(tile), n = first_row(tile + 1) - lo;
+        // Another warp of the group begins each time.
+        for (int e = ((wk + tile) & (a.warps_k - 1)) * 32 + lane; e < kQ4Rows * a.vectors; e += a.warps_k * 32) {
+            const int v = e / kQ4Rows, r = e % kQ4Rows, row = lo + r;
+            if (r >= n) continue;
+            const float *p = red + ((buffer * kQ4Warps + wm * a.warps_k) * kQ4Rows + r) * 8 * NT + v * a.parts * SUB;
             float sum = 0.0f;
-            for (int w = 0; w < a.warps_k; ++w)
-                for (int i = 0; i < per_vector; ++i) sum += p[w * kQ4Rows * 8 * NT + i];
+            for (int w = 0; w < a.warps_k; ++w, p += kQ4Rows * 8 * NT)
+                for (int i = 0; i < a.parts; ++i)
+#pragma unroll
+                    for (int c = 0; c < SUB; ++c) sum += p[i * SUB + c];
+            if (odd_vectors) sum = add_odd_ones(sum * 4096.0f, kb, row, v) * 0x1p-12f;
             if (a.y_rows) {
                 float *y = ysum + row * a.vectors + v;
-                sum += at.kb ? *y : 0.0f;
+                sum += kb ? *y : 0.0f;
                 *y = sum;  // this thread again the next time
             }
-            if (at.kb == a.blocks_k - 1) dev::store_as(a.y, a.dtype_y, v * a.stride_y + r0 + row, sum);
+            if (h_lo + (kb + 1) * a.stage_h >= h_hi && a.ranks == 1) dev::store_as(a.y, a.dtype_y, v * a.stride_y + r0 + row, sum * 4096.0f);
         }
-        buffer ^= 1;
+        if (NT == 1) buffer ^= 1;
     };
 
-    Q4Chunk<SUB, ZEROS> even, odd;
-    At now = {0, 0, 0, chunks_in(0)}, next = now;
-    load(even, next);
-    advance(next);
-    load(odd, next);
-    advance(next);
-    auto step = [&](Q4Chunk<SUB, ZEROS> &c) {
-        if (now.i == 0 && now.round == 0) {
-            if (now.kb) __syncthreads();
-            stage(now.kb);
+    for (int kb = 0; h_lo + kb * a.stage_h < h_hi; ++kb) {
+        // The staging's halves: whole steps, an even share for each warp, and what is left, a half for a warp.
+        const int first = h_lo + kb * a.stage_h, n = min(h_hi - first, a.stage_h);
+        const bool cut = (first + n) * kQ4Half > a.N;  // the last half is not whole
+        const int whole = (n - (cut ? 1 : 0)) / kQ4Deep, rest = n - whole * kQ4Deep;
+        const int k0 = whole * wk / a.warps_k, mine = whole * (wk + 1) / a.warps_k - k0;
+        Q4Part<E, ZEROS> part[kQ4Deep] = {}, extra = {};
+        Rows at = {};
+        if (S == 0) {  // the offsets of the scales are needed before the first load
+            if (kb) __syncthreads();
+            for (int h = tid; h < n; h += kQ4Threads) offsets[h] = group_of(min((first + h) * kQ4Half, a.N - 1));
             __syncthreads();
         }
-        consume(c, now);
-        load(c, next);
-        advance(next);
-        if (now.i == now.n - 1) finish(now);
-        advance(now);
-        return now.kb < a.blocks_k;
-    };
-    while (step(even) && step(odd)) {
+        if (tiles && mine) {
+            at = rows_of(0, first + k0 * kQ4Deep);
+#pragma unroll
+            for (int h = 0; h < kQ4Deep; ++h) load(part[h], at, h, k0 * kQ4Deep + h, kb, false);
+        }
+        if (S && kb) __syncthreads();  // all are done with the x before
+        odd_vectors = __syncthreads_or(stage(kb)) != 0;
+
+        for (int tile = 0; tile < tiles; ++tile) {
+            const int left = (wk + tile) & (a.warps_k - 1);  // which of the left halves this warp takes
+            for (int i = left; i < rest; i += a.warps_k) {
+                const int half = whole * kQ4Deep + i;
+                load(extra, rows_of(tile, first + half), 0, half, kb, cut && half == n - 1);
+                multiply(extra, half);
+            }
+            for (int i = 0; i < mine; ++i) {
+                const bool end = i == mine - 1;
+                const int half = (k0 + i) * kQ4Deep;
+                if (!(end && tile == tiles - 1)) {
+                    int to = half + kQ4Deep;
+                    if (end) {
+                        to = k0 * kQ4Deep;
+                        at = rows_of(tile + 1, first + to);
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            at.w[r] += 64 * kQ4Deep;
+                            if (S) at.s[r] += SUB * kQ4Deep * s_size;
+                            if (S && ZEROS) at.z[r] += SUB * kQ4Deep;
+                        }
+                    }
+#pragma unroll
+                    for (int h = 0; h < kQ4Deep; ++h) {
+                        multiply(part[h], half + h);
+                        load(part[h], at, h, to + h, kb, false);
+                    }
+                } else {
+#pragma unroll
+                    for (int h = 0; h < kQ4Deep; ++h) multiply(part[h], half + h);
+                }
+            }
+            finish(kb, tile);
+        }
+    }
+
+    if (a.ranks > 1) {  // the ranks' sums, each rank for its share of the rows
+        namespace cg = cooperative_groups;
+        cg::cluster_group cluster = cg::this_cluster();
+        cluster.sync();
+        const int lo = rows * rank / a.ranks, n = rows * (rank + 1) / a.ranks - lo;
+        for (int e = tid; e < n * a.vectors; e += kQ4Threads) {
+            const int v = e / n, row = lo + e - v * n;
+            float sum = 0.0f;
+            for (int r = 0; r < a.ranks; ++r) sum += cluster.map_shared_rank(ysum, r)[row * a.vectors + v];
+            dev::store_as(a.y, a.dtype_y, v * a.stride_y + r0 + row, sum * 4096.0f);
+        }
+        cluster.sync();  // nobody leaves while its sums are read
     }
 }
 
@@ -415,20 +495,21 @@ struct Q4Entry {
     std::atomic<uint64_t> *smem_set;
 };
 
-template <typename X, int NT, bool SUB, bool ZEROS>
+template <int NT, int S, bool ZEROS, bool WORDS>
 Q4Entry q4_entry() {
     static std::atomic<uint64_t> set{0};
-    return {k_q4_gemv<X, NT, SUB, ZEROS>, &set};
+    return {k_q4_gemv<NT, S, ZEROS, WORDS>, &set};
 }
-template <typename X, int NT>
-Q4Entry q4_entry(bool sub, bool zeros) {
-    if (sub) return zeros ? q4_entry<X, NT, true, true>() : q4_entry<X, NT, true, false>();
-    return zeros ? q4_entry<X, NT, false, true>() : q4_entry<X, NT, false, false>();
+template <int NT, int S>
+Q4Entry q4_entry(bool zeros, bool words) {
+    if (words) return zeros ? q4_entry<NT, S, true, true>() : q4_entry<NT, S, false, true>();
+    return q4_entry<NT, S, true, false>();
 }
-template <typename X>
-Q4Entry q4_entry(int nt, bool sub, bool zeros) {
-    if (nt == 1) return q4_entry<X, 1>(sub, zeros);
-    return nt == 2 ? q4_entry<X, 2>(sub, zeros) : q4_entry<X, 4>(sub, zeros);
+template <int NT>
+Q4Entry q4_entry(int group, bool zeros, bool words) {
+    if (group == 32) return q4_entry<NT, 4>(zeros, words);
+    if (group == 64) return q4_entry<NT, 2>(zeros, words);
+    return group == 128 ? q4_entry<NT, 1>(zeros, words) : q4_entry<NT, 0>(zeros, words);
 }
 
 // No columns: every sum is empty.
@@ -436,6 +517,26 @@ __global__ void k_q4_zero(Q4Args a) {
     dev::wait_for_previous();
     for (int64_t e = blockIdx.x * int64_t(blockDim.x) + threadIdx.x; e < a.M * a.vectors; e += int64_t(gridDim.x) * blockDim.x)
         dev::store_as(a.y, a.dtype_y, e / a.M * a.stride_y + e % a.M, 0.0f);
+}
+
+// Blocks of a cluster: as many as it takes for a block's weights to outweigh its x four to one, if there are
+// columns for them.
+int q4_ranks(int64_t M, int steps, int columns, int sms) {
+    (void)M, (void)columns, (void)sms;
+    return 1;
+}
+
+// Warps that share a tile: the number that gives the least work for each (a tile's end counts two halves).
+int q4_warps_k(int rows, int halves) {
+    int best = 1;
+    int64_t least = INT64_MAX;
+    for (int wk = 1; wk <= kQ4Warps; wk *= 2) {
+        const int groups = kQ4Warps / wk, each = (rows + groups - 1) / groups, steps = halves / kQ4Deep;
+        const int64_t share = (steps + wk - 1) / wk * kQ4Deep + (halves % kQ4Deep + wk - 1) / wk;
+        const int64_t work = int64_t((each + kQ4Rows - 1) / kQ4Rows) * (share + 2);
+        if (work < least) least = work, best = wk;
+    }
+    return best;
 }
 
 }  // namespace l2d
@@ -449,8 +550,8 @@ int l2d_q4_gemv(const l2d_q4_desc *desc, const void *x, int64_t stride_x, void *
     if (!desc) return set_error(L2D_ERR_INVALID, "null descriptor");
     const l2d_q4_desc &d = *desc;
     constexpr int64_t kMax = int64_t(1) << 31;
-    if (d.M < 0 || d.N < 0 || d.M >= kMax || d.N >= kMax / 2)
-        return set_error(L2D_ERR_INVALID, "M = %lld, N = %lld: M below 2^31 and N below 2^30 are supported",
+    if (d.M < 0 || d.N < 0 || d.M >= kMax || d.N >= kMax / 16)
+        return set_error(L2D_ERR_INVALID, "M = %lld, N = %lld: M below 2^31 and N below 2^27 are supported",
                          static_cast<long long>(d.M), static_cast<long long>(d.N));
     if (vectors < 0 || vectors >= kMax) return set_error(L2D_ERR_INVALID, "%lld vectors", static_cast<long long>(vectors));
     if (!valid_dtype(d.dtype_x) || !valid_dtype(d.dtype_y) || !valid_dtype(d.dtype_s))
@@ -493,15 +594,12 @@ int l2d_q4_gemv(const l2d_q4_desc *desc, const void *x, int64_t stride_x, void *
     a.dtype_x = d.dtype_x;
     a.dtype_y = d.dtype_y;
     a.dtype_s = d.dtype_s;
-    a.aligned = reinterpret_cast<uintptr_t>(d.W) % 16 == 0 && ldw % 16 == 0;
-    a.sub_shift = d.group == 32 ? 2 : d.group == 64 ? 1 : 0;
-    a.parts = d.dtype_x == L2D_F32 ? 3 : 1;
-    const int each = a.parts << a.sub_shift;  // columns of B per vector
-    const int most = 32 / each;               // vectors of one pass over the weights
-    const int64_t chunks = (d.N + kQ4Chunk - 1) / kQ4Chunk;
-    a.warps_k = 1;
-    while (a.warps_k < kQ4Warps && a.warps_k < chunks) a.warps_k *= 2;
-    const int64_t blocks = std::max<int64_t>(std::min<int64_t>(d.M, 2 * sms), (d.M + kQ4MaxRows - 1) / kQ4MaxRows);
+    a.per_group = ((uint64_t(1) << 40) + d.group / 128 - 1) / std::max(d.group / 128, 1);
+    const bool words = reinterpret_cast<uintptr_t>(d.W) % 16 == 0 && ldw % 16 == 0 && d.N % 32 == 0 && d.dtype_s != L2D_F32;
+    a.parts = d.dtype_x == L2D_F32 ? 2 : 1;
+    const int each = a.parts * (d.group == 32 ? 4 : d.group == 64 ? 2 : 1);  // columns of B per vector
+    const int most = 32 / each;                                             // vectors of one pass over the weights
+    const int halves = static_cast<int>((d.N + kQ4Half - 1) / kQ4Half);
     for (int64_t v = 0; v < vectors; v += most) {
         a.vectors = static_cast<int>(std::min<int64_t>(most, vectors - v));
         a.x = static_cast<const char *>(x) + v * stride_x * elem_bytes(d.dtype_x);
@@ -512,28 +610,29 @@ int l2d_q4_gemv(const l2d_q4_desc *desc, const void *x, int64_t stride_x, void *
         }
         const int tiles_n = a.vectors * each <= 8 ? 1 : a.vectors * each <= 16 ? 2 : 4;
         const int columns = a.vectors * a.parts;
-        // x is staged whole where two blocks with it fit an SM, else as many times as it takes.
-        const int rows = static_cast<int>((d.M + blocks - 1) / blocks);
-        constexpr int kRoom = 112 * 1024;
-        const int64_t whole = chunks * kQ4Chunk;
-        if (whole * columns * 2 <= kRoom - q4_smem(tiles_n, columns, 0, 0).bytes) {
-            a.block_k = static_cast<int>(whole);
-            a.blocks_k = 1;
-            a.y_rows = 0;
-        } else {
-            const int step = kQ4Chunk * a.warps_k;
-            const int fits = (kRoom - q4_smem(tiles_n, columns, 0, rows).bytes) / (columns * 2) / step * step;
-            a.block_k = std::max(fits, step);
-            a.blocks_k = static_cast<int>((d.N + a.block_k - 1) / a.block_k);
+        a.ranks = q4_ranks(d.M, halves / kQ4Deep, columns, sms);
+        const int64_t shares = std::max<int64_t>(std::min<int64_t>(d.M, std::max(1, sms / a.ranks)), (d.M + kQ4MaxRows - 1) / kQ4MaxRows);
+        const int rows = static_cast<int>((d.M + shares - 1) / shares);
+        // x is staged whole where it fits, else in as many parts as it takes.
+        constexpr int kRoom = 227 * 1024 - 64;
+        const int mine = ((halves + kQ4Deep - 1) / kQ4Deep + a.ranks - 1) / a.ranks * kQ4Deep;  // of a block
+        a.y_rows = a.ranks > 1 ? rows : 0;
+        const int per_half = q4_smem(tiles_n, columns, 4, 0).bytes - q4_smem(tiles_n, columns, 0, 0).bytes;  // four of them
+        int fits = (kRoom - q4_smem(tiles_n, columns, 0, a.y_rows * a.vectors).bytes) / per_half * 4;
+        if (fits < mine) {
             a.y_rows = rows;
+            fits = (kRoom - q4_smem(tiles_n, columns, 0, rows * a.vectors).bytes) / per_half * 4;
+            const int times = (mine + fits - 1) / fits;
+            fits = ((mine + times - 1) / times + kQ4Deep - 1) / kQ4Deep * kQ4Deep;
         }
-        const int smem = q4_smem(tiles_n, columns, a.block_k, a.y_rows).bytes;
-        const bool sub = a.sub_shift > 0, zeros = d.zeros != nullptr;
-        const Q4Entry k = d.dtype_x == L2D_F32 ? q4_entry<float>(tiles_n, sub, zeros)
-                          : d.dtype_x == L2D_F16 ? q4_entry<__half>(tiles_n, sub, zeros)
-                                                 : q4_entry<__nv_bfloat16>(tiles_n, sub, zeros);
+        a.stage_h = std::min(fits, mine);
+        a.warps_k = q4_warps_k(rows, a.stage_h);
+        const int smem = q4_smem(tiles_n, columns, a.stage_h, a.y_rows * a.vectors).bytes;
+        const bool zeros = d.zeros != nullptr;
+        const Q4Entry k = tiles_n == 1   ? q4_entry<1>(d.group, zeros, words)
+                          : tiles_n == 2 ? q4_entry<2>(d.group, zeros, words) : q4_entry<4>(d.group, zeros, words);
         L2D_CUDA_TRY(allow_smem(k.run, 227 * 1024, d.device, *k.smem_set));
-        L2D_CUDA_TRY(launch(k.run, dim3(static_cast<unsigned>(blocks)), kQ4Threads, smem, stream, a));
+        L2D_CUDA_TRY(launch_clusters(k.run, dim3(static_cast<unsigned>(shares * a.ranks)), a.ranks, kQ4Threads, smem, stream, a));
     }
     return L2D_OK;
 }
