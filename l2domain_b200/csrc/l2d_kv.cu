@@ -885,8 +885,6 @@ int check_cache(const l2d_kv_cache *cache, Cache *c) {
     return L2D_OK;
 }
 
-bool misaligned(const void *p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
-
 }  // namespace l2d
 
 using namespace l2d;

@@ -35,6 +35,8 @@ inline int device_sms(int device, int *sms) {
     return L2D_OK;
 }
 
+inline bool misaligned(const void *p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
+
 // Makes `device` current for a scope.
 struct OnDevice {
     int prev = -1;

@@ -3,33 +3,35 @@
 //   y[b][i] = sum_j s[i][j / g] * (q[i][j] - z[i][j / g]) * x[b][j]
 //
 // Memory bound: a weight is half a byte and is used once per vector.  At the bandwidth of HBM an SM
-// gets about 52 weights a cycle and has 128 lanes to treat them, so a weight may cost little over two
-// instructions; a fused multiply-add in fp32 with its conversion would be three or four.  So the products
-// run on matrix instructions (m16n8k16, fp32 sums), 16 rows of weights as the A operand and the vectors
+// gets about 52 weights a cycle and has 128 lanes to treat them (64 of them for logic), so a weight may
+// cost little over two instructions; a fused multiply-add in fp32 with its conversion would be three or
+// four.  So the products run on matrix instructions, 16 rows of weights as the A operand and the vectors
 // as columns of B, and everything else is arranged to spend next to nothing per weight:
 //
-//  * A nibble masked into the low mantissa bits of a 16-bit float is the subnormal q 2^-24, one higher up
-//    16 q 2^-24: both exact, and no instruction but the mask.  x of the columns that end up higher is a
-//    sixteenth of itself.  What the zero point takes away is z times the group's sum of x, which is
-//    computed once per block: sum (q - z) x = sum q x - z sum x, in fp32.
-//  * x is held in shared memory as fp16, each 128 columns of a vector scaled by a power of two to a
-//    largest value just under 2^15, in one part (fp16 and bf16) or two (fp32: 11 bits, and the next 11 as a
-//    column of their own).  That keeps fp16 and bf16 exact and fp32 to one rounding of 2^-24 for values
-//    down to 2^-28 of the largest among its 128 columns; smaller ones are off by up to 2^-36 of the largest.
-//  * Infinities and NaNs do not survive sum q x - z sum x.  They are staged as zeros, and the threads that
-//    store a vector's results add the terms of its infinities and NaNs at the end, one by one.
+//  * One vector (two, for groups of 128 and more) is multiplied in integers (m16n8k32, bytes): two masks and
+//    a shift turn eight nibbles into bytes.  x of each 128 columns is a 30-bit integer times a power of
+//    two, in four signed digits of 8 bits, a column of B each.  Sums are exact up to the end of a group;
+//    values of x are exact down to 2^-6 (fp32), 2^-19 (fp16) or 2^-22 (bf16) of the largest among their 128
+//    columns, and otherwise off by at most 2^-30 of it.
+//  * More vectors are multiplied in fp16 with fp32 sums (m16n8k16): one column a vector (two for fp32, 11
+//    bits each, which leaves one rounding of 2^-24).  A nibble masked into the low mantissa bits of an fp16
+//    number is the subnormal q 2^-24, one higher up 16 q 2^-24: both exact, and no instruction but the mask.
+//    x of the columns that end up higher is a sixteenth of itself.  Each 128 columns of a vector are scaled
+//    by a power of two to a largest value just under 2^15; what is below 2^-28 of it may lose bits.
+//  * What the zero point takes away is z times the group's sum of x, which is computed once per block:
+//    sum (q - z) x = sum q x - z sum x.  Infinities and NaNs do not survive that.  They are staged as zeros,
+//    and the threads that store a vector's results add the terms of its infinities and NaNs at the end.
 //  * The scales are applied to the fp32 sums of each group.  One instruction sums over the four lanes of a
 //    row, 128 columns; where groups are shorter, x of the different groups goes to different columns of B
 //    (zeros elsewhere), so that each group still has a sum of its own: S = 128 / group columns per part.
 //  * A lane's 16 bytes (32 columns of one row) are loaded straight into registers from the row-major
-//    weights, a chunk ahead.  A product's order of columns is free, so nibbles are used in the order in
-//    which masks deliver them, and x is put into that order when it is staged.
+//    weights, a step of 512 columns ahead, in code without branches.  A product's order of columns is free,
+//    so nibbles are used in the order in which masks deliver them, and x is put into that order when it is
+//    staged.  A request for eight rows occupies the L1 for eight cycles whatever its width, so the scales of
+//    a whole step are loaded as one word per row.
 //  * A block's rows are its even share of M, in tiles of at most 16 rows of nearly equal size, so that
 //    blocks finish together whatever M is; groups of its warps take a tile each, split its columns and
-//    meet in shared memory at its end, in a fixed order.  Where a block has
-//    few rows, staging all of x for them would cost as much as their weights: a cluster of blocks then
-//    takes more rows together, each block a share of the columns, and adds its sums over distributed
-//    shared memory, in rank order.
+//    meet in shared memory at its end, in a fixed order.
 #include "l2d_launch.cuh"
 
 #include <cooperative_groups.h>
@@ -61,16 +63,16 @@ constexpr int kQ4Half = 128;       // columns of one sum: 64 bytes of each row
 constexpr int kQ4Deep = 4;         // of them in a step, which a warp has in registers or on their way
 constexpr int kQ4Rows = 16;
 constexpr int kQ4MaxRows = 896;    // rows of a block, at most
-constexpr int kQ4Column = 320;     // bytes between columns of x in shared memory: 256 used, so that two lie in other banks
+// Bytes between columns of x in shared memory: 256 used (128 by bytes), and 64 so that two lie in other banks.
+__host__ __device__ constexpr int q4_column(bool bytes) { return bytes ? 192 : 320; }
 
-// Byte offsets in dynamic shared memory: x, zeros, its sums and factors, offsets of scales, the warps' sums, y.
+// Byte offsets in dynamic shared memory: x, its sums and factors, offsets of scales, the warps' sums, y.
 struct Q4Smem {
-    int zero, sums, offsets, red, y, bytes;
+    int sums, offsets, red, y, bytes;
 };
-__host__ __device__ inline Q4Smem q4_smem(int tiles_n, int columns, int stage_h, int y_floats) {
+__host__ __device__ inline Q4Smem q4_smem(int tiles_n, bool bytes, int columns, int stage_h, int y_floats) {
     Q4Smem s;
-    s.zero = columns * stage_h * kQ4Column;
-    s.sums = s.zero + 256;
+    s.sums = columns * stage_h * q4_column(bytes);
     s.offsets = s.sums + stage_h * 8 * tiles_n * 8;
     s.red = s.offsets + (stage_h + 3) / 4 * 16;
     s.y = s.red + (tiles_n == 1 ? 2 : 1) * kQ4Warps * kQ4Rows * 8 * tiles_n * 4;
@@ -88,6 +90,20 @@ __device__ __forceinline__ void q4_mma(float (&c)[4], const uint32_t (&a)[4], ui
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// c += a b in integers: a unsigned, b signed bytes, 32 columns.
+__device__ __forceinline__ void q4_mma_bytes(uint32_t (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// 16 bytes of shared memory where `real`; v stays as it is elsewhere.
+__device__ __forceinline__ void load_if(uint4 &v, const char *p, bool real) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %5, 0;\n@p ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n}"
+        : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w)
+        : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))), "r"(static_cast<uint32_t>(real)));
 }
 
 // Eight nibbles as fp16 numbers, p[i] nibbles i and i + 4: q 2^-24, and 16 q 2^-24 in p[1] and p[3].
@@ -132,25 +148,37 @@ __device__ __forceinline__ uint4 load_any(const uint8_t *p, int left, const uint
     return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-// What a warp holds of 128 columns of a tile: this lane's 16 bytes of rows g and g + 8, the scales of those
-// rows' sums and the zeros of the same groups.
-template <int E, bool ZEROS>
+// What a warp holds of 128 columns of a tile: this lane's 16 bytes of rows g and g + 8.
 struct Q4Part {
     uint4 w[2];
-    uint32_t s[2][E];              // [row][column of C], as stored
-    uint32_t z[2][ZEROS ? E : 1];
+};
+// And of a step of four such halves: the scales and zeros of its columns 2t, 2t + 1 of C for both rows, as
+// stored.  Two to a word (zeros: bytes); S = 0: those of the first and of the last half.
+template <int S, bool ZEROS>
+struct Q4Scales {
+    uint32_t s[2][S > 1 ? 4 : 2];
+    uint32_t z[2][!ZEROS || S == 1 ? 1 : S == 4 ? 4 : 2];
+    int from;  // S = 0: the first half whose scale is the last one's
 };
 
+__device__ __forceinline__ float scale_value(uint32_t word, bool high, bool is_half) {
+    const float wide = __uint_as_float(high ? word & 0xffff0000u : word << 16);
+    return is_half ? __half2float(__ushort_as_half(static_cast<unsigned short>(high ? word >> 16 : word))) : wide;
+}
+
 // S: columns of B per part of a vector (4, 2, 1 for groups of 32, 64, 128 columns), 0 for longer groups.
-// WORDS: every row of W is whole 16-byte words on 16-byte boundaries, and scales have 16 bits.
-template <int NT, int S, bool ZEROS, bool WORDS>
+// WORDS: every row of W is whole 16-byte words on 16-byte boundaries, and the 16-bit scales (and zeros) of a step
+// can be read in words.
+// BYTES: integer products.
+template <int NT, int S, bool ZEROS, bool WORDS, bool BYTES>
 __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
-    constexpr int SUB = S > 1 ? S : 1, kShift = S == 4 ? 2 : S == 2 ? 1 : 0, E = S > 1 ? 2 : 1;
+    constexpr int SUB = S > 1 ? S : 1, kShift = S == 4 ? 2 : S == 2 ? 1 : 0, E = S > 1 ? 2 : 1, kColumn = q4_column(BYTES);
+    constexpr float kUnit = BYTES ? 1.0f : 4096.0f;  // of the sums
     extern __shared__ __align__(16) char smem[];
     const int tid = threadIdx.x, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // known to be the same in all lanes
     const int columns = a.vectors * a.parts;                 // of x in shared memory
-    const Q4Smem lay = q4_smem(NT, columns, a.stage_h, a.y_rows * a.vectors);
+    const Q4Smem lay = q4_smem(NT, BYTES, columns, a.stage_h, a.y_rows * a.vectors);
     float2 *sums = reinterpret_cast<float2 *>(smem + lay.sums);
     int *offsets = reinterpret_cast<int *>(smem + lay.offsets);
     float *red = reinterpret_cast<float *>(smem + lay.red), *ysum = reinterpret_cast<float *>(smem + lay.y);
@@ -172,52 +200,60 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
     auto group_of = [&](int col) {
         return S > 1 ? col >> (7 - kShift) : static_cast<int>(static_cast<uint64_t>(col >> 7) * a.per_group >> 40);
     };
-    const int s_size = WORDS ? 2 : a.dtype_s == L2D_F32 ? 4 : 2;
     dev::wait_for_previous();
 
     // The column of x that this lane feeds into column g of each n-tile: part (8 n + g) / S, if the lane's columns
-    // of W belong to that column's subgroup; else zeros, from a place that does not move.
-    const char *x_at[NT];
-    int x_half[NT];
+    // of W belong to that column's subgroup.  b stays zero where it feeds none.
+    constexpr int kAhead = NT == 1 ? 2 : 1;
+    bool feeds[NT];
+    uint4 b[NT][kAhead];
     float acc[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        const int column = (8 * n + g) >> kShift;
-        const bool feeds = (g & (SUB - 1)) == (t * SUB >> 2) && column < columns;
-        x_at[n] = feeds ? smem + column * kQ4Column + t * 16 : smem + lay.zero;
-        x_half[n] = feeds ? columns * kQ4Column : 0;
+        feeds[n] = (g & (SUB - 1)) == (t * SUB >> 2) && ((8 * n + g) >> kShift) < columns;
+#pragma unroll
+        for (int e = 0; e < kAhead; ++e) b[n][e] = make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[n][e] = 0.0f;
     }
+    const char *x_lane = smem + (g >> kShift) * kColumn + t * 16;
+    const int x_half = columns * kColumn;
+    const bool is_half = a.dtype_s == L2D_F16;
 
-    // Adds the products of half `half` of the staging.
-    auto multiply = [&](const Q4Part<E, ZEROS> &c, int half) {
+    // Adds the products of half `half` of the staging: scales s and zeros z of [row][column of C].
+    auto multiply = [&](const Q4Part &c, int half, const float (&s)[2][E], const float (&z)[2][E]) {
         const uint32_t w0[4] = {c.w[0].x, c.w[0].y, c.w[0].z, c.w[0].w}, w1[4] = {c.w[1].x, c.w[1].y, c.w[1].z, c.w[1].w};
         float sum[NT][4];
-        const char *x[NT];
+        const char *x = x_lane + half * x_half;
+        if constexpr (BYTES) {
+            // Sums of products of bytes, on top of the bits of 1.5 * 2^23: as a float they are that much more.
+            uint32_t c0[4] = {0x4b400000u, 0x4b400000u, 0x4b400000u, 0x4b400000u};
 #pragma unroll
-        for (int n = 0; n < NT; ++n) x[n] = x_at[n] + half * x_half[n];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            uint32_t p0[4], p1[4];
-            unpack(w0[j], p0);
-            unpack(w1[j], p1);
-            const uint32_t a0[4] = {p0[0], p1[0], p0[1], p1[1]}, a1[4] = {p0[2], p1[2], p0[3], p1[3]};
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const uint4 b = *reinterpret_cast<const uint4 *>(x[n] + j * 64);
-                if (j == 0) q4_mma_first(sum[n], a0, b.x, b.y);
-                else q4_mma(sum[n], a0, b.x, b.y);
-                q4_mma(sum[n], a1, b.z, b.w);
+            for (int j = 0; j < 4; j += 2) {
+                load_if(b[0][j / 2], x + j * 32, feeds[0]);
+                const uint32_t a0[4] = {w0[j] & 0x0F0F0F0F, w1[j] & 0x0F0F0F0F, w0[j] >> 4 & 0x0F0F0F0F, w1[j] >> 4 & 0x0F0F0F0F};
+                const uint32_t a1[4] = {w0[j + 1] & 0x0F0F0F0F, w1[j + 1] & 0x0F0F0F0F, w0[j + 1] >> 4 & 0x0F0F0F0F, w1[j + 1] >> 4 & 0x0F0F0F0F};
+                q4_mma_bytes(c0, a0, b[0][j / 2].x, b[0][j / 2].y);
+                q4_mma_bytes(c0, a1, b[0][j / 2].z, b[0][j / 2].w);
             }
-        }
-        float s[2][E], z[2][E];
 #pragma unroll
-        for (int e = 0; e < 2 * E; ++e) {
-            const uint32_t v = c.s[e / E][e % E];
-            const float wide = __uint_as_float(WORDS || s_size == 2 ? v << 16 : v);
-            s[e / E][e % E] = a.dtype_s == L2D_F16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(v))) : wide;
-            z[e / E][e % E] = ZEROS ? static_cast<float>(c.z[e / E][ZEROS ? e % E : 0] & 15) : 8.0f;
+            for (int e = 0; e < 4; ++e) sum[0][e] = __uint_as_float(c0[e]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                uint32_t p0[4], p1[4];
+                unpack(w0[j], p0);
+                unpack(w1[j], p1);
+                const uint32_t a0[4] = {p0[0], p1[0], p0[1], p1[1]}, a1[4] = {p0[2], p1[2], p0[3], p1[3]};
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    uint4 &bb = b[n][j % kAhead];
+                    load_if(bb, x + n * (8 >> kShift) * kColumn + j * 64, feeds[n]);
+                    if (j == 0) q4_mma_first(sum[n], a0, bb.x, bb.y);
+                    else q4_mma(sum[n], a0, bb.x, bb.y);
+                    q4_mma(sum[n], a1, bb.z, bb.w);
+                }
+            }
         }
         const float4 *xs = reinterpret_cast<const float4 *>(sums + half * 8 * NT) + t;
 #pragma unroll
@@ -225,10 +261,28 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
             const float4 f = xs[4 * n];  // sum and factor of columns 2t and 2t + 1
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float v = fmaf(-z[e >> 1][(e & 1) % E], e & 1 ? f.z : f.x, sum[n][e]);
+                const float zero = z[e >> 1][(e & 1) % E], xsum = e & 1 ? f.z : f.x;
+                // By bytes all of this is integers below 2^24, and exact (without zeros the sum is 8 of it and the bias).
+                const float v = BYTES ? sum[n][e] - (ZEROS ? fmaf(zero, xsum, 12582912.0f) : xsum) : fmaf(-zero, xsum, sum[n][e]);
                 acc[n][e] = fmaf(s[e >> 1][(e & 1) % E], v * fabsf(e & 1 ? f.w : f.y), acc[n][e]);
             }
         }
+    };
+    // Half h of a step.
+    auto multiply_of = [&](const Q4Part &c, const Q4Scales<S, ZEROS> &q, int h, int half) {
+        float s[2][E], z[2][E];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const bool second = S == 0 && h >= q.from;
+            const uint32_t word = S == 0 ? (second ? q.s[r][1] : q.s[r][0]) : q.s[r][S == 1 ? h / 2 : h];
+#pragma unroll
+            for (int e = 0; e < E; ++e) s[r][e] = scale_value(word, S == 1 ? h & 1 : e, is_half);
+            uint32_t zeros = 0;
+            if constexpr (ZEROS) zeros = S == 0 ? (second ? q.z[r][1] : q.z[r][0]) : S == 1 ? q.z[r][0] >> (8 * h) : S == 2 ? q.z[r][h / 2] >> (16 * (h & 1)) : q.z[r][h];
+#pragma unroll
+            for (int e = 0; e < E; ++e) z[r][e] = ZEROS ? static_cast<float>(zeros >> (8 * e) & 15) : 8.0f;
+        }
+        multiply(c, half, s, z);
     };
 
     // Where this lane reads: rows g and g + 8 of a tile, or the tile's last row where it has fewer (their sums are
@@ -237,7 +291,7 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
         const uint8_t *w[2], *s[2], *z[2];
     };
     // Scales of the columns 2t, 2t + 1 of C, which belong to the subgroups (2t) % S and (2t + 1) % S.
-    const int sub = S > 1 ? (2 * t) & (SUB - 1) : 0;
+    const int sub = S == 4 ? (2 * t) & 3 : 0;
     auto rows_of = [&](int tile, int half) {
         Rows at;
         const int last = first_row(tile + 1) - 1, lo = first_row(tile);
@@ -245,31 +299,77 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
         for (int r = 0; r < 2; ++r) {
             const int64_t row = r0 + min(lo + g + 8 * r, last), first = S ? half * SUB + sub : 0;
             at.w[r] = a.W + row * a.ldw + half * 64 + 16 * t;
-            at.s[r] = a.scales + (row * a.lds + first) * s_size;
+            at.s[r] = a.scales + (row * a.lds + first) * 2;
             at.z[r] = ZEROS ? a.zeros + row * a.lds + first : nullptr;
         }
         return at;
     };
-    // Loads half h after those, which is half `half` of the staging.  `last`: the last one of a row that is not
-    // whole, where there may be fewer bytes and groups; scales past the last column belong to sums that are zero.
-    auto load = [&](Q4Part<E, ZEROS> &c, const Rows &at, int h, int half, int kb, bool last) {
-        const int col = (h_lo + kb * a.stage_h + half) * kQ4Half, left = row_bytes - (col >> 1) - 16 * t;
-        const int more = S > 1 && last && sub + 1 > group_of(a.N - 1) - group_of(col) ? 0 : 1, skip = S > 1 && last ? min(0, group_of(a.N - 1) - group_of(col) - sub) : 0;
+    auto load = [&](Q4Part &c, const Rows &at, int h) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) c.w[r] = load_weights(at.w[r] + h * 64);
+    };
+    // The scales of the step from half `half` of the staging on.
+    auto load_scales = [&](Q4Scales<S, ZEROS> &q, const Rows &at, int half) {
+        const int first = S == 0 ? offsets[half] : 0, last = S == 0 ? offsets[half + kQ4Deep - 1] : 0;
+        if (S == 0) q.from = offsets[half + 1] != first ? 1 : offsets[half + 2] != first ? 2 : 3;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            const uint8_t *p = at.w[r] + h * 64;
-            if constexpr (!WORDS) c.w[r] = load_any(p, left, a.W, w_end);
-            else if (!last) c.w[r] = load_weights(p);
-            else c.w[r] = left > 0 ? load_weights(p) : make_uint4(0, 0, 0, 0);
-            const int first = S ? h * SUB + skip : offsets[half];
+            if constexpr (S == 0) {
+                q.s[r][0] = __ldg(reinterpret_cast<const uint16_t *>(at.s[r]) + first);
+                q.s[r][1] = __ldg(reinterpret_cast<const uint16_t *>(at.s[r]) + last);
+                if constexpr (ZEROS) q.z[r][0] = __ldg(at.z[r] + first), q.z[r][1] = __ldg(at.z[r] + last);
+            } else if constexpr (S == 1) {
+                const uint2 v = __ldg(reinterpret_cast<const uint2 *>(at.s[r]));
+                q.s[r][0] = v.x, q.s[r][1] = v.y;
+                if constexpr (ZEROS) q.z[r][0] = __ldg(reinterpret_cast<const uint32_t *>(at.z[r]));
+            } else if constexpr (S == 2) {
+                const uint4 v = __ldg(reinterpret_cast<const uint4 *>(at.s[r]));
+                q.s[r][0] = v.x, q.s[r][1] = v.y, q.s[r][2] = v.z, q.s[r][3] = v.w;
+                if constexpr (ZEROS) {
+                    const uint2 u = __ldg(reinterpret_cast<const uint2 *>(at.z[r]));
+                    q.z[r][0] = u.x, q.z[r][1] = u.y;
+                }
+            } else {
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int i = first + (e ? more : 0);
-                if (WORDS || s_size == 2) c.s[r][e] = __ldg(reinterpret_cast<const uint16_t *>(at.s[r]) + i);
-                else c.s[r][e] = __ldg(reinterpret_cast<const uint32_t *>(at.s[r]) + i);
-                if constexpr (ZEROS) c.z[r][e] = a.zeros ? __ldg(at.z[r] + i) : 8;
+                for (int h = 0; h < kQ4Deep; ++h) {
+                    q.s[r][h] = __ldg(reinterpret_cast<const uint32_t *>(at.s[r]) + 2 * h);
+                    if constexpr (ZEROS) q.z[r][h] = __ldg(reinterpret_cast<const uint16_t *>(at.z[r]) + 2 * h);
+                }
             }
         }
+    };
+    // One half by itself, whatever its alignment, and be it the last one of a row that is not whole: fewer bytes,
+    // fewer groups (scales past the last column belong to sums that are zero).
+    struct Alone {
+        Q4Part c;
+        uint32_t s[2][E], z[2][E];
+    };
+    auto load_alone = [&](Alone &x, int tile, int half) {
+        const int col = half * kQ4Half, left = row_bytes - (col >> 1) - 16 * t;
+        const int last = first_row(tile + 1) - 1, lo = first_row(tile);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int64_t row = r0 + min(lo + g + 8 * r, last);
+            x.c.w[r] = load_any(a.W + row * a.ldw + (col >> 1) + 16 * t, left, a.W, w_end);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int64_t i = row * a.lds + group_of(min(col + (S > 1 ? (sub + e) * (kQ4Half / SUB) : 0), a.N - 1));
+                x.s[r][e] = a.dtype_s == L2D_F32 ? __ldg(reinterpret_cast<const uint32_t *>(a.scales) + i)
+                                                 : __ldg(reinterpret_cast<const uint16_t *>(a.scales) + i);
+                x.z[r][e] = a.zeros ? __ldg(a.zeros + i) : 8;
+            }
+        }
+    };
+    auto multiply_alone = [&](const Alone &x, int half) {
+        float s[2][E], z[2][E];
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                s[r][e] = a.dtype_s == L2D_F32 ? __uint_as_float(x.s[r][e]) : scale_value(x.s[r][e], false, is_half);
+                z[r][e] = static_cast<float>(x.z[r][e] & 15);
+            }
+        multiply(x.c, half, s, z);
     };
 
     // x of one staging: 16 lanes take 128 columns of one vector, eight columns each.  16 bytes hold columns
@@ -313,6 +413,35 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
             }
 #pragma unroll
             for (int d = 1; d < 16; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+            const bool odd = __ballot_sync(0xffffffffu, odd_ones) >> (lane & 16) & 0xffff;  // in these 128 columns
+            any_odd = any_odd || (real && odd);
+            const int column = v * a.parts, tt = u >> 2, j = u & 3;
+            float2 *to = sums + half * 8 * NT + (column << kShift) + u / (16 / SUB);
+            const bool stores_sums = real && u % (16 / SUB) == 0;
+            if constexpr (BYTES) {
+                // 2^(p - 127) takes the largest to [2^29, 2^30); four signed digits of 8 bits, a column each.
+                const uint32_t p = min(283u - (top >> 23), 253u);
+                const float up = __uint_as_float(p << 23), back = __uint_as_float((254u - p) << 23);
+                uint32_t digits[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) digits[i] = (static_cast<uint32_t>(__float2int_rn(f[i] * up)) + 0x00808080u) ^ 0x00808080u;
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    const uint32_t pick = d | (4 + d) << 4;
+                    const uint32_t even = __byte_perm(__byte_perm(digits[0], digits[2], pick), __byte_perm(digits[4], digits[6], pick), 0x5410);
+                    const uint32_t odds = __byte_perm(__byte_perm(digits[1], digits[3], pick), __byte_perm(digits[5], digits[7], pick), 0x5410);
+                    if (real)
+                        *reinterpret_cast<uint2 *>(smem + (half * columns + column + d) * kColumn + (j >> 1) * 64 + tt * 16 + (j & 1) * 8) = make_uint2(even, odds);
+                    int total = __dp4a(static_cast<int>(even), 0x01010101, __dp4a(static_cast<int>(odds), 0x01010101, 0));
+#pragma unroll
+                    for (int o = 1; o < 16 / SUB; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+                    const float factor = back * static_cast<float>(1 << 8 * d);
+                    if (stores_sums)
+                        to[d << kShift] = make_float2(ZEROS ? static_cast<float>(total) : 12582912.0f + 8.0f * static_cast<float>(total),
+                                                      odd && d == 0 ? -factor : factor);  // the sign: see add_odd_ones()
+                }
+                continue;
+            }
             // 2^(p - 127) takes the largest to [2^14, 2^15); the factor back is short of 2^12, which the end makes good.
             const uint32_t p = min(268u - (top >> 23), 254u);
             const float up = __uint_as_float(p << 23), back = __uint_as_float((266u - p) << 23);
@@ -338,25 +467,20 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
                 total_hi += __shfl_xor_sync(0xffffffffu, total_hi, d);
                 total_lo += __shfl_xor_sync(0xffffffffu, total_lo, d);
             }
-            const bool odd = __ballot_sync(0xffffffffu, odd_ones) >> (lane & 16) & 0xffff;  // in these 128 columns
-            any_odd = any_odd || (real && odd);
             if (real) {
-                const int column = v * a.parts, tt = u >> 2, j = u & 3;
-                uint4 *dst = reinterpret_cast<uint4 *>(smem + (half * columns + column) * kQ4Column) + j * 4 + tt;
+                uint4 *dst = reinterpret_cast<uint4 *>(smem + (half * columns + column) * kColumn) + j * 4 + tt;
                 dst[0] = make_uint4(hi[0] | hi[4] << 16, hi[1] | hi[5] << 16, hi[2] | hi[6] << 16, hi[3] | hi[7] << 16);
                 if (a.parts == 2)
-                    dst[kQ4Column / 16] = make_uint4(lo[0] | lo[4] << 16, lo[1] | lo[5] << 16, lo[2] | lo[6] << 16, lo[3] | lo[7] << 16);
-                if (u % (16 / SUB) == 0) {
-                    float2 *to = sums + half * 8 * NT + (column << kShift) + u / (16 / SUB);
-                    to[0] = make_float2(total_hi * 0x1p-24f, odd ? -back : back);  // the sign: see add_odd_ones()
-                    if (a.parts == 2) to[SUB] = make_float2(total_lo * 0x1p-24f, back * 0x1p-11f);
-                }
+                    dst[kColumn / 16] = make_uint4(lo[0] | lo[4] << 16, lo[1] | lo[5] << 16, lo[2] | lo[6] << 16, lo[3] | lo[7] << 16);
+            }
+            if (stores_sums) {
+                to[0] = make_float2(total_hi * 0x1p-24f, odd ? -back : back);
+                if (a.parts == 2) to[SUB] = make_float2(total_lo * 0x1p-24f, back * 0x1p-11f);
             }
         }
         // Columns of B without a vector: their sums are dropped, but stay finite.
         const int used = columns << kShift, unused = 8 * NT - used;
         for (int e = tid; e < halves * unused; e += kQ4Threads) sums[e / unused * 8 * NT + used + e % unused] = make_float2(0.0f, 0.0f);
-        if (tid < 16) reinterpret_cast<uint4 *>(smem + lay.zero)[tid] = make_uint4(0, 0, 0, 0);
         return any_odd;
     };
 
@@ -405,13 +529,13 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
                 for (int i = 0; i < a.parts; ++i)
 #pragma unroll
                     for (int c = 0; c < SUB; ++c) sum += p[i * SUB + c];
-            if (odd_vectors) sum = add_odd_ones(sum * 4096.0f, kb, row, v) * 0x1p-12f;
+            if (odd_vectors) sum = add_odd_ones(sum * kUnit, kb, row, v) / kUnit;
             if (a.y_rows) {
                 float *y = ysum + row * a.vectors + v;
                 sum += kb ? *y : 0.0f;
                 *y = sum;  // this thread again the next time
             }
-            if (h_lo + (kb + 1) * a.stage_h >= h_hi && a.ranks == 1) dev::store_as(a.y, a.dtype_y, v * a.stride_y + r0 + row, sum * 4096.0f);
+            if (h_lo + (kb + 1) * a.stage_h >= h_hi && a.ranks == 1) dev::store_as(a.y, a.dtype_y, v * a.stride_y + r0 + row, sum * kUnit);
         }
         if (NT == 1) buffer ^= 1;
     };
@@ -420,9 +544,10 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
         // The staging's halves: whole steps, an even share for each warp, and what is left, a half for a warp.
         const int first = h_lo + kb * a.stage_h, n = min(h_hi - first, a.stage_h);
         const bool cut = (first + n) * kQ4Half > a.N;  // the last half is not whole
-        const int whole = (n - (cut ? 1 : 0)) / kQ4Deep, rest = n - whole * kQ4Deep;
+        const int whole = WORDS ? (n - (cut ? 1 : 0)) / kQ4Deep : 0, rest = n - whole * kQ4Deep;
         const int k0 = whole * wk / a.warps_k, mine = whole * (wk + 1) / a.warps_k - k0;
-        Q4Part<E, ZEROS> part[kQ4Deep] = {}, extra = {};
+        Q4Part part[kQ4Deep] = {};
+        Q4Scales<S, ZEROS> now = {}, next = {};
         Rows at = {};
         if (S == 0) {  // the offsets of the scales are needed before the first load
             if (kb) __syncthreads();
@@ -432,42 +557,45 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
         if (tiles && mine) {
             at = rows_of(0, first + k0 * kQ4Deep);
 #pragma unroll
-            for (int h = 0; h < kQ4Deep; ++h) load(part[h], at, h, k0 * kQ4Deep + h, kb, false);
+            for (int h = 0; h < kQ4Deep; ++h) load(part[h], at, h);
+            load_scales(now, at, k0 * kQ4Deep);
         }
         if (S && kb) __syncthreads();  // all are done with the x before
         odd_vectors = __syncthreads_or(stage(kb)) != 0;
 
         for (int tile = 0; tile < tiles; ++tile) {
-            const int left = (wk + tile) & (a.warps_k - 1);  // which of the left halves this warp takes
-            for (int i = left; i < rest; i += a.warps_k) {
-                const int half = whole * kQ4Deep + i;
-                load(extra, rows_of(tile, first + half), 0, half, kb, cut && half == n - 1);
-                multiply(extra, half);
+            for (int i = (wk + tile) & (a.warps_k - 1); i < rest; i += 2 * a.warps_k) {
+                const int half = whole * kQ4Deep + i, other = half + a.warps_k;
+                Alone x, y;
+                load_alone(x, tile, first + half);
+                if (other < n) load_alone(y, tile, first + other);
+                multiply_alone(x, half);
+                if (other < n) multiply_alone(y, other);
             }
             for (int i = 0; i < mine; ++i) {
                 const bool end = i == mine - 1;
                 const int half = (k0 + i) * kQ4Deep;
                 if (!(end && tile == tiles - 1)) {
-                    int to = half + kQ4Deep;
                     if (end) {
-                        to = k0 * kQ4Deep;
-                        at = rows_of(tile + 1, first + to);
+                        at = rows_of(tile + 1, first + k0 * kQ4Deep);
                     } else {
 #pragma unroll
                         for (int r = 0; r < 2; ++r) {
                             at.w[r] += 64 * kQ4Deep;
-                            if (S) at.s[r] += SUB * kQ4Deep * s_size;
+                            if (S) at.s[r] += SUB * kQ4Deep * 2;
                             if (S && ZEROS) at.z[r] += SUB * kQ4Deep;
                         }
                     }
+                    load_scales(next, at, end ? k0 * kQ4Deep : half + kQ4Deep);
 #pragma unroll
                     for (int h = 0; h < kQ4Deep; ++h) {
-                        multiply(part[h], half + h);
-                        load(part[h], at, h, to + h, kb, false);
+                        multiply_of(part[h], now, h, half + h);
+                        load(part[h], at, h);
                     }
+                    now = next;
                 } else {
 #pragma unroll
-                    for (int h = 0; h < kQ4Deep; ++h) multiply(part[h], half + h);
+                    for (int h = 0; h < kQ4Deep; ++h) multiply_of(part[h], now, h, half + h);
                 }
             }
             finish(kb, tile);
@@ -483,7 +611,7 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
             const int v = e / n, row = lo + e - v * n;
             float sum = 0.0f;
             for (int r = 0; r < a.ranks; ++r) sum += cluster.map_shared_rank(ysum, r)[row * a.vectors + v];
-            dev::store_as(a.y, a.dtype_y, v * a.stride_y + r0 + row, sum * 4096.0f);
+            dev::store_as(a.y, a.dtype_y, v * a.stride_y + r0 + row, sum * kUnit);
         }
         cluster.sync();  // nobody leaves while its sums are read
     }
@@ -495,21 +623,26 @@ struct Q4Entry {
     std::atomic<uint64_t> *smem_set;
 };
 
-template <int NT, int S, bool ZEROS, bool WORDS>
+template <int NT, int S, bool ZEROS, bool WORDS, bool BYTES>
 Q4Entry q4_entry() {
     static std::atomic<uint64_t> set{0};
-    return {k_q4_gemv<NT, S, ZEROS, WORDS>, &set};
+    return {k_q4_gemv<NT, S, ZEROS, WORDS, BYTES>, &set};
 }
 template <int NT, int S>
 Q4Entry q4_entry(bool zeros, bool words) {
-    if (words) return zeros ? q4_entry<NT, S, true, true>() : q4_entry<NT, S, false, true>();
-    return q4_entry<NT, S, true, false>();
+    if (words) return zeros ? q4_entry<NT, S, true, true, false>() : q4_entry<NT, S, false, true, false>();
+    return q4_entry<NT, S, true, false, false>();
 }
 template <int NT>
 Q4Entry q4_entry(int group, bool zeros, bool words) {
     if (group == 32) return q4_entry<NT, 4>(zeros, words);
     if (group == 64) return q4_entry<NT, 2>(zeros, words);
     return group == 128 ? q4_entry<NT, 1>(zeros, words) : q4_entry<NT, 0>(zeros, words);
+}
+Q4Entry q4_entry_bytes(int group, bool zeros) {
+    if (group == 64) return zeros ? q4_entry<1, 2, true, true, true>() : q4_entry<1, 2, false, true, true>();
+    if (group == 128) return zeros ? q4_entry<1, 1, true, true, true>() : q4_entry<1, 1, false, true, true>();
+    return zeros ? q4_entry<1, 0, true, true, true>() : q4_entry<1, 0, false, true, true>();
 }
 
 // No columns: every sum is empty.
@@ -527,12 +660,12 @@ int q4_ranks(int64_t M, int steps, int columns, int sms) {
 }
 
 // Warps that share a tile: the number that gives the least work for each (a tile's end counts two halves).
-int q4_warps_k(int rows, int halves) {
+int q4_warps_k(int rows, int halves, int deep) {
     int best = 1;
     int64_t least = INT64_MAX;
     for (int wk = 1; wk <= kQ4Warps; wk *= 2) {
-        const int groups = kQ4Warps / wk, each = (rows + groups - 1) / groups, steps = halves / kQ4Deep;
-        const int64_t share = (steps + wk - 1) / wk * kQ4Deep + (halves % kQ4Deep + wk - 1) / wk;
+        const int groups = kQ4Warps / wk, each = (rows + groups - 1) / groups, steps = halves / deep;
+        const int64_t share = (steps + wk - 1) / wk * deep + (halves % deep + wk - 1) / wk;
         const int64_t work = int64_t((each + kQ4Rows - 1) / kQ4Rows) * (share + 2);
         if (work < least) least = work, best = wk;
     }
@@ -572,8 +705,7 @@ int l2d_q4_gemv(const l2d_q4_desc *desc, const void *x, int64_t stride_x, void *
         return set_error(L2D_ERR_INVALID, "strides too large");
     if (d.M == 0 || vectors == 0) return L2D_OK;
     if (!y || (d.N && (!x || !d.W || !d.scales))) return set_error(L2D_ERR_INVALID, "null pointer");
-    if (reinterpret_cast<uintptr_t>(x) % elem_bytes(d.dtype_x) || reinterpret_cast<uintptr_t>(y) % elem_bytes(d.dtype_y) ||
-        reinterpret_cast<uintptr_t>(d.scales) % elem_bytes(d.dtype_s))
+    if (misaligned(x, elem_bytes(d.dtype_x)) || misaligned(y, elem_bytes(d.dtype_y)) || misaligned(d.scales, elem_bytes(d.dtype_s)))
         return set_error(L2D_ERR_INVALID, "x, y and scales must be aligned to their elements");
     int sms = 0;
     const int st = device_sms(d.device, &sms);
@@ -595,9 +727,13 @@ int l2d_q4_gemv(const l2d_q4_desc *desc, const void *x, int64_t stride_x, void *
     a.dtype_y = d.dtype_y;
     a.dtype_s = d.dtype_s;
     a.per_group = ((uint64_t(1) << 40) + d.group / 128 - 1) / std::max(d.group / 128, 1);
-    const bool words = reinterpret_cast<uintptr_t>(d.W) % 16 == 0 && ldw % 16 == 0 && d.N % 32 == 0 && d.dtype_s != L2D_F32;
-    a.parts = d.dtype_x == L2D_F32 ? 2 : 1;
-    const int each = a.parts * (d.group == 32 ? 4 : d.group == 64 ? 2 : 1);  // columns of B per vector
+    const int word = d.group == 32 ? 2 : d.group == 64 ? 8 : d.group == 128 ? 4 : 1;  // scales that are read together
+    const bool words = !misaligned(d.W, 16) && ldw % 16 == 0 && d.dtype_s != L2D_F32 && lds % word == 0 &&
+                       !misaligned(d.scales, 2 * word) && !misaligned(d.zeros, word);
+    const int sub = d.group == 32 ? 4 : d.group == 64 ? 2 : 1;
+    const bool bytes = words && vectors * sub <= 2;
+    a.parts = bytes ? 4 : d.dtype_x == L2D_F32 ? 2 : 1;
+    const int each = a.parts * sub;                                         // columns of B per vector
     const int most = 32 / each;                                             // vectors of one pass over the weights
     const int halves = static_cast<int>((d.N + kQ4Half - 1) / kQ4Half);
     for (int64_t v = 0; v < vectors; v += most) {
@@ -617,19 +753,20 @@ int l2d_q4_gemv(const l2d_q4_desc *desc, const void *x, int64_t stride_x, void *
         constexpr int kRoom = 227 * 1024 - 64;
         const int mine = ((halves + kQ4Deep - 1) / kQ4Deep + a.ranks - 1) / a.ranks * kQ4Deep;  // of a block
         a.y_rows = a.ranks > 1 ? rows : 0;
-        const int per_half = q4_smem(tiles_n, columns, 4, 0).bytes - q4_smem(tiles_n, columns, 0, 0).bytes;  // four of them
-        int fits = (kRoom - q4_smem(tiles_n, columns, 0, a.y_rows * a.vectors).bytes) / per_half * 4;
+        const int per_half = q4_smem(tiles_n, bytes, columns, 4, 0).bytes - q4_smem(tiles_n, bytes, columns, 0, 0).bytes;  // four of them
+        int fits = (kRoom - q4_smem(tiles_n, bytes, columns, 0, a.y_rows * a.vectors).bytes) / per_half * 4;
         if (fits < mine) {
             a.y_rows = rows;
-            fits = (kRoom - q4_smem(tiles_n, columns, 0, rows * a.vectors).bytes) / per_half * 4;
+            fits = (kRoom - q4_smem(tiles_n, bytes, columns, 0, rows * a.vectors).bytes) / per_half * 4;
             const int times = (mine + fits - 1) / fits;
             fits = ((mine + times - 1) / times + kQ4Deep - 1) / kQ4Deep * kQ4Deep;
         }
         a.stage_h = std::min(fits, mine);
-        a.warps_k = q4_warps_k(rows, a.stage_h);
-        const int smem = q4_smem(tiles_n, columns, a.stage_h, a.y_rows * a.vectors).bytes;
+        a.warps_k = q4_warps_k(rows, a.stage_h, words ? kQ4Deep : 1);
+        const int smem = q4_smem(tiles_n, bytes, columns, a.stage_h, a.y_rows * a.vectors).bytes;
         const bool zeros = d.zeros != nullptr;
-        const Q4Entry k = tiles_n == 1   ? q4_entry<1>(d.group, zeros, words)
+        const Q4Entry k = bytes          ? q4_entry_bytes(d.group, zeros)
+                          : tiles_n == 1 ? q4_entry<1>(d.group, zeros, words)
                           : tiles_n == 2 ? q4_entry<2>(d.group, zeros, words) : q4_entry<4>(d.group, zeros, words);
         L2D_CUDA_TRY(allow_smem(k.run, 227 * 1024, d.device, *k.smem_set));
         L2D_CUDA_TRY(launch_clusters(k.run, dim3(static_cast<unsigned>(shares * a.ranks)), a.ranks, kQ4Threads, smem, stream, a));
