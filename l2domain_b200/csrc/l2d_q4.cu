@@ -3,35 +3,33 @@
 //   y[b][i] = sum_j s[i][j / g] * (q[i][j] - z[i][j / g]) * x[b][j]
 //
 // Memory bound: a weight is half a byte and is used once per vector.  At the bandwidth of HBM an SM
-// gets about 52 weights a cycle and has 128 lanes to treat them (64 of them for logic), so a weight may
-// cost little over two instructions; a fused multiply-add in fp32 with its conversion would be three or
-// four.  So the products run on matrix instructions, 16 rows of weights as the A operand and the vectors
+// gets about 52 weights a cycle and has 128 lanes to treat them, so a weight may cost little over two
+// instructions; a fused multiply-add in fp32 with its conversion would be three or four.  So the products
+// run on matrix instructions (m16n8k16, fp32 sums), 16 rows of weights as the A operand and the vectors
 // as columns of B, and everything else is arranged to spend next to nothing per weight:
 //
-//  * One vector (two, for groups of 128 and more) is multiplied in integers (m16n8k32, bytes): two masks and
-//    a shift turn eight nibbles into bytes.  x of each 128 columns is a 30-bit integer times a power of
-//    two, in four signed digits of 8 bits, a column of B each.  Sums are exact up to the end of a group;
-//    values of x are exact down to 2^-6 (fp32), 2^-19 (fp16) or 2^-22 (bf16) of the largest among their 128
-//    columns, and otherwise off by at most 2^-30 of it.
-//  * More vectors are multiplied in fp16 with fp32 sums (m16n8k16): one column a vector (two for fp32, 11
-//    bits each, which leaves one rounding of 2^-24).  A nibble masked into the low mantissa bits of an fp16
-//    number is the subnormal q 2^-24, one higher up 16 q 2^-24: both exact, and no instruction but the mask.
-//    x of the columns that end up higher is a sixteenth of itself.  Each 128 columns of a vector are scaled
-//    by a power of two to a largest value just under 2^15; what is below 2^-28 of it may lose bits.
-//  * What the zero point takes away is z times the group's sum of x, which is computed once per block:
-//    sum (q - z) x = sum q x - z sum x.  Infinities and NaNs do not survive that.  They are staged as zeros,
-//    and the threads that store a vector's results add the terms of its infinities and NaNs at the end.
+//  * A nibble masked into the low mantissa bits of a 16-bit float is the subnormal q 2^-24, one higher up
+//    16 q 2^-24: both exact, and no instruction but the mask.  x of the columns that end up higher is a
+//    sixteenth of itself.  What the zero point takes away is z times the group's sum of x, which is
+//    computed once per block: sum (q - z) x = sum q x - z sum x, in fp32.
+//  * x is held in shared memory as fp16, each 128 columns of a vector scaled by a power of two to a
+//    largest value just under 2^15, in one part (fp16 and bf16) or two (fp32: 11 bits, and the next 11 as a
+//    column of their own).  That keeps fp16 and bf16 exact and fp32 to one rounding of 2^-24 for values
+//    down to 2^-28 of the largest among its 128 columns; smaller ones are off by up to 2^-36 of the largest.
+//  * Infinities and NaNs do not survive sum q x - z sum x.  They are staged as zeros, and the threads that
+//    store a vector's results add the terms of its infinities and NaNs at the end, one by one.
 //  * The scales are applied to the fp32 sums of each group.  One instruction sums over the four lanes of a
 //    row, 128 columns; where groups are shorter, x of the different groups goes to different columns of B
 //    (zeros elsewhere), so that each group still has a sum of its own: S = 128 / group columns per part.
 //  * A lane's 16 bytes (32 columns of one row) are loaded straight into registers from the row-major
-//    weights, a step of 512 columns ahead, in code without branches.  A product's order of columns is free,
-//    so nibbles are used in the order in which masks deliver them, and x is put into that order when it is
-//    staged.  A request for eight rows occupies the L1 for eight cycles whatever its width, so the scales of
-//    a whole step are loaded as one word per row.
+//    weights, a chunk ahead.  A product's order of columns is free, so nibbles are used in the order in
+//    which masks deliver them, and x is put into that order when it is staged.
 //  * A block's rows are its even share of M, in tiles of at most 16 rows of nearly equal size, so that
 //    blocks finish together whatever M is; groups of its warps take a tile each, split its columns and
-//    meet in shared memory at its end, in a fixed order.
+//    meet in shared memory at its end, in a fixed order.  Where a block has
+//    few rows, staging all of x for them would cost as much as their weights: a cluster of blocks then
+//    takes more rows together, each block a share of the columns, and adds its sums over distributed
+//    shared memory, in rank order.
 #include "l2d_launch.cuh"
 
 #include <cooperative_groups.h>
@@ -54,6 +52,7 @@ struct Q4Args {
     int ranks;       // blocks of a cluster, which split the columns
     int stage_h;     // halves of 128 columns of x staged at a time
     int y_rows;      // rows of the block's sums kept (0: one staging and no cluster)
+    int wide;        // scales and zeros of a step as one word
     uint64_t per_group;  // ceil(2^40 / (group / 128)): a half's group without a division
 };
 
@@ -157,7 +156,7 @@ struct Q4Part {
 template <int S, bool ZEROS>
 struct Q4Scales {
     uint32_t s[2][S > 1 ? 4 : 2];
-    uint32_t z[2][!ZEROS || S == 1 ? 1 : S == 4 ? 4 : 2];
+    uint32_t z[2][!ZEROS ? 1 : S == 4 ? 4 : 2];
     int from;  // S = 0: the first half whose scale is the last one's
 };
 
@@ -278,7 +277,7 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
 #pragma unroll
             for (int e = 0; e < E; ++e) s[r][e] = scale_value(word, S == 1 ? h & 1 : e, is_half);
             uint32_t zeros = 0;
-            if constexpr (ZEROS) zeros = S == 0 ? (second ? q.z[r][1] : q.z[r][0]) : S == 1 ? q.z[r][0] >> (8 * h) : S == 2 ? q.z[r][h / 2] >> (16 * (h & 1)) : q.z[r][h];
+            if constexpr (ZEROS) zeros = S == 0 ? (second ? q.z[r][1] : q.z[r][0]) : S == 1 ? q.z[r][h / 2] >> (8 * (h & 1)) : S == 2 ? q.z[r][h / 2] >> (16 * (h & 1)) : q.z[r][h];
 #pragma unroll
             for (int e = 0; e < E; ++e) z[r][e] = ZEROS ? static_cast<float>(zeros >> (8 * e) & 15) : 8.0f;
         }
@@ -319,15 +318,32 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
                 q.s[r][1] = __ldg(reinterpret_cast<const uint16_t *>(at.s[r]) + last);
                 if constexpr (ZEROS) q.z[r][0] = __ldg(at.z[r] + first), q.z[r][1] = __ldg(at.z[r] + last);
             } else if constexpr (S == 1) {
-                const uint2 v = __ldg(reinterpret_cast<const uint2 *>(at.s[r]));
-                q.s[r][0] = v.x, q.s[r][1] = v.y;
-                if constexpr (ZEROS) q.z[r][0] = __ldg(reinterpret_cast<const uint32_t *>(at.z[r]));
-            } else if constexpr (S == 2) {
-                const uint4 v = __ldg(reinterpret_cast<const uint4 *>(at.s[r]));
-                q.s[r][0] = v.x, q.s[r][1] = v.y, q.s[r][2] = v.z, q.s[r][3] = v.w;
+                if (a.wide) {
+                    const uint2 v = __ldg(reinterpret_cast<const uint2 *>(at.s[r]));
+                    q.s[r][0] = v.x, q.s[r][1] = v.y;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) q.s[r][i] = __ldg(reinterpret_cast<const uint32_t *>(at.s[r]) + i);
+                }
                 if constexpr (ZEROS) {
-                    const uint2 u = __ldg(reinterpret_cast<const uint2 *>(at.z[r]));
-                    q.z[r][0] = u.x, q.z[r][1] = u.y;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) q.z[r][i] = __ldg(reinterpret_cast<const uint16_t *>(at.z[r]) + i);
+                }
+            } else if constexpr (S == 2) {
+                if (a.wide) {
+                    const uint4 v = __ldg(reinterpret_cast<const uint4 *>(at.s[r]));
+                    q.s[r][0] = v.x, q.s[r][1] = v.y, q.s[r][2] = v.z, q.s[r][3] = v.w;
+                    if constexpr (ZEROS) {
+                        const uint2 u = __ldg(reinterpret_cast<const uint2 *>(at.z[r]));
+                        q.z[r][0] = u.x, q.z[r][1] = u.y;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint2 v = __ldg(reinterpret_cast<const uint2 *>(at.s[r]) + i);
+                        q.s[r][2 * i] = v.x, q.s[r][2 * i + 1] = v.y;
+                        if constexpr (ZEROS) q.z[r][i] = __ldg(reinterpret_cast<const uint32_t *>(at.z[r]) + i);
+                    }
                 }
             } else {
 #pragma unroll
@@ -377,36 +393,45 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
     auto stage = [&](int kb) {
         bool any_odd = false;
         const int first = h_lo + kb * a.stage_h, halves = min(h_hi - first, a.stage_h);
-        const int u = lane & 15;
-        for (int e = warp * 2 + (lane >> 4); e - (lane >> 4) < halves * a.vectors; e += kQ4Warps * 2) {
-            const bool real = e < halves * a.vectors;
-            const int v = real ? e / halves : 0, half = real ? e - v * halves : 0, col = (first + half) * kQ4Half + 8 * u;
-            float f[8];
-            const int eb = a.dtype_x == L2D_F32 ? 4 : 2;
-            const char *src = static_cast<const char *>(a.x) + (v * a.stride_x + col) * eb;
-            uint32_t raw[8];
+        const int u = lane & 15, units = halves * a.vectors;
+        // Eight columns of x as stored: 16 bytes, or 32 of fp32.
+        struct Raw {
+            uint4 lo, hi;
+        };
+        auto fetch = [&](int e) {
+            Raw r = {};
+            if (e >= units) return r;
+            const int v = e / halves, col = (first + e - v * halves) * kQ4Half + 8 * u, size = a.dtype_x == L2D_F32 ? 4 : 2;
+            const char *src = static_cast<const char *>(a.x) + (v * a.stride_x + col) * size;
             if (col + 8 <= a.N && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-                const uint4 q = *reinterpret_cast<const uint4 *>(src);
-                if (a.dtype_x == L2D_F32) {
-                    const uint4 r = *reinterpret_cast<const uint4 *>(src + 16);
-                    raw[0] = q.x, raw[1] = q.y, raw[2] = q.z, raw[3] = q.w, raw[4] = r.x, raw[5] = r.y, raw[6] = r.z, raw[7] = r.w;
-                } else {
-                    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) raw[i] = w[i >> 1] >> (16 * (i & 1)) & 0xffff;
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    raw[i] = col + i >= a.N ? 0
-                             : a.dtype_x == L2D_F32 ? reinterpret_cast<const uint32_t *>(src)[i] : reinterpret_cast<const uint16_t *>(src)[i];
+                r.lo = __ldg(reinterpret_cast<const uint4 *>(src));
+                if (size == 4) r.hi = __ldg(reinterpret_cast<const uint4 *>(src) + 1);
+                return r;
             }
+            uint32_t w[8] = {};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (col + i >= a.N) continue;
+                if (size == 4) w[i] = __ldg(reinterpret_cast<const uint32_t *>(src) + i);
+                else w[i / 2] |= static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t *>(src) + i)) << (16 * (i & 1));
+            }
+            r.lo = make_uint4(w[0], w[1], w[2], w[3]);
+            r.hi = make_uint4(w[4], w[5], w[6], w[7]);
+            return r;
+        };
+        Raw ahead = fetch(warp * 2 + (lane >> 4));
+        for (int e = warp * 2 + (lane >> 4); e - (lane >> 4) < units; e += kQ4Warps * 2) {
+            const Raw r = ahead;
+            ahead = fetch(e + kQ4Warps * 2);
+            const bool real = e < units;
+            const int v = real ? e / halves : 0, half = real ? e - v * halves : 0;
+            const uint32_t raw[8] = {r.lo.x, r.lo.y, r.lo.z, r.lo.w, r.hi.x, r.hi.y, r.hi.z, r.hi.w};
+            float f[8];
             uint32_t top = 0;
             bool odd_ones = false;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                f[i] = a.dtype_x == L2D_F16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(raw[i])))
-                                            : __uint_as_float(a.dtype_x == L2D_F32 ? raw[i] : raw[i] << 16);
+                f[i] = a.dtype_x == L2D_F32 ? __uint_as_float(raw[i]) : scale_value(raw[i / 2], i & 1, a.dtype_x == L2D_F16);
                 const uint32_t m = __float_as_uint(f[i]) & 0x7fffffffu;
                 if (m < 0x7f800000u) top = max(top, m);
                 else f[i] = 0.0f, odd_ones = true;
@@ -652,22 +677,62 @@ __global__ void k_q4_zero(Q4Args a) {
         dev::store_as(a.y, a.dtype_y, e / a.M * a.stride_y + e % a.M, 0.0f);
 }
 
-// Blocks of a cluster: as many as it takes for a block's weights to outweigh its x four to one, if there are
-// columns for them.
-int q4_ranks(int64_t M, int steps, int columns, int sms) {
-    (void)M, (void)columns, (void)sms;
-    return 1;
+// How many clusters of 1, 2, 4 and 8 blocks of one SM each run at the same time; looked up once per device.
+int q4_clusters(int device, const Q4Entry &k, const int **clusters) {
+    static int known[kMaxDevices][4];
+    static std::atomic<bool> done[kMaxDevices];
+    if (!done[device].load(std::memory_order_acquire)) {
+        int found[4];
+        for (int i = 0; i < 4; ++i) {
+            cudaLaunchConfig_t cfg = {};
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = 1u << i;
+            attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+            cfg.gridDim = dim3(1u << i);
+            cfg.blockDim = dim3(kQ4Threads);
+            cfg.dynamicSmemBytes = 200 * 1024;
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            L2D_CUDA_TRY(cudaOccupancyMaxActiveClusters(&found[i], k.run, &cfg));
+        }
+        std::copy(found, found + 4, known[device]);  // the same for every thread that gets here
+        done[device].store(true, std::memory_order_release);
+    }
+    *clusters = known[device];
+    return L2D_OK;
 }
 
-// Warps that share a tile: the number that gives the least work for each (a tile's end counts two halves).
-int q4_warps_k(int rows, int halves, int deep) {
-    int best = 1;
-    int64_t least = INT64_MAX;
-    for (int wk = 1; wk <= kQ4Warps; wk *= 2) {
-        const int groups = kQ4Warps / wk, each = (rows + groups - 1) / groups, steps = halves / deep;
-        const int64_t share = (steps + wk - 1) / wk * deep + (halves % deep + wk - 1) / wk;
-        const int64_t work = int64_t((each + kQ4Rows - 1) / kQ4Rows) * (share + 2);
-        if (work < least) least = work, best = wk;
+// Blocks of a cluster and warps of a tile: the choice that gives a warp the least to do, in units of 128 columns
+// of a tile of fp16 products in one n-tile (105 warp instructions).  Measured with every choice forced on nine
+// shapes of 360 x 171 to 28672 x 8192 and 1 to 16 vectors: this picks the fastest of them or one within 10 %.
+struct Q4Shape {
+    int ranks, warps_k, rows;
+    int64_t shares;
+};
+Q4Shape q4_shape(int64_t M, int halves, int vectors, int tiles_n, bool bytes, int deep, const int *clusters) {
+    constexpr double kStage = 2.4;    // 128 columns of two vectors staged
+    constexpr double kCluster = 2.4;  // two barriers and the sums' way over distributed shared memory
+    constexpr double kEnd = 2.0;      // a tile's end
+    const double unit = bytes ? 0.6 : tiles_n == 1 ? 1.0 : tiles_n == 2 ? 1.5 : 2.4;
+    Q4Shape best = {};
+    double least = 1e300;
+    for (int i = 0; i < 4; ++i) {
+        const int ranks = 1 << i, steps = (halves + kQ4Deep - 1) / kQ4Deep;
+        if (ranks > steps || (i && clusters[i] < 1)) break;
+        const int64_t shares = std::max<int64_t>(std::min<int64_t>(M, std::max(1, clusters[i])), (M + kQ4MaxRows - 1) / kQ4MaxRows);
+        const int rows = static_cast<int>((M + shares - 1) / shares), mine = std::min(halves, (steps + ranks - 1) / ranks * kQ4Deep);
+        const double stage = (int64_t(mine) * vectors + 2 * kQ4Warps - 1) / (2 * kQ4Warps) * kStage + (i ? kCluster : 0.0);
+        for (int wk = 1; wk <= kQ4Warps; wk *= 2) {
+            const int groups = kQ4Warps / wk, each = (rows + groups - 1) / groups;
+            const int share = (mine / deep + wk - 1) / wk * deep + (mine % deep + wk - 1) / wk;
+            const int64_t waves = (shares + std::max(1, clusters[i]) - 1) / std::max(1, clusters[i]);
+            const double work = waves * (stage + ((each + kQ4Rows - 1) / kQ4Rows) * (share * unit + kEnd));
+            if (work < least) {
+                least = work;
+                best = {ranks, wk, rows, shares};
+            }
+        }
     }
     return best;
 }
@@ -727,9 +792,11 @@ int l2d_q4_gemv(const l2d_q4_desc *desc, const void *x, int64_t stride_x, void *
     a.dtype_y = d.dtype_y;
     a.dtype_s = d.dtype_s;
     a.per_group = ((uint64_t(1) << 40) + d.group / 128 - 1) / std::max(d.group / 128, 1);
-    const int word = d.group == 32 ? 2 : d.group == 64 ? 8 : d.group == 128 ? 4 : 1;  // scales that are read together
-    const bool words = !misaligned(d.W, 16) && ldw % 16 == 0 && d.dtype_s != L2D_F32 && lds % word == 0 &&
-                       !misaligned(d.scales, 2 * word) && !misaligned(d.zeros, word);
+    // Scales that are read together: at least `word` of them, and twice as many where they are aligned to that.
+    const int word = d.group == 32 ? 2 : d.group == 64 ? 4 : d.group == 128 ? 2 : 1;
+    auto together = [&](int n) { return lds % n == 0 && !misaligned(d.scales, 2 * n) && !misaligned(d.zeros, n); };
+    const bool words = !misaligned(d.W, 16) && ldw % 16 == 0 && d.dtype_s != L2D_F32 && together(word);
+    a.wide = together(2 * word);
     const int sub = d.group == 32 ? 4 : d.group == 64 ? 2 : 1;
     const bool bytes = words && vectors * sub <= 2;
     a.parts = bytes ? 4 : d.dtype_x == L2D_F32 ? 2 : 1;
@@ -746,9 +813,18 @@ int l2d_q4_gemv(const l2d_q4_desc *desc, const void *x, int64_t stride_x, void *
         }
         const int tiles_n = a.vectors * each <= 8 ? 1 : a.vectors * each <= 16 ? 2 : 4;
         const int columns = a.vectors * a.parts;
-        a.ranks = q4_ranks(d.M, halves / kQ4Deep, columns, sms);
-        const int64_t shares = std::max<int64_t>(std::min<int64_t>(d.M, std::max(1, sms / a.ranks)), (d.M + kQ4MaxRows - 1) / kQ4MaxRows);
-        const int rows = static_cast<int>((d.M + shares - 1) / shares);
+        const bool zeros = d.zeros != nullptr;
+        const Q4Entry k = bytes          ? q4_entry_bytes(d.group, zeros)
+                          : tiles_n == 1 ? q4_entry<1>(d.group, zeros, words)
+                          : tiles_n == 2 ? q4_entry<2>(d.group, zeros, words) : q4_entry<4>(d.group, zeros, words);
+        L2D_CUDA_TRY(allow_smem(k.run, 227 * 1024, d.device, *k.smem_set));
+        const int *clusters = nullptr;
+        const int known = q4_clusters(d.device, k, &clusters);
+        if (known != L2D_OK) return known;
+        const Q4Shape shape = q4_shape(d.M, halves, a.vectors, tiles_n, bytes, words ? kQ4Deep : 1, clusters);
+        a.ranks = shape.ranks;
+        a.warps_k = shape.warps_k;
+        const int rows = shape.rows;
         // x is staged whole where it fits, else in as many parts as it takes.
         constexpr int kRoom = 227 * 1024 - 64;
         const int mine = ((halves + kQ4Deep - 1) / kQ4Deep + a.ranks - 1) / a.ranks * kQ4Deep;  // of a block
@@ -762,14 +838,8 @@ int l2d_q4_gemv(const l2d_q4_desc *desc, const void *x, int64_t stride_x, void *
             fits = ((mine + times - 1) / times + kQ4Deep - 1) / kQ4Deep * kQ4Deep;
         }
         a.stage_h = std::min(fits, mine);
-        a.warps_k = q4_warps_k(rows, a.stage_h, words ? kQ4Deep : 1);
         const int smem = q4_smem(tiles_n, bytes, columns, a.stage_h, a.y_rows * a.vectors).bytes;
-        const bool zeros = d.zeros != nullptr;
-        const Q4Entry k = bytes          ? q4_entry_bytes(d.group, zeros)
-                          : tiles_n == 1 ? q4_entry<1>(d.group, zeros, words)
-                          : tiles_n == 2 ? q4_entry<2>(d.group, zeros, words) : q4_entry<4>(d.group, zeros, words);
-        L2D_CUDA_TRY(allow_smem(k.run, 227 * 1024, d.device, *k.smem_set));
-        L2D_CUDA_TRY(launch_clusters(k.run, dim3(static_cast<unsigned>(shares * a.ranks)), a.ranks, kQ4Threads, smem, stream, a));
+        L2D_CUDA_TRY(launch_clusters(k.run, dim3(static_cast<unsigned>(shape.shares * a.ranks)), a.ranks, kQ4Threads, smem, stream, a));
     }
     return L2D_OK;
 }
