@@ -371,7 +371,8 @@ L2D_API int l2d_pool_release(int device);
 enum {
     L2D_KV_BAD_PAGE = 1,    /* a page number outside [0, num_pages), a position or length past the page
                                table, or a sequence outside it */
-    L2D_KV_BAD_POSITION = 2 /* a position past the rotation tables */
+    L2D_KV_BAD_POSITION = 2, /* a position past the rotation tables */
+    L2D_KV_TIMEOUT = 4       /* a wait inside the attention ran out of time (never expected): the output is not valid */
 };
 
 /* Matrix-vector products with 4-bit weights and group scales.

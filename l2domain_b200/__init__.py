@@ -584,7 +584,7 @@ class PeerShard:
 # Decoding operators: 4-bit weights, the paged cache, attention over it
 # --------------------------------------------------------------------------------------------
 
-KV_BAD_PAGE, KV_BAD_POSITION = 1, 2
+KV_BAD_PAGE, KV_BAD_POSITION, KV_TIMEOUT = 1, 2, 4
 
 
 class Q4Matrix:

@@ -2,6 +2,8 @@
 // token per sequence over it (l2d_attn_*).
 #include "l2d_launch.cuh"
 
+#include <cuda.h>
+
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -104,10 +106,13 @@ __global__ void __launch_bounds__(256) k_append(AppendArgs a) {
 //
 // Memory bound: each key and value is read once, for all query heads of its group.  A block of four
 // warps works on one key-value head of one sequence at a time; each warp streams its own 16 keys of
-// every 64 through a ring of shared memory of its own (asynchronous copies, no block-wide barrier in
-// the loop) and keeps a running maximum and sum per query head, so the data is passed over once.
-// 16-bit caches feed matrix instructions with the query heads as the 16 rows; 32-bit caches use fp32
-// fused multiply-adds.
+// every 64 through a ring of shared memory of its own (no block-wide barrier in the loop) and keeps a
+// running maximum and sum per query head, so the data is passed over once.  16-bit caches feed matrix
+// instructions with the query heads as the 16 rows; 32-bit caches use fp32 fused multiply-adds.
+//
+// A tile of 16 keys that lies in one page is one box of a tensor map over the cache (elements, heads,
+// slots, pages), and one thread starts its copies; with a page size that is no multiple of 16, or rows off
+// 16-byte boundaries, the lanes look up the page of each key and copy its rows themselves.
 //
 // The tiles of all sequences and heads form one line that is cut into equal pieces, one per resident
 // block, whatever the lengths are: a long sequence is split over many blocks and a block may take
@@ -139,6 +144,32 @@ __device__ __forceinline__ void copies_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+// A box of a tensor map to shared memory, counted by a barrier there.
+__device__ __forceinline__ void copy_box(uint32_t dst, const CUtensorMap *map, int x, int head, int slot, int page, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+                 "l"(map), "r"(x), "r"(head), "r"(slot), "r"(page), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void barrier_init(uint32_t bar) { asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void barrier_expect(uint32_t bar, int bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// Waits for the barrier's phase of this parity; false if it does not come in some seconds.
+__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity) {
+    uint32_t done = 0;
+    for (int i = 0; i < (1 << 22) && !done; ++i)
+        asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    return done;
+}
+// What this thread did to shared memory comes before copies of boxes that are started after the next barrier.
+__device__ __forceinline__ void before_boxes() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Rows of keys and values in shared memory: boxes of 128 bytes a row, 16-byte chunks exchanged by the row
+// (chunk ^ row, as the tensor map's 128-byte swizzle has it), so that eight rows' chunks meet all banks.
+template <int ROWS>
+__device__ __forceinline__ int chunk_at(int row, int chunk) {
+    return (chunk >> 3) * (ROWS * 128) + row * 128 + (((chunk ^ row) & 7) << 4);
+}
+
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -158,13 +189,13 @@ template <typename T>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
 template <>
 __device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 template <>
 __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -191,8 +222,9 @@ struct MmaCore {
     static constexpr int kKeys = 16;                       // keys of a warp's tile
     static constexpr int kRows = SPLIT ? 8 : 16;           // query heads
     static constexpr int kDim = KS * 16;                   // head_dim, padded
-    static constexpr int kChunks = KS * 2;                 // 16-byte chunks of a row
-    static constexpr int kPitch = (kChunks + 1) * 16;      // an odd number of chunks: eight rows meet all banks
+    static constexpr int kBoxes = (KS + 3) / 4;            // of 64 elements
+    static constexpr int kChunks = kBoxes * 8;             // 16-byte chunks of a row, padding included
+    static constexpr int kPitch = (KS * 2 + 1) * 16;       // of queries: an odd number of chunks
     static constexpr bool kQueryInSmem = !SPLIT && KS > 8; // registers would not hold queries and sums
     static constexpr int kQueryBytes = kRows * kPitch;
     static constexpr int kWarpBytes = 0;
@@ -200,20 +232,22 @@ struct MmaCore {
     float o[2 * KS][4], m[2], l[2];
     uint32_t query;
 
-    // q: this group's first head; `heads` rows are real.  All threads of the block call it.
-    __device__ __forceinline__ void begin(const T *q, int heads, int D, bool aligned, char *smem_q, char *) {
+    // q: this group's first head; `heads` rows are real, `flip` takes their negatives.  All threads of the block call it.
+    __device__ __forceinline__ void begin(const T *q, int heads, int D, bool aligned, bool flip, char *smem_q, char *) {
         const int lane = threadIdx.x & 31;
+        const uint32_t sign = flip ? 0x80008000u : 0u;
         if (aligned) {
-            for (int e = threadIdx.x; e < kRows * kChunks; e += kAttnThreads) {
-                const int r = e / kChunks, ch = e - r * kChunks;
+            for (int e = threadIdx.x; e < kRows * KS * 2; e += kAttnThreads) {
+                const int r = e / (KS * 2), ch = e - r * (KS * 2);
                 uint4 x = make_uint4(0, 0, 0, 0);
                 if (r < heads && ch * 8 < D) x = *reinterpret_cast<const uint4 *>(q + r * D + ch * 8);
-                *reinterpret_cast<uint4 *>(smem_q + r * kPitch + ch * 16) = x;
+                *reinterpret_cast<uint4 *>(smem_q + r * kPitch + ch * 16) = make_uint4(x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign);
             }
         } else {
             for (int e = threadIdx.x; e < kRows * kDim; e += kAttnThreads) {
                 const int r = e / kDim, i = e - r * kDim;
-                reinterpret_cast<T *>(smem_q + r * kPitch)[i] = r < heads && i < D ? q[r * D + i] : dev::narrow<T>(0.0f);
+                const uint16_t x = r < heads && i < D ? reinterpret_cast<const uint16_t *>(q)[r * D + i] : 0;
+                reinterpret_cast<uint16_t *>(smem_q + r * kPitch)[i] = static_cast<uint16_t>(x ^ sign);
             }
         }
         __syncthreads();
@@ -222,7 +256,7 @@ struct MmaCore {
             uint32_t r[4];
 #pragma unroll
             for (int k = 0; k < KS; k += 2) {
-                ldmatrix4(r, query + (lane & 7) * kPitch + min(2 * k + (lane >> 3), kChunks - 1) * 16);
+                ldmatrix4(r, query + (lane & 7) * kPitch + min(2 * k + (lane >> 3), KS * 2 - 1) * 16);
                 qa[k][0] = r[0];
                 qa[k][1] = r[1];
                 if (k + 1 < KS) {
@@ -247,11 +281,12 @@ struct MmaCore {
         ldmatrix4(a, query + (((lane >> 3) & 1) * 8 + (lane & 7)) * kPitch + (lane >> 4) * 16 + k * 32);
     }
 
-    // One tile: keys at ks, values at vs (shared memory), bit j of live: key j counts.
+    // One tile: keys at ks, values at vs (shared memory), bit j of live: key j counts.  scale2 > 0.
     __device__ __forceinline__ void step(const char *ks, const char *vs, uint32_t live, float scale2) {
         const int lane = threadIdx.x & 31, t = lane & 3;
-        const uint32_t ka = smem_addr(ks) + ((lane >> 4) * 8 + (lane & 7)) * kPitch + ((lane >> 3) & 1) * 16;
-        const uint32_t va = smem_addr(vs) + (((lane >> 3) & 1) * 8 + (lane & 7)) * kPitch + (lane >> 4) * 16;
+        // Chunk 2k + hi of row r is at chunk_at(r, hi) ^ (2k & 7) * 16, in box k / 4.
+        const uint32_t ka = smem_addr(ks) + chunk_at<kKeys>((lane >> 4) * 8 + (lane & 7), (lane >> 3) & 1);
+        const uint32_t va = smem_addr(vs) + chunk_at<kKeys>(((lane >> 3) & 1) * 8 + (lane & 7), lane >> 4);
         float s[2][4] = {};
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
@@ -267,24 +302,25 @@ struct MmaCore {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) a[e] = qa[k][e];
             }
-            ldmatrix4(b, ka + k * 32);
+            ldmatrix4(b, (ka ^ ((2 * k & 7) << 4)) + (k / 4) * (kKeys * 128));
             mma16816<T>(s[0], a, b[0], b[1]);
             mma16816<T>(s[1], a, b[2], b[3]);
+        }
+        if (live != (1u << kKeys) - 1) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (!(live >> ((e >> 2) * 8 + 2 * t + (e & 1)) & 1)) s[e >> 2][e & 3] = -INFINITY;
         }
         uint32_t p[4];
 #pragma unroll
         for (int r = 0; r < (SPLIT ? 1 : 2); ++r) {
-            float x[4], top = -INFINITY;
-            bool ok[4];
+            float x[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                ok[e] = live >> ((e >> 1) * 8 + 2 * t + (e & 1)) & 1;
-                x[e] = s[e >> 1][2 * r + (e & 1)];
-                top = fmaxf(top, ok[e] ? x[e] * scale2 : -INFINITY);
-            }
+            for (int e = 0; e < 4; ++e) x[e] = s[e >> 1][2 * r + (e & 1)];
+            float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const float m2 = fmaxf(m[r], top), base = finite_base(m2);
+            const float m2 = fmaxf(m[r], top * scale2), base = finite_base(m2);
             if (__any_sync(0xffffffffu, m2 != m[r])) {
                 const float f = exp2_approx(m[r] - base);
                 l[r] *= f;
@@ -299,24 +335,20 @@ struct MmaCore {
                 }
                 m[r] = m2;
             }
-            T hi[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x[e] = ok[e] ? exp2_approx(fmaf(x[e], scale2, -base)) : 0.0f;
-                l[r] += x[e];
-                hi[e] = dev::narrow<T>(x[e]);
-            }
-            p[r] = pack2(hi[0], hi[1]);
-            p[r + 2] = pack2(hi[2], hi[3]);
-            if constexpr (SPLIT) {
-                p[1] = pack2(dev::narrow<T>(x[0] - dev::widen(hi[0])), dev::narrow<T>(x[1] - dev::widen(hi[1])));
-                p[3] = pack2(dev::narrow<T>(x[2] - dev::widen(hi[2])), dev::narrow<T>(x[3] - dev::widen(hi[3])));
+            for (int e = 0; e < 4; ++e) x[e] = exp2_approx(fmaf(x[e], scale2, -base));
+            l[r] += (x[0] + x[1]) + (x[2] + x[3]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const T a = dev::narrow<T>(x[2 * h]), b = dev::narrow<T>(x[2 * h + 1]);
+                p[r + 2 * h] = pack2(a, b);
+                if constexpr (SPLIT) p[1 + 2 * h] = pack2(dev::narrow<T>(x[2 * h] - dev::widen(a)), dev::narrow<T>(x[2 * h + 1] - dev::widen(b)));
             }
         }
 #pragma unroll
         for (int n = 0; n < KS; ++n) {
             uint32_t b[4];
-            ldmatrix4_trans(b, va + n * 32);
+            ldmatrix4_trans(b, (va ^ ((2 * n & 7) << 4)) + (n / 4) * (kKeys * 128));
             mma16816<T>(o[2 * n], p, b[0], b[1]);
             mma16816<T>(o[2 * n + 1], p, b[2], b[3]);
         }
@@ -352,8 +384,8 @@ struct SimdCore {
     static constexpr int kKeys = DV == 1 ? 16 : 8;
     static constexpr int kRows = GT;
     static constexpr int kDim = DV * 128;
+    static constexpr int kBoxes = kDim / 32;
     static constexpr int kChunks = kDim / 4;
-    static constexpr int kPitch = (kChunks + 1) * 16;
     static constexpr int kQueryBytes = GT * kDim * 4;
     static constexpr int kWarpBytes = GT * kKeys * 4;  // weights of the warp's tile
     static constexpr int kParts = 32 / kKeys;
@@ -362,14 +394,15 @@ struct SimdCore {
     float *weights;
     int chunks;
 
-    __device__ __forceinline__ void begin(const float *q, int heads, int D, bool, char *smem_q, char *warp_smem) {
+    __device__ __forceinline__ void begin(const float *q, int heads, int D, bool, bool flip, char *smem_q, char *warp_smem) {
         float *sq = reinterpret_cast<float *>(smem_q);
         query = sq;
         weights = reinterpret_cast<float *>(warp_smem);
         chunks = (D + 3) / 4;
         for (int e = threadIdx.x; e < GT * kDim; e += kAttnThreads) {
             const int r = e / kDim, i = e - r * kDim;
-            sq[e] = r < heads && i < D ? q[r * D + i] : 0.0f;
+            const float x = r < heads && i < D ? q[r * D + i] : 0.0f;
+            sq[e] = flip ? -x : x;
         }
         __syncthreads();
 #pragma unroll
@@ -386,9 +419,8 @@ struct SimdCore {
     __device__ __forceinline__ void step(const char *ks, const char *vs, uint32_t live, float scale2) {
         const int lane = threadIdx.x & 31, key = lane % kKeys, sub = lane / kKeys;
         float s[GT] = {};
-        const float4 *row = reinterpret_cast<const float4 *>(ks + key * kPitch);
         for (int c = sub; c < chunks; c += kParts) {
-            const float4 k = row[c];
+            const float4 k = *reinterpret_cast<const float4 *>(ks + chunk_at<kKeys>(key, c));
 #pragma unroll
             for (int g = 0; g < GT; ++g) {
                 const float4 q = reinterpret_cast<const float4 *>(query + g * kDim)[c];
@@ -424,7 +456,7 @@ struct SimdCore {
                 if (lane + 32 * v >= chunks) continue;
                 float4 x[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4 *>(vs + (j + i) * kPitch + (lane + 32 * v) * 16);
+                for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4 *>(vs + chunk_at<kKeys>(j + i, lane + 32 * v));
 #pragma unroll
                 for (int g = 0; g < GT; ++g) {
                     const float4 w = *reinterpret_cast<const float4 *>(weights + g * kKeys + j);
@@ -461,11 +493,12 @@ struct SimdCore {
 };
 
 // Shared memory of a block: the rings (reused for the warps' sums at the end of a piece), queries, the
-// cores' own words, row offsets and live bits per stage, maxima and sums.
+// cores' own words, barriers, row offsets and live bits, maxima and sums.
 constexpr int kJoin = 128;  // pieces whose factors are held at a time when a sequence's pieces are joined
 template <typename Core, int STAGES>
 struct AttnSmem {
-    static constexpr int kStage = 2 * Core::kKeys * Core::kPitch;
+    static constexpr int kTile = Core::kKeys * 128 * Core::kBoxes;  // of keys, and of values
+    static constexpr int kStage = 2 * kTile;
     static constexpr int kRing = kAttnWarps * STAGES * kStage;
     static constexpr int kSums = kAttnWarps * Core::kRows * Core::kDim * 4;
     static constexpr int kFactors = kSums;  // behind the sums
@@ -473,35 +506,43 @@ struct AttnSmem {
     static constexpr int kQuery = kRing > kEnd ? kRing : kEnd;
     static constexpr int kWarp = kQuery + Core::kQueryBytes;
     static constexpr int kRowAt = kWarp + kAttnWarps * Core::kWarpBytes;
-    static constexpr int kLive = kRowAt + kAttnWarps * Core::kKeys * 16;
+    static constexpr int kBars = kRowAt + kAttnWarps * Core::kKeys * 16;
+    static constexpr int kLive = kBars + kAttnWarps * STAGES * 8;
     static constexpr int kMl = kLive + kAttnWarps * STAGES * 4;
     static constexpr int kFlag = kMl + kAttnWarps * 2 * kMaxRows * 4;
     static constexpr int kBytes = kFlag + 16;
 };
 
-// A warp's view of the keys of one sequence and head: page lookups run one tile ahead of the copies.
+// How keys and values come to shared memory: as boxes, as 16-byte chunks, or element by element.
+enum { kBoxes = 2, kWords = 1, kElements = 0 };
+
+struct AttnMaps {
+    CUtensorMap k, v;
+};
+
+// A warp's view of the keys of one sequence and head.  Page lookups run one tile ahead of the copies.
 template <typename Core, int STAGES>
 struct Stream {
     using T = typename Core::Elem;
+    using Sm = AttnSmem<Core, STAGES>;
     const Cache &c;
-    const char *k, *v;  // this head's rows
+    const AttnMaps &maps;
+    int how, head;
     const int32_t *table;
     char *ring;
-    longlong2 *row_at;  // where the rows of the tile being started are, in bytes from k and v
+    longlong2 *row_at;    // where the rows of the tile being started are, in bytes from k and v
+    uint32_t bars;
     uint32_t *live;
-    int64_t next;       // the key of lane 0 in the tile whose pages are in `page`
-    int len, step;      // keys of the sequence; keys between this warp's tiles
-    int slot, page;
-    bool aligned;
-
-    __device__ __forceinline__ Stream(const Cache &cache, char *r, longlong2 *ra, uint32_t *lv, bool al)
-        : c(cache), ring(r), row_at(ra), live(lv), aligned(al) {}
+    uint32_t phases;      // parity of each stage's barrier
+    int64_t next;         // the first key of the tile whose pages are in `page`
+    int lo, len, step;    // keys lo .. len - 1 count; keys between this warp's tiles
+    int slot, page;       // of this lane's key; of the tile's first key, with boxes
 
     __device__ __forceinline__ void lookup() {
         const int lane = threadIdx.x & 31;
-        const int64_t key = next + lane;
+        const int64_t key = how == kBoxes ? next : next + lane;
         page = -2;  // no such key
-        if (lane < Core::kKeys && key < len) {
+        if (key < len && (how == kBoxes ? key + Core::kKeys > lo : key >= lo && lane < Core::kKeys)) {
             const unsigned i = static_cast<unsigned>(key) / static_cast<unsigned>(c.page_size);
             slot = static_cast<int>(static_cast<unsigned>(key) - i * static_cast<unsigned>(c.page_size));
             page = max(table[i], -1);
@@ -511,50 +552,98 @@ struct Stream {
     // Starts the copies of the next tile into a stage of the ring.
     __device__ __forceinline__ void issue(int stage) {
         const int lane = threadIdx.x & 31;
+        constexpr uint32_t kAll = (1u << Core::kKeys) - 1;
         const bool real = page >= 0 && page < c.num_pages;
         if (!real && page != -2) report(c.status, L2D_KV_BAD_PAGE);
-        const uint32_t bits = __ballot_sync(0xffffffffu, real);
-        if (lane == 0) live[stage] = bits;
-        if (bits) {
-            constexpr int64_t eb = sizeof(T);
-            __syncwarp();  // the rows of the tile before have been read
-            if (lane < Core::kKeys)
-                row_at[lane] = real ? make_longlong2((page * c.k_page + slot * c.k_slot) * eb, (page * c.v_page + slot * c.v_slot) * eb)
-                                    : make_longlong2(0, 0);
-            __syncwarp();
-            char *dst = ring + stage * AttnSmem<Core, STAGES>::kStage;
-            if (aligned) {
-                const uint32_t to = smem_addr(dst);
-                const int row_bytes = c.head_dim * static_cast<int>(eb);
-#pragma unroll 8
-                for (int e = lane; e < Core::kKeys * Core::kChunks; e += 32) {
-                    const int r = e / Core::kChunks, ch = e - r * Core::kChunks;
-                    const longlong2 at = row_at[r];
-                    const bool in = (bits >> r & 1) && ch * 16 < row_bytes;
-                    const int off = in ? ch * 16 : 0;
-                    copy16(to + r * Core::kPitch + ch * 16, k + at.x + off, in);
-                    copy16(to + (Core::kKeys + r) * Core::kPitch + ch * 16, v + at.y + off, in);
-                }
-            } else {
-                for (int r = 0; r < Core::kKeys; ++r) {
-                    const longlong2 at = row_at[r];
-                    T *kd = reinterpret_cast<T *>(dst + r * Core::kPitch), *vd = reinterpret_cast<T *>(dst + (Core::kKeys + r) * Core::kPitch);
-                    for (int i = lane; i < Core::kDim; i += 32) {
-                        const bool in = (bits >> r & 1) && i < c.head_dim;
-                        kd[i] = in ? reinterpret_cast<const T *>(k + at.x)[i] : dev::narrow<T>(0.0f);
-                        vd[i] = in ? reinterpret_cast<const T *>(v + at.y)[i] : dev::narrow<T>(0.0f);
+        char *tile = ring + stage * Sm::kStage;
+        if (how == kBoxes) {
+            uint32_t bits = 0;
+            if (real) {
+                bits = kAll;
+                if (next < lo) bits &= kAll << (lo - static_cast<int>(next));  // by less than kKeys: lookup()
+                if (next + Core::kKeys > len) bits &= kAll >> (static_cast<int>(next) + Core::kKeys - len);
+            }
+            if (lane == 0) {
+                live[stage] = bits;
+                if (bits) {
+                    const uint32_t bar = bars + 8 * stage, to = smem_addr(tile);
+                    barrier_expect(bar, Sm::kStage);
+#pragma unroll
+                    for (int b = 0; b < Core::kBoxes; ++b) {
+                        const int x = b * (128 / static_cast<int>(sizeof(T)));
+                        copy_box(to + b * Core::kKeys * 128, &maps.k, x, head, slot, page, bar);
+                        copy_box(to + Sm::kTile + b * Core::kKeys * 128, &maps.v, x, head, slot, page, bar);
                     }
                 }
             }
+        } else {
+            const uint32_t bits = __ballot_sync(0xffffffffu, real);
+            if (lane == 0) live[stage] = bits;
+            if (bits) {
+                constexpr int64_t eb = sizeof(T);
+                __syncwarp();  // the rows of the tile before have been read
+                if (lane < Core::kKeys)
+                    row_at[lane] = real ? make_longlong2((page * c.k_page + slot * c.k_slot + head * c.k_head) * eb,
+                                                         (page * c.v_page + slot * c.v_slot + head * c.v_head) * eb)
+                                        : make_longlong2(0, 0);
+                __syncwarp();
+                const uint32_t to = smem_addr(tile);
+                const int row_bytes = c.head_dim * static_cast<int>(eb);
+                if (how == kWords) {
+#pragma unroll 4
+                    for (int e = lane; e < Core::kKeys * Core::kChunks; e += 32) {
+                        const int r = e / Core::kChunks, ch = e - r * Core::kChunks;
+                        const longlong2 at = row_at[r];
+                        const bool in = (bits >> r & 1) && ch * 16 < row_bytes;
+                        const int off = in ? ch * 16 : 0;
+                        copy16(to + chunk_at<Core::kKeys>(r, ch), c.k + at.x + off, in);
+                        copy16(to + Sm::kTile + chunk_at<Core::kKeys>(r, ch), c.v + at.y + off, in);
+                    }
+                } else {
+                    constexpr int kPer = 16 / static_cast<int>(sizeof(T));
+                    for (int r = 0; r < Core::kKeys; ++r) {
+                        const longlong2 at = row_at[r];
+                        for (int i = lane; i < Core::kChunks * kPer; i += 32) {
+                            const bool in = (bits >> r & 1) && i < c.head_dim;
+                            const int dst = chunk_at<Core::kKeys>(r, i / kPer) + i % kPer * static_cast<int>(eb);
+                            *reinterpret_cast<T *>(tile + dst) = in ? reinterpret_cast<const T *>(c.k + at.x)[i] : dev::narrow<T>(0.0f);
+                            *reinterpret_cast<T *>(tile + Sm::kTile + dst) = in ? reinterpret_cast<const T *>(c.v + at.y)[i] : dev::narrow<T>(0.0f);
+                        }
+                    }
+                }
+            }
+            copies_commit();
         }
-        copies_commit();
         next += step;
         lookup();
+    }
+
+    // The live bits of a stage, once its copies are there.  Values of keys that do not count are made zeros, as
+    // their weights are: slots that were never written may hold anything.
+    __device__ __forceinline__ uint32_t take(int stage) {
+        if (how != kBoxes) copies_wait<STAGES - 2>();
+        __syncwarp();
+        const uint32_t bits = live[stage];
+        if (how == kBoxes && bits) {
+            if (!barrier_wait(bars + 8 * stage, phases >> stage & 1)) report(c.status, L2D_KV_TIMEOUT);
+            phases ^= 1u << stage;
+            if (bits != (1u << Core::kKeys) - 1) {
+                char *values = ring + stage * Sm::kStage + Sm::kTile;
+                for (int r = 0; r < Core::kKeys; ++r)
+                    if (!(bits >> r & 1))
+                        for (int ch = threadIdx.x & 31; ch < Core::kChunks; ch += 32)
+                            *reinterpret_cast<uint4 *>(values + chunk_at<Core::kKeys>(r, ch)) = make_uint4(0, 0, 0, 0);
+                before_boxes();
+                __syncwarp();
+            }
+        }
+        return bits;
     }
 };
 
 struct Span {
-    int lo, len, tiles;
+    int lo, len;      // the keys that count
+    int from, tiles;  // tiles from a multiple of their size on
 };
 
 template <int TILE>
@@ -563,7 +652,8 @@ __device__ __forceinline__ Span span_of(const AttnArgs &a, int b) {
     const int room = a.c.table_width * a.c.page_size;  // below 2^31
     s.len = min(max(a.lens[b], 0), room);
     s.lo = a.window && s.len > a.window ? s.len - a.window : 0;
-    s.tiles = (s.len - s.lo) / TILE + ((s.len - s.lo) % TILE != 0);
+    s.from = s.lo & ~(TILE - 1);
+    s.tiles = s.len > s.lo ? (s.len - s.from) / TILE + ((s.len - s.from) % TILE != 0) : 0;
     return s;
 }
 
@@ -657,11 +747,11 @@ __device__ __forceinline__ void join(const AttnArgs &a, const AttnScratch &sc, i
 }
 
 template <typename Core, int STAGES>
-__global__ void __launch_bounds__(kAttnThreads) k_attn(AttnArgs a, AttnScratch sc, int m_tiles, int least, bool aligned, bool q_aligned) {
+__global__ void __launch_bounds__(kAttnThreads) k_attn(const __grid_constant__ AttnArgs a, const __grid_constant__ AttnMaps maps, AttnScratch sc, int m_tiles, int least, int how, bool q_aligned) {
     using T = typename Core::Elem;
     using Sm = AttnSmem<Core, STAGES>;
     constexpr int TILE = kAttnWarps * Core::kKeys;
-    extern __shared__ __align__(16) char smem[];
+    extern __shared__ __align__(1024) char smem[];
     float *sm_m = reinterpret_cast<float *>(smem + Sm::kMl), *sm_l = sm_m + kAttnWarps * kMaxRows;
     int *flag = reinterpret_cast<int *>(smem + Sm::kFlag);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -670,9 +760,17 @@ __global__ void __launch_bounds__(kAttnThreads) k_attn(AttnArgs a, AttnScratch s
 
     // All tiles of one head, and rows without a position.
     int64_t total = 0;
-    for (int b = lane; b < a.batch; b += 32) total += span_of<TILE>(a, b).tiles;
+    int longest = 0;
+    for (int b = lane; b < a.batch; b += 32) {
+        const int n = span_of<TILE>(a, b).tiles;
+        total += n;
+        longest = max(longest, n);
+    }
 #pragma unroll
-    for (int d = 16; d; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+    for (int d = 16; d; d >>= 1) {
+        total += __shfl_xor_sync(0xffffffffu, total, d);
+        longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, d));
+    }
     for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
         if (tid == 0 && a.lens[b] > a.c.table_width * a.c.page_size) report(a.c.status, L2D_KV_BAD_PAGE);
         if (span_of<TILE>(a, b).tiles) continue;
@@ -683,7 +781,7 @@ __global__ void __launch_bounds__(kAttnThreads) k_attn(AttnArgs a, AttnScratch s
 
     // This block's piece of the line of tiles, and the sequence it starts in (every warp looks for itself).
     total *= items;
-    const int64_t per = max(quotient(total + gridDim.x - 1, gridDim.x), static_cast<int64_t>(least));
+    const int64_t per = max(quotient(total + gridDim.x - 1, gridDim.x), static_cast<int64_t>(min(least, longest)));
     int64_t u = blockIdx.x * per;
     const int64_t first_unit = u, stop = min(total, u + per);
     if (u >= stop) return;
@@ -708,9 +806,16 @@ __global__ void __launch_bounds__(kAttnThreads) k_attn(AttnArgs a, AttnScratch s
         before = __shfl_sync(0xffffffffu, upto, 31);
     }
 
-    const float scale2 = a.scale * 1.4426950408889634f;
-    Stream<Core, STAGES> in(a.c, smem + warp * STAGES * Sm::kStage, reinterpret_cast<longlong2 *>(smem + Sm::kRowAt) + warp * Core::kKeys,
-                            reinterpret_cast<uint32_t *>(smem + Sm::kLive) + warp * STAGES, aligned);
+    const float scale2 = fabsf(a.scale) * 1.4426950408889634f;  // a negative one turns the queries' signs
+    Stream<Core, STAGES> in{a.c, maps, how};
+    in.ring = smem + warp * STAGES * Sm::kStage;
+    in.row_at = reinterpret_cast<longlong2 *>(smem + Sm::kRowAt) + warp * Core::kKeys;
+    in.bars = smem_addr(smem + Sm::kBars) + warp * STAGES * 8;
+    in.live = reinterpret_cast<uint32_t *>(smem + Sm::kLive) + warp * STAGES;
+    in.phases = 0;
+    if (lane < STAGES) barrier_init(in.bars + 8 * lane);
+    before_boxes();
+    __syncwarp();
     Core core;
     while (u < stop) {
         const Span s = span_of<TILE>(a, b);
@@ -726,26 +831,24 @@ __global__ void __launch_bounds__(kAttnThreads) k_attn(AttnArgs a, AttnScratch s
         const int hk = item / m_tiles, row0 = (item - hk * m_tiles) * Core::kRows, rows = min(G - row0, Core::kRows);
         const int head0 = hk * G + row0;
 
-        in.k = a.c.k + hk * a.c.k_head * static_cast<int64_t>(sizeof(T));
-        in.v = a.c.v + hk * a.c.v_head * static_cast<int64_t>(sizeof(T));
+        in.head = hk;
         in.table = a.c.table + b * a.c.table_stride;
-        in.len = static_cast<int>(min(static_cast<int64_t>(s.len), s.lo + static_cast<int64_t>(t0 + n) * TILE));
-        in.next = s.lo + static_cast<int64_t>(t0) * TILE + warp * Core::kKeys;
+        in.lo = s.lo;
+        in.len = static_cast<int>(min(static_cast<int64_t>(s.len), s.from + static_cast<int64_t>(t0 + n) * TILE));
+        in.next = s.from + static_cast<int64_t>(t0) * TILE + warp * Core::kKeys;
         in.step = TILE;
         in.lookup();
 #pragma unroll 1
         for (int i = 0; i < STAGES - 1; ++i) in.issue(i);
-        core.begin(static_cast<const T *>(a.q) + b * a.q_token + static_cast<int64_t>(head0) * D, rows, D, q_aligned, smem + Sm::kQuery,
+        core.begin(static_cast<const T *>(a.q) + b * a.q_token + static_cast<int64_t>(head0) * D, rows, D, q_aligned, a.scale < 0.0f, smem + Sm::kQuery,
                    smem + Sm::kWarp + warp * Core::kWarpBytes);
         int stage = 0;
 #pragma unroll 1
         for (int i = 0; i < n; ++i) {
-            copies_wait<STAGES - 2>();
-            __syncwarp();
-            in.issue(stage == 0 ? STAGES - 1 : stage - 1);
-            const uint32_t live = in.live[stage];
+            const uint32_t live = in.take(stage);
+            in.issue(stage == 0 ? STAGES - 1 : stage - 1);  // every lane is done with that one: take()
             const char *ks = in.ring + stage * Sm::kStage;
-            if (live) core.step(ks, ks + Core::kKeys * Core::kPitch, live, scale2);
+            if (live) core.step(ks, ks + Sm::kTile, live, scale2);
             stage = stage + 1 == STAGES ? 0 : stage + 1;
         }
         copies_wait<0>();
@@ -802,18 +905,19 @@ __global__ void __launch_bounds__(kAttnThreads) k_attn(AttnArgs a, AttnScratch s
             }
         }
         u += n;
+        before_boxes();
         __syncthreads();  // the rings hold sums until here
     }
 }
 
 struct AttnKernel {
-    void (*run)(AttnArgs, AttnScratch, int, int, bool, bool);
-    int smem, rows, dim, tile;
+    void (*run)(AttnArgs, AttnMaps, AttnScratch, int, int, int, bool);
+    int smem, rows, dim, tile, keys;
 };
 
 template <typename Core, int STAGES>
 AttnKernel attn_kernel() {
-    return {k_attn<Core, STAGES>, AttnSmem<Core, STAGES>::kBytes, Core::kRows, Core::kDim, kAttnWarps * Core::kKeys};
+    return {k_attn<Core, STAGES>, AttnSmem<Core, STAGES>::kBytes, Core::kRows, Core::kDim, kAttnWarps * Core::kKeys, Core::kKeys};
 }
 
 template <typename T, bool SPLIT>
@@ -889,11 +993,36 @@ int check_cache(const l2d_kv_cache *cache, Cache *c) {
 
 using namespace l2d;
 
+namespace l2d {
+
+// A tensor map over keys or values: boxes of 128 bytes by `keys` slots of one head in one page.
+bool encode_map(CUtensorMap *map, void *base, int dtype, const Cache &c, int64_t head, int64_t slot, int64_t page, int keys) {
+    static const auto encode = [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) f = nullptr;
+        return reinterpret_cast<decltype(&cuTensorMapEncodeTiled)>(f);
+    }();
+    if (!encode) return false;
+    const cuuint64_t eb = elem_bytes(dtype);
+    const cuuint64_t sizes[4] = {static_cast<cuuint64_t>(c.head_dim), static_cast<cuuint64_t>(c.heads), static_cast<cuuint64_t>(c.page_size),
+                                 static_cast<cuuint64_t>(c.num_pages)};
+    const cuuint64_t strides[3] = {head * eb, slot * eb, page * eb};
+    const cuuint32_t box[4] = {static_cast<cuuint32_t>(128 / eb), 1, static_cast<cuuint32_t>(keys), 1}, ones[4] = {1, 1, 1, 1};
+    const CUtensorMapDataType type = dtype == L2D_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : dtype == L2D_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                                                        : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    return encode(map, type, 4, base, sizes, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace l2d
+
 struct l2d_attn_plan {
     Cache cache;
     l2d_attn_desc desc;
     int dtype, device, grid, m_tiles;
-    bool aligned;
+    int how;
+    AttnMaps maps;
     AttnKernel kernel;
     AttnScratch scratch;
     void *memory;
@@ -1016,10 +1145,15 @@ int l2d_attn_plan_create(const l2d_kv_cache *cache, const l2d_attn_desc *desc, l
     p->kernel = k;
     p->scratch = {reinterpret_cast<float *>(base), reinterpret_cast<float *>(base + part), reinterpret_cast<unsigned *>(base + part + ml)};
     p->memory = memory;
-    // Asynchronous copies of 16 bytes need rows of whole 16-byte chunks on 16-byte boundaries.
+    // 16-byte copies need rows of whole 16-byte words on 16-byte boundaries; boxes also pages of whole tiles.
     const int64_t eb = elem_bytes(cache->dtype);
     const int64_t any = cache->head_dim | c.k_page | c.k_slot | c.k_head | c.v_page | c.v_slot | c.v_head;
-    p->aligned = (any * eb) % 16 == 0 && !misaligned(c.k, 16) && !misaligned(c.v, 16);
+    p->how = (any * eb) % 16 || misaligned(c.k, 16) || misaligned(c.v, 16) ? kElements : kWords;
+    if (p->how == kWords && cache->page_size % k.keys == 0 && c.num_pages > 0) {
+        const bool ok = encode_map(&p->maps.k, c.k, cache->dtype, c, c.k_head, c.k_slot, c.k_page, k.keys) &&
+                        encode_map(&p->maps.v, c.v, cache->dtype, c, c.v_head, c.v_slot, c.v_page, k.keys);
+        if (ok) p->how = kBoxes;
+    }
     *plan = p;
     return L2D_OK;
 }
@@ -1037,10 +1171,10 @@ int l2d_attn_decode(l2d_attn_plan *p, const void *q, void *out, float *lse, cons
     const bool q_aligned = !misaligned(q, 16) && (p->desc.q_token * eb) % 16 == 0 && (p->cache.head_dim * eb) % 16 == 0;
     // No more blocks than pieces the page table leaves room for.
     const int64_t room = int64_t(p->cache.table_width) * p->cache.page_size, tiles = (room + p->kernel.tile - 1) / p->kernel.tile;
-    const int64_t most = std::max<int64_t>(1, (tiles * batch * p->cache.heads * p->m_tiles + kLeastTiles - 1) / kLeastTiles);
+    const int64_t most = std::max<int64_t>(1, (tiles + kLeastTiles - 1) / kLeastTiles) * batch * p->cache.heads * p->m_tiles;
     const dim3 grid(static_cast<unsigned>(std::min<int64_t>(p->grid, most)));
     AttnArgs a = {p->cache, q, out, lse, lens, p->desc.q_token, p->desc.out_token, p->desc.heads_q, p->desc.window, batch, p->desc.scale};
-    L2D_CUDA_TRY(launch(p->kernel.run, grid, kAttnThreads, p->kernel.smem, stream, a, p->scratch, p->m_tiles, kLeastTiles, p->aligned, q_aligned));
+    L2D_CUDA_TRY(launch(p->kernel.run, grid, kAttnThreads, p->kernel.smem, stream, a, p->maps, p->scratch, p->m_tiles, kLeastTiles, p->how, q_aligned));
     return L2D_OK;
 }
 
