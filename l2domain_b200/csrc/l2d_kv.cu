@@ -20,6 +20,7 @@ struct Cache {
     const int32_t *table;
     int64_t table_stride, num_pages;
     int num_seqs, table_width, page_size, heads, head_dim;
+    int page_shift;  // log2 of page_size, -1 if it is no power of two
     uint32_t *status;
 };
 
@@ -44,59 +45,151 @@ struct AttnArgs {
     float scale;
 };
 
+// The page of its sequence that holds a position.
+__device__ __forceinline__ unsigned page_index(const Cache &c, unsigned pos) {
+    return c.page_shift >= 0 ? pos >> c.page_shift : pos / static_cast<unsigned>(c.page_size);
+}
+
 __device__ __forceinline__ void report(uint32_t *status, uint32_t bit) {
     if (status) atomicOr(status, bit);
 }
 
 // The page of position p of sequence s, or -1 if it has none.
 __device__ __forceinline__ int64_t page_of(const Cache &c, int64_t s, int p) {
-    const int i = p / c.page_size;
+    const int i = static_cast<int>(page_index(c, p));
     if (s < 0 || s >= c.num_seqs || i >= c.table_width) return -1;
     const int32_t page = c.table[s * c.table_stride + i];
     return page >= 0 && page < c.num_pages ? page : -1;
 }
 
-// One block per token; a thread takes single elements (of a pair, the first one and its partner).
-template <typename T>
-__global__ void __launch_bounds__(256) k_append(AppendArgs a) {
+// ---------------------------------------------------------------------------------------------
+// Appending.
+//
+// A copy with a few multiplications: every element is read once and written once.  A head is cut into units
+// of VEC pairs (the rotated part: for the half layout VEC elements and their VEC partners, for the interleaved
+// one 2 VEC elements side by side) and of 2 VEC elements (the rest, and values), so that a thread moves 32 bytes
+// of 16-bit elements.  A thread keeps its unit's cosines and sines for as many heads of its token as the grid
+// leaves it: heads are split over blocks only while there are too few tokens to fill the GPU.
+// ---------------------------------------------------------------------------------------------
+
+template <typename T, int N>
+struct Pack {
+    T v[N];
+};
+
+// N consecutive elements; one load or store of up to 16 bytes each where N > 1 (the host checked the alignment).
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> load_pack(const T *p) {
+    Pack<T, N> r;
+    if constexpr (N * sizeof(T) >= 16) {
+#pragma unroll
+        for (int i = 0; i < N * static_cast<int>(sizeof(T)) / 16; ++i) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(reinterpret_cast<const char *>(p) + 16 * i);
+            memcpy(reinterpret_cast<char *>(r.v) + 16 * i, &x, 16);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) r.v[i] = p[i];
+    }
+    return r;
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_pack(T *p, const Pack<T, N> &r) {
+    if constexpr (N * sizeof(T) >= 16) {
+#pragma unroll
+        for (int i = 0; i < N * static_cast<int>(sizeof(T)) / 16; ++i) {
+            uint4 x;
+            memcpy(&x, reinterpret_cast<const char *>(r.v) + 16 * i, 16);
+            *reinterpret_cast<uint4 *>(reinterpret_cast<char *>(p) + 16 * i) = x;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) p[i] = r.v[i];
+    }
+}
+
+constexpr int kAppendThreads = 256;
+
+// units: rotated units of a head (rot_units), then plain ones.  A thread's unit is fixed; the threads of a token
+// for which `rows` are left take every rows-th of its heads.
+template <typename T, int VEC, bool INTERLEAVED>
+__global__ void __launch_bounds__(kAppendThreads) k_append(const __grid_constant__ AppendArgs a, int units, int rot_units, int rows) {
     dev::wait_for_previous();
-    const int D = a.c.head_dim, half = a.rot_dim / 2, hk = a.c.heads;
-    for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
-        const int p = a.pos[t];
-        if (p < 0) continue;
-        if (a.rot_dim && p >= a.max_pos) {
-            if (threadIdx.x == 0) report(a.c.status, L2D_KV_BAD_POSITION);
-            continue;
+    const int D = a.c.head_dim, half = a.rot_dim / 2, hk = a.c.heads, heads = a.heads_q + 2 * hk;
+    const int64_t thread = static_cast<int64_t>(blockIdx.x) * kAppendThreads + threadIdx.x;
+    const int64_t t = thread / (units * rows);
+    if (t >= a.tokens) return;
+    const int rest = static_cast<int>(thread - t * (units * rows)), row = rest / units, unit = rest - row * units;
+    const int p = a.pos[t];
+    if (p < 0) return;
+    if (a.rot_dim && p >= a.max_pos) {
+        if (rest == 0) report(a.c.status, L2D_KV_BAD_POSITION);
+        return;
+    }
+    const int64_t page = page_of(a.c, a.seq ? a.seq[t] : t, p);
+    if (page < 0) {
+        if (rest == 0) report(a.c.status, L2D_KV_BAD_PAGE);
+        return;
+    }
+    const int slot = p - static_cast<int>(page_index(a.c, p)) * a.c.page_size;
+    const T *k = static_cast<const T *>(a.k) + t * a.k_token, *v = static_cast<const T *>(a.v) + t * a.v_token;
+    const T *q = static_cast<const T *>(a.q) + t * a.q_token;
+    T *q_out = static_cast<T *>(a.q_out) + t * a.q_out_token;
+    T *kc = reinterpret_cast<T *>(a.c.k) + page * a.c.k_page + slot * a.c.k_slot;
+    T *vc = reinterpret_cast<T *>(a.c.v) + page * a.c.v_page + slot * a.c.v_slot;
+
+    // Where the unit's two halves are, and its angles.
+    const bool rotated = unit < rot_units;
+    const int pair = unit * VEC;  // first pair of a rotated unit
+    const int first = !rotated ? a.rot_dim + (unit - rot_units) * 2 * VEC : INTERLEAVED ? 2 * pair : pair;
+    const int second = rotated && !INTERLEAVED ? pair + half : first + VEC;
+    const bool both = rotated || second < D;  // the plain part may end with one half
+    float c[VEC], s[VEC];
+    if (rotated) {
+        const Pack<float, VEC> cc = load_pack<float, VEC>(a.cos + static_cast<int64_t>(p) * half + pair);
+        const Pack<float, VEC> ss = load_pack<float, VEC>(a.sin + static_cast<int64_t>(p) * half + pair);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) c[i] = cc.v[i], s[i] = ss.v[i];
+    }
+    // Heads in order: queries, keys, values; a few at a time, loads first.
+    auto at = [&](int h, const T *&src, T *&dst) {
+        const int g = h - a.heads_q, w = g - hk;
+        if (g < 0) src = q + static_cast<int64_t>(h) * D, dst = q_out + static_cast<int64_t>(h) * D;
+        else if (w < 0) src = k + static_cast<int64_t>(g) * D, dst = kc + g * a.c.k_head;
+        else src = v + static_cast<int64_t>(w) * D, dst = vc + w * a.c.v_head;
+    };
+    constexpr int kHeads = 4;
+    for (int h0 = row; h0 < heads; h0 += kHeads * rows) {
+        Pack<T, VEC> x[kHeads], y[kHeads];
+        T *dst[kHeads];
+#pragma unroll
+        for (int j = 0; j < kHeads; ++j) {
+            const T *src = nullptr;
+            dst[j] = nullptr;
+            if (h0 + j * rows >= heads) continue;
+            at(h0 + j * rows, src, dst[j]);
+            x[j] = load_pack<T, VEC>(src + first);
+            if (both) y[j] = load_pack<T, VEC>(src + second);
         }
-        const int64_t page = page_of(a.c, a.seq ? a.seq[t] : t, p);
-        if (page < 0) {
-            if (threadIdx.x == 0) report(a.c.status, L2D_KV_BAD_PAGE);
-            continue;
-        }
-        const int slot = p % a.c.page_size;
-        T *kc = reinterpret_cast<T *>(a.c.k) + page * a.c.k_page + slot * a.c.k_slot;
-        T *vc = reinterpret_cast<T *>(a.c.v) + page * a.c.v_page + slot * a.c.v_slot;
-        for (int e = threadIdx.x; e < hk * D; e += blockDim.x) {
-            const int h = e / D, i = e - h * D;
-            vc[h * a.c.v_head + i] = static_cast<const T *>(a.v)[t * a.v_token + e];
-        }
-        for (int e = threadIdx.x; e < (a.heads_q + hk) * D; e += blockDim.x) {
-            const int hh = e / D, i = e - hh * D;
-            const bool is_q = hh < a.heads_q;
-            const int h = is_q ? hh : hh - a.heads_q;
-            const T *src = is_q ? static_cast<const T *>(a.q) + t * a.q_token + int64_t(h) * D
-                                : static_cast<const T *>(a.k) + t * a.k_token + int64_t(h) * D;
-            T *dst = is_q ? static_cast<T *>(a.q_out) + t * a.q_out_token + int64_t(h) * D : kc + h * a.c.k_head;
-            if (i >= a.rot_dim) {
-                dst[i] = src[i];
-                continue;
+#pragma unroll
+        for (int j = 0; j < kHeads; ++j) {
+            if (h0 + j * rows >= heads) continue;
+            if (rotated && h0 + j * rows < a.heads_q + hk) {
+                float u[2 * VEC];
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) u[i] = dev::widen(x[j].v[i]), u[VEC + i] = dev::widen(y[j].v[i]);
+                T r[2 * VEC];
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    const int lo = INTERLEAVED ? 2 * i : i, hi = INTERLEAVED ? 2 * i + 1 : VEC + i;
+                    r[lo] = dev::narrow<T>(fmaf(u[lo], c[i], -(u[hi] * s[i])));
+                    r[hi] = dev::narrow<T>(fmaf(u[hi], c[i], u[lo] * s[i]));
+                }
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) x[j].v[i] = r[i], y[j].v[i] = r[VEC + i];
             }
-            if (a.interleaved ? (i & 1) : i >= half) continue;
-            const int j = a.interleaved ? i + 1 : i + half, r = a.interleaved ? i / 2 : i;
-            const float c = a.cos[int64_t(p) * half + r], s = a.sin[int64_t(p) * half + r];
-            const float u = dev::widen(src[i]), w = dev::widen(src[j]);
-            dst[i] = dev::narrow<T>(fmaf(u, c, -(w * s)));
-            dst[j] = dev::narrow<T>(fmaf(w, c, u * s));
+            store_pack<T, VEC>(dst[j] + first, x[j]);
+            if (both) store_pack<T, VEC>(dst[j] + second, y[j]);
         }
     }
 }
@@ -121,10 +214,8 @@ __global__ void __launch_bounds__(256) k_append(AppendArgs a) {
 // not depend on which block came last.
 // ---------------------------------------------------------------------------------------------
 
-constexpr int kAttnWarps = 4;
-constexpr int kAttnThreads = kAttnWarps * 32;
 constexpr int kMaxRows = 16;    // query heads a block works on
-constexpr int kLeastTiles = 4;  // tiles of a block's piece, at least
+constexpr int kLeastTiles = 2;  // tiles of a block's piece, at least
 
 struct AttnScratch {
     float *part;         // [grid][2][kMaxRows][head_dim padded] unnormalised sums
@@ -220,6 +311,8 @@ template <typename T, int KS, bool SPLIT>
 struct MmaCore {
     using Elem = T;
     static constexpr int kKeys = 16;                       // keys of a warp's tile
+    static constexpr int kWarps = KS <= 8 ? 8 : 4;         // whose rings fit an SM
+    static constexpr int kThreads = kWarps * 32;
     static constexpr int kRows = SPLIT ? 8 : 16;           // query heads
     static constexpr int kDim = KS * 16;                   // head_dim, padded
     static constexpr int kBoxes = (KS + 3) / 4;            // of 64 elements
@@ -232,25 +325,28 @@ struct MmaCore {
     float o[2 * KS][4], m[2], l[2];
     uint32_t query;
 
-    // q: this group's first head; `heads` rows are real, `flip` takes their negatives.  All threads of the block call it.
-    __device__ __forceinline__ void begin(const T *q, int heads, int D, bool aligned, bool flip, char *smem_q, char *) {
-        const int lane = threadIdx.x & 31;
+    // q: this group's first head; `heads` rows are real, `flip` takes their negatives.  All threads of the block call
+    // it, and a barrier before begin().
+    static __device__ __forceinline__ void stage_query(const T *q, int heads, int D, bool aligned, bool flip, char *smem_q) {
         const uint32_t sign = flip ? 0x80008000u : 0u;
         if (aligned) {
-            for (int e = threadIdx.x; e < kRows * KS * 2; e += kAttnThreads) {
+            for (int e = threadIdx.x; e < kRows * KS * 2; e += kThreads) {
                 const int r = e / (KS * 2), ch = e - r * (KS * 2);
                 uint4 x = make_uint4(0, 0, 0, 0);
                 if (r < heads && ch * 8 < D) x = *reinterpret_cast<const uint4 *>(q + r * D + ch * 8);
                 *reinterpret_cast<uint4 *>(smem_q + r * kPitch + ch * 16) = make_uint4(x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign);
             }
         } else {
-            for (int e = threadIdx.x; e < kRows * kDim; e += kAttnThreads) {
+            for (int e = threadIdx.x; e < kRows * kDim; e += kThreads) {
                 const int r = e / kDim, i = e - r * kDim;
                 const uint16_t x = r < heads && i < D ? reinterpret_cast<const uint16_t *>(q)[r * D + i] : 0;
                 reinterpret_cast<uint16_t *>(smem_q + r * kPitch)[i] = static_cast<uint16_t>(x ^ sign);
             }
         }
-        __syncthreads();
+    }
+
+    __device__ __forceinline__ void begin(char *smem_q, char *, int) {
+        const int lane = threadIdx.x & 31;
         query = smem_addr(smem_q);
         if constexpr (SPLIT) {  // matrices of 8 heads x 8 elements, two steps of 16 at once
             uint32_t r[4];
@@ -287,7 +383,7 @@ struct MmaCore {
         // Chunk 2k + hi of row r is at chunk_at(r, hi) ^ (2k & 7) * 16, in box k / 4.
         const uint32_t ka = smem_addr(ks) + chunk_at<kKeys>((lane >> 4) * 8 + (lane & 7), (lane >> 3) & 1);
         const uint32_t va = smem_addr(vs) + chunk_at<kKeys>(((lane >> 3) & 1) * 8 + (lane & 7), lane >> 4);
-        float s[2][4] = {};
+        float s[2][4] = {}, s2[2][4] = {};  // of even and odd steps: shorter chains
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
             uint32_t a[4], b[4];
@@ -303,9 +399,11 @@ struct MmaCore {
                 for (int e = 0; e < 4; ++e) a[e] = qa[k][e];
             }
             ldmatrix4(b, (ka ^ ((2 * k & 7) << 4)) + (k / 4) * (kKeys * 128));
-            mma16816<T>(s[0], a, b[0], b[1]);
-            mma16816<T>(s[1], a, b[2], b[3]);
+            mma16816<T>(k & 1 ? s2[0] : s[0], a, b[0], b[1]);
+            mma16816<T>(k & 1 ? s2[1] : s[1], a, b[2], b[3]);
         }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e >> 2][e & 3] += s2[e >> 2][e & 3];
         if (live != (1u << kKeys) - 1) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
@@ -381,7 +479,9 @@ struct MmaCore {
 template <int GT, int DV>
 struct SimdCore {
     using Elem = float;
-    static constexpr int kKeys = DV == 1 ? 16 : 8;
+    static constexpr int kKeys = 8;
+    static constexpr int kWarps = DV == 1 ? 8 : 4;
+    static constexpr int kThreads = kWarps * 32;
     static constexpr int kRows = GT;
     static constexpr int kDim = DV * 128;
     static constexpr int kBoxes = kDim / 32;
@@ -394,17 +494,18 @@ struct SimdCore {
     float *weights;
     int chunks;
 
-    __device__ __forceinline__ void begin(const float *q, int heads, int D, bool, bool flip, char *smem_q, char *warp_smem) {
-        float *sq = reinterpret_cast<float *>(smem_q);
-        query = sq;
-        weights = reinterpret_cast<float *>(warp_smem);
-        chunks = (D + 3) / 4;
-        for (int e = threadIdx.x; e < GT * kDim; e += kAttnThreads) {
+    static __device__ __forceinline__ void stage_query(const float *q, int heads, int D, bool, bool flip, char *smem_q) {
+        for (int e = threadIdx.x; e < GT * kDim; e += kThreads) {
             const int r = e / kDim, i = e - r * kDim;
             const float x = r < heads && i < D ? q[r * D + i] : 0.0f;
-            sq[e] = flip ? -x : x;
+            reinterpret_cast<float *>(smem_q)[e] = flip ? -x : x;
         }
-        __syncthreads();
+    }
+
+    __device__ __forceinline__ void begin(char *smem_q, char *warp_smem, int D) {
+        query = reinterpret_cast<float *>(smem_q);
+        weights = reinterpret_cast<float *>(warp_smem);
+        chunks = (D + 3) / 4;
 #pragma unroll
         for (int g = 0; g < GT; ++g) {
             m[g] = -INFINITY;
@@ -492,24 +593,25 @@ struct SimdCore {
     }
 };
 
-// Shared memory of a block: the rings (reused for the warps' sums at the end of a piece), queries, the
+// Shared memory of a block: the rings, stage by stage (the last one, which the first tiles of the next piece do
+// not need, is reused for the warps' sums at the end of a piece), queries, the
 // cores' own words, barriers, row offsets and live bits, maxima and sums.
-constexpr int kJoin = 128;  // pieces whose factors are held at a time when a sequence's pieces are joined
+constexpr int kJoin = 64;  // pieces whose factors are held at a time when a sequence's pieces are joined
 template <typename Core, int STAGES>
 struct AttnSmem {
     static constexpr int kTile = Core::kKeys * 128 * Core::kBoxes;  // of keys, and of values
-    static constexpr int kStage = 2 * kTile;
-    static constexpr int kRing = kAttnWarps * STAGES * kStage;
-    static constexpr int kSums = kAttnWarps * Core::kRows * Core::kDim * 4;
-    static constexpr int kFactors = kSums;  // behind the sums
-    static constexpr int kEnd = kFactors + kJoin * kMaxRows * 4;
+    static constexpr int kStage = 2 * kTile;  // of one warp
+    static constexpr int kRing = Core::kWarps * STAGES * kStage;
+    static constexpr int kSums = Core::kWarps * (STAGES - 1) * kStage;
+    static constexpr int kFactors = kSums + Core::kWarps * Core::kRows * Core::kDim * 4;
+    static constexpr int kEnd = kFactors + 2 * kJoin * kMaxRows * 4;
     static constexpr int kQuery = kRing > kEnd ? kRing : kEnd;
     static constexpr int kWarp = kQuery + Core::kQueryBytes;
-    static constexpr int kRowAt = kWarp + kAttnWarps * Core::kWarpBytes;
-    static constexpr int kBars = kRowAt + kAttnWarps * Core::kKeys * 16;
-    static constexpr int kLive = kBars + kAttnWarps * STAGES * 8;
-    static constexpr int kMl = kLive + kAttnWarps * STAGES * 4;
-    static constexpr int kFlag = kMl + kAttnWarps * 2 * kMaxRows * 4;
+    static constexpr int kRowAt = kWarp + Core::kWarps * Core::kWarpBytes;
+    static constexpr int kBars = kRowAt + Core::kWarps * Core::kKeys * 16;
+    static constexpr int kLive = kBars + Core::kWarps * STAGES * 8;
+    static constexpr int kMl = kLive + Core::kWarps * STAGES * 4;
+    static constexpr int kFlag = kMl + Core::kWarps * 2 * kMaxRows * 4;
     static constexpr int kBytes = kFlag + 16;
 };
 
@@ -543,7 +645,7 @@ struct Stream {
         const int64_t key = how == kBoxes ? next : next + lane;
         page = -2;  // no such key
         if (key < len && (how == kBoxes ? key + Core::kKeys > lo : key >= lo && lane < Core::kKeys)) {
-            const unsigned i = static_cast<unsigned>(key) / static_cast<unsigned>(c.page_size);
+            const unsigned i = page_index(c, static_cast<unsigned>(key));
             slot = static_cast<int>(static_cast<unsigned>(key) - i * static_cast<unsigned>(c.page_size));
             page = max(table[i], -1);
         }
@@ -555,7 +657,7 @@ struct Stream {
         constexpr uint32_t kAll = (1u << Core::kKeys) - 1;
         const bool real = page >= 0 && page < c.num_pages;
         if (!real && page != -2) report(c.status, L2D_KV_BAD_PAGE);
-        char *tile = ring + stage * Sm::kStage;
+        char *tile = ring + stage * (Core::kWarps * Sm::kStage);
         if (how == kBoxes) {
             uint32_t bits = 0;
             if (real) {
@@ -628,7 +730,7 @@ struct Stream {
             if (!barrier_wait(bars + 8 * stage, phases >> stage & 1)) report(c.status, L2D_KV_TIMEOUT);
             phases ^= 1u << stage;
             if (bits != (1u << Core::kKeys) - 1) {
-                char *values = ring + stage * Sm::kStage + Sm::kTile;
+                char *values = ring + stage * (Core::kWarps * Sm::kStage) + Sm::kTile;
                 for (int r = 0; r < Core::kKeys; ++r)
                     if (!(bits >> r & 1))
                         for (int ch = threadIdx.x & 31; ch < Core::kChunks; ch += 32)
@@ -681,78 +783,106 @@ __device__ __forceinline__ void join(const AttnArgs &a, const AttnScratch &sc, i
                                      float *sums, float *factors, float *sm_m, float *sm_l) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, D = a.c.head_dim, n = c1 - c0 + 1;
     auto slot = [&](int j) { return static_cast<int64_t>(c0 + j) * 2 + (j == 0 ? odd : 0); };
-    // Each row's maximum and sum of weights, lanes over the pieces.
-    for (int r = warp; r < rows; r += kAttnWarps) {
-        float top = -INFINITY, sum = 0.0f;
-        for (int j = lane; j < n; j += 32) top = fmaxf(top, __ldcg(sc.ml + slot(j) * 2 * kMaxRows + r));
-#pragma unroll
-        for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        for (int j = lane; j < n; j += 32) {
-            const float *ml = sc.ml + slot(j) * 2 * kMaxRows + r;
-            sum = fmaf(exp2_approx(__ldcg(ml) - finite_base(top)), __ldcg(ml + kMaxRows), sum);
-        }
-#pragma unroll
-        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        if (lane == 0) {
-            sm_m[r] = finite_base(top);
-            sm_l[r] = sum;
-        }
-    }
-    __syncthreads();
-    // The sums, warps over the pieces, up to 1024 elements (of whole rows' float4s) at a time.
-    constexpr int kQuads = Core::kRows * Core::kDim / 4, kEach = kQuads < 256 ? kQuads / 32 : 8, kRowQuads = Core::kDim / 4;
-    static_assert(kQuads % 32 == 0, "a warp covers whole rows");
+    float *weights = factors + kJoin * kMaxRows;  // the pieces' sums of weights
+    // The sums, warps over the pieces, up to 1024 elements (of whole rows' float4s) at a time; kJoin pieces at a
+    // time, relative to the largest maximum so far.
+    constexpr int kQuads = Core::kRows * Core::kDim / 4, kEach = kQuads % 256 == 0 ? 8 : kQuads % 128 == 0 ? 4 : 1, kRowQuads = Core::kDim / 4;
+    static_assert(kQuads % (32 * kEach) == 0, "every lane has as many");
     for (int first = 0; first < kQuads; first += 32 * kEach) {
         float4 acc[kEach];
 #pragma unroll
         for (int j = 0; j < kEach; ++j) acc[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (tid < kMaxRows) {
+            sm_m[tid] = -INFINITY;
+            sm_l[tid] = 0.0f;
+        }
         for (int p0 = 0; p0 < n; p0 += kJoin) {
             const int pn = min(n - p0, kJoin);
             __syncthreads();
-            for (int e = tid; e < pn * kMaxRows; e += kAttnThreads) {
+#pragma unroll 4
+            for (int e = tid; e < pn * kMaxRows; e += Core::kThreads) {
                 const int j = e / kMaxRows, r = e % kMaxRows;
-                factors[e] = r < rows ? exp2_approx(__ldcg(sc.ml + slot(p0 + j) * 2 * kMaxRows + r) - sm_m[r]) : 0.0f;
+                const float *ml = sc.ml + slot(p0 + j) * 2 * kMaxRows + r;
+                factors[e] = r < rows ? __ldcg(ml) : -INFINITY;
+                weights[e] = r < rows ? __ldcg(ml + kMaxRows) : 0.0f;
             }
             __syncthreads();
-#pragma unroll 2
-            for (int j = warp; j < pn; j += kAttnWarps) {
-                const float4 *part = reinterpret_cast<const float4 *>(sc.part + slot(p0 + j) * kMaxRows * Core::kDim);
+            for (int r = warp; r < kMaxRows; r += Core::kWarps) {  // a warp a row, lanes over the pieces
+                const float was = sm_m[r], m0 = lane < pn ? factors[lane * kMaxRows + r] : -INFINITY,
+                            m1 = lane + 32 < pn ? factors[(lane + 32) * kMaxRows + r] : -INFINITY;
+                float top = fmaxf(was, fmaxf(m0, m1));
+#pragma unroll
+                for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                const float base = finite_base(top), f0 = exp2_approx(m0 - base), f1 = exp2_approx(m1 - base);
+                float sum = (lane < pn ? f0 * weights[lane * kMaxRows + r] : 0.0f) + (lane + 32 < pn ? f1 * weights[(lane + 32) * kMaxRows + r] : 0.0f);
+                if (lane < pn) factors[lane * kMaxRows + r] = f0;
+                if (lane + 32 < pn) factors[(lane + 32) * kMaxRows + r] = f1;
+#pragma unroll
+                for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                __syncwarp();
+                if (lane == 0) {
+                    const float f = exp2_approx(was - base);  // what the pieces before are worth now
+                    sm_m[r] = top;
+                    sm_l[r] = fmaf(sm_l[r], f, sum);
+                    sm_m[kMaxRows + r] = f;
+                }
+            }
+            __syncthreads();
+            if (p0) {
 #pragma unroll
                 for (int i = 0; i < kEach; ++i) {
-                    const int q = first + lane + 32 * i, r = q / kRowQuads;
-                    if (q < kQuads && r < rows) {
-                        const float f = factors[j * kMaxRows + r];
-                        const float4 x = __ldcg(part + q);
-                        acc[i] = make_float4(fmaf(f, x.x, acc[i].x), fmaf(f, x.y, acc[i].y), fmaf(f, x.z, acc[i].z), fmaf(f, x.w, acc[i].w));
+                    const float f = sm_m[kMaxRows + (first + lane + 32 * i) / kRowQuads];
+                    acc[i] = make_float4(acc[i].x * f, acc[i].y * f, acc[i].z * f, acc[i].w * f);
+                }
+            }
+            // Four pieces' loads at a time (rows that are not real: of anything, and dropped).
+            constexpr int kPieces = 4;
+            for (int j0 = warp; j0 < pn; j0 += kPieces * Core::kWarps) {
+                float4 x[kPieces][kEach];
+#pragma unroll
+                for (int k = 0; k < kPieces; ++k) {
+                    const int j = min(j0 + k * Core::kWarps, pn - 1);
+                    const float4 *part = reinterpret_cast<const float4 *>(sc.part + slot(p0 + j) * kMaxRows * Core::kDim) + first + lane;
+#pragma unroll
+                    for (int i = 0; i < kEach; ++i) x[k][i] = __ldcg(part + 32 * i);
+                }
+#pragma unroll
+                for (int k = 0; k < kPieces; ++k) {
+                    const int j = j0 + k * Core::kWarps;
+                    if (j >= pn) break;
+#pragma unroll
+                    for (int i = 0; i < kEach; ++i) {
+                        const float f = factors[j * kMaxRows + (first + lane + 32 * i) / kRowQuads];
+                        acc[i] = make_float4(fmaf(f, x[k][i].x, acc[i].x), fmaf(f, x[k][i].y, acc[i].y), fmaf(f, x[k][i].z, acc[i].z), fmaf(f, x[k][i].w, acc[i].w));
                     }
                 }
             }
         }
 #pragma unroll
         for (int i = 0; i < kEach; ++i)
-            if (first + lane + 32 * i < kQuads) reinterpret_cast<float4 *>(sums)[warp * kQuads + first + lane + 32 * i] = acc[i];
+            reinterpret_cast<float4 *>(sums)[warp * kQuads + first + lane + 32 * i] = acc[i];
     }
     __syncthreads();
-    for (int q = tid; q < rows * kRowQuads; q += kAttnThreads) {
+    for (int q = tid; q < rows * kRowQuads; q += Core::kThreads) {
         const int r = q / kRowQuads, i = (q - r * kRowQuads) * 4;
         if (i >= D) continue;
         float4 x = reinterpret_cast<const float4 *>(sums)[q];
 #pragma unroll
-        for (int w = 1; w < kAttnWarps; ++w) {
+        for (int w = 1; w < Core::kWarps; ++w) {
             const float4 y = reinterpret_cast<const float4 *>(sums)[w * kQuads + q];
             x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
         }
-        store_row4<typename Core::Elem>(a, b, head0 + r, i, D, x, sm_m[r], sm_l[r]);
+        store_row4<typename Core::Elem>(a, b, head0 + r, i, D, x, finite_base(sm_m[r]), sm_l[r]);
     }
 }
 
 template <typename Core, int STAGES>
-__global__ void __launch_bounds__(kAttnThreads) k_attn(const __grid_constant__ AttnArgs a, const __grid_constant__ AttnMaps maps, AttnScratch sc, int m_tiles, int least, int how, bool q_aligned) {
+__global__ void __launch_bounds__(Core::kThreads, 1) k_attn(const __grid_constant__ AttnArgs a, const __grid_constant__ AttnMaps maps, AttnScratch sc, int m_tiles, int least, int how, bool q_aligned) {
     using T = typename Core::Elem;
     using Sm = AttnSmem<Core, STAGES>;
-    constexpr int TILE = kAttnWarps * Core::kKeys;
+    constexpr int TILE = Core::kWarps * Core::kKeys;
     extern __shared__ __align__(1024) char smem[];
-    float *sm_m = reinterpret_cast<float *>(smem + Sm::kMl), *sm_l = sm_m + kAttnWarps * kMaxRows;
+    float *sm_m = reinterpret_cast<float *>(smem + Sm::kMl), *sm_l = sm_m + Core::kWarps * kMaxRows;
     int *flag = reinterpret_cast<int *>(smem + Sm::kFlag);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int D = a.c.head_dim, G = a.heads_q / a.c.heads, items = a.c.heads * m_tiles;
@@ -774,9 +904,9 @@ __global__ void __launch_bounds__(kAttnThreads) k_attn(const __grid_constant__ A
     for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
         if (tid == 0 && a.lens[b] > a.c.table_width * a.c.page_size) report(a.c.status, L2D_KV_BAD_PAGE);
         if (span_of<TILE>(a, b).tiles) continue;
-        for (int i = tid; i < a.heads_q * D; i += kAttnThreads) static_cast<T *>(a.out)[b * a.out_token + i] = dev::narrow<T>(0.0f);
+        for (int i = tid; i < a.heads_q * D; i += Core::kThreads) static_cast<T *>(a.out)[b * a.out_token + i] = dev::narrow<T>(0.0f);
         if (a.lse)
-            for (int h = tid; h < a.heads_q; h += kAttnThreads) a.lse[static_cast<int64_t>(b) * a.heads_q + h] = -INFINITY;
+            for (int h = tid; h < a.heads_q; h += Core::kThreads) a.lse[static_cast<int64_t>(b) * a.heads_q + h] = -INFINITY;
     }
 
     // This block's piece of the line of tiles, and the sequence it starts in (every warp looks for itself).
@@ -808,7 +938,7 @@ __global__ void __launch_bounds__(kAttnThreads) k_attn(const __grid_constant__ A
 
     const float scale2 = fabsf(a.scale) * 1.4426950408889634f;  // a negative one turns the queries' signs
     Stream<Core, STAGES> in{a.c, maps, how};
-    in.ring = smem + warp * STAGES * Sm::kStage;
+    in.ring = smem + warp * Sm::kStage;
     in.row_at = reinterpret_cast<longlong2 *>(smem + Sm::kRowAt) + warp * Core::kKeys;
     in.bars = smem_addr(smem + Sm::kBars) + warp * STAGES * 8;
     in.live = reinterpret_cast<uint32_t *>(smem + Sm::kLive) + warp * STAGES;
@@ -816,69 +946,100 @@ __global__ void __launch_bounds__(kAttnThreads) k_attn(const __grid_constant__ A
     if (lane < STAGES) barrier_init(in.bars + 8 * lane);
     before_boxes();
     __syncwarp();
-    Core core;
-    while (u < stop) {
-        const Span s = span_of<TILE>(a, b);
-        const int64_t at = u - before * items;
-        if (!s.tiles || at >= static_cast<int64_t>(s.tiles) * items) {
-            before += s.tiles;
-            ++b;
-            continue;
+    // What a block does at a time: some tiles of one head group of a sequence.
+    struct Piece {
+        Span s;
+        int b, item, t0, n, head0, rows;
+    };
+    auto find = [&](int64_t at_unit) {
+        Piece p;
+        for (;; ++b) {
+            p.s = span_of<TILE>(a, b);
+            if (at_unit - before * items < static_cast<int64_t>(p.s.tiles) * items) break;
+            before += p.s.tiles;
         }
-        const int item = static_cast<int>(quotient(at, s.tiles));
-        const int t0 = static_cast<int>(at - static_cast<int64_t>(item) * s.tiles);
-        const int n = static_cast<int>(min(static_cast<int64_t>(s.tiles - t0), stop - u));
-        const int hk = item / m_tiles, row0 = (item - hk * m_tiles) * Core::kRows, rows = min(G - row0, Core::kRows);
-        const int head0 = hk * G + row0;
-
-        in.head = hk;
-        in.table = a.c.table + b * a.c.table_stride;
-        in.lo = s.lo;
-        in.len = static_cast<int>(min(static_cast<int64_t>(s.len), s.from + static_cast<int64_t>(t0 + n) * TILE));
-        in.next = s.from + static_cast<int64_t>(t0) * TILE + warp * Core::kKeys;
+        const int64_t at = at_unit - before * items;
+        p.b = b;
+        p.item = static_cast<int>(quotient(at, p.s.tiles));
+        p.t0 = static_cast<int>(at - static_cast<int64_t>(p.item) * p.s.tiles);
+        p.n = static_cast<int>(min(static_cast<int64_t>(p.s.tiles - p.t0), stop - at_unit));
+        const int hk = p.item / m_tiles, row0 = (p.item - hk * m_tiles) * Core::kRows;
+        p.rows = min(G - row0, Core::kRows);
+        p.head0 = hk * G + row0;
+        return p;
+    };
+    auto start = [&](const Piece &p) {  // its first tiles
+        in.head = p.item / m_tiles;
+        in.table = a.c.table + p.b * a.c.table_stride;
+        in.lo = p.s.lo;
+        in.len = static_cast<int>(min(static_cast<int64_t>(p.s.len), p.s.from + static_cast<int64_t>(p.t0 + p.n) * TILE));
+        in.next = p.s.from + static_cast<int64_t>(p.t0) * TILE + warp * Core::kKeys;
         in.step = TILE;
         in.lookup();
 #pragma unroll 1
         for (int i = 0; i < STAGES - 1; ++i) in.issue(i);
-        core.begin(static_cast<const T *>(a.q) + b * a.q_token + static_cast<int64_t>(head0) * D, rows, D, q_aligned, a.scale < 0.0f, smem + Sm::kQuery,
-                   smem + Sm::kWarp + warp * Core::kWarpBytes);
+    };
+    auto stage_query = [&](const Piece &p) {
+        Core::stage_query(static_cast<const T *>(a.q) + p.b * a.q_token + static_cast<int64_t>(p.head0) * D, p.rows, D, q_aligned, a.scale < 0.0f,
+                          smem + Sm::kQuery);
+    };
+
+    Core core;
+    Piece p = find(u);
+    start(p);
+    stage_query(p);
+    __syncthreads();
+    for (;;) {
+        core.begin(smem + Sm::kQuery, smem + Sm::kWarp + warp * Core::kWarpBytes, D);
         int stage = 0;
 #pragma unroll 1
-        for (int i = 0; i < n; ++i) {
+        for (int i = 0; i < p.n; ++i) {
             const uint32_t live = in.take(stage);
             in.issue(stage == 0 ? STAGES - 1 : stage - 1);  // every lane is done with that one: take()
-            const char *ks = in.ring + stage * Sm::kStage;
+            const char *ks = in.ring + stage * (Core::kWarps * Sm::kStage);
             if (live) core.step(ks, ks + Sm::kTile, live, scale2);
             stage = stage + 1 == STAGES ? 0 : stage + 1;
         }
-        copies_wait<0>();
+        if (how != kBoxes) copies_wait<0>();
+        // The next piece's first tiles are on their way while this one's sums meet.
+        const bool more = u + p.n < stop;
+        Piece following = p;
+        before_boxes();
+        __syncwarp();
+        if (more) {
+            following = find(u + p.n);
+            start(following);
+        }
         __syncthreads();
+        if (more) stage_query(following);
 
         // The warps' sums meet.
-        float *sums = reinterpret_cast<float *>(smem);
+        const Span s = p.s;
+        const int n = p.n, t0 = p.t0, item = p.item, head0 = p.head0, rows = p.rows;
+        float *sums = reinterpret_cast<float *>(smem + Sm::kSums);
         core.end(sums + warp * Core::kRows * Core::kDim, sm_m + warp * kMaxRows, sm_l + warp * kMaxRows);
         __syncthreads();
         const bool whole = n == s.tiles;
         const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + (u != first_unit);
         constexpr int kRowQuads = Core::kDim / 4;
-        for (int q = tid; q < rows * kRowQuads; q += kAttnThreads) {
+        for (int q = tid; q < rows * kRowQuads; q += Core::kThreads) {
             const int r = q / kRowQuads, i = (q - r * kRowQuads) * 4;
             if (i >= D) continue;
             float top = sm_m[r];
 #pragma unroll
-            for (int w = 1; w < kAttnWarps; ++w) top = fmaxf(top, sm_m[w * kMaxRows + r]);
+            for (int w = 1; w < Core::kWarps; ++w) top = fmaxf(top, sm_m[w * kMaxRows + r]);
             const float base = finite_base(top);
             float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             float sum = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kAttnWarps; ++w) {
+            for (int w = 0; w < Core::kWarps; ++w) {
                 const float f = exp2_approx(sm_m[w * kMaxRows + r] - base);
                 const float4 y = *reinterpret_cast<const float4 *>(sums + (w * Core::kRows + r) * Core::kDim + i);
                 x = make_float4(fmaf(f, y.x, x.x), fmaf(f, y.y, x.y), fmaf(f, y.z, x.z), fmaf(f, y.w, x.w));
                 sum = fmaf(f, sm_l[w * kMaxRows + r], sum);
             }
             if (whole) {
-                store_row4<T>(a, b, head0 + r, i, D, x, base, sum);
+                store_row4<T>(a, p.b, head0 + r, i, D, x, base, sum);
             } else {
                 *reinterpret_cast<float4 *>(sc.part + (slot * kMaxRows + r) * Core::kDim + i) = x;
                 if (i == 0) {
@@ -893,7 +1054,7 @@ __global__ void __launch_bounds__(kAttnThreads) k_attn(const __grid_constant__ A
             __threadfence();
             __syncthreads();
             if (tid == 0) {
-                unsigned *count = sc.arrived + static_cast<int64_t>(b) * items + item;
+                unsigned *count = sc.arrived + static_cast<int64_t>(p.b) * items + item;
                 const bool last = atomicAdd(count, 1u) == static_cast<unsigned>(c1 - c0);
                 if (last) *count = 0;
                 *flag = last;
@@ -901,30 +1062,32 @@ __global__ void __launch_bounds__(kAttnThreads) k_attn(const __grid_constant__ A
             __syncthreads();
             if (*flag) {
                 __threadfence();
-                join<Core>(a, sc, c0, c1, u0 != c0 * per, b, head0, rows, sums, reinterpret_cast<float *>(smem + Sm::kFactors), sm_m, sm_l);
+                join<Core>(a, sc, c0, c1, u0 != c0 * per, p.b, head0, rows, sums, reinterpret_cast<float *>(smem + Sm::kFactors), sm_m, sm_l);
             }
         }
-        u += n;
         before_boxes();
-        __syncthreads();  // the rings hold sums until here
+        __syncthreads();  // the last stage holds sums until here
+        if (!more) break;
+        u += n;
+        p = following;
     }
 }
 
 struct AttnKernel {
     void (*run)(AttnArgs, AttnMaps, AttnScratch, int, int, int, bool);
-    int smem, rows, dim, tile, keys;
+    int smem, threads, rows, dim, tile, keys;
 };
 
 template <typename Core, int STAGES>
 AttnKernel attn_kernel() {
-    return {k_attn<Core, STAGES>, AttnSmem<Core, STAGES>::kBytes, Core::kRows, Core::kDim, kAttnWarps * Core::kKeys, Core::kKeys};
+    return {k_attn<Core, STAGES>, AttnSmem<Core, STAGES>::kBytes, Core::kThreads, Core::kRows, Core::kDim, Core::kWarps * Core::kKeys, Core::kKeys};
 }
 
 template <typename T, bool SPLIT>
 AttnKernel pick_mma(int D) {
-    if (D <= 64) return attn_kernel<MmaCore<T, 4, SPLIT>, 4>();
-    if (D <= 80) return attn_kernel<MmaCore<T, 5, SPLIT>, 4>();
-    if (D <= 96) return attn_kernel<MmaCore<T, 6, SPLIT>, 4>();
+    if (D <= 64) return attn_kernel<MmaCore<T, 4, SPLIT>, 3>();
+    if (D <= 80) return attn_kernel<MmaCore<T, 5, SPLIT>, 3>();
+    if (D <= 96) return attn_kernel<MmaCore<T, 6, SPLIT>, 3>();
     if (D <= 128) return attn_kernel<MmaCore<T, 8, SPLIT>, 3>();
     if (D <= 192) return attn_kernel<MmaCore<T, 12, SPLIT>, 3>();
     return attn_kernel<MmaCore<T, 16, SPLIT>, 3>();
@@ -972,6 +1135,7 @@ int check_cache(const l2d_kv_cache *cache, Cache *c) {
     c->num_seqs = k.num_seqs;
     c->table_width = k.table_width;
     c->page_size = k.page_size;
+    c->page_shift = k.page_size & (k.page_size - 1) ? -1 : __builtin_ctz(static_cast<unsigned>(k.page_size));
     c->heads = k.heads;
     c->head_dim = k.head_dim;
     c->status = k.status;
@@ -1079,9 +1243,27 @@ int l2d_kv_append(const l2d_kv_cache *cache, const l2d_append_desc *desc, const 
     a.heads_q = d.heads_q;
     a.rot_dim = d.rot_dim;
     a.interleaved = d.interleaved;
-    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(tokens, int64_t(sms) * 64)));
-    auto kernel = cache->dtype == L2D_F32 ? k_append<float> : cache->dtype == L2D_F16 ? k_append<__half> : k_append<__nv_bfloat16>;
-    L2D_CUDA_TRY(launch(kernel, grid, 256, 0, stream, a));
+    // Units of 16-byte words where everything is aligned to them.
+    const int vec = 16 / eb, half = d.rot_dim / 2;
+    int64_t all = D | a.k_token | a.v_token | a.c.k_page | a.c.k_slot | a.c.k_head | a.c.v_page | a.c.v_slot | a.c.v_head | half;
+    if (d.heads_q) all |= a.q_token | a.q_out_token;
+    const bool words = all % vec == 0 && !misaligned(k, 16) && !misaligned(v, 16) && !misaligned(q, 16) && !misaligned(q_out, 16) &&
+                       !misaligned(a.c.k, 16) && !misaligned(a.c.v, 16) && !misaligned(d.cos, 16) && !misaligned(d.sin, 16);
+    const int each = words ? vec : 1, rot_units = half / each, units = rot_units + (D - d.rot_dim + 2 * each - 1) / (2 * each);
+    // Heads of a token in one thread: all of them, or as few as it takes for two blocks a SM.
+    const int heads = d.heads_q + 2 * cache->heads;
+    const int64_t want = int64_t(sms) * 2 * kAppendThreads, have = tokens * units;
+    const int rows = static_cast<int>(std::min<int64_t>(heads, std::max<int64_t>(1, (want + have - 1) / have)));
+    const int64_t blocks = (have * rows + kAppendThreads - 1) / kAppendThreads;
+    if (blocks > INT32_MAX) return set_error(L2D_ERR_INVALID, "%lld tokens are too many", static_cast<long long>(tokens));
+    auto pick = [&](auto type) {
+        using T = decltype(type);
+        constexpr int kVec = 16 / sizeof(T);
+        if (words) return d.interleaved ? k_append<T, kVec, true> : k_append<T, kVec, false>;
+        return d.interleaved ? k_append<T, 1, true> : k_append<T, 1, false>;
+    };
+    auto kernel = cache->dtype == L2D_F32 ? pick(float()) : cache->dtype == L2D_F16 ? pick(__half()) : pick(__nv_bfloat16());
+    L2D_CUDA_TRY(launch(kernel, dim3(static_cast<unsigned>(blocks)), kAppendThreads, 0, stream, a, units, rot_units, rows));
     return L2D_OK;
 }
 
@@ -1117,7 +1299,7 @@ int l2d_attn_plan_create(const l2d_kv_cache *cache, const l2d_attn_desc *desc, l
     const int m_tiles = (G + k.rows - 1) / k.rows;
     int blocks = 0;
     L2D_CUDA_TRY(cudaFuncSetAttribute(k.run, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem));
-    L2D_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, k.run, kAttnThreads, k.smem));
+    L2D_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, k.run, k.threads, k.smem));
     if (blocks < 1) return set_error(L2D_ERR_CUDA, "the attention kernel does not fit an SM");
     const int grid = sms * blocks;
     const size_t part = size_t(grid) * 2 * kMaxRows * k.dim * 4, ml = size_t(grid) * 4 * kMaxRows * 4;
@@ -1174,7 +1356,7 @@ int l2d_attn_decode(l2d_attn_plan *p, const void *q, void *out, float *lse, cons
     const int64_t most = std::max<int64_t>(1, (tiles + kLeastTiles - 1) / kLeastTiles) * batch * p->cache.heads * p->m_tiles;
     const dim3 grid(static_cast<unsigned>(std::min<int64_t>(p->grid, most)));
     AttnArgs a = {p->cache, q, out, lse, lens, p->desc.q_token, p->desc.out_token, p->desc.heads_q, p->desc.window, batch, p->desc.scale};
-    L2D_CUDA_TRY(launch(p->kernel.run, grid, kAttnThreads, p->kernel.smem, stream, a, p->maps, p->scratch, p->m_tiles, kLeastTiles, p->how, q_aligned));
+    L2D_CUDA_TRY(launch(p->kernel.run, grid, p->kernel.threads, p->kernel.smem, stream, a, p->maps, p->scratch, p->m_tiles, kLeastTiles, p->how, q_aligned));
     return L2D_OK;
 }
 
