@@ -312,6 +312,7 @@ struct MmaCore {
     using Elem = T;
     static constexpr int kKeys = 16;                       // keys of a warp's tile
     static constexpr int kWarps = KS <= 8 ? 8 : 4;         // whose rings fit an SM
+    static constexpr bool kWholeRows = true;               // products reach the padding of a row
     static constexpr int kThreads = kWarps * 32;
     static constexpr int kRows = SPLIT ? 8 : 16;           // query heads
     static constexpr int kDim = KS * 16;                   // head_dim, padded
@@ -481,6 +482,7 @@ struct SimdCore {
     using Elem = float;
     static constexpr int kKeys = 8;
     static constexpr int kWarps = DV == 1 ? 8 : 4;
+    static constexpr bool kWholeRows = false;
     static constexpr int kThreads = kWarps * 32;
     static constexpr int kRows = GT;
     static constexpr int kDim = DV * 128;
@@ -595,7 +597,7 @@ struct SimdCore {
 
 // Shared memory of a block: the rings, stage by stage (the last one, which the first tiles of the next piece do
 // not need, is reused for the warps' sums at the end of a piece), queries, the
-// cores' own words, barriers, row offsets and live bits, maxima and sums.
+// cores' own words, barriers, live bits, maxima and sums.
 constexpr int kJoin = 64;  // pieces whose factors are held at a time when a sequence's pieces are joined
 template <typename Core, int STAGES>
 struct AttnSmem {
@@ -607,8 +609,7 @@ struct AttnSmem {
     static constexpr int kEnd = kFactors + 2 * kJoin * kMaxRows * 4;
     static constexpr int kQuery = kRing > kEnd ? kRing : kEnd;
     static constexpr int kWarp = kQuery + Core::kQueryBytes;
-    static constexpr int kRowAt = kWarp + Core::kWarps * Core::kWarpBytes;
-    static constexpr int kBars = kRowAt + Core::kWarps * Core::kKeys * 16;
+    static constexpr int kBars = kWarp + Core::kWarps * Core::kWarpBytes;
     static constexpr int kLive = kBars + Core::kWarps * STAGES * 8;
     static constexpr int kMl = kLive + Core::kWarps * STAGES * 4;
     static constexpr int kFlag = kMl + Core::kWarps * 2 * kMaxRows * 4;
@@ -632,19 +633,18 @@ struct Stream {
     int how, head;
     const int32_t *table;
     char *ring;
-    longlong2 *row_at;    // where the rows of the tile being started are, in bytes from k and v
     uint32_t bars;
     uint32_t *live;
     uint32_t phases;      // parity of each stage's barrier
     int64_t next;         // the first key of the tile whose pages are in `page`
     int lo, len, step;    // keys lo .. len - 1 count; keys between this warp's tiles
-    int slot, page;       // of this lane's key; of the tile's first key, with boxes
+    int slot, page;       // of this lane's key (lanes kLanes j .. kLanes j + kLanes - 1: key j); with boxes, of the tile's first
+    static constexpr int kLanes = 32 / Core::kKeys;
 
     __device__ __forceinline__ void lookup() {
-        const int lane = threadIdx.x & 31;
-        const int64_t key = how == kBoxes ? next : next + lane;
+        const int64_t key = how == kBoxes ? next : next + (threadIdx.x & 31) / kLanes;
         page = -2;  // no such key
-        if (key < len && (how == kBoxes ? key + Core::kKeys > lo : key >= lo && lane < Core::kKeys)) {
+        if (key < len && (how == kBoxes ? key + Core::kKeys : key + 1) > lo) {
             const unsigned i = page_index(c, static_cast<unsigned>(key));
             slot = static_cast<int>(static_cast<unsigned>(key) - i * static_cast<unsigned>(c.page_size));
             page = max(table[i], -1);
@@ -679,38 +679,36 @@ struct Stream {
                 }
             }
         } else {
-            const uint32_t bits = __ballot_sync(0xffffffffu, real);
+            // Bit kLanes j of the vote to bit j.
+            const uint32_t vote = __ballot_sync(0xffffffffu, real);
+            const uint32_t bits = __ballot_sync(0xffffffffu, lane < Core::kKeys && (vote >> (lane * kLanes & 31) & 1));
             if (lane == 0) live[stage] = bits;
             if (bits) {
                 constexpr int64_t eb = sizeof(T);
-                __syncwarp();  // the rows of the tile before have been read
-                if (lane < Core::kKeys)
-                    row_at[lane] = real ? make_longlong2((page * c.k_page + slot * c.k_slot + head * c.k_head) * eb,
-                                                         (page * c.v_page + slot * c.v_slot + head * c.v_head) * eb)
-                                        : make_longlong2(0, 0);
-                __syncwarp();
-                const uint32_t to = smem_addr(tile);
-                const int row_bytes = c.head_dim * static_cast<int>(eb);
+                const int r = lane / kLanes, first = lane % kLanes;
+                const char *k = c.k, *v = c.v;
+                if (real) {
+                    k += (page * c.k_page + slot * c.k_slot + head * c.k_head) * eb;
+                    v += (page * c.v_page + slot * c.v_slot + head * c.v_head) * eb;
+                }
                 if (how == kWords) {
+                    const int have = c.head_dim * static_cast<int>(eb) / 16, need = Core::kWholeRows ? Core::kDim / 8 : have;
+                    const uint32_t to = smem_addr(tile);
 #pragma unroll 4
-                    for (int e = lane; e < Core::kKeys * Core::kChunks; e += 32) {
-                        const int r = e / Core::kChunks, ch = e - r * Core::kChunks;
-                        const longlong2 at = row_at[r];
-                        const bool in = (bits >> r & 1) && ch * 16 < row_bytes;
+                    for (int ch = first; ch < need; ch += kLanes) {
+                        const bool in = real && ch < have;
                         const int off = in ? ch * 16 : 0;
-                        copy16(to + chunk_at<Core::kKeys>(r, ch), c.k + at.x + off, in);
-                        copy16(to + Sm::kTile + chunk_at<Core::kKeys>(r, ch), c.v + at.y + off, in);
+                        copy16(to + chunk_at<Core::kKeys>(r, ch), k + off, in);
+                        copy16(to + Sm::kTile + chunk_at<Core::kKeys>(r, ch), v + off, in);
                     }
                 } else {
                     constexpr int kPer = 16 / static_cast<int>(sizeof(T));
-                    for (int r = 0; r < Core::kKeys; ++r) {
-                        const longlong2 at = row_at[r];
-                        for (int i = lane; i < Core::kChunks * kPer; i += 32) {
-                            const bool in = (bits >> r & 1) && i < c.head_dim;
-                            const int dst = chunk_at<Core::kKeys>(r, i / kPer) + i % kPer * static_cast<int>(eb);
-                            *reinterpret_cast<T *>(tile + dst) = in ? reinterpret_cast<const T *>(c.k + at.x)[i] : dev::narrow<T>(0.0f);
-                            *reinterpret_cast<T *>(tile + Sm::kTile + dst) = in ? reinterpret_cast<const T *>(c.v + at.y)[i] : dev::narrow<T>(0.0f);
-                        }
+                    const int need = Core::kWholeRows ? Core::kDim : (c.head_dim + 3) / 4 * 4;
+                    for (int i = first; i < need; i += kLanes) {
+                        const bool in = real && i < c.head_dim;
+                        const int dst = chunk_at<Core::kKeys>(r, i / kPer) + i % kPer * static_cast<int>(eb);
+                        *reinterpret_cast<T *>(tile + dst) = in ? reinterpret_cast<const T *>(k)[i] : dev::narrow<T>(0.0f);
+                        *reinterpret_cast<T *>(tile + Sm::kTile + dst) = in ? reinterpret_cast<const T *>(v)[i] : dev::narrow<T>(0.0f);
                     }
                 }
             }
@@ -723,7 +721,7 @@ struct Stream {
     // The live bits of a stage, once its copies are there.  Values of keys that do not count are made zeros, as
     // their weights are: slots that were never written may hold anything.
     __device__ __forceinline__ uint32_t take(int stage) {
-        if (how != kBoxes) copies_wait<STAGES - 2>();
+        if (how != kBoxes) copies_wait<STAGES - 1>();
         __syncwarp();
         const uint32_t bits = live[stage];
         if (how == kBoxes && bits) {
@@ -939,7 +937,6 @@ __global__ void __launch_bounds__(Core::kThreads, 1) k_attn(const __grid_constan
     const float scale2 = fabsf(a.scale) * 1.4426950408889634f;  // a negative one turns the queries' signs
     Stream<Core, STAGES> in{a.c, maps, how};
     in.ring = smem + warp * Sm::kStage;
-    in.row_at = reinterpret_cast<longlong2 *>(smem + Sm::kRowAt) + warp * Core::kKeys;
     in.bars = smem_addr(smem + Sm::kBars) + warp * STAGES * 8;
     in.live = reinterpret_cast<uint32_t *>(smem + Sm::kLive) + warp * STAGES;
     in.phases = 0;
@@ -994,8 +991,9 @@ __global__ void __launch_bounds__(Core::kThreads, 1) k_attn(const __grid_constan
         int stage = 0;
 #pragma unroll 1
         for (int i = 0; i < p.n; ++i) {
+            __syncwarp();  // every lane is done with the stage before this one
+            in.issue(stage == 0 ? STAGES - 1 : stage - 1);
             const uint32_t live = in.take(stage);
-            in.issue(stage == 0 ? STAGES - 1 : stage - 1);  // every lane is done with that one: take()
             const char *ks = in.ring + stage * (Core::kWarps * Sm::kStage);
             if (live) core.step(ks, ks + Sm::kTile, live, scale2);
             stage = stage + 1 == STAGES ? 0 : stage + 1;
@@ -1159,7 +1157,8 @@ using namespace l2d;
 
 namespace l2d {
 
-// A tensor map over keys or values: boxes of 128 bytes by `keys` slots of one head in one page.
+// A tensor map over keys or values: boxes of 128 bytes by `keys` slots of one head in one page.  Fetching 256 bytes
+// at a time into L2 costs 20 % where a row has only 128 (32 x 4096 keys of 64 fp16 elements: 127 us, 104 us without).
 bool encode_map(CUtensorMap *map, void *base, int dtype, const Cache &c, int64_t head, int64_t slot, int64_t page, int keys) {
     static const auto encode = [] {
         void *f = nullptr;
@@ -1176,7 +1175,7 @@ bool encode_map(CUtensorMap *map, void *base, int dtype, const Cache &c, int64_t
     const CUtensorMapDataType type = dtype == L2D_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : dtype == L2D_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                                                                         : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     return encode(map, type, 4, base, sizes, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+                  c.head_dim * eb >= 256 ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 }  // namespace l2d
