@@ -451,10 +451,16 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
         struct Raw {
             uint4 lo, hi;
         };
-        auto fetch = [&](int e) {
+        struct Unit {
+            int v, half;
+        };
+        auto step = [&](Unit &e) {
+            for (e.half += kQ4Warps * 2; e.half >= halves; e.half -= halves) ++e.v;
+        };
+        auto fetch = [&](const Unit &e) {
             Raw r = {};
-            if (e >= units) return r;
-            const int v = e / halves, col = (first + e - v * halves) * kQ4Half + 8 * u, size = a.dtype_x == L2D_F32 ? 4 : 2;
+            if (e.v >= a.vectors) return r;
+            const int v = e.v, col = (first + e.half) * kQ4Half + 8 * u, size = a.dtype_x == L2D_F32 ? 4 : 2;
             const char *src = static_cast<const char *>(a.x) + (v * a.stride_x + col) * size;
             if (col + 8 <= a.N && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
                 r.lo = __ldg(reinterpret_cast<const uint4 *>(src));
@@ -472,12 +478,58 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
             r.hi = make_uint4(w[4], w[5], w[6], w[7]);
             return r;
         };
-        Raw ahead = fetch(warp * 2 + (lane >> 4));
-        for (int e = warp * 2 + (lane >> 4); e - (lane >> 4) < units; e += kQ4Warps * 2) {
+        const int mine = warp * 2 + (lane >> 4);
+        Unit at = {mine / halves, mine % halves};
+        Raw ahead = fetch(at);
+        for (int e = mine; e - (lane >> 4) < units; e += kQ4Warps * 2) {
             const Raw r = ahead;
-            ahead = fetch(e + kQ4Warps * 2);
             const bool real = e < units;
-            const int v = real ? e / halves : 0, half = real ? e - v * halves : 0;
+            const int v = real ? at.v : 0, half = real ? at.half : 0, column = v * a.parts, tt = u >> 2, j = u & 3;
+            float2 *to = sums + half * 8 * NT + (column << kShift) + u / (16 / SUB);
+            const bool stores_sums = real && u % (16 / SUB) == 0;
+            step(at);
+            ahead = fetch(at);
+            if constexpr (KIND == kQ4Fast) {  // 16-bit inputs: the same as below in fewer instructions
+                uint32_t w[4] = {r.lo.x, r.lo.y, r.lo.z, r.lo.w};
+                const bool is_fp16 = a.dtype_x == L2D_F16;
+                const uint32_t inf = is_fp16 ? 0x7c00u : 0x7f80u;
+                auto largest = [&] {
+                    const uint32_t m = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+                    return max(m & 0xffffu, m >> 16);
+                };
+                uint32_t top = largest();
+                const uint32_t odd_votes = __ballot_sync(0xffffffffu, top >= inf);
+                const bool odd = odd_votes >> (lane & 16) & 0xffff;
+                any_odd = any_odd || (real && odd);
+                if (odd_votes) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if ((w[i] & 0x7fffu) >= inf) w[i] &= 0xffff0000u;
+                        if ((w[i] >> 16 & 0x7fffu) >= inf) w[i] &= 0xffffu;
+                    }
+                    top = largest();
+                }
+#pragma unroll
+                for (int d = 1; d < 16; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+                const uint32_t p = min(268u - (__float_as_uint(scale_value(top, false, is_fp16)) >> 23), 254u);
+                const float up = __uint_as_float(p << 23), back = __uint_as_float((266u - p) << 23);
+                float f[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) f[i] = scale_value(w[i / 2], i & 1, is_fp16) * up;
+                uint32_t out[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const __half2 h = i & 1 ? __floats2half2_rn(f[i] * 0.0625f, f[i + 4] * 0.0625f) : __floats2half2_rn(f[i], f[i + 4]);
+                    memcpy(&out[i], &h, 4);
+                }
+                // Of the values as they were: what rounding takes off the smallest is below 2^-39 of the largest.
+                float total = ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
+#pragma unroll
+                for (int d = 1; d < 16 / SUB; d <<= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+                if (real) reinterpret_cast<uint4 *>(smem + (half * columns + column) * kColumn)[j * 4 + tt] = make_uint4(out[0], out[1], out[2], out[3]);
+                if (stores_sums) to[0] = make_float2(total * 0x1p-24f, odd ? -back : back);  // the sign: see add_odd_ones()
+                continue;
+            }
             const uint32_t raw[8] = {r.lo.x, r.lo.y, r.lo.z, r.lo.w, r.hi.x, r.hi.y, r.hi.z, r.hi.w};
             float f[8];
             uint32_t top = 0;
@@ -493,9 +545,6 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
             for (int d = 1; d < 16; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
             const bool odd = __ballot_sync(0xffffffffu, odd_ones) >> (lane & 16) & 0xffff;  // in these 128 columns
             any_odd = any_odd || (real && odd);
-            const int column = v * a.parts, tt = u >> 2, j = u & 3;
-            float2 *to = sums + half * 8 * NT + (column << kShift) + u / (16 / SUB);
-            const bool stores_sums = real && u % (16 / SUB) == 0;
             if constexpr (BYTES) {
                 // 2^(p - 127) takes the largest to [2^29, 2^30); four signed digits of 8 bits, a column each.
                 const uint32_t p = min(283u - (top >> 23), 253u);
