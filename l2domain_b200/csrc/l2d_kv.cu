@@ -724,7 +724,7 @@ struct Stream {
     // The live bits of a stage, once its copies are there.  Values of keys that do not count are made zeros, as
     // their weights are: slots that were never written may hold anything.
     __device__ __forceinline__ uint32_t take(int stage) {
-        if (how != kBoxes) copies_wait<STAGES - 1>();
+        if (how != kBoxes) copies_wait<STAGES - 2>();
         __syncwarp();
         const uint32_t bits = live[stage];
         if (how == kBoxes && bits) {
@@ -887,6 +887,11 @@ __global__ void __launch_bounds__(Core::kThreads, 1) k_attn(const __grid_constan
     int *flag = reinterpret_cast<int *>(smem + Sm::kFlag);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int D = a.c.head_dim, G = a.heads_q / a.c.heads, items = a.c.heads * m_tiles;
+    // What needs nothing of the kernels before: the maps' way to the copy unit, and the barriers.
+    const uint32_t bars = smem_addr(smem + Sm::kBars) + warp * STAGES * 8;
+    if (how == kBoxes && tid < 2) asm volatile("prefetch.tensormap [%0];" ::"l"(tid ? &maps.v : &maps.k) : "memory");
+    if (lane < STAGES) barrier_init(bars + 8 * lane);
+    before_boxes();
     dev::wait_for_previous();
 
     // All tiles of one head, and rows without a position.
@@ -940,11 +945,9 @@ __global__ void __launch_bounds__(Core::kThreads, 1) k_attn(const __grid_constan
     const float scale2 = fabsf(a.scale) * 1.4426950408889634f;  // a negative one turns the queries' signs
     Stream<Core, STAGES> in{a.c, maps, how};
     in.ring = smem + warp * Sm::kStage;
-    in.bars = smem_addr(smem + Sm::kBars) + warp * STAGES * 8;
+    in.bars = bars;
     in.live = reinterpret_cast<uint32_t *>(smem + Sm::kLive) + warp * STAGES;
     in.phases = 0;
-    if (lane < STAGES) barrier_init(in.bars + 8 * lane);
-    before_boxes();
     __syncwarp();
     // What a block does at a time: some tiles of one head group of a sequence.
     struct Piece {
@@ -994,9 +997,8 @@ __global__ void __launch_bounds__(Core::kThreads, 1) k_attn(const __grid_constan
         int stage = 0;
 #pragma unroll 1
         for (int i = 0; i < p.n; ++i) {
-            __syncwarp();  // every lane is done with the stage before this one
-            in.issue(stage == 0 ? STAGES - 1 : stage - 1);
             const uint32_t live = in.take(stage);
+            in.issue(stage == 0 ? STAGES - 1 : stage - 1);  // every lane is done with that one: take()
             const char *ks = in.ring + stage * (Core::kWarps * Sm::kStage);
             if (live) core.step(ks, ks + Sm::kTile, live, scale2);
             stage = stage + 1 == STAGES ? 0 : stage + 1;
