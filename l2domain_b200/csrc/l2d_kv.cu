@@ -1147,8 +1147,8 @@ int check_cache(const l2d_kv_cache *cache, Cache *c) {
         return set_error(L2D_ERR_INVALID, "cache strides overlap (the least of them is %lld elements)", static_cast<long long>(least));
     const int64_t most = std::max({c->k_page, c->v_page, c->k_slot, c->v_slot, c->k_head, c->v_head, c->table_stride});
     if (most > (int64_t(1) << 40)) return set_error(L2D_ERR_INVALID, "cache strides too large");
-    const bool used = k.num_seqs && k.table_width && k.num_pages;
-    if (used && (!k.k || !k.v || !k.table)) return set_error(L2D_ERR_INVALID, "null cache pointer");
+    const bool used = k.num_seqs && k.table_width;  // the table is read then, and pages where there are any
+    if (used && (!k.table || (k.num_pages && (!k.k || !k.v)))) return set_error(L2D_ERR_INVALID, "null cache pointer");
     const uintptr_t align = elem_bytes(k.dtype) - 1;
     if ((reinterpret_cast<uintptr_t>(k.k) & align) || (reinterpret_cast<uintptr_t>(k.v) & align) ||
         (reinterpret_cast<uintptr_t>(k.table) & 3) || (reinterpret_cast<uintptr_t>(k.status) & 3))

@@ -65,6 +65,7 @@ def call(op, cache=None, table=None, desc=None, **kw):
     (dict(k_strides=(2048, 63, 64)), {}, INVALID, "strides"), (dict(v_strides=(-1, 128, 64)), {}, INVALID, "strides"),
     ({}, dict(table_stride=3), INVALID, "strides"), (dict(k_strides=(1 << 41, 128, 64)), {}, INVALID, "too large"),
     (dict(k=None), {}, INVALID, "null"), (dict(v=None), {}, INVALID, "null"), ({}, dict(table=None), INVALID, "null"),
+    (dict(num_pages=0), dict(table=None), INVALID, "null"),
     (dict(k=PTR + 1), {}, INVALID, "aligned"), (dict(v=PTR + 1), {}, INVALID, "aligned"),
     ({}, dict(table=PTR + 2), INVALID, "aligned"), ({}, dict(status=PTR + 1), INVALID, "aligned"),
 ])

@@ -168,6 +168,30 @@ def test_q4_vector_alone_equals_vector_in_company():
     assert torch.equal(both, again)
 
 
+@pytest.mark.parametrize("vectors", [1, 3, 9])
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("dt,dt_y", [(L.F32, L.F32), (L.BF16, L.F32)])
+def test_q4_one_sided_activations_do_not_cancel(vectors, group, dt, dt_y):
+    """Activations around 100: the sums of q x and of z x are hundreds of times the result.  An fp32 result is held to
+    the rounding of sums of (q - z) x themselves: at most 8 products in a row in a matrix instruction's sum, each off
+    by 2u of what it holds, and 2048 / 128 + 16 additions of groups' sums."""
+    w, s, z, x = q4_case(150, 2048, group, dt, vectors, True, seed=7)
+    x = (x.float() + 100).to(TORCH[dt])
+    y = torch.empty(vectors, 150, dtype=TORCH[dt_y], device="cuda")
+    L.Q4Matrix(w, s, 150, 2048, group, zeros=z, dtype_x=dt, dtype_y=dt_y, ldw=w.stride(0), lds=s.stride(0)).gemv(x, y, vectors=vectors)
+    want, total = q4_exact(w, s, z, x, 2048, group)
+    close(y, want, 2 * U * (8 + 2048 / 128 + 16) * total, dt_y)
+
+
+@pytest.mark.parametrize("N,group", [(4096, 128), (2048, 64), (1536, 32), (4096, 512), (4224, 384), (11008, 128), (5120, 256)])
+@pytest.mark.parametrize("vectors", [1, 2, 6])
+def test_q4_whole_steps_and_remainders(N, group, vectors):
+    """Rows of whole 512-column steps and of steps and a rest, with scales read in words and by twos."""
+    for zeros in (False, True):
+        for dt in (L.F16, L.F32):
+            q4_check(*q4_case(600, N, group, dt, vectors, zeros, L.BF16, seed=N), N, group, dt, dt_s=L.BF16)
+
+
 # ------------------------------------------------------------------------------------------------
 # The paged cache
 # ------------------------------------------------------------------------------------------------
@@ -308,6 +332,40 @@ def test_attention_slots_past_the_end_may_hold_anything(dt):
     P.table[2, :] = 1 << 30
     got = attn_check(P, lens, 8, dt, window=window)
     assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
+
+
+@pytest.mark.parametrize("dt", [L.F32, L.BF16])
+@pytest.mark.parametrize("page", [16, 10])
+def test_attention_does_not_look_up_pages_before_the_window(dt, page):
+    """A sliding window's old pages may have been given back: their entries are never used."""
+    P = Pages(dt, 3, 40, page, 2, 64, seed=13)
+    lens, window = [390, 200, 77], 50
+    want = attn_check(P, lens, 4, dt, window=window)
+    for b, n in enumerate(lens):
+        P.table[b, : (n - window) // page] = -1
+        P.table[b, -(-n // page):] = -1
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    plan = L.PagedAttention(P.cache(), P.table, P.seqs, P.width, 4, window=window, status=status)
+    got = attn_check(P, lens, 4, dt, window=window, plan=plan)
+    assert status.item() == 0 and torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
+
+
+@pytest.mark.parametrize("dt", [L.F32, L.BF16])
+def test_cache_without_pages_reports_every_key(dt):
+    """A table that points into a cache of no pages: nothing is read, the rows are empty and the status says so."""
+    table = torch.zeros(2, 3, dtype=torch.int32, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    cache = L.KvCache(None, None, dt, 0, 16, 1, 64)
+    q, lens = normal(gen(1), dt, 2, 2, 64), torch.tensor([40, 0], dtype=torch.int32, device="cuda")
+    out, lse = torch.ones_like(q), torch.zeros(2, 2, device="cuda")
+    L.PagedAttention(cache, table, 2, 3, 2, status=status).decode(q, out, lens, 2, lse=lse)
+    torch.cuda.synchronize()
+    assert status.item() == L.KV_BAD_PAGE and (out == 0).all() and (lse == -math.inf).all()
+    status.zero_()
+    k = normal(gen(2), dt, 2, 1, 64)
+    L.KvAppend(cache, table, 2, 3, status=status).append(k, k, lens, 2)
+    torch.cuda.synchronize()
+    assert status.item() == L.KV_BAD_PAGE
 
 
 @pytest.mark.parametrize("dt", [L.F32, L.F16, L.BF16])
