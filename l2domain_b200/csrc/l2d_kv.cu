@@ -642,24 +642,25 @@ struct Stream {
     int64_t next;         // the first key of the tile whose pages are in `page`
     int lo, len, step;    // keys lo .. len - 1 count; keys between this warp's tiles
     int slot, page;       // of this lane's key (lanes kLanes j .. kLanes j + kLanes - 1: key j); with boxes, of the tile's first
+    bool wanted;          // that key, or one of the tile's, counts
     static constexpr int kLanes = 32 / Core::kKeys;
 
+    // The entry is not looked at before the next tile is started: an instruction that used it here would wait for
+    // it, and the products with it.
     __device__ __forceinline__ void lookup() {
         const int64_t key = how == kBoxes ? next : next + (threadIdx.x & 31) / kLanes;
-        page = -2;  // no such key
-        if (key < len && (how == kBoxes ? key + Core::kKeys : key + 1) > lo) {
-            const unsigned i = page_index(c, static_cast<unsigned>(key));
-            slot = static_cast<int>(static_cast<unsigned>(key) - i * static_cast<unsigned>(c.page_size));
-            page = max(table[i], -1);
-        }
+        wanted = key < len && (how == kBoxes ? key + Core::kKeys : key + 1) > lo;
+        const unsigned i = page_index(c, static_cast<unsigned>(key));
+        slot = static_cast<int>(static_cast<unsigned>(key) - i * static_cast<unsigned>(c.page_size));
+        if (wanted) page = __ldg(table + i);
     }
 
     // Starts the copies of the next tile into a stage of the ring.
     __device__ __forceinline__ void issue(int stage) {
         const int lane = threadIdx.x & 31;
         constexpr uint32_t kAll = (1u << Core::kKeys) - 1;
-        const bool real = page >= 0 && page < c.num_pages;
-        if (!real && page != -2) report(c.status, L2D_KV_BAD_PAGE);
+        const bool real = wanted && page >= 0 && page < c.num_pages;
+        if (wanted && !real) report(c.status, L2D_KV_BAD_PAGE);
         char *tile = ring + stage * (Core::kWarps * Sm::kStage);
         if (how == kBoxes) {
             uint32_t bits = 0;
@@ -948,6 +949,7 @@ __global__ void __launch_bounds__(Core::kThreads, 1) k_attn(const __grid_constan
     in.bars = bars;
     in.live = reinterpret_cast<uint32_t *>(smem + Sm::kLive) + warp * STAGES;
     in.phases = 0;
+    in.page = -1;
     __syncwarp();
     // What a block does at a time: some tiles of one head group of a sequence.
     struct Piece {
