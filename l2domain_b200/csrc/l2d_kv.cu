@@ -197,18 +197,19 @@ __global__ void __launch_bounds__(kAppendThreads) k_append(const __grid_constant
 // ---------------------------------------------------------------------------------------------
 // Attention of one token over the cache.
 //
-// Memory bound: each key and value is read once, for all query heads of its group.  A block of four
-// warps works on one key-value head of one sequence at a time; each warp streams its own 16 keys of
-// every 64 through a ring of shared memory of its own (no block-wide barrier in the loop) and keeps a
-// running maximum and sum per query head, so the data is passed over once.  16-bit caches feed matrix
+// Memory bound: each key and value is read once, for all query heads of its group.  A block of
+// eight warps (four for heads of more than 128 elements, whose rings would not fit) works on one
+// key-value head of one sequence at a time; each warp streams its own 16 keys (8 of 32 bits) of every 128
+// through a ring of shared memory of its own (no block-wide barrier in the loop) and keeps a running
+// maximum and sum per query head, so the data is passed over once.  16-bit caches feed matrix
 // instructions with the query heads as the 16 rows; 32-bit caches use fp32 fused multiply-adds.
 //
 // A tile of 16 keys that lies in one page is one box of a tensor map over the cache (elements, heads,
 // slots, pages), and one thread starts its copies; with a page size that is no multiple of 16, or rows off
 // 16-byte boundaries, the lanes look up the page of each key and copy its rows themselves.
 //
-// The tiles of all sequences and heads form one line that is cut into equal pieces, one per resident
-// block, whatever the lengths are: a long sequence is split over many blocks and a block may take
+// The tiles of all sequences and heads, and kSwitch units before each head's, form one line that is cut into
+// equal pieces, one per resident block, whatever the lengths are: a long sequence is split over many blocks and a block may take
 // several short ones.  A piece that ends inside a sequence leaves its unnormalised sums in the plan's
 // scratch, and the last piece of that sequence to arrive adds them in piece order, so the result does
 // not depend on which block came last.
@@ -219,6 +220,13 @@ constexpr int kMaxRows = 16;    // query heads a block works on
 // (one sequence, 8 key-value heads of 128: 300 keys 8.7 us whole and 9.8 us split, 500 keys 10.2 and 9.9, 1000 keys
 // 15.1 and 10.1).
 constexpr int kWholeTiles = 3;
+// What a block spends on a head of a sequence besides its tiles (finding it, its first pages and queries, the sum over
+// the warps), as so many tiles of the line that the blocks share evenly.  With none, blocks of many short sequences end
+// last; 0, 1, 2, 3, 4 (8 key-value heads of 128, ragged): 64 x 8192 keys 195, 180, 174, 172, 172 us; 32 x 4000 71, 56,
+// 53, 52, 52; 100 x 1000 82, 62, 56, 57, 57; 200 x 300 77, 66, 63, 65, 66; equal lengths 64 x 2048 89, 92, 90, 91, 92.
+constexpr int kSwitch = 2;
+
+__host__ __device__ __forceinline__ int64_t units_of(int64_t tiles) { return tiles ? tiles + kSwitch : 0; }
 
 struct AttnScratch {
     float *part;         // [grid][2][kMaxRows][head_dim padded] unnormalised sums
@@ -895,12 +903,12 @@ __global__ void __launch_bounds__(Core::kThreads, 1) k_attn(const __grid_constan
     before_boxes();
     dev::wait_for_previous();
 
-    // All tiles of one head, and rows without a position.
+    // All units of one head, and rows without a position.
     int64_t total = 0;
     int longest = 0;
     for (int b = lane; b < a.batch; b += 32) {
         const int n = span_of<TILE>(a, b).tiles;
-        total += n;
+        total += units_of(n);
         longest = max(longest, n);
     }
 #pragma unroll
@@ -916,16 +924,15 @@ __global__ void __launch_bounds__(Core::kThreads, 1) k_attn(const __grid_constan
             for (int h = tid; h < a.heads_q; h += Core::kThreads) a.lse[static_cast<int64_t>(b) * a.heads_q + h] = -INFINITY;
     }
 
-    // This block's piece of the line of tiles, and the sequence it starts in (every warp looks for itself).
+    // This block's piece of the line of units, and the sequence it starts in (every warp looks for itself).
     total *= items;
-    const int64_t per = max(quotient(total + gridDim.x - 1, gridDim.x), static_cast<int64_t>(longest <= kWholeTiles ? longest : 1));
-    int64_t u = blockIdx.x * per;
-    const int64_t first_unit = u, stop = min(total, u + per);
-    if (u >= stop) return;
-    int64_t before = 0;  // tiles of one head in the sequences before b
+    const int64_t per = max(quotient(total + gridDim.x - 1, gridDim.x), longest <= kWholeTiles ? units_of(longest) : 1);
+    const int64_t first_unit = blockIdx.x * per, stop = min(total, first_unit + per);
+    if (first_unit >= stop) return;
+    int64_t before = 0;  // units of one head in the sequences before b
     int b = 0;
     for (;; b += 32) {
-        const int64_t n = b + lane < a.batch ? span_of<TILE>(a, b + lane).tiles : 0;
+        const int64_t n = b + lane < a.batch ? units_of(span_of<TILE>(a, b + lane).tiles) : 0;
         int64_t upto = n;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -933,7 +940,7 @@ __global__ void __launch_bounds__(Core::kThreads, 1) k_attn(const __grid_constan
             if (lane >= d) upto += x;
         }
         upto += before;
-        const unsigned found = __ballot_sync(0xffffffffu, n && u < upto * items);
+        const unsigned found = __ballot_sync(0xffffffffu, n && first_unit < upto * items);
         if (found) {
             const int l = __ffs(found) - 1;
             before = __shfl_sync(0xffffffffu, upto - n, l);
@@ -951,26 +958,33 @@ __global__ void __launch_bounds__(Core::kThreads, 1) k_attn(const __grid_constan
     in.phases = 0;
     in.page = -1;
     __syncwarp();
-    // What a block does at a time: some tiles of one head group of a sequence.
+    // What a block does at a time: n tiles from t0 of one head group of a sequence, whose first tile is unit u0.
     struct Piece {
         Span s;
         int b, item, t0, n, head0, rows;
+        int64_t u0;
     };
-    auto find = [&](int64_t at_unit) {
+    auto find = [&](int64_t at_unit) {  // the first piece from that unit on; n = 0: none
         Piece p;
-        for (;; ++b) {
+        p.n = 0;
+        while (at_unit < stop) {
             p.s = span_of<TILE>(a, b);
-            if (at_unit - before * items < static_cast<int64_t>(p.s.tiles) * items) break;
-            before += p.s.tiles;
+            const int64_t units = units_of(p.s.tiles), at = at_unit - before * items;
+            if (at >= units * items) {
+                before += units;
+                ++b;
+                continue;
+            }
+            p.b = b;
+            p.item = static_cast<int>(quotient(at, units));
+            p.u0 = before * items + p.item * units + kSwitch;
+            p.t0 = static_cast<int>(max(at_unit - p.u0, static_cast<int64_t>(0)));
+            p.n = static_cast<int>(max(min(static_cast<int64_t>(p.s.tiles), stop - p.u0) - p.t0, static_cast<int64_t>(0)));
+            const int hk = p.item / m_tiles, row0 = (p.item - hk * m_tiles) * Core::kRows;
+            p.rows = min(G - row0, Core::kRows);
+            p.head0 = hk * G + row0;
+            break;  // without a tile it is at its end
         }
-        const int64_t at = at_unit - before * items;
-        p.b = b;
-        p.item = static_cast<int>(quotient(at, p.s.tiles));
-        p.t0 = static_cast<int>(at - static_cast<int64_t>(p.item) * p.s.tiles);
-        p.n = static_cast<int>(min(static_cast<int64_t>(p.s.tiles - p.t0), stop - at_unit));
-        const int hk = p.item / m_tiles, row0 = (p.item - hk * m_tiles) * Core::kRows;
-        p.rows = min(G - row0, Core::kRows);
-        p.head0 = hk * G + row0;
         return p;
     };
     auto start = [&](const Piece &p) {  // its first tiles
@@ -990,7 +1004,8 @@ __global__ void __launch_bounds__(Core::kThreads, 1) k_attn(const __grid_constan
     };
 
     Core core;
-    Piece p = find(u);
+    Piece p = find(first_unit);
+    if (p.n == 0) return;
     start(p);
     stage_query(p);
     __syncthreads();
@@ -1007,14 +1022,11 @@ __global__ void __launch_bounds__(Core::kThreads, 1) k_attn(const __grid_constan
         }
         if (how != kBoxes) copies_wait<0>();
         // The next piece's first tiles are on their way while this one's sums meet.
-        const bool more = u + p.n < stop;
-        Piece following = p;
+        Piece following = find(p.u0 + p.t0 + p.n);
+        const bool more = following.n;
         before_boxes();
         __syncwarp();
-        if (more) {
-            following = find(u + p.n);
-            start(following);
-        }
+        if (more) start(following);
         __syncthreads();
         if (more) stage_query(following);
 
@@ -1025,7 +1037,7 @@ __global__ void __launch_bounds__(Core::kThreads, 1) k_attn(const __grid_constan
         core.end(sums + warp * Core::kRows * Core::kDim, sm_m + warp * kMaxRows, sm_l + warp * kMaxRows);
         __syncthreads();
         const bool whole = n == s.tiles;
-        const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + (u != first_unit);
+        const int64_t u0 = p.u0, slot = static_cast<int64_t>(blockIdx.x) * 2 + (u0 + t0 != first_unit);
         constexpr int kRowQuads = Core::kDim / 4;
         for (int q = tid; q < rows * kRowQuads; q += Core::kThreads) {
             const int r = q / kRowQuads, i = (q - r * kRowQuads) * 4;
@@ -1054,7 +1066,6 @@ __global__ void __launch_bounds__(Core::kThreads, 1) k_attn(const __grid_constan
             }
         }
         if (!whole) {
-            const int64_t u0 = u - t0;
             const int c0 = static_cast<int>(quotient(u0, per)), c1 = static_cast<int>(quotient(u0 + s.tiles - 1, per));
             __threadfence();
             __syncthreads();
@@ -1073,7 +1084,6 @@ __global__ void __launch_bounds__(Core::kThreads, 1) k_attn(const __grid_constan
         before_boxes();
         __syncthreads();  // the last stage holds sums until here
         if (!more) break;
-        u += n;
         p = following;
     }
 }
@@ -1359,7 +1369,7 @@ int l2d_attn_decode(l2d_attn_plan *p, const void *q, void *out, float *lse, cons
     const bool q_aligned = !misaligned(q, 16) && (p->desc.q_token * eb) % 16 == 0 && (p->cache.head_dim * eb) % 16 == 0;
     // No more blocks than pieces the page table leaves room for.
     const int64_t room = int64_t(p->cache.table_width) * p->cache.page_size, tiles = (room + p->kernel.tile - 1) / p->kernel.tile;
-    const int64_t most = (tiles <= kWholeTiles ? 1 : tiles) * batch * p->cache.heads * p->m_tiles;
+    const int64_t most = (tiles <= kWholeTiles ? 1 : units_of(tiles)) * batch * p->cache.heads * p->m_tiles;
     const dim3 grid(static_cast<unsigned>(std::min<int64_t>(p->grid, most)));
     AttnArgs a = {p->cache, q, out, lse, lens, p->desc.q_token, p->desc.out_token, p->desc.heads_q, p->desc.window, batch, p->desc.scale};
     L2D_CUDA_TRY(launch(p->kernel.run, grid, p->kernel.threads, p->kernel.smem, stream, a, p->maps, p->scratch, p->m_tiles, p->how, q_aligned));
