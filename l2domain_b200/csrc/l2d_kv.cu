@@ -216,9 +216,10 @@ __global__ void __launch_bounds__(kAppendThreads) k_append(const __grid_constant
 // ---------------------------------------------------------------------------------------------
 
 constexpr int kMaxRows = 16;    // query heads a block works on
-// Sequences of up to so many tiles are not split: a tile takes about 1.2 us of its block, and joining pieces 4 us
-// (one sequence, 8 key-value heads of 128: 300 keys 8.7 us whole and 9.8 us split, 500 keys 10.2 and 9.9, 1000 keys
-// 15.1 and 10.1).
+// Heads of sequences of up to so many tiles are not split, the block in whose piece their first unit lies does them
+// whole: a tile takes about 1.2 us of its block, and joining pieces 4 us (8 key-value heads of 128; one sequence of 300
+// keys 8.4 us whole and 9.8 us split, of 500 keys 9.8 and 9.6, of 1000 keys 14.3 and 9.9; ragged 30 x 380 with 4 heads
+// 10.2 and 15.5, 200 x 300 61 and 63; ragged 100 x 1000 is 56.5 us with 3 here, 54.8 with 5).
 constexpr int kWholeTiles = 3;
 // What a block spends on a head of a sequence besides its tiles (finding it, its first pages and queries, the sum over
 // the warps), as so many tiles of the line that the blocks share evenly.  With none, blocks of many short sequences end
@@ -905,17 +906,9 @@ __global__ void __launch_bounds__(Core::kThreads, 1) k_attn(const __grid_constan
 
     // All units of one head, and rows without a position.
     int64_t total = 0;
-    int longest = 0;
-    for (int b = lane; b < a.batch; b += 32) {
-        const int n = span_of<TILE>(a, b).tiles;
-        total += units_of(n);
-        longest = max(longest, n);
-    }
+    for (int b = lane; b < a.batch; b += 32) total += units_of(span_of<TILE>(a, b).tiles);
 #pragma unroll
-    for (int d = 16; d; d >>= 1) {
-        total += __shfl_xor_sync(0xffffffffu, total, d);
-        longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, d));
-    }
+    for (int d = 16; d; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
     for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
         if (tid == 0 && a.lens[b] > a.c.table_width * a.c.page_size) report(a.c.status, L2D_KV_BAD_PAGE);
         if (span_of<TILE>(a, b).tiles) continue;
@@ -926,7 +919,7 @@ __global__ void __launch_bounds__(Core::kThreads, 1) k_attn(const __grid_constan
 
     // This block's piece of the line of units, and the sequence it starts in (every warp looks for itself).
     total *= items;
-    const int64_t per = max(quotient(total + gridDim.x - 1, gridDim.x), longest <= kWholeTiles ? units_of(longest) : 1);
+    const int64_t per = max(quotient(total + gridDim.x - 1, gridDim.x), static_cast<int64_t>(1));
     const int64_t first_unit = blockIdx.x * per, stop = min(total, first_unit + per);
     if (first_unit >= stop) return;
     int64_t before = 0;  // units of one head in the sequences before b
@@ -978,8 +971,17 @@ __global__ void __launch_bounds__(Core::kThreads, 1) k_attn(const __grid_constan
             p.b = b;
             p.item = static_cast<int>(quotient(at, units));
             p.u0 = before * items + p.item * units + kSwitch;
-            p.t0 = static_cast<int>(max(at_unit - p.u0, static_cast<int64_t>(0)));
-            p.n = static_cast<int>(max(min(static_cast<int64_t>(p.s.tiles), stop - p.u0) - p.t0, static_cast<int64_t>(0)));
+            if (p.s.tiles <= kWholeTiles) {
+                if (at_unit > p.u0 - kSwitch) {  // the block before has it
+                    at_unit = p.u0 + p.s.tiles;
+                    continue;
+                }
+                p.t0 = 0;
+                p.n = p.s.tiles;
+            } else {
+                p.t0 = static_cast<int>(max(at_unit - p.u0, static_cast<int64_t>(0)));
+                p.n = static_cast<int>(max(min(static_cast<int64_t>(p.s.tiles), stop - p.u0) - p.t0, static_cast<int64_t>(0)));
+            }
             const int hk = p.item / m_tiles, row0 = (p.item - hk * m_tiles) * Core::kRows;
             p.rows = min(G - row0, Core::kRows);
             p.head0 = hk * G + row0;
