@@ -339,15 +339,14 @@ struct MmaCore {
     uint32_t query;
 
     // q: this group's first head; `heads` rows are real, `flip` takes their negatives.  All threads of the block call
-    // it, and a barrier before begin().
+    // it, and wait for their copies (copies_wait) and for each other before begin().
     static __device__ __forceinline__ void stage_query(const T *q, int heads, int D, bool aligned, bool flip, char *smem_q) {
-        const uint32_t sign = flip ? 0x80008000u : 0u;
-        if (aligned) {
+        const uint16_t sign = flip ? 0x8000 : 0;
+        if (aligned && !flip) {
             for (int e = threadIdx.x; e < kRows * KS * 2; e += kThreads) {
                 const int r = e / (KS * 2), ch = e - r * (KS * 2);
-                uint4 x = make_uint4(0, 0, 0, 0);
-                if (r < heads && ch * 8 < D) x = *reinterpret_cast<const uint4 *>(q + r * D + ch * 8);
-                *reinterpret_cast<uint4 *>(smem_q + r * kPitch + ch * 16) = make_uint4(x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign);
+                const bool real = r < heads && ch * 8 < D;
+                copy16(smem_addr(smem_q + r * kPitch + ch * 16), real ? q + r * D + ch * 8 : q, real);
             }
         } else {
             for (int e = threadIdx.x; e < kRows * kDim; e += kThreads) {
@@ -508,7 +507,15 @@ struct SimdCore {
     float *weights;
     int chunks;
 
-    static __device__ __forceinline__ void stage_query(const float *q, int heads, int D, bool, bool flip, char *smem_q) {
+    static __device__ __forceinline__ void stage_query(const float *q, int heads, int D, bool aligned, bool flip, char *smem_q) {
+        if (aligned && !flip) {
+            for (int e = threadIdx.x; e < GT * kDim / 4; e += kThreads) {
+                const int r = e / (kDim / 4), i = (e - r * (kDim / 4)) * 4;
+                const bool real = r < heads && i < D;
+                copy16(smem_addr(smem_q + e * 16), real ? q + r * D + i : q, real);
+            }
+            return;
+        }
         for (int e = threadIdx.x; e < GT * kDim; e += kThreads) {
             const int r = e / kDim, i = e - r * kDim;
             const float x = r < heads && i < D ? q[r * D + i] : 0.0f;
@@ -620,7 +627,7 @@ struct AttnSmem {
     static constexpr int kFactors = kSums + Core::kWarps * Core::kRows * Core::kDim * 4;
     static constexpr int kEnd = kFactors + 2 * kJoin * kMaxRows * 4;
     static constexpr int kQuery = kRing > kEnd ? kRing : kEnd;
-    static constexpr int kWarp = kQuery + Core::kQueryBytes;
+    static constexpr int kWarp = kQuery + 2 * Core::kQueryBytes;  // of this piece and of the next one
     static constexpr int kBars = kWarp + Core::kWarps * Core::kWarpBytes;
     static constexpr int kLive = kBars + Core::kWarps * STAGES * 8;
     static constexpr int kMl = kLive + Core::kWarps * STAGES * 4;
@@ -1000,19 +1007,27 @@ __global__ void __launch_bounds__(Core::kThreads, 1) k_attn(const __grid_constan
 #pragma unroll 1
         for (int i = 0; i < STAGES - 1; ++i) in.issue(i);
     };
-    auto stage_query = [&](const Piece &p) {
+    auto stage_query = [&](const Piece &p, char *to) {
         Core::stage_query(static_cast<const T *>(a.q) + p.b * a.q_token + static_cast<int64_t>(p.head0) * D, p.rows, D, q_aligned, a.scale < 0.0f,
-                          smem + Sm::kQuery);
+                          to);
     };
 
     Core core;
     Piece p = find(first_unit);
     if (p.n == 0) return;
     start(p);
-    stage_query(p);
+    char *query = smem + Sm::kQuery, *next_query = query + Core::kQueryBytes;
+    stage_query(p, query);
+    copies_commit();
+    copies_wait<0>();
     __syncthreads();
     for (;;) {
-        core.begin(smem + Sm::kQuery, smem + Sm::kWarp + warp * Core::kWarpBytes, D);
+        core.begin(query, smem + Sm::kWarp + warp * Core::kWarpBytes, D);
+        // While the first tiles come: what follows, and its queries (with those loaded while the sums meet, heads of 256
+        // elements took 49 us and not 46, ragged 64 x 8192 keys of 128 170 and not 169).
+        Piece following = find(p.u0 + p.t0 + p.n);
+        const bool more = following.n;
+        if (more) stage_query(following, next_query);
         int stage = 0;
 #pragma unroll 1
         for (int i = 0; i < p.n; ++i) {
@@ -1022,15 +1037,13 @@ __global__ void __launch_bounds__(Core::kThreads, 1) k_attn(const __grid_constan
             if (live) core.step(ks, ks + Sm::kTile, live, scale2);
             stage = stage + 1 == STAGES ? 0 : stage + 1;
         }
-        if (how != kBoxes) copies_wait<0>();
+        copies_commit();
+        copies_wait<0>();
         // The next piece's first tiles are on their way while this one's sums meet.
-        Piece following = find(p.u0 + p.t0 + p.n);
-        const bool more = following.n;
         before_boxes();
         __syncwarp();
         if (more) start(following);
         __syncthreads();
-        if (more) stage_query(following);
 
         // The warps' sums meet.
         const Span s = p.s;
@@ -1087,6 +1100,9 @@ __global__ void __launch_bounds__(Core::kThreads, 1) k_attn(const __grid_constan
         __syncthreads();  // the last stage holds sums until here
         if (!more) break;
         p = following;
+        char *const used = query;
+        query = next_query;
+        next_query = used;
     }
 }
 
