@@ -319,6 +319,21 @@ def test_attention_many_sequences():
     attn_check(P, lens, 4, L.BF16)
 
 
+@pytest.mark.parametrize("dt", [L.F32, L.BF16])
+@pytest.mark.parametrize("D", [64, 160])
+@pytest.mark.parametrize("seqs", [1, 5, 40, 150])
+def test_attention_short_and_long_sequences_in_one_batch(dt, D, seqs):
+    """Heads that one block does whole next to heads that are cut, from fewer to many more than there are blocks."""
+    tile = 128 if D <= 128 and dt == L.BF16 else 64 if dt == L.BF16 or D <= 128 else 32
+    some = [1, tile, 0, 3 * tile, 3 * tile + 1, tile + 1, 12 * tile + 5, 0, 0, 4 * tile, 2 * tile - 1]
+    lens = [some[(i * i + 3) % len(some)] for i in range(seqs)]
+    P = Pages(dt, seqs, -(-max(max(lens), 1) // 16), 16, 3, D, seed=seqs)
+    for scale in (0.0, -0.25):
+        first = attn_check(P, lens, 6, dt, scale=scale)
+        again = attn_check(P, lens, 6, dt, scale=scale)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
 @pytest.mark.parametrize("dt", [L.F32, L.F16, L.BF16])
 def test_attention_slots_past_the_end_may_hold_anything(dt):
     P = Pages(dt, 4, 10, 16, 2, 64, seed=3)
