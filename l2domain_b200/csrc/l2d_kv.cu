@@ -392,7 +392,10 @@ struct MmaCore {
         ldmatrix4(a, query + (((lane >> 3) & 1) * 8 + (lane & 7)) * kPitch + (lane >> 4) * 16 + k * 32);
     }
 
-    // One tile: keys at ks, values at vs (shared memory), bit j of live: key j counts.  scale2 > 0.
+    // One tile: keys at ks, values at vs (shared memory), bit j of live: key j counts.  scale2 > 0.  Scores are scaled,
+    // and rounded, before the maximum is taken and taken off: the largest is then 0 whatever its size.  With one
+    // rounding fewer, by a fused multiply-add on the unscaled ones, it would be what that rounding left: hundreds for
+    // scores of 2^31.
     __device__ __forceinline__ void step(const char *ks, const char *vs, uint32_t live, float scale2) {
         const int lane = threadIdx.x & 31, t = lane & 3;
         // Chunk 2k + hi of row r is at chunk_at(r, hi) ^ (2k & 7) * 16, in box k / 4.
@@ -418,7 +421,7 @@ struct MmaCore {
             mma16816<T>(k & 1 ? s2[1] : s[1], a, b[2], b[3]);
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s[e >> 2][e & 3] += s2[e >> 2][e & 3];
+        for (int e = 0; e < 8; ++e) s[e >> 2][e & 3] = (s[e >> 2][e & 3] + s2[e >> 2][e & 3]) * scale2;
         if (live != (1u << kKeys) - 1) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
@@ -433,7 +436,7 @@ struct MmaCore {
             float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const float m2 = fmaxf(m[r], top * scale2), base = finite_base(m2);
+            const float m2 = fmaxf(m[r], top), base = finite_base(m2);
             if (__any_sync(0xffffffffu, m2 != m[r])) {
                 const float f = exp2_approx(m[r] - base);
                 l[r] *= f;
@@ -449,7 +452,7 @@ struct MmaCore {
                 m[r] = m2;
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = exp2_approx(fmaf(x[e], scale2, -base));
+            for (int e = 0; e < 4; ++e) x[e] = exp2_approx(x[e] - base);
             l[r] += (x[0] + x[1]) + (x[2] + x[3]);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -560,11 +563,12 @@ struct SimdCore {
         for (int g = 0; g < GT; ++g) {
 #pragma unroll
             for (int d = kKeys; d < 32; d <<= 1) s[g] += __shfl_xor_sync(0xffffffffu, s[g], d);
-            float top = ok ? s[g] * scale2 : -INFINITY;
+            s[g] *= scale2;
+            float top = ok ? s[g] : -INFINITY;
 #pragma unroll
             for (int d = 1; d < kKeys; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
             const float m2 = fmaxf(m[g], top), base = finite_base(m2), f = exp2_approx(m[g] - base);
-            const float w = ok ? exp2_approx(fmaf(s[g], scale2, -base)) : 0.0f;
+            const float w = ok ? exp2_approx(s[g] - base) : 0.0f;
             l[g] = fmaf(l[g], f, w);
             m[g] = m2;
             if (sub == 0) weights[g * kKeys + key] = w;

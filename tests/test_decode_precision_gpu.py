@@ -1,0 +1,72 @@
+"""The decoding operators where 32-bit arithmetic has to be kept: sums whose largest terms cancel, weigh nothing or
+lie far above the rest.
+
+The tolerances come from rounding alone (u = 2^-24), with the bounds that test_decode_ops_gpu.py derives:
+
+* q4: 2u (160 + n / 32) S, S the sum of the terms' absolute values; what has the weight zero adds nothing to S.
+* attention: scores here are single products, exact but for the scale (two roundings, 2u |score|); a weight is off
+  by 2^-20 for exp and by what its two 16-bit parts leave: 2^-16 of it for bf16; for fp16 2^-22 of it or 2^-39 of the
+  largest weight, whichever is more.
+"""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+import l2domain_b200 as L  # noqa: E402
+from test_decode_ops_gpu import TORCH, U, Pages, attn_check, close, gen, gpu, normal, q4_exact  # noqa: E402,F401
+
+
+# ------------------------------------------------------------------------------------------------
+# Attention
+# ------------------------------------------------------------------------------------------------
+
+def steered(P, n, heads_q, dt, scores, values, q0):
+    """Attention over n keys of each head whose only non-zero element is the first: key p of every head has the score
+    q0[h] * scores[p] (scale 1).  (out, lse, want, want lse, slack, slack of lse) for one sequence."""
+    D = P.D
+    q = torch.zeros(1, heads_q, D, dtype=TORCH[dt], device="cuda")
+    q[0, :, 0] = q0.to(TORCH[dt])
+    at = torch.arange(n, device="cuda")
+    rows = P.table[0].long()[at // P.page], at % P.page
+    P.k[rows] = 0
+    keys = torch.zeros(n, P.heads, D, dtype=TORCH[dt], device="cuda")
+    keys[:, :, 0] = scores.to(TORCH[dt])[:, None]
+    P.k[rows], P.v[rows] = keys, values.to(TORCH[dt])
+    out = torch.full_like(q, math.nan)
+    lse = torch.full((1, heads_q), math.nan, device="cuda")
+    L.PagedAttention(P.cache(), P.table, P.seqs, P.width, heads_q, scale=1.0).decode(
+        q, out, torch.tensor([n], dtype=torch.int32, device="cuda"), 1, lse=lse)
+    torch.cuda.synchronize()
+    k, v = (t.double().repeat_interleave(heads_q // P.heads, 1) for t in P.rows(0, 0, n))
+    s = torch.einsum("hd,nhd->hn", q[0].double(), k)
+    l = torch.logsumexp(s, -1)
+    w = torch.exp(s - l[:, None])
+    off = 2 * U * s.abs().amax(-1, keepdim=True) * 2 + 2.0 ** -20 + 2 * U * (160 + n / 16)
+    part = {L.F32: 0 * w, L.BF16: w * 2.0 ** -16, L.F16: torch.maximum(w * 2.0 ** -22, w.amax(-1, keepdim=True) * 2.0 ** -39)}[dt]
+    slack = torch.einsum("hn,nhd->hd", w * off + part, v.abs())
+    return out[0], lse[0], torch.einsum("hn,nhd->hd", w, v), l, slack, off[:, 0]
+
+
+@pytest.mark.parametrize("dt", [L.F32, L.F16, L.BF16])
+@pytest.mark.parametrize("G,D", [(2, 64), (16, 64), (1, 128), (5, 256), (12, 128)])
+@pytest.mark.parametrize("power", [14, 27, 31, 36])
+def test_attention_scores_far_apart(dt, G, D, power):
+    """Scores of up to 2^power, each key's far below the next one's: the largest takes all, whatever the rounding of the
+    others is worth."""
+    power = min(power, 30) if dt == L.F16 else power
+    P = Pages(dt, 1, 20, 16, 2, D, seed=power)
+    n = 300
+    low = min(power - power // 2, 15)
+    scores = (torch.randperm(n, device="cuda", generator=gen(power)) + 1).float() * 2.0 ** (low - 9)
+    scores = scores.to(TORCH[dt]).float()  # rounded: several may be the largest
+    q0 = torch.full((2 * G,), 2.0 ** (power - low), device="cuda")
+    g = gen(G)
+    values = normal(g, dt, n, 2, D)
+    top = torch.nonzero(scores == scores.max())[:, 0]
+    values[top] = values[top[:1]].clone()
+    out, lse, want, want_lse, _, _ = steered(P, n, 2 * G, dt, scores, values, q0)
+    close(out, want, 2.0 ** -15 * want.abs(), dt)
+    close(lse, want_lse, 2.0 ** -20 * want_lse.abs(), L.F32)
