@@ -321,7 +321,7 @@ __device__ __forceinline__ float finite_base(float m) { return m == -INFINITY ? 
 // One warp's part of one head group of a 16-bit cache: KS steps of 16 elements of the head, the query
 // heads as the rows of m16n8k16.  Groups of up to eight heads (SPLIT) use the other eight rows for the
 // low halves of the weights: p = hi + lo in two 16-bit numbers, so rounding p costs nothing there.
-// Larger groups round p once to the cache's type, 2^-9 (bf16) or 2^-12 (fp16) of each term.
+// Larger groups multiply twice, by hi and by lo.
 template <typename T, int KS, bool SPLIT>
 struct MmaCore {
     using Elem = T;
@@ -427,7 +427,7 @@ struct MmaCore {
             for (int e = 0; e < 8; ++e)
                 if (!(live >> ((e >> 2) * 8 + 2 * t + (e & 1)) & 1)) s[e >> 2][e & 3] = -INFINITY;
         }
-        uint32_t p[4];
+        uint32_t p[4], lo[SPLIT ? 1 : 4];
 #pragma unroll
         for (int r = 0; r < (SPLIT ? 1 : 2); ++r) {
             float x[4];
@@ -458,7 +458,7 @@ struct MmaCore {
             for (int h = 0; h < 2; ++h) {
                 const T a = dev::narrow<T>(x[2 * h]), b = dev::narrow<T>(x[2 * h + 1]);
                 p[r + 2 * h] = pack2(a, b);
-                if constexpr (SPLIT) p[1 + 2 * h] = pack2(dev::narrow<T>(x[2 * h] - dev::widen(a)), dev::narrow<T>(x[2 * h + 1] - dev::widen(b)));
+                (SPLIT ? p[1 + 2 * h] : lo[r + 2 * h]) = pack2(dev::narrow<T>(x[2 * h] - dev::widen(a)), dev::narrow<T>(x[2 * h + 1] - dev::widen(b)));
             }
         }
 #pragma unroll
@@ -467,6 +467,10 @@ struct MmaCore {
             ldmatrix4_trans(b, (va ^ ((2 * n & 7) << 4)) + (n / 4) * (kKeys * 128));
             mma16816<T>(o[2 * n], p, b[0], b[1]);
             mma16816<T>(o[2 * n + 1], p, b[2], b[3]);
+            if constexpr (!SPLIT) {
+                mma16816<T>(o[2 * n], lo, b[0], b[1]);
+                mma16816<T>(o[2 * n + 1], lo, b[2], b[3]);
+            }
         }
     }
 

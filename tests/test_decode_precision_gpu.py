@@ -70,3 +70,36 @@ def test_attention_scores_far_apart(dt, G, D, power):
     out, lse, want, want_lse, _, _ = steered(P, n, 2 * G, dt, scores, values, q0)
     close(out, want, 2.0 ** -15 * want.abs(), dt)
     close(lse, want_lse, 2.0 ** -20 * want_lse.abs(), L.F32)
+
+
+@pytest.mark.parametrize("dt", [L.F32, L.F16, L.BF16])
+@pytest.mark.parametrize("G,D", [(1, 128), (8, 64), (7, 256), (9, 128), (12, 64), (16, 80), (16, 96), (16, 128), (16, 192), (16, 256), (33, 128)])
+def test_attention_values_that_cancel(dt, G, D):
+    """Two keys of nearly the same score and opposite values, among others that weigh little: the difference of their
+    weights comes out, which weights of 8 or 11 bits would not have."""
+    P = Pages(dt, 1, 20, 16, 1, D, seed=G)
+    n = 300
+    scores = torch.full((n,), -40.0, device="cuda")
+    scores[4], scores[6] = 0.0, -0.015625  # of one tile: weights are relative to the largest in it
+    g = gen(D)
+    values = normal(g, L.F32, n, 1, D)
+    values[6] = -values[4]
+    q0 = (torch.arange(G, device="cuda") + 1) / 64.0 + 0.5
+    out, lse, want, want_lse, slack, off = steered(P, n, G, dt, scores, values, q0)
+    close(out, want, slack, dt)
+    close(lse, want_lse, off, L.F32)
+
+
+@pytest.mark.parametrize("dt", [L.F16, L.BF16])
+@pytest.mark.parametrize("D", [80, 96, 128, 192, 250, 256])
+@pytest.mark.parametrize("G", [9, 16, 40])
+def test_attention_large_groups_on_wide_heads(dt, D, G):
+    P = Pages(dt, 3, 20, 16, 2, D, seed=G)
+    attn_check(P, [300, 0, 129], 2 * G, dt)
+
+
+@pytest.mark.parametrize("D", [136, 160, 200, 256])
+@pytest.mark.parametrize("G", [1, 5, 8, 17])
+def test_attention_fp32_groups_on_wide_heads(D, G):
+    P = Pages(L.F32, 3, 20, 16, 2, D, seed=G)
+    attn_check(P, [300, 0, 129], 2 * G, L.F32)
