@@ -318,10 +318,18 @@ __device__ __forceinline__ uint32_t pack2(T lo, T hi) {
 // A running softmax's maximum, and what exponents are taken relative to: never -inf.
 __device__ __forceinline__ float finite_base(float m) { return m == -INFINITY ? 0.0f : m; }
 
+// Weights, 1 for the largest score, as numbers of the cache's type: bf16 has the exponents of fp32, but fp16 ends at
+// 2^-24, so there they are taken 2^15 times as large (and sums of values too, until they leave the registers).
+template <typename T>
+constexpr float kWeightUnit = 1.0f;
+template <>
+constexpr float kWeightUnit<__half> = 0x1p15f;
+
 // One warp's part of one head group of a 16-bit cache: KS steps of 16 elements of the head, the query
 // heads as the rows of m16n8k16.  Groups of up to eight heads (SPLIT) use the other eight rows for the
-// low halves of the weights: p = hi + lo in two 16-bit numbers, so rounding p costs nothing there.
-// Larger groups multiply twice, by hi and by lo.
+// low halves of the weights: p = hi + lo in two 16-bit numbers, which leaves 2^-17 of p (bf16), or 2^-23 of it and
+// at least 2^-51 of the largest (fp16, whose low halves are taken another 2^11 times as large).
+// Larger groups multiply twice, by hi and by lo, into the same sums, which for fp16 leaves at least 2^-40 of the largest.
 template <typename T, int KS, bool SPLIT>
 struct MmaCore {
     using Elem = T;
@@ -337,6 +345,8 @@ struct MmaCore {
     static constexpr bool kQueryInSmem = !SPLIT && KS > 8; // registers would not hold queries and sums
     static constexpr int kQueryBytes = kRows * kPitch;
     static constexpr int kWarpBytes = 0;
+    static constexpr float kUnit = kWeightUnit<T>;
+    static constexpr float kLow = SPLIT && kUnit != 1.0f ? 0x1p11f : 1.0f;  // of low halves, beyond kUnit
     uint32_t qa[kQueryInSmem ? 1 : KS][SPLIT ? 2 : 4];
     float o[2 * KS][4], m[2], l[2];
     uint32_t query;
@@ -456,9 +466,10 @@ struct MmaCore {
             l[r] += (x[0] + x[1]) + (x[2] + x[3]);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const T a = dev::narrow<T>(x[2 * h]), b = dev::narrow<T>(x[2 * h + 1]);
+                const float u = x[2 * h] * kUnit, v = x[2 * h + 1] * kUnit;
+                const T a = dev::narrow<T>(u), b = dev::narrow<T>(v);
                 p[r + 2 * h] = pack2(a, b);
-                (SPLIT ? p[1 + 2 * h] : lo[r + 2 * h]) = pack2(dev::narrow<T>(x[2 * h] - dev::widen(a)), dev::narrow<T>(x[2 * h + 1] - dev::widen(b)));
+                (SPLIT ? p[1 + 2 * h] : lo[r + 2 * h]) = pack2(dev::narrow<T>((u - dev::widen(a)) * kLow), dev::narrow<T>((v - dev::widen(b)) * kLow));
             }
         }
 #pragma unroll
@@ -488,7 +499,8 @@ struct MmaCore {
 #pragma unroll
             for (int n = 0; n < 2 * KS; ++n) {
                 float2 v = make_float2(o[n][2 * r], o[n][2 * r + 1]);
-                if constexpr (SPLIT) v = make_float2(v.x + o[n][2], v.y + o[n][3]);
+                if constexpr (SPLIT) v = make_float2(fmaf(o[n][2], 1.0f / kLow, v.x), fmaf(o[n][3], 1.0f / kLow, v.y));
+                v = make_float2(v.x * (1.0f / kUnit), v.y * (1.0f / kUnit));
                 *reinterpret_cast<float2 *>(so + (g + 8 * r) * kDim + 8 * n + 2 * t) = v;
             }
         }

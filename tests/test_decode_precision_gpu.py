@@ -72,6 +72,24 @@ def test_attention_scores_far_apart(dt, G, D, power):
     close(lse, want_lse, 2.0 ** -20 * want_lse.abs(), L.F32)
 
 
+@pytest.mark.parametrize("G,D", [(1, 64), (8, 128), (12, 64), (16, 128), (16, 256), (33, 80)])
+@pytest.mark.parametrize("nats", [8, 12, 18])
+def test_attention_keeps_small_weights(G, D, nats):
+    """A key far above the others whose values are zero: what comes out is all of the others'."""
+    for dt in (L.F16, L.BF16):
+        P = Pages(dt, 1, 30, 16, 1, D, seed=nats)
+        n = 450
+        g = gen(nats)
+        scores = -(torch.rand(n, device="cuda", generator=g) + nats)
+        scores[7] = 0.0
+        values = normal(g, L.F32, n, 1, D).abs() * 500 + 100
+        values[7] = 0.0
+        q0 = torch.linspace(0.75, 1.0, G, device="cuda")
+        out, lse, want, want_lse, slack, off = steered(P, n, G, dt, scores, values, q0)
+        close(out, want, slack, dt)
+        close(lse, want_lse, off, L.F32)
+
+
 @pytest.mark.parametrize("dt", [L.F32, L.F16, L.BF16])
 @pytest.mark.parametrize("G,D", [(1, 128), (8, 64), (7, 256), (9, 128), (12, 64), (16, 80), (16, 96), (16, 128), (16, 192), (16, 256), (33, 128)])
 def test_attention_values_that_cancel(dt, G, D):
@@ -103,3 +121,11 @@ def test_attention_large_groups_on_wide_heads(dt, D, G):
 def test_attention_fp32_groups_on_wide_heads(D, G):
     P = Pages(L.F32, 3, 20, 16, 2, D, seed=G)
     attn_check(P, [300, 0, 129], 2 * G, L.F32)
+
+
+def test_attention_large_scores_fp16():
+    P = Pages(L.F16, 2, 20, 16, 2, 64, seed=5)
+    P.k.mul_(64)
+    for scale in (0.25, -0.25):
+        attn_check(P, [300, 31], 4, L.F16, scale=scale)
+        attn_check(P, [300, 31], 24, L.F16, scale=scale)
