@@ -259,10 +259,11 @@ __device__ __forceinline__ void barrier_init(uint32_t bar) { asm volatile("mbarr
 __device__ __forceinline__ void barrier_expect(uint32_t bar, int bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-// Waits for the barrier's phase of this parity; false if it does not come in some seconds.
+// Waits for the barrier's phase of this parity; false if it does not come in about two seconds (a try suspends the
+// thread for up to 4 us).
 __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity) {
     uint32_t done = 0;
-    for (int i = 0; i < (1 << 22) && !done; ++i)
+    for (int i = 0; i < (1 << 19) && !done; ++i)
         asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
     return done;
 }
@@ -677,12 +678,13 @@ struct Stream {
     char *ring;
     uint32_t bars;
     uint32_t *live;
-    uint32_t phases;      // parity of each stage's barrier
+    uint32_t phases;      // parity of each stage's barrier; kLate: a box did not come
     int64_t next;         // the first key of the tile whose pages are in `page`
     int lo, len, step;    // keys lo .. len - 1 count; keys between this warp's tiles
     int slot, page;       // of this lane's key (lanes kLanes j .. kLanes j + kLanes - 1: key j); with boxes, of the tile's first
     bool wanted;          // that key, or one of the tile's, counts
     static constexpr int kLanes = 32 / Core::kKeys;
+    static constexpr uint32_t kLate = 1u << 31;
 
     // The entry is not looked at before the next tile is started: an instruction that used it here would wait for
     // it, and the products with it.
@@ -761,6 +763,21 @@ struct Stream {
         lookup();
     }
 
+    // A box did not come: no more are started (lane 0 starts them), and the ones under way are waited for.
+    __device__ __forceinline__ void give_up(int stage) {
+        report(c.status, L2D_KV_TIMEOUT);
+        phases |= kLate;
+        len = 0;
+        wanted = false;
+        if (threadIdx.x & 31) return;
+#pragma unroll 1
+        for (int j = 1; j < STAGES - 1; ++j) {
+            const int s = (stage + j) % STAGES;
+            if (live[s]) barrier_wait(bars + 8 * s, phases >> s & 1);
+            live[s] = 0;
+        }
+    }
+
     // The live bits of a stage, once its copies are there.  Values of keys that do not count are made zeros, as
     // their weights are: slots that were never written may hold anything.
     __device__ __forceinline__ uint32_t take(int stage) {
@@ -768,7 +785,7 @@ struct Stream {
         __syncwarp();
         const uint32_t bits = live[stage];
         if (how == kBoxes && bits) {
-            if (!barrier_wait(bars + 8 * stage, phases >> stage & 1)) report(c.status, L2D_KV_TIMEOUT);
+            if (!barrier_wait(bars + 8 * stage, phases >> stage & 1)) give_up(stage);
             phases ^= 1u << stage;
             if (bits != (1u << Core::kKeys) - 1) {
                 char *values = ring + stage * (Core::kWarps * Sm::kStage) + Sm::kTile;
@@ -1024,6 +1041,7 @@ __global__ void __launch_bounds__(Core::kThreads, 1) k_attn(const __grid_constan
         in.table = a.c.table + p.b * a.c.table_stride;
         in.lo = p.s.lo;
         in.len = static_cast<int>(min(static_cast<int64_t>(p.s.len), p.s.from + static_cast<int64_t>(p.t0 + p.n) * TILE));
+        if (in.phases & in.kLate) in.len = 0;
         in.next = p.s.from + static_cast<int64_t>(p.t0) * TILE + warp * Core::kKeys;
         in.step = TILE;
         in.lookup();
