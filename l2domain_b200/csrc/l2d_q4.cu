@@ -134,8 +134,7 @@ int l2d_q4_gemv(const l2d_q4_desc *desc, const void *x, int64_t stride_x, void *
     const bool words = !misaligned(d.W, 16) && ldw % 16 == 0 && d.dtype_s != L2D_F32 && together(word);
     a.wide = together(2 * word);
     const int sub = d.group == 32 ? 4 : d.group == 64 ? 2 : 1;
-    const bool wide = d.dtype_x == L2D_F32 || d.dtype_y == L2D_F32;
-    const Q4Kind kind = vectors * sub <= 2 ? kQ4Bytes : wide ? kQ4Exact : kQ4Fast;
+    const Q4Kind kind = vectors * sub <= 2 ? kQ4Bytes : d.dtype_x == L2D_F32 ? kQ4From32 : kQ4From16;
     const bool bytes = kind == kQ4Bytes;
     a.parts = bytes ? 4 : d.dtype_x == L2D_F32 ? 2 : 1;
     const int each = a.parts * sub;                                         // columns of B per vector
@@ -153,8 +152,8 @@ int l2d_q4_gemv(const l2d_q4_desc *desc, const void *x, int64_t stride_x, void *
         const int columns = a.vectors * a.parts;
         const bool zeros = d.zeros != nullptr;
         const Q4Entry k = bytes              ? q4_entry_bytes(d.group, zeros, words)
-                          : kind == kQ4Exact ? q4_entry_exact(tiles_n, d.group, zeros, words)
-                                             : q4_entry_fast(tiles_n, d.group, zeros, words);
+                          : kind == kQ4From32 ? q4_entry_float(tiles_n, d.group, zeros, words)
+                                             : q4_entry_half(tiles_n, d.group, zeros, words);
         L2D_CUDA_TRY(allow_smem(k.run, 227 * 1024, d.device, *k.smem_set));
         const int *clusters = nullptr;
         const int known = q4_clusters(d.device, k, &clusters);

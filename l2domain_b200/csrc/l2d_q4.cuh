@@ -12,17 +12,15 @@
 //    bytes.  x of each 128 columns is a 30-bit integer times a power of two, in four signed digits of 8 bits, a
 //    column of B each.  Sums are exact up to the end of a group; values of x are exact down to 2^-6 (fp32),
 //    2^-19 (fp16) or 2^-22 (bf16) of the largest among their 128 columns, and otherwise off by at most 2^-30 of it.
-//  * More vectors are multiplied in fp16 with fp32 sums (m16n8k16), one column a vector.  A nibble masked into
-//    the low mantissa bits of an fp16 number is the subnormal q 2^-24, one higher up 16 q 2^-24: both exact, and
-//    no instruction but the mask.  x of the columns that end up higher is a sixteenth of itself.  Each 128 columns
-//    of a vector are scaled by a power of two to a largest value just under 2^15; what is below 2^-28 of it may
-//    lose bits.
-//  * If inputs or results are fp32, that is not enough: sum q x and z sum x may nearly cancel.  There the
-//    difference q - z is taken first, exactly, from 1024 + q and 1024 + z (two instructions more for every two
-//    weights), and fp32 vectors take two columns, 11 bits each, which leaves one rounding of 2^-24.
-//  * Otherwise what the zero point takes away is z times the group's sum of x, which is computed once per block:
-//    sum (q - z) x = sum q x - z sum x.  Infinities and NaNs do not survive that.  They are staged as zeros,
-//    and the threads that store a vector's results add the terms of its infinities and NaNs at the end.
+//  * More vectors are multiplied in fp16 with fp32 sums (m16n8k16), one column a vector.  The difference q - z is
+//    taken first, exactly, from 1024 + q and 1024 + z, because sum q x and z sum x may nearly cancel: where the largest
+//    x meets a weight of zero, or a row has few others, their difference has few right bits left.  (A nibble masked
+//    into the low mantissa bits of an fp16 number is exact as it is, and two instructions less for every two weights:
+//    8 vectors 28672 x 8192 on groups of 128 take 42 us so, and 48 with the differences.)  A mask higher up gives 16 (q - z), with
+//    a sixteenth of x.  Each 128 columns of a vector are scaled by a power of two to a largest value just under 2^15;
+//    what is below 2^-28 of it may lose bits.
+//  * fp32 vectors take two columns of fp16, 11 bits each, which leaves one rounding of 2^-24.
+//  * Infinities and NaNs are staged as zeros, and the threads that store a vector's results add their terms at the end.
 //  * The scales are applied to the fp32 sums of each group.  One instruction sums over the four lanes of a
 //    row, 128 columns; where groups are shorter, x of the different groups goes to different columns of B
 //    (zeros elsewhere), so that each group still has a sum of its own: S = 128 / group columns per part.
@@ -56,7 +54,7 @@ struct Q4Args {
     void *y;
     int64_t M, ldw, lds, stride_x, stride_y;
     int N, vectors, group, dtype_x, dtype_y, dtype_s;
-    int parts;       // columns of x per vector: 4 by bytes, 2 for fp32 in fp16, else 1
+    int parts;       // columns of x per vector: 4 by bytes, 2 for fp32, else 1
     int warps_k;     // warps that split a tile's columns
     int ranks;       // blocks of a cluster, which split the columns
     int stage_h;     // halves of 128 columns of x staged at a time
@@ -133,15 +131,6 @@ __device__ __forceinline__ void unpack_less(uint32_t w, uint32_t z, uint32_t (&p
     p[3] = sub_half2((w & 0x00F000F0) | 0x64006400, hi);
 }
 
-// Eight nibbles as fp16 numbers, p[i] nibbles i and i + 4: q 2^-24, and 16 q 2^-24 in p[1] and p[3].
-__device__ __forceinline__ void unpack(uint32_t w, uint32_t (&p)[4]) {
-    p[0] = w & 0x000F000F;
-    p[1] = w & 0x00F000F0;
-    w >>= 8;
-    p[2] = w & 0x000F000F;
-    p[3] = w & 0x00F000F0;
-}
-
 __device__ __forceinline__ uint4 load_weights(const uint8_t *p) {
     uint4 v;
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
@@ -196,8 +185,8 @@ __device__ __forceinline__ float scale_value(uint32_t word, bool high, bool is_h
 // S: columns of B per part of a vector (4, 2, 1 for groups of 32, 64, 128 columns), 0 for longer groups.
 // WORDS: every row of W is whole 16-byte words on 16-byte boundaries, and the 16-bit scales (and zeros) of a step
 // can be read in words.
-// KIND: how products are taken.
-enum Q4Kind { kQ4Fast, kQ4Exact, kQ4Bytes };
+// KIND: how products are taken: in fp16 with 16-bit or fp32 vectors, or by bytes.
+enum Q4Kind { kQ4From16, kQ4From32, kQ4Bytes };
 template <int NT, int S, bool ZEROS, bool WORDS, Q4Kind KIND>
 __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
     constexpr bool BYTES = KIND == kQ4Bytes;
@@ -250,7 +239,7 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
     const bool is_half = a.dtype_s == L2D_F16;
 
     // Adds the products of half `half` of the staging: scales s and zeros z of [row][column of C].
-    auto multiply = [&](const Q4Part &part, int half, const float (&s)[2][E], const float (&z)[2][E]) {
+    auto multiply = [&](const Q4Part &part, int half, const float (&s)[2][E], const uint32_t (&z)[2][E]) {
         const uint32_t w0[4] = {part.w[0].x, part.w[0].y, part.w[0].z, part.w[0].w}, w1[4] = {part.w[1].x, part.w[1].y, part.w[1].z, part.w[1].w};
         float sum[NT][4];
         const char *x = x_lane + half * x_half;
@@ -276,25 +265,20 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sum[n][e] = __uint_as_float(c[n][e]);
         } else {
-            uint32_t z0 = 8, z1 = 8;  // of this lane's own columns, which the lane of their subgroup's sum has
-            if constexpr (KIND == kQ4Exact) {
-                const int own = t * SUB >> 2, from = S > 1 ? (lane & ~3) | own >> 1 : lane;
-                uint32_t v[2][E];
+            uint32_t z0 = z[0][0], z1 = z[1][0];  // of this lane's own columns, which the lane of their subgroup's sum has
+            if constexpr (ZEROS && S > 1) {
+                const int own = t * SUB >> 2, from = (lane & ~3) | own >> 1;
+                uint32_t v[2][2];
 #pragma unroll
-                for (int e = 0; e < 2 * E; ++e) v[e / E][e % E] = __shfl_sync(0xffffffffu, static_cast<uint32_t>(z[e / E][e % E]), from);
-                z0 = v[0][own & 1 ? E - 1 : 0];
-                z1 = v[1][own & 1 ? E - 1 : 0];
+                for (int e = 0; e < 4; ++e) v[e / 2][e % 2] = __shfl_sync(0xffffffffu, z[e / 2][e % E], from);
+                z0 = v[0][own & 1];
+                z1 = v[1][own & 1];
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 uint32_t p0[4], p1[4];
-                if constexpr (KIND == kQ4Exact) {
-                    unpack_less(w0[j], z0, p0);
-                    unpack_less(w1[j], z1, p1);
-                } else {
-                    unpack(w0[j], p0);
-                    unpack(w1[j], p1);
-                }
+                unpack_less(w0[j], z0, p0);
+                unpack_less(w1[j], z1, p1);
                 const uint32_t a0[4] = {p0[0], p1[0], p0[1], p1[1]}, a1[4] = {p0[2], p1[2], p0[3], p1[3]};
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
@@ -312,17 +296,17 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
             const float4 f = xs[4 * n];  // sum and factor of columns 2t and 2t + 1
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float zero = z[e >> 1][(e & 1) % E], xsum = e & 1 ? f.z : f.x;
                 // By bytes all of this is integers below 2^24, and exact (without zeros the sum is 8 of it and the bias).
-                const float v = BYTES              ? sum[n][e] - (ZEROS ? fmaf(zero, xsum, 12582912.0f) : xsum)
-                                : KIND == kQ4Exact ? sum[n][e] * 0x1p-24f : fmaf(-zero, xsum, sum[n][e]);
+                const float xsum = e & 1 ? f.z : f.x;
+                const float v = BYTES ? sum[n][e] - (ZEROS ? fmaf(static_cast<float>(z[e >> 1][(e & 1) % E]), xsum, 12582912.0f) : xsum) : sum[n][e];
                 acc[n][e] = fmaf(s[e >> 1][(e & 1) % E], v * fabsf(e & 1 ? f.w : f.y), acc[n][e]);
             }
         }
     };
     // Half h of a step.
     auto multiply_of = [&](const Q4Part &c, const Q4Scales<S, ZEROS> &q, int h, int half) {
-        float s[2][E], z[2][E];
+        float s[2][E];
+        uint32_t z[2][E];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             const bool second = S == 0 && h >= q.from;
@@ -332,7 +316,7 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
             uint32_t zeros = 0;
             if constexpr (ZEROS) zeros = S == 0 ? (second ? q.z[r][1] : q.z[r][0]) : S == 1 ? q.z[r][h / 2] >> (8 * (h & 1)) : S == 2 ? q.z[r][h / 2] >> (16 * (h & 1)) : q.z[r][h];
 #pragma unroll
-            for (int e = 0; e < E; ++e) z[r][e] = ZEROS ? static_cast<float>(zeros >> (8 * e) & 15) : 8.0f;
+            for (int e = 0; e < E; ++e) z[r][e] = ZEROS ? zeros >> (8 * e) & 15 : 8;
         }
         multiply(c, half, s, z);
     };
@@ -430,13 +414,14 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
         }
     };
     auto multiply_alone = [&](const Alone &x, int half) {
-        float s[2][E], z[2][E];
+        float s[2][E];
+        uint32_t z[2][E];
 #pragma unroll
         for (int r = 0; r < 2; ++r)
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 s[r][e] = a.dtype_s == L2D_F32 ? __uint_as_float(x.s[r][e]) : scale_value(x.s[r][e], false, is_half);
-                z[r][e] = static_cast<float>(x.z[r][e] & 15);
+                z[r][e] = x.z[r][e] & 15;
             }
         multiply(x.c, half, s, z);
     };
@@ -489,7 +474,7 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
             const bool stores_sums = real && u % (16 / SUB) == 0;
             step(at);
             ahead = fetch(at);
-            if constexpr (KIND == kQ4Fast) {  // 16-bit inputs: the same as below in fewer instructions
+            if constexpr (KIND == kQ4From16) {  // the same as below in fewer instructions
                 uint32_t w[4] = {r.lo.x, r.lo.y, r.lo.z, r.lo.w};
                 const bool is_fp16 = a.dtype_x == L2D_F16;
                 const uint32_t inf = is_fp16 ? 0x7c00u : 0x7f80u;
@@ -512,7 +497,7 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
 #pragma unroll
                 for (int d = 1; d < 16; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
                 const uint32_t p = min(268u - (__float_as_uint(scale_value(top, false, is_fp16)) >> 23), 254u);
-                const float up = __uint_as_float(p << 23), back = __uint_as_float((266u - p) << 23);
+                const float up = __uint_as_float(p << 23), back = __uint_as_float((266u - p) << 23) * 0x1p-24f;
                 float f[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) f[i] = scale_value(w[i / 2], i & 1, is_fp16) * up;
@@ -522,12 +507,8 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
                     const __half2 h = i & 1 ? __floats2half2_rn(f[i] * 0.0625f, f[i + 4] * 0.0625f) : __floats2half2_rn(f[i], f[i + 4]);
                     memcpy(&out[i], &h, 4);
                 }
-                // Of the values as they were: what rounding takes off the smallest is below 2^-39 of the largest.
-                float total = ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
-#pragma unroll
-                for (int d = 1; d < 16 / SUB; d <<= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
                 if (real) reinterpret_cast<uint4 *>(smem + (half * columns + column) * kColumn)[j * 4 + tt] = make_uint4(out[0], out[1], out[2], out[3]);
-                if (stores_sums) to[0] = make_float2(total * 0x1p-24f, odd ? -back : back);  // the sign: see add_odd_ones()
+                if (stores_sums) to[0] = make_float2(0.0f, odd ? -back : back);  // the sign: see add_odd_ones()
                 continue;
             }
             const uint32_t raw[8] = {r.lo.x, r.lo.y, r.lo.z, r.lo.w, r.hi.x, r.hi.y, r.hi.z, r.hi.w};
@@ -571,28 +552,23 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
             }
             // 2^(p - 127) takes the largest to [2^14, 2^15); the factor back is short of 2^12, which the end makes good.
             const uint32_t p = min(268u - (top >> 23), 254u);
-            const float up = __uint_as_float(p << 23), back = __uint_as_float((266u - p) << 23);
-            uint32_t hi[8];
-            float total_hi = 0.0f;
+            const float up = __uint_as_float(p << 23), back = __uint_as_float((266u - p) << 23) * 0x1p-24f;
+            uint32_t hi[8], lo[8];  // lo: what the first part leaves, 2^11 times as large
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 f[i] *= i & 1 ? up * 0.0625f : up;
                 const __half h = __float2half_rn(f[i]);
                 hi[i] = __half_as_ushort(h);
-                total_hi = fmaf(i & 1 ? 16.0f : 1.0f, __half2float(h), total_hi);
+                lo[i] = __half_as_ushort(__float2half_rn((f[i] - __half2float(h)) * 2048.0f));
             }
-#pragma unroll
-            for (int d = 1; d < 16 / SUB; d <<= 1) total_hi += __shfl_xor_sync(0xffffffffu, total_hi, d);
             uint4 *dst = reinterpret_cast<uint4 *>(smem + (half * columns + column) * kColumn) + j * 4 + tt;
-            if (real) dst[0] = make_uint4(hi[0] | hi[4] << 16, hi[1] | hi[5] << 16, hi[2] | hi[6] << 16, hi[3] | hi[7] << 16);
-            if (stores_sums) to[0] = make_float2(total_hi * 0x1p-24f, odd ? -back : back);
-            if (KIND == kQ4Exact && a.parts == 2) {  // what the first part leaves, 2^11 times as large
-                uint32_t lo[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    lo[i] = __half_as_ushort(__float2half_rn((f[i] - __half2float(__ushort_as_half(static_cast<unsigned short>(hi[i])))) * 2048.0f));
-                if (real) dst[kColumn / 16] = make_uint4(lo[0] | lo[4] << 16, lo[1] | lo[5] << 16, lo[2] | lo[6] << 16, lo[3] | lo[7] << 16);
-                if (stores_sums) to[SUB] = make_float2(0.0f, back * 0x1p-11f);  // no sum: it is not taken off
+            if (real) {
+                dst[0] = make_uint4(hi[0] | hi[4] << 16, hi[1] | hi[5] << 16, hi[2] | hi[6] << 16, hi[3] | hi[7] << 16);
+                dst[kColumn / 16] = make_uint4(lo[0] | lo[4] << 16, lo[1] | lo[5] << 16, lo[2] | lo[6] << 16, lo[3] | lo[7] << 16);
+            }
+            if (stores_sums) {
+                to[0] = make_float2(0.0f, odd ? -back : back);
+                to[SUB] = make_float2(0.0f, back * 0x1p-11f);
             }
         }
         // Columns of B without a vector: their sums are dropped, but stay finite.
@@ -757,8 +733,8 @@ Q4Entry q4_entry(int group, bool zeros, bool words) {
     return group == 128 ? q4_entry<NT, 1, KIND>(zeros, words) : q4_entry<NT, 0, KIND>(zeros, words);
 }
 // The kernels of one kind each, compiled apart; tiles_n: how many eights of columns B has (1, 2 or 4; by bytes 1).
-Q4Entry q4_entry_fast(int tiles_n, int group, bool zeros, bool words);
-Q4Entry q4_entry_exact(int tiles_n, int group, bool zeros, bool words);
+Q4Entry q4_entry_half(int tiles_n, int group, bool zeros, bool words);
+Q4Entry q4_entry_float(int tiles_n, int group, bool zeros, bool words);
 Q4Entry q4_entry_bytes(int group, bool zeros, bool words);
 
 }  // namespace l2d

@@ -129,3 +129,60 @@ def test_attention_large_scores_fp16():
     for scale in (0.25, -0.25):
         attn_check(P, [300, 31], 4, L.F16, scale=scale)
         attn_check(P, [300, 31], 24, L.F16, scale=scale)
+
+
+# ------------------------------------------------------------------------------------------------
+# 4-bit products
+# ------------------------------------------------------------------------------------------------
+
+def product(w, s, z, x, N, group, dt, dt_y):
+    M, vectors = w.shape[0], x.shape[0]
+    y = torch.full((vectors, M), math.nan, dtype=TORCH[dt_y], device="cuda")
+    L.Q4Matrix(w, s, M, N, group, zeros=z, dtype_x=dt, dtype_y=dt_y, ldw=w.stride(0), lds=s.stride(0)).gemv(x, y, vectors=vectors, stride_x=x.stride(0))
+    torch.cuda.synchronize()
+    return y
+
+
+def weights(M, N, group, zeros, seed, pad=0):
+    g = gen(seed)
+    groups = -(-N // group)
+    w = torch.randint(0, 256, (M, (N + 1) // 2 + pad), dtype=torch.uint8, device="cuda", generator=g)
+    s = torch.empty(M, groups, device="cuda").uniform_(0.01, 0.02, generator=g).half()
+    z = torch.randint(0, 16, (M, groups), dtype=torch.uint8, device="cuda", generator=g) if zeros else None
+    return w, s, z
+
+
+def set_weight(w, column, value):
+    """q of a column of every row."""
+    byte, shift = w[:, column // 2], 4 * (column % 2)
+    w[:, column // 2] = (byte & (0xF0 if shift == 0 else 0x0F)) | (value.to(torch.uint8) << shift)
+
+
+def zero_point(z, column, group, M):
+    return z[:, column // group] & 15 if z is not None else torch.full((M,), 8, dtype=torch.uint8, device="cuda")
+
+
+def tolerance(N, total):
+    return 2 * U * (160 + N / 32) * total
+
+
+@pytest.mark.parametrize("dt,dt_y", [(L.F32, L.F32), (L.F16, L.F16), (L.BF16, L.BF16), (L.BF16, L.F32)])
+@pytest.mark.parametrize("group", [32, 64, 128, 256])
+@pytest.mark.parametrize("vectors", [1, 2, 5])
+def test_q4_rows_of_few_weights(dt, dt_y, group, vectors):
+    """Rows with one weight that is not zero, and one with none: the other columns leave nothing behind."""
+    M, N = 40, 768
+    w, s, z = weights(M, N, group, group == 256, seed=7)
+    for column in range(N):
+        set_weight(w, column, zero_point(z, column, group, M))
+    for row in range(1, M):
+        column = 19 * row
+        q = int(w[row, column // 2]) ^ (7 << (4 * (column % 2)))
+        w[row, column // 2] = q
+    x = normal(gen(8), L.F32, vectors, N)
+    x[:, 19 * 3] = 0.0078125
+    x = x.to(TORCH[dt])
+    want, total = q4_exact(w, s, z, x, N, group)
+    y = product(w, s, z, x, N, group, dt, dt_y)
+    assert (y[:, 0] == 0).all()
+    close(y, want, tolerance(N, total), dt_y)
