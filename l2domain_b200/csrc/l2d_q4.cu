@@ -149,7 +149,6 @@ int l2d_q4_gemv(const l2d_q4_desc *desc, const void *x, int64_t stride_x, void *
             continue;
         }
         const int tiles_n = a.vectors * each <= 8 ? 1 : a.vectors * each <= 16 ? 2 : 4;
-        const int columns = a.vectors * a.parts;
         const bool zeros = d.zeros != nullptr;
         const Q4Entry k = bytes              ? q4_entry_bytes(d.group, zeros, words)
                           : kind == kQ4From32 ? q4_entry_float(tiles_n, d.group, zeros, words)
@@ -166,16 +165,16 @@ int l2d_q4_gemv(const l2d_q4_desc *desc, const void *x, int64_t stride_x, void *
         constexpr int kRoom = 227 * 1024 - 64;
         const int mine = ((halves + kQ4Deep - 1) / kQ4Deep + a.ranks - 1) / a.ranks * kQ4Deep;  // of a block
         a.y_rows = a.ranks > 1 ? rows : 0;
-        const int per_half = q4_smem(tiles_n, bytes, columns, 4, 0).bytes - q4_smem(tiles_n, bytes, columns, 0, 0).bytes;  // four of them
-        int fits = (kRoom - q4_smem(tiles_n, bytes, columns, 0, a.y_rows * a.vectors).bytes) / per_half * 4;
+        const int per_half = q4_smem(tiles_n, bytes, a.vectors, a.parts, 4, 0).bytes - q4_smem(tiles_n, bytes, a.vectors, a.parts, 0, 0).bytes;  // four of them
+        int fits = (kRoom - q4_smem(tiles_n, bytes, a.vectors, a.parts, 0, a.y_rows * a.vectors).bytes) / per_half * 4;
         if (fits < mine) {
             a.y_rows = rows;
-            fits = (kRoom - q4_smem(tiles_n, bytes, columns, 0, rows * a.vectors).bytes) / per_half * 4;
+            fits = (kRoom - q4_smem(tiles_n, bytes, a.vectors, a.parts, 0, rows * a.vectors).bytes) / per_half * 4;
             const int times = (mine + fits - 1) / fits;
             fits = ((mine + times - 1) / times + kQ4Deep - 1) / kQ4Deep * kQ4Deep;
         }
         a.stage_h = std::min(fits, mine);
-        const int smem = q4_smem(tiles_n, bytes, columns, a.stage_h, a.y_rows * a.vectors).bytes;
+        const int smem = q4_smem(tiles_n, bytes, a.vectors, a.parts, a.stage_h, a.y_rows * a.vectors).bytes;
         L2D_CUDA_TRY(launch_clusters(k.run, dim3(static_cast<unsigned>(shape.shares * a.ranks)), a.ranks, kQ4Threads, smem, stream, a));
     }
     return L2D_OK;

@@ -17,10 +17,11 @@
 //    x meets a weight of zero, or a row has few others, their difference has few right bits left.  (A nibble masked
 //    into the low mantissa bits of an fp16 number is exact as it is, and two instructions less for every two weights:
 //    8 vectors 28672 x 8192 on groups of 128 take 42 us so, and 48 with the differences.)  A mask higher up gives 16 (q - z), with
-//    a sixteenth of x.  Each 128 columns of a vector are scaled by a power of two to a largest value just under 2^15;
-//    what is below 2^-28 of it may lose bits.
-//  * fp32 vectors take two columns of fp16, 11 bits each, which leaves one rounding of 2^-24.
-//  * Infinities and NaNs are staged as zeros, and the threads that store a vector's results add their terms at the end.
+//    a sixteenth of x.  Each 128 columns of a vector are scaled by a power of two to a largest value just under 2^15.
+//  * fp32 vectors take two columns of fp16, 11 bits each and a sign between them: the last of 24 bits of x may be lost.
+//  * Infinities and NaNs, and values so far below the largest of their 128 columns that the scaled number loses bits of
+//    them, are staged as zeros, and the threads that store a vector's results add their terms at the end: what is below
+//    2^-23 of the largest (fp32), or below 2^-24 of it and has bits that would be lost (16-bit vectors).
 //  * The scales are applied to the fp32 sums of each group.  One instruction sums over the four lanes of a
 //    row, 128 columns; where groups are shorter, x of the different groups goes to different columns of B
 //    (zeros elsewhere), so that each group still has a sum of its own: S = 128 / group columns per part.
@@ -72,15 +73,17 @@ constexpr int kQ4MaxRows = 896;    // rows of a block, at most
 // Bytes between columns of x in shared memory: 256 used (128 by bytes), and 64 so that two lie in other banks.
 __host__ __device__ constexpr int q4_column(bool bytes) { return bytes ? 192 : 320; }
 
-// Byte offsets in dynamic shared memory: x, its sums and factors, offsets of scales, the warps' sums, y.
+// Byte offsets in dynamic shared memory: x, its sums and factors, offsets of scales, marks of what of x is left out
+// (16 bytes for 128 columns of a vector), the warps' sums, y.
 struct Q4Smem {
-    int sums, offsets, red, y, bytes;
+    int sums, offsets, marks, red, y, bytes;
 };
-__host__ __device__ inline Q4Smem q4_smem(int tiles_n, bool bytes, int columns, int stage_h, int y_floats) {
+__host__ __device__ inline Q4Smem q4_smem(int tiles_n, bool bytes, int vectors, int parts, int stage_h, int y_floats) {
     Q4Smem s;
-    s.sums = columns * stage_h * q4_column(bytes);
+    s.sums = vectors * parts * stage_h * q4_column(bytes);
     s.offsets = s.sums + stage_h * 8 * tiles_n * 8;
-    s.red = s.offsets + (stage_h + 3) / 4 * 16;
+    s.marks = s.offsets + (stage_h + 3) / 4 * 16;
+    s.red = s.marks + vectors * stage_h * 16;
     s.y = s.red + (tiles_n == 1 ? 2 : 1) * kQ4Warps * kQ4Rows * 8 * tiles_n * 4;
     s.bytes = s.y + y_floats * 4;
     return s;
@@ -196,9 +199,10 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
     const int tid = threadIdx.x, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // known to be the same in all lanes
     const int columns = a.vectors * a.parts;                 // of x in shared memory
-    const Q4Smem lay = q4_smem(NT, BYTES, columns, a.stage_h, a.y_rows * a.vectors);
+    const Q4Smem lay = q4_smem(NT, BYTES, a.vectors, a.parts, a.stage_h, a.y_rows * a.vectors);
     float2 *sums = reinterpret_cast<float2 *>(smem + lay.sums);
     int *offsets = reinterpret_cast<int *>(smem + lay.offsets);
+    uint8_t *marks = reinterpret_cast<uint8_t *>(smem + lay.marks);
     float *red = reinterpret_cast<float *>(smem + lay.red), *ysum = reinterpret_cast<float *>(smem + lay.y);
     // This block's rows, and its halves of 128 columns.
     const int shares = gridDim.x / a.ranks, share = blockIdx.x / a.ranks, rank = blockIdx.x % a.ranks;
@@ -482,15 +486,12 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
                     const uint32_t m = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
                     return max(m & 0xffffu, m >> 16);
                 };
-                uint32_t top = largest();
-                const uint32_t odd_votes = __ballot_sync(0xffffffffu, top >= inf);
-                const bool odd = odd_votes >> (lane & 16) & 0xffff;
-                any_odd = any_odd || (real && odd);
-                if (odd_votes) {
+                uint32_t top = largest(), mark = 0;
+                if (top >= inf) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        if ((w[i] & 0x7fffu) >= inf) w[i] &= 0xffff0000u;
-                        if ((w[i] >> 16 & 0x7fffu) >= inf) w[i] &= 0xffffu;
+                        if ((w[i] & 0x7fffu) >= inf) w[i] &= 0xffff0000u, mark |= 1u << 2 * i;
+                        if ((w[i] >> 16 & 0x7fffu) >= inf) w[i] &= 0xffffu, mark |= 2u << 2 * i;
                     }
                     top = largest();
                 }
@@ -501,6 +502,17 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
                 float f[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) f[i] = scale_value(w[i / 2], i & 1, is_fp16) * up;
+                // All 11 bits of a value are above 2^-24, sixteenths included, down to 2^-10; each that is not is looked at.
+                const uint32_t m = __vminu2(__vminu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vminu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+                if ((__float_as_uint(scale_value(min(m & 0xffffu, m >> 16), false, is_fp16)) >> 23) + p < 244) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float g = i & 1 ? f[i] * 0.0625f : f[i];
+                        if (__half2float(__float2half_rn(g)) != g || (g == 0.0f && scale_value(w[i / 2], i & 1, is_fp16) != 0.0f)) f[i] = 0.0f, mark |= 1u << i;
+                    }
+                }
+                const bool odd = __ballot_sync(0xffffffffu, mark != 0) >> (lane & 16) & 0xffff;  // in these 128 columns
+                any_odd = any_odd || (real && odd);
                 uint32_t out[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -509,24 +521,25 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
                 }
                 if (real) reinterpret_cast<uint4 *>(smem + (half * columns + column) * kColumn)[j * 4 + tt] = make_uint4(out[0], out[1], out[2], out[3]);
                 if (stores_sums) to[0] = make_float2(0.0f, odd ? -back : back);  // the sign: see add_odd_ones()
+                if (real && odd) marks[(half * a.vectors + v) * 16 + u] = static_cast<uint8_t>(mark);
                 continue;
             }
             const uint32_t raw[8] = {r.lo.x, r.lo.y, r.lo.z, r.lo.w, r.hi.x, r.hi.y, r.hi.z, r.hi.w};
             float f[8];
-            uint32_t top = 0;
-            bool odd_ones = false;
+            uint32_t top = 0, mark = 0;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 f[i] = a.dtype_x == L2D_F32 ? __uint_as_float(raw[i]) : scale_value(raw[i / 2], i & 1, a.dtype_x == L2D_F16);
                 const uint32_t m = __float_as_uint(f[i]) & 0x7fffffffu;
                 if (m < 0x7f800000u) top = max(top, m);
-                else f[i] = 0.0f, odd_ones = true;
+                else f[i] = 0.0f, mark |= 1u << i;
             }
 #pragma unroll
             for (int d = 1; d < 16; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
-            const bool odd = __ballot_sync(0xffffffffu, odd_ones) >> (lane & 16) & 0xffff;  // in these 128 columns
-            any_odd = any_odd || (real && odd);
             if constexpr (BYTES) {
+                const bool odd = __ballot_sync(0xffffffffu, mark != 0) >> (lane & 16) & 0xffff;
+                any_odd = any_odd || (real && odd);
+                if (real && odd) marks[(half * a.vectors + v) * 16 + u] = static_cast<uint8_t>(mark);
                 // 2^(p - 127) takes the largest to [2^29, 2^30); four signed digits of 8 bits, a column each.
                 const uint32_t p = min(283u - (top >> 23), 253u);
                 const float up = __uint_as_float(p << 23), back = __uint_as_float((254u - p) << 23);
@@ -553,6 +566,18 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
             // 2^(p - 127) takes the largest to [2^14, 2^15); the factor back is short of 2^12, which the end makes good.
             const uint32_t p = min(268u - (top >> 23), 254u);
             const float up = __uint_as_float(p << 23), back = __uint_as_float((266u - p) << 23) * 0x1p-24f;
+            // The two parts keep 23 bits of what is not below 2^-13, sixteenths included.
+            bool far = false;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) far = far || (fabsf(f[i] * up) < (i & 1 ? 0x1p-9f : 0x1p-13f) && f[i] != 0.0f);
+            if (far) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (fabsf(f[i] * up) < (i & 1 ? 0x1p-9f : 0x1p-13f) && f[i] != 0.0f) f[i] = 0.0f, mark |= 1u << i;
+            }
+            const bool odd = __ballot_sync(0xffffffffu, mark != 0) >> (lane & 16) & 0xffff;
+            any_odd = any_odd || (real && odd);
+            if (real && odd) marks[(half * a.vectors + v) * 16 + u] = static_cast<uint8_t>(mark);
             uint32_t hi[8], lo[8];  // lo: what the first part leaves, 2^11 times as large
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -578,17 +603,20 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
     };
 
     bool odd_vectors = false;
-    // The terms of infinities and NaNs of x in this staging, for one result: row of the block, vector v.
+    // The terms of what of x was left out of this staging, for one result: row of the block, vector v.
     auto add_odd_ones = [&](float sum, int kb, int row, int v) {
         const int first = h_lo + kb * a.stage_h, halves = min(h_hi - first, a.stage_h);
         for (int half = 0; half < halves; ++half) {
             if (!(sums[half * 8 * NT + ((v * a.parts) << kShift)].y < 0.0f)) continue;
-            for (int col = (first + half) * kQ4Half; col < min(a.N, (first + half + 1) * kQ4Half); ++col) {
-                const float x = dev::load_as_float(a.x, a.dtype_x, v * a.stride_x + col);
-                if (isfinite(x)) continue;
-                const int64_t i = (r0 + row) * a.lds + group_of(col);
-                const int q = a.W[(r0 + row) * a.ldw + col / 2] >> (4 * (col & 1)) & 15, z = a.zeros ? a.zeros[i] & 15 : 8;
-                sum += dev::load_as_float(a.scales, a.dtype_s, i) * (static_cast<float>(q - z) * x);
+            const uint32_t *bits = reinterpret_cast<const uint32_t *>(marks + (half * a.vectors + v) * 16);
+            for (int w = 0; w < 4; ++w) {
+                for (uint32_t left = bits[w]; left; left &= left - 1) {
+                    const int col = (first + half) * kQ4Half + 32 * w + __ffs(left) - 1;
+                    const int64_t i = (r0 + row) * a.lds + group_of(col);
+                    const int q = a.W[(r0 + row) * a.ldw + col / 2] >> (4 * (col & 1)) & 15, z = a.zeros ? a.zeros[i] & 15 : 8;
+                    const float x = dev::load_as_float(a.x, a.dtype_x, v * a.stride_x + col);
+                    sum += dev::load_as_float(a.scales, a.dtype_s, i) * (static_cast<float>(q - z) * x);
+                }
             }
         }
         return sum;

@@ -166,6 +166,55 @@ def tolerance(N, total):
     return 2 * U * (160 + N / 32) * total
 
 
+LARGE = [(L.F32, L.F32, 1e4), (L.F32, L.F32, 1e6), (L.F32, L.F32, 2.0 ** 32), (L.F32, L.F32, 1e10), (L.F32, L.F32, 1e30),
+         (L.BF16, L.F32, 1e6), (L.BF16, L.F32, 1e12), (L.BF16, L.BF16, 1e8), (L.BF16, L.BF16, 3e35), (L.F16, L.F32, 6e4),
+         (L.F16, L.F16, 6e4), (L.F32, L.BF16, 1e9)]
+
+
+def large_activation(dt, dt_y, large, group, vectors):
+    """What the largest activation is multiplied with is zero: the others have all their bits."""
+    M, N = 70, 1152
+    w, s, z = weights(M, N, group, group == 64, seed=group)
+    x = normal(gen(3), L.F32, vectors, N)
+    if dt == L.F16:
+        x *= 0.01
+    for b in range(vectors):
+        for column in (5 + 17 * b, 640 + b):
+            set_weight(w, column, zero_point(z, column, group, M))
+            x[b, column] = -large if b % 2 else large
+    x = x.to(TORCH[dt])
+    want, total = q4_exact(w, s, z, x, N, group)
+    close(product(w, s, z, x, N, group, dt, dt_y), want, tolerance(N, total), dt_y)
+
+
+def every_size(dt, group, vectors):
+    """Powers of two from 2^-40 to 2^40 in one vector, the largest on weights of zero; and all of them scaled by 2^60."""
+    M, N = 33, 1024
+    w, s, z = weights(M, N, group, True, seed=vectors)
+    g = gen(5)
+    size = torch.randint(-40, 41, (vectors, N), device="cuda", generator=g).float()
+    x = normal(g, L.F32, vectors, N) * torch.exp2(size)
+    for column in torch.unique(torch.nonzero(size > 0)[:, 1]).tolist():
+        set_weight(w, column, zero_point(z, column, group, M))
+    for scale in (1.0, 2.0 ** 60, 2.0 ** -60):
+        xx = (x * scale).to(TORCH[dt])
+        want, total = q4_exact(w, s, z, xx, N, group)
+        close(product(w, s, z, xx, N, group, dt, L.F32), want, tolerance(N, total), L.F32)
+
+
+@pytest.mark.parametrize("dt,dt_y,large", LARGE)
+@pytest.mark.parametrize("group", [32, 64, 128, 384])
+@pytest.mark.parametrize("vectors", [3, 9])
+def test_q4_large_activation_on_a_zero_weight_several_vectors(dt, dt_y, large, group, vectors):
+    large_activation(dt, dt_y, large, group, vectors)
+
+
+@pytest.mark.parametrize("dt", [L.F32, L.BF16])
+@pytest.mark.parametrize("group", [32, 64, 128, 512])
+def test_q4_activations_of_every_size_several_vectors(dt, group):
+    every_size(dt, group, 4)
+
+
 @pytest.mark.parametrize("dt,dt_y", [(L.F32, L.F32), (L.F16, L.F16), (L.BF16, L.BF16), (L.BF16, L.F32)])
 @pytest.mark.parametrize("group", [32, 64, 128, 256])
 @pytest.mark.parametrize("vectors", [1, 2, 5])
@@ -186,3 +235,30 @@ def test_q4_rows_of_few_weights(dt, dt_y, group, vectors):
     y = product(w, s, z, x, N, group, dt, dt_y)
     assert (y[:, 0] == 0).all()
     close(y, want, tolerance(N, total), dt_y)
+
+
+def infinities_and_nans(dt, group, vectors):
+    """They reach their own vector, beside activations of wide range, which keep their bits in the others."""
+    M, N = 50, 640
+    w, s, z = weights(M, N, group, True, seed=11)
+    set_weight(w, 300, zero_point(z, 300, group, M))
+    set_weight(w, 200, (zero_point(z, 200, group, M) + 1) % 16)  # z + 1, or -15 where z is 15
+    x = normal(gen(4), L.F32, vectors, N).to(TORCH[dt])
+    x[:, 300] = 60000.0
+    clean = product(w, s, z, x, N, group, dt, L.F32)
+    want, total = q4_exact(w, s, z, x, N, group)
+    close(clean, want, tolerance(N, total), L.F32)
+    last = vectors - 1
+    for odd in (math.inf, -math.inf, math.nan):
+        x[last, 200] = odd
+        y = product(w, s, z, x, N, group, dt, L.F32)
+        assert torch.equal(y[:last], clean[:last])
+        up = zero_point(z, 200, group, M) != 15
+        assert torch.isnan(y[last]).all() if math.isnan(odd) else torch.equal(y[last], torch.where(up, odd, -odd))
+
+
+@pytest.mark.parametrize("dt", [L.F32, L.F16, L.BF16])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("vectors", [3, 10])
+def test_q4_infinities_and_nans_several_vectors(dt, group, vectors):
+    infinities_and_nans(dt, group, vectors)
