@@ -134,10 +134,10 @@ int l2d_q4_gemv(const l2d_q4_desc *desc, const void *x, int64_t stride_x, void *
     const bool words = !misaligned(d.W, 16) && ldw % 16 == 0 && d.dtype_s != L2D_F32 && together(word);
     a.wide = together(2 * word);
     const int sub = d.group == 32 ? 4 : d.group == 64 ? 2 : 1;
-    const Q4Kind kind = vectors * sub <= 2 ? kQ4Bytes : d.dtype_x == L2D_F32 ? kQ4From32 : kQ4From16;
-    const bool bytes = kind == kQ4Bytes;
-    a.parts = bytes ? 4 : d.dtype_x == L2D_F32 ? 2 : 1;
-    const int each = a.parts * sub;                                         // columns of B per vector
+    const bool fp32 = d.dtype_x == L2D_F32;
+    const bool bytes = vectors * sub * q4_parts(fp32 ? kQ4Bytes32 : kQ4Bytes16) <= 8;  // columns of B
+    const int parts = q4_parts(bytes ? fp32 ? kQ4Bytes32 : kQ4Bytes16 : fp32 ? kQ4Half32 : kQ4Half16);
+    const int each = parts * sub;                                           // columns of B per vector
     const int most = 32 / each;                                             // vectors of one pass over the weights
     const int halves = static_cast<int>((d.N + kQ4Half - 1) / kQ4Half);
     for (int64_t v = 0; v < vectors; v += most) {
@@ -150,9 +150,9 @@ int l2d_q4_gemv(const l2d_q4_desc *desc, const void *x, int64_t stride_x, void *
         }
         const int tiles_n = a.vectors * each <= 8 ? 1 : a.vectors * each <= 16 ? 2 : 4;
         const bool zeros = d.zeros != nullptr;
-        const Q4Entry k = bytes              ? q4_entry_bytes(d.group, zeros, words)
-                          : kind == kQ4From32 ? q4_entry_float(tiles_n, d.group, zeros, words)
-                                             : q4_entry_half(tiles_n, d.group, zeros, words);
+        const Q4Entry k = bytes  ? q4_entry_bytes(fp32, d.group, zeros, words)
+                          : fp32 ? q4_entry_float(tiles_n, d.group, zeros, words)
+                                 : q4_entry_half(tiles_n, d.group, zeros, words);
         L2D_CUDA_TRY(allow_smem(k.run, 227 * 1024, d.device, *k.smem_set));
         const int *clusters = nullptr;
         const int known = q4_clusters(d.device, k, &clusters);
@@ -165,16 +165,16 @@ int l2d_q4_gemv(const l2d_q4_desc *desc, const void *x, int64_t stride_x, void *
         constexpr int kRoom = 227 * 1024 - 64;
         const int mine = ((halves + kQ4Deep - 1) / kQ4Deep + a.ranks - 1) / a.ranks * kQ4Deep;  // of a block
         a.y_rows = a.ranks > 1 ? rows : 0;
-        const int per_half = q4_smem(tiles_n, bytes, a.vectors, a.parts, 4, 0).bytes - q4_smem(tiles_n, bytes, a.vectors, a.parts, 0, 0).bytes;  // four of them
-        int fits = (kRoom - q4_smem(tiles_n, bytes, a.vectors, a.parts, 0, a.y_rows * a.vectors).bytes) / per_half * 4;
+        const int per_half = q4_smem(tiles_n, bytes, a.vectors, parts, 4, 0).bytes - q4_smem(tiles_n, bytes, a.vectors, parts, 0, 0).bytes;  // four of them
+        int fits = (kRoom - q4_smem(tiles_n, bytes, a.vectors, parts, 0, a.y_rows * a.vectors).bytes) / per_half * 4;
         if (fits < mine) {
             a.y_rows = rows;
-            fits = (kRoom - q4_smem(tiles_n, bytes, a.vectors, a.parts, 0, rows * a.vectors).bytes) / per_half * 4;
+            fits = (kRoom - q4_smem(tiles_n, bytes, a.vectors, parts, 0, rows * a.vectors).bytes) / per_half * 4;
             const int times = (mine + fits - 1) / fits;
             fits = ((mine + times - 1) / times + kQ4Deep - 1) / kQ4Deep * kQ4Deep;
         }
         a.stage_h = std::min(fits, mine);
-        const int smem = q4_smem(tiles_n, bytes, a.vectors, a.parts, a.stage_h, a.y_rows * a.vectors).bytes;
+        const int smem = q4_smem(tiles_n, bytes, a.vectors, parts, a.stage_h, a.y_rows * a.vectors).bytes;
         L2D_CUDA_TRY(launch_clusters(k.run, dim3(static_cast<unsigned>(shape.shares * a.ranks)), a.ranks, kQ4Threads, smem, stream, a));
     }
     return L2D_OK;

@@ -10,8 +10,7 @@
 //
 //  * Few vectors are multiplied in integers (m16n8k32, bytes): two masks and a shift turn eight nibbles into
 //    bytes.  x of each 128 columns is a 30-bit integer times a power of two, in four signed digits of 8 bits, a
-//    column of B each.  Sums are exact up to the end of a group; values of x are exact down to 2^-6 (fp32),
-//    2^-19 (fp16) or 2^-22 (bf16) of the largest among their 128 columns, and otherwise off by at most 2^-30 of it.
+//    column of B each, and one of fp32 a 60-bit integer in eight.  x is exact, and so are sums up to the end of a group.
 //  * More vectors are multiplied in fp16 with fp32 sums (m16n8k16), one column a vector.  The difference q - z is
 //    taken first, exactly, from 1024 + q and 1024 + z, because sum q x and z sum x may nearly cancel: where the largest
 //    x meets a weight of zero, or a row has few others, their difference has few right bits left.  (A nibble masked
@@ -20,8 +19,9 @@
 //    a sixteenth of x.  Each 128 columns of a vector are scaled by a power of two to a largest value just under 2^15.
 //  * fp32 vectors take two columns of fp16, 11 bits each and a sign between them: the last of 24 bits of x may be lost.
 //  * Infinities and NaNs, and values so far below the largest of their 128 columns that the scaled number loses bits of
-//    them, are staged as zeros, and the threads that store a vector's results add their terms at the end: what is below
-//    2^-23 of the largest (fp32), or below 2^-24 of it and has bits that would be lost (16-bit vectors).
+//    them, are staged as zeros, and the threads that store a vector's results add their terms at the end.  In fp16 that
+//    is what is below 2^-23 of the largest (fp32), or below 2^-24 of it with bits that would be lost (16-bit vectors); in
+//    integers, below 2^-36 (fp32), 2^-19 (fp16) or 2^-22 (bf16) of it with such bits.
 //  * The scales are applied to the fp32 sums of each group.  One instruction sums over the four lanes of a
 //    row, 128 columns; where groups are shorter, x of the different groups goes to different columns of B
 //    (zeros elsewhere), so that each group still has a sum of its own: S = 128 / group columns per part.
@@ -55,7 +55,6 @@ struct Q4Args {
     void *y;
     int64_t M, ldw, lds, stride_x, stride_y;
     int N, vectors, group, dtype_x, dtype_y, dtype_s;
-    int parts;       // columns of x per vector: 4 by bytes, 2 for fp32, else 1
     int warps_k;     // warps that split a tile's columns
     int ranks;       // blocks of a cluster, which split the columns
     int stage_h;     // halves of 128 columns of x staged at a time
@@ -188,18 +187,21 @@ __device__ __forceinline__ float scale_value(uint32_t word, bool high, bool is_h
 // S: columns of B per part of a vector (4, 2, 1 for groups of 32, 64, 128 columns), 0 for longer groups.
 // WORDS: every row of W is whole 16-byte words on 16-byte boundaries, and the 16-bit scales (and zeros) of a step
 // can be read in words.
-// KIND: how products are taken: in fp16 with 16-bit or fp32 vectors, or by bytes.
-enum Q4Kind { kQ4From16, kQ4From32, kQ4Bytes };
+// KIND: how products are taken, in fp16 or by bytes, and whether vectors have 16 or 32 bits.
+enum Q4Kind { kQ4Half16, kQ4Half32, kQ4Bytes16, kQ4Bytes32 };
+// Columns of x per vector.
+__host__ __device__ constexpr int q4_parts(Q4Kind kind) { return kind == kQ4Bytes32 ? 8 : kind == kQ4Bytes16 ? 4 : kind == kQ4Half32 ? 2 : 1; }
 template <int NT, int S, bool ZEROS, bool WORDS, Q4Kind KIND>
 __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
-    constexpr bool BYTES = KIND == kQ4Bytes;
+    constexpr bool BYTES = KIND == kQ4Bytes16 || KIND == kQ4Bytes32, FP32 = KIND == kQ4Half32 || KIND == kQ4Bytes32;
+    constexpr int PARTS = q4_parts(KIND);
     constexpr int SUB = S > 1 ? S : 1, kShift = S == 4 ? 2 : S == 2 ? 1 : 0, E = S > 1 ? 2 : 1, kColumn = q4_column(BYTES);
     constexpr float kUnit = BYTES ? 1.0f : 4096.0f;  // of the sums
     extern __shared__ __align__(16) char smem[];
     const int tid = threadIdx.x, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // known to be the same in all lanes
-    const int columns = a.vectors * a.parts;                 // of x in shared memory
-    const Q4Smem lay = q4_smem(NT, BYTES, a.vectors, a.parts, a.stage_h, a.y_rows * a.vectors);
+    const int columns = a.vectors * PARTS;                 // of x in shared memory
+    const Q4Smem lay = q4_smem(NT, BYTES, a.vectors, PARTS, a.stage_h, a.y_rows * a.vectors);
     float2 *sums = reinterpret_cast<float2 *>(smem + lay.sums);
     int *offsets = reinterpret_cast<int *>(smem + lay.offsets);
     uint8_t *marks = reinterpret_cast<uint8_t *>(smem + lay.marks);
@@ -449,7 +451,7 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
         auto fetch = [&](const Unit &e) {
             Raw r = {};
             if (e.v >= a.vectors) return r;
-            const int v = e.v, col = (first + e.half) * kQ4Half + 8 * u, size = a.dtype_x == L2D_F32 ? 4 : 2;
+            const int v = e.v, col = (first + e.half) * kQ4Half + 8 * u, size = FP32 ? 4 : 2;
             const char *src = static_cast<const char *>(a.x) + (v * a.stride_x + col) * size;
             if (col + 8 <= a.N && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
                 r.lo = __ldg(reinterpret_cast<const uint4 *>(src));
@@ -473,12 +475,12 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
         for (int e = mine; e - (lane >> 4) < units; e += kQ4Warps * 2) {
             const Raw r = ahead;
             const bool real = e < units;
-            const int v = real ? at.v : 0, half = real ? at.half : 0, column = v * a.parts, tt = u >> 2, j = u & 3;
+            const int v = real ? at.v : 0, half = real ? at.half : 0, column = v * PARTS, tt = u >> 2, j = u & 3;
             float2 *to = sums + half * 8 * NT + (column << kShift) + u / (16 / SUB);
             const bool stores_sums = real && u % (16 / SUB) == 0;
             step(at);
             ahead = fetch(at);
-            if constexpr (KIND == kQ4From16) {  // the same as below in fewer instructions
+            if constexpr (KIND == kQ4Half16) {  // the same as below in fewer instructions
                 uint32_t w[4] = {r.lo.x, r.lo.y, r.lo.z, r.lo.w};
                 const bool is_fp16 = a.dtype_x == L2D_F16;
                 const uint32_t inf = is_fp16 ? 0x7c00u : 0x7f80u;
@@ -529,7 +531,7 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
             uint32_t top = 0, mark = 0;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                f[i] = a.dtype_x == L2D_F32 ? __uint_as_float(raw[i]) : scale_value(raw[i / 2], i & 1, a.dtype_x == L2D_F16);
+                f[i] = FP32 ? __uint_as_float(raw[i]) : scale_value(raw[i / 2], i & 1, a.dtype_x == L2D_F16);
                 const uint32_t m = __float_as_uint(f[i]) & 0x7fffffffu;
                 if (m < 0x7f800000u) top = max(top, m);
                 else f[i] = 0.0f, mark |= 1u << i;
@@ -537,29 +539,53 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
 #pragma unroll
             for (int d = 1; d < 16; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
             if constexpr (BYTES) {
+                // 2^(p - 127) takes the largest to [2^29, 2^30); four signed digits of 8 bits, a column each, and for fp32
+                // four more of the next 30 bits.
+                const uint32_t p = min(283u - (top >> 23), 253u);
+                const float up = __uint_as_float(p << 23), back = __uint_as_float((254u - p) << 23);
+                const float least = FP32 ? 0x1p-7f : 0x1p10f;  // from here on all bits of a value are there
+                bool far = false;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) far = far || (fabsf(f[i] * up) < least && f[i] != 0.0f);
+                if (far) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float n = f[i] * up;
+                        float left = n - rintf(n);
+                        if (FP32) left = left * 0x1p30f - rintf(left * 0x1p30f);
+                        if (left != 0.0f || (n == 0.0f && f[i] != 0.0f)) f[i] = 0.0f, mark |= 1u << i;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) f[i] *= up;
                 const bool odd = __ballot_sync(0xffffffffu, mark != 0) >> (lane & 16) & 0xffff;
                 any_odd = any_odd || (real && odd);
                 if (real && odd) marks[(half * a.vectors + v) * 16 + u] = static_cast<uint8_t>(mark);
-                // 2^(p - 127) takes the largest to [2^29, 2^30); four signed digits of 8 bits, a column each.
-                const uint32_t p = min(283u - (top >> 23), 253u);
-                const float up = __uint_as_float(p << 23), back = __uint_as_float((254u - p) << 23);
-                uint32_t digits[8];
+                auto four_digits = [&](int part, float unit) {
+                    uint32_t digits[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) digits[i] = (static_cast<uint32_t>(__float2int_rn(f[i] * up)) + 0x00808080u) ^ 0x00808080u;
+                    for (int i = 0; i < 8; ++i) digits[i] = (static_cast<uint32_t>(__float2int_rn(f[i])) + 0x00808080u) ^ 0x00808080u;
 #pragma unroll
-                for (int d = 0; d < 4; ++d) {
-                    const uint32_t pick = d | (4 + d) << 4;
-                    const uint32_t even = __byte_perm(__byte_perm(digits[0], digits[2], pick), __byte_perm(digits[4], digits[6], pick), 0x5410);
-                    const uint32_t odds = __byte_perm(__byte_perm(digits[1], digits[3], pick), __byte_perm(digits[5], digits[7], pick), 0x5410);
-                    if (real)
-                        *reinterpret_cast<uint2 *>(smem + (half * columns + column + d) * kColumn + (j >> 1) * 64 + tt * 16 + (j & 1) * 8) = make_uint2(even, odds);
-                    int total = __dp4a(static_cast<int>(even), 0x01010101, __dp4a(static_cast<int>(odds), 0x01010101, 0));
+                    for (int d = 0; d < 4; ++d) {
+                        const uint32_t pick = d | (4 + d) << 4;
+                        const uint32_t even = __byte_perm(__byte_perm(digits[0], digits[2], pick), __byte_perm(digits[4], digits[6], pick), 0x5410);
+                        const uint32_t odds = __byte_perm(__byte_perm(digits[1], digits[3], pick), __byte_perm(digits[5], digits[7], pick), 0x5410);
+                        if (real)
+                            *reinterpret_cast<uint2 *>(smem + (half * columns + column + part + d) * kColumn + (j >> 1) * 64 + tt * 16 + (j & 1) * 8) = make_uint2(even, odds);
+                        int total = __dp4a(static_cast<int>(even), 0x01010101, __dp4a(static_cast<int>(odds), 0x01010101, 0));
 #pragma unroll
-                    for (int o = 1; o < 16 / SUB; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-                    const float factor = back * static_cast<float>(1 << 8 * d);
-                    if (stores_sums)
-                        to[d << kShift] = make_float2(ZEROS ? static_cast<float>(total) : 12582912.0f + 8.0f * static_cast<float>(total),
-                                                      odd && d == 0 ? -factor : factor);  // the sign: see add_odd_ones()
+                        for (int o = 1; o < 16 / SUB; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+                        const float factor = unit * static_cast<float>(1 << 8 * d);
+                        if (stores_sums)
+                            to[(part + d) << kShift] = make_float2(ZEROS ? static_cast<float>(total) : 12582912.0f + 8.0f * static_cast<float>(total),
+                                                                   odd && part + d == 0 ? -factor : factor);  // the sign: see add_odd_ones()
+                    }
+                };
+                four_digits(0, back);
+                if constexpr (FP32) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) f[i] = (f[i] - rintf(f[i])) * 0x1p30f;
+                    four_digits(4, back * 0x1p-30f);
                 }
                 continue;
             }
@@ -607,7 +633,7 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
     auto add_odd_ones = [&](float sum, int kb, int row, int v) {
         const int first = h_lo + kb * a.stage_h, halves = min(h_hi - first, a.stage_h);
         for (int half = 0; half < halves; ++half) {
-            if (!(sums[half * 8 * NT + ((v * a.parts) << kShift)].y < 0.0f)) continue;
+            if (!(sums[half * 8 * NT + ((v * PARTS) << kShift)].y < 0.0f)) continue;
             const uint32_t *bits = reinterpret_cast<const uint32_t *>(marks + (half * a.vectors + v) * 16);
             for (int w = 0; w < 4; ++w) {
                 for (uint32_t left = bits[w]; left; left &= left - 1) {
@@ -644,10 +670,10 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
         for (int e = ((wk + tile) & (a.warps_k - 1)) * 32 + lane; e < kQ4Rows * a.vectors; e += a.warps_k * 32) {
             const int v = e / kQ4Rows, r = e % kQ4Rows, row = lo + r;
             if (r >= n) continue;
-            const float *p = red + ((buffer * kQ4Warps + wm * a.warps_k) * kQ4Rows + r) * 8 * NT + v * a.parts * SUB;
+            const float *p = red + ((buffer * kQ4Warps + wm * a.warps_k) * kQ4Rows + r) * 8 * NT + v * PARTS * SUB;
             float sum = 0.0f;
             for (int w = 0; w < a.warps_k; ++w, p += kQ4Rows * 8 * NT)
-                for (int i = 0; i < a.parts; ++i)
+                for (int i = 0; i < PARTS; ++i)
 #pragma unroll
                     for (int c = 0; c < SUB; ++c) sum += p[i * SUB + c];
             if (odd_vectors) sum = add_odd_ones(sum * kUnit, kb, row, v) / kUnit;
@@ -763,6 +789,6 @@ Q4Entry q4_entry(int group, bool zeros, bool words) {
 // The kernels of one kind each, compiled apart; tiles_n: how many eights of columns B has (1, 2 or 4; by bytes 1).
 Q4Entry q4_entry_half(int tiles_n, int group, bool zeros, bool words);
 Q4Entry q4_entry_float(int tiles_n, int group, bool zeros, bool words);
-Q4Entry q4_entry_bytes(int group, bool zeros, bool words);
+Q4Entry q4_entry_bytes(bool fp32, int group, bool zeros, bool words);
 
 }  // namespace l2d

@@ -209,10 +209,24 @@ def test_q4_large_activation_on_a_zero_weight_several_vectors(dt, dt_y, large, g
     large_activation(dt, dt_y, large, group, vectors)
 
 
+@pytest.mark.parametrize("dt,dt_y,large", LARGE)
+@pytest.mark.parametrize("group", [32, 64, 128, 384])
+@pytest.mark.parametrize("vectors", [1, 2])
+def test_q4_large_activation_on_a_zero_weight(dt, dt_y, large, group, vectors):
+    large_activation(dt, dt_y, large, group, vectors)
+
+
 @pytest.mark.parametrize("dt", [L.F32, L.BF16])
 @pytest.mark.parametrize("group", [32, 64, 128, 512])
 def test_q4_activations_of_every_size_several_vectors(dt, group):
     every_size(dt, group, 4)
+
+
+@pytest.mark.parametrize("dt", [L.F32, L.BF16])
+@pytest.mark.parametrize("group", [32, 64, 128, 512])
+@pytest.mark.parametrize("vectors", [1, 2])
+def test_q4_activations_of_every_size(dt, group, vectors):
+    every_size(dt, group, vectors)
 
 
 @pytest.mark.parametrize("dt,dt_y", [(L.F32, L.F32), (L.F16, L.F16), (L.BF16, L.BF16), (L.BF16, L.F32)])
@@ -261,4 +275,11 @@ def infinities_and_nans(dt, group, vectors):
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("vectors", [3, 10])
 def test_q4_infinities_and_nans_several_vectors(dt, group, vectors):
+    infinities_and_nans(dt, group, vectors)
+
+
+@pytest.mark.parametrize("dt", [L.F32, L.F16, L.BF16])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("vectors", [1, 2])
+def test_q4_infinities_and_nans(dt, group, vectors):
     infinities_and_nans(dt, group, vectors)
