@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
     constexpr bool BYTES = KIND == kQ4Bytes16 || KIND == kQ4Bytes32, FP32 = KIND == kQ4Half32 || KIND == kQ4Bytes32;
     constexpr int PARTS = q4_parts(KIND);
     constexpr int SUB = S > 1 ? S : 1, kShift = S == 4 ? 2 : S == 2 ? 1 : 0, E = S > 1 ? 2 : 1, kColumn = q4_column(BYTES);
-    constexpr float kUnit = BYTES ? 1.0f : 4096.0f;  // of the sums
+    constexpr float kUnit = BYTES ? 0x1p16f : 0x1p12f;  // of the sums: those of (q - z) x may pass the range before their scale
     extern __shared__ __align__(16) char smem[];
     const int tid = threadIdx.x, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // known to be the same in all lanes
@@ -540,9 +540,9 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
             for (int d = 1; d < 16; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
             if constexpr (BYTES) {
                 // 2^(p - 127) takes the largest to [2^29, 2^30); four signed digits of 8 bits, a column each, and for fp32
-                // four more of the next 30 bits.
+                // four more of the next 30 bits.  The factor back is short of 2^16, which the end makes good.
                 const uint32_t p = min(283u - (top >> 23), 253u);
-                const float up = __uint_as_float(p << 23), back = __uint_as_float((254u - p) << 23);
+                const float up = __uint_as_float(p << 23), back = __uint_as_float((254u - p) << 23) * 0x1p-16f;
                 const float least = FP32 ? 0x1p-7f : 0x1p10f;  // from here on all bits of a value are there
                 bool far = false;
 #pragma unroll

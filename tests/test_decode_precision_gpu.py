@@ -251,6 +251,21 @@ def test_q4_rows_of_few_weights(dt, dt_y, group, vectors):
     close(y, want, tolerance(N, total), dt_y)
 
 
+@pytest.mark.parametrize("dt", [L.F32, L.BF16])
+@pytest.mark.parametrize("group", [32, 64, 128, 256])
+@pytest.mark.parametrize("vectors", [1, 2, 5])
+def test_q4_sums_that_pass_the_range_before_their_scale(dt, group, vectors):
+    """Activations of 2^122: sums of (q - z) x pass the range of fp32, the scaled ones do not."""
+    M, N = 20, 512
+    w, s, z = weights(M, N, group, False, seed=9)
+    w |= 0x88  # all weights positive
+    s *= 2.0 ** -6
+    x = ((normal(gen(2), L.F32, vectors, N).abs() + 1) * 2.0 ** 122).to(TORCH[dt])
+    want, total = q4_exact(w, s, z, x, N, group)
+    assert want.max() < 2.0 ** 127
+    close(product(w, s, z, x, N, group, dt, dt), want, tolerance(N, total), dt)
+
+
 def infinities_and_nans(dt, group, vectors):
     """They reach their own vector, beside activations of wide range, which keep their bits in the others."""
     M, N = 50, 640
