@@ -316,11 +316,18 @@ __device__ __forceinline__ uint32_t pack2(T lo, T hi) {
     return static_cast<uint32_t>(a) | static_cast<uint32_t>(b) << 16;
 }
 
+// What is added to the largest score before exponents are taken relative to it: weights of 2^-24 and less leave sums of
+// 2^24 of the largest values inside the range.  Values of fp16 need no such room.
+template <typename T>
+constexpr float kRoom = 24.0f;
+template <>
+constexpr float kRoom<__half> = 0.0f;
+
 // A running softmax's maximum, and what exponents are taken relative to: never -inf.
 __device__ __forceinline__ float finite_base(float m) { return m == -INFINITY ? 0.0f : m; }
 
-// Weights, 1 for the largest score, as numbers of the cache's type: bf16 has the exponents of fp32, but fp16 ends at
-// 2^-24, so there they are taken 2^15 times as large (and sums of values too, until they leave the registers).
+// Weights as numbers of the cache's type: bf16 has the exponents of fp32, but fp16 ends at
+// 2^-24, so there they, 1 for the largest score, are taken 2^15 times as large (and sums of values too, until they leave the registers).
 template <typename T>
 constexpr float kWeightUnit = 1.0f;
 template <>
@@ -404,7 +411,7 @@ struct MmaCore {
     }
 
     // One tile: keys at ks, values at vs (shared memory), bit j of live: key j counts.  scale2 > 0.  Scores are scaled,
-    // and rounded, before the maximum is taken and taken off: the largest is then 0 whatever its size.  With one
+    // and rounded, before the maximum is taken and taken off: the largest is then -kRoom or close to it whatever its size.  With one
     // rounding fewer, by a fused multiply-add on the unscaled ones, it would be what that rounding left: hundreds for
     // scores of 2^31.
     __device__ __forceinline__ void step(const char *ks, const char *vs, uint32_t live, float scale2) {
@@ -447,7 +454,7 @@ struct MmaCore {
             float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const float m2 = fmaxf(m[r], top), base = finite_base(m2);
+            const float m2 = fmaxf(m[r], top + kRoom<T>), base = finite_base(m2);
             if (__any_sync(0xffffffffu, m2 != m[r])) {
                 const float f = exp2_approx(m[r] - base);
                 l[r] *= f;
@@ -584,7 +591,7 @@ struct SimdCore {
             float top = ok ? s[g] : -INFINITY;
 #pragma unroll
             for (int d = 1; d < kKeys; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-            const float m2 = fmaxf(m[g], top), base = finite_base(m2), f = exp2_approx(m[g] - base);
+            const float m2 = fmaxf(m[g], top + kRoom<float>), base = finite_base(m2), f = exp2_approx(m[g] - base);
             const float w = ok ? exp2_approx(s[g] - base) : 0.0f;
             l[g] = fmaf(l[g], f, w);
             m[g] = m2;

@@ -123,6 +123,21 @@ def test_attention_fp32_groups_on_wide_heads(D, G):
     attn_check(P, [300, 0, 129], 2 * G, L.F32)
 
 
+@pytest.mark.parametrize("dt", [L.F32, L.F16, L.BF16])
+@pytest.mark.parametrize("G,D", [(1, 64), (8, 128), (16, 64), (4, 256)])
+def test_attention_values_near_the_end_of_the_range(dt, G, D):
+    """Their mean is in the range, and their sum is not."""
+    P = Pages(dt, 1, 130, 16, 1, D, seed=G)
+    n = 2000
+    largest = torch.finfo(TORCH[dt]).max
+    scores = torch.rand(n, device="cuda", generator=gen(D)) * 0.25
+    values = (0.5 + 0.25 * torch.rand(n, 1, D, device="cuda", generator=gen(G))) * largest
+    values[:, :, 1::2] *= -1
+    out, lse, want, want_lse, slack, off = steered(P, n, G, dt, scores, values, torch.ones(G, device="cuda"))
+    close(out, want, slack, dt)
+    close(lse, want_lse, off, L.F32)
+
+
 def test_attention_large_scores_fp16():
     P = Pages(L.F16, 2, 20, 16, 2, 64, seed=5)
     P.k.mul_(64)
