@@ -123,7 +123,6 @@ int l2d_q4_gemv(const l2d_q4_desc *desc, const void *x, int64_t stride_x, void *
     a.lds = lds;
     a.stride_x = stride_x;
     a.stride_y = stride_y;
-    a.group = d.group;
     a.dtype_x = d.dtype_x;
     a.dtype_y = d.dtype_y;
     a.dtype_s = d.dtype_s;

@@ -54,7 +54,7 @@ struct Q4Args {
     const void *x;
     void *y;
     int64_t M, ldw, lds, stride_x, stride_y;
-    int N, vectors, group, dtype_x, dtype_y, dtype_s;
+    int N, vectors, dtype_x, dtype_y, dtype_s;
     int warps_k;     // warps that split a tile's columns
     int ranks;       // blocks of a cluster, which split the columns
     int stage_h;     // halves of 128 columns of x staged at a time
