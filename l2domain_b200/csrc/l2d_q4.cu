@@ -13,12 +13,12 @@ __global__ void k_q4_zero(Q4Args a) {
         dev::store_as(a.y, a.dtype_y, e / a.M * a.stride_y + e % a.M, 0.0f);
 }
 
-// How many clusters of 1, 2, 4 and 8 blocks of one SM each run at the same time; looked up once per device.
-int q4_clusters(int device, const Q4Entry &k, const int **clusters) {
-    static int known[kMaxDevices][4];
-    static std::atomic<bool> done[kMaxDevices];
-    if (!done[device].load(std::memory_order_acquire)) {
-        int found[4];
+// How many clusters of 1, 2, 4 and 8 blocks of one SM each run at the same time; looked up once per device, and kept
+// as four numbers of 16 bits in one word.
+int q4_clusters(int device, const Q4Entry &k, int (&clusters)[4]) {
+    static std::atomic<uint64_t> known[kMaxDevices];
+    uint64_t word = known[device].load(std::memory_order_relaxed);
+    if (!word) {
         for (int i = 0; i < 4; ++i) {
             cudaLaunchConfig_t cfg = {};
             cudaLaunchAttribute attr[1];
@@ -30,12 +30,13 @@ int q4_clusters(int device, const Q4Entry &k, const int **clusters) {
             cfg.dynamicSmemBytes = 200 * 1024;
             cfg.attrs = attr;
             cfg.numAttrs = 1;
-            L2D_CUDA_TRY(cudaOccupancyMaxActiveClusters(&found[i], k.run, &cfg));
+            int found = 0;
+            L2D_CUDA_TRY(cudaOccupancyMaxActiveClusters(&found, k.run, &cfg));
+            word |= static_cast<uint64_t>(std::min(found, 0xffff)) << (16 * i);
         }
-        std::copy(found, found + 4, known[device]);  // the same for every thread that gets here
-        done[device].store(true, std::memory_order_release);
+        known[device].store(word, std::memory_order_relaxed);
     }
-    *clusters = known[device];
+    for (int i = 0; i < 4; ++i) clusters[i] = static_cast<int>(word >> (16 * i) & 0xffff);
     return L2D_OK;
 }
 
@@ -153,8 +154,8 @@ int l2d_q4_gemv(const l2d_q4_desc *desc, const void *x, int64_t stride_x, void *
                           : fp32 ? q4_entry_float(tiles_n, d.group, zeros, words)
                                  : q4_entry_half(tiles_n, d.group, zeros, words);
         L2D_CUDA_TRY(allow_smem(k.run, 227 * 1024, d.device, *k.smem_set));
-        const int *clusters = nullptr;
-        const int known = q4_clusters(d.device, k, &clusters);
+        int clusters[4];
+        const int known = q4_clusters(d.device, k, clusters);
         if (known != L2D_OK) return known;
         const Q4Shape shape = q4_shape(d.M, halves, a.vectors, tiles_n, bytes, words ? kQ4Deep : 1, clusters);
         a.ranks = shape.ranks;
