@@ -93,7 +93,9 @@ namespace dev {
 
 // Waits until every kernel before this one on the stream has completed and its writes are visible, then
 // lets the next kernel's blocks become resident.  In that order: a kernel that starts on the release
-// finds everything before this kernel complete.
+// finds everything before this kernel complete: only what this kernel itself writes (results, and new keys and values)
+// may change under a resident block that still waits, and must not be read by loads for read-only data (__ldg, .nc).
+// Weights, scales and page tables may, no kernel that releases early writes them.
 __device__ __forceinline__ void wait_for_previous() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
