@@ -141,6 +141,24 @@ __device__ __forceinline__ uint4 load_weights(const uint8_t *p) {
     return v;
 }
 
+// Of x, by ordinary loads: the kernel before may still have been writing it when this one's blocks became resident, so
+// it is no read-only data.
+__device__ __forceinline__ uint4 load_words(const char *p) {
+    uint4 v;
+    asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint32_t load_word(const char *p) {
+    uint32_t v;
+    asm volatile("ld.global.u32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint32_t load_short(const char *p) {
+    uint16_t v;
+    asm volatile("ld.global.u16 %0, [%1];" : "=h"(v) : "l"(p));
+    return v;
+}
+
 // 16 bytes at any address, of which `left` belong to the row (zeros after them), inside [begin, end): from the
 // two aligned ones around them where those are inside too, else byte by byte.
 __device__ __forceinline__ uint4 load_any(const uint8_t *p, int left, const uint8_t *begin, const uint8_t *end) {
@@ -456,16 +474,16 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
             const int v = e.v, col = (first + e.half) * kQ4Half + 8 * u, size = FP32 ? 4 : 2;
             const char *src = static_cast<const char *>(a.x) + (v * a.stride_x + col) * size;
             if (col + 8 <= a.N && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-                r.lo = __ldg(reinterpret_cast<const uint4 *>(src));
-                if (size == 4) r.hi = __ldg(reinterpret_cast<const uint4 *>(src) + 1);
+                r.lo = load_words(src);
+                if (size == 4) r.hi = load_words(src + 16);
                 return r;
             }
             uint32_t w[8] = {};
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 if (col + i >= a.N) continue;
-                if (size == 4) w[i] = __ldg(reinterpret_cast<const uint32_t *>(src) + i);
-                else w[i / 2] |= static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t *>(src) + i)) << (16 * (i & 1));
+                if (size == 4) w[i] = load_word(src + 4 * i);
+                else w[i / 2] |= load_short(src + 2 * i) << (16 * (i & 1));
             }
             r.lo = make_uint4(w[0], w[1], w[2], w[3]);
             r.hi = make_uint4(w[4], w[5], w[6], w[7]);
