@@ -430,7 +430,7 @@ typedef struct {
 } l2d_append_desc;
 /* pos[t]: the position of token t, both in its sequence's cache and for the rotation; a negative one
  * marks padding, for which nothing is written.  seq[t]: its row of the page table (NULL: t).  q_out may
- * be q.  Two tokens of one call must not share a slot.  A token with a bad page or position (status) is
+ * be q, with the same stride, and must not overlap it otherwise.  Two tokens of one call must not share a slot.  A token with a bad page or position (status) is
  * left out whole. */
 L2D_API int l2d_kv_append(const l2d_kv_cache *cache, const l2d_append_desc *desc, const void *k, const void *v,
                           const void *q, void *q_out, const int32_t *pos, const int32_t *seq, int64_t tokens,

@@ -648,7 +648,7 @@ class KvAppend:
 
     def append(self, k, v, pos, tokens: int, seq=None, q=None, q_out=None, stream=None) -> None:
         """``pos`` (int32): each token's position, negative for padding; ``seq`` (int32): its row of the
-        page table (None: token t belongs to row t); ``q_out`` may be ``q``."""
+        page table (None: token t belongs to row t); ``q_out`` may be ``q``, with q_token and q_out_token alike."""
         check(self._call(self._refs[0], self._refs[1], _ptr(k), _ptr(v), _ptr(q), _ptr(q_out), _ptr(pos), _ptr(seq),
                          tokens, _stream_handle(stream)))
 

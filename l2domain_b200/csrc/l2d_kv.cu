@@ -1306,6 +1306,9 @@ int l2d_kv_append(const l2d_kv_cache *cache, const l2d_append_desc *desc, const 
     if (misaligned(k, eb) || misaligned(v, eb) || misaligned(q, eb) || misaligned(q_out, eb) || misaligned(pos, 4) ||
         misaligned(seq, 4) || misaligned(d.cos, 4) || misaligned(d.sin, 4))
         return set_error(L2D_ERR_INVALID, "pointers must be aligned to their elements");
+    if (d.heads_q && q == q_out && tokens > 1 && a.q_token != a.q_out_token)
+        return set_error(L2D_ERR_INVALID, "q_out is q, but q_token is %lld and q_out_token %lld", static_cast<long long>(a.q_token),
+                         static_cast<long long>(a.q_out_token));
     if (d.rot_dim && d.max_pos < 0) return set_error(L2D_ERR_INVALID, "max_pos %lld", static_cast<long long>(d.max_pos));
     int sms = 0;
     st = device_sms(cache->device, &sms);
