@@ -127,6 +127,7 @@ def main() -> int:
     pos = torch.full((args.batch,), args.length - 1, dtype=torch.int32, device="cuda")
     lens = pos + 1
     side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())  # which fills the cache, x, pos and lens
     with torch.cuda.stream(side):
         layer.step(x, pos, lens, out, stream=side)
     side.synchronize()
