@@ -136,7 +136,8 @@ def main() -> int:
         layer.step(x, pos, lens, out, stream=torch.cuda.current_stream())
         pos.add_(1)
         lens.add_(1)
-    for _ in range(10):
+    before = 10  # steps, each of which leaves the cache a token longer
+    for _ in range(before):
         graph.replay()
     start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
     start.record()
@@ -145,7 +146,8 @@ def main() -> int:
     end.record()
     end.synchronize()
     us = start.elapsed_time(end) / args.steps * 1e3
-    cache = 2 * args.batch * args.length * args.kv_heads * args.head_dim * 2
+    keys = args.length + before + (args.steps - 1) / 2  # of a sequence in the timed steps, on average
+    cache = int(2 * args.batch * keys * args.kv_heads * args.head_dim * 2)
     weights = (row * args.hidden + args.hidden * args.heads * args.head_dim) * (0.5 + 2 / 128)
     print(json.dumps({"us_per_step": round(us, 2), "cache_bytes": cache, "weight_bytes": int(weights),
                       "gb_per_s": round((cache + weights) / us / 1e3, 1), "status": int(layer.status.item())}))

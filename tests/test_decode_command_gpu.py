@@ -33,3 +33,10 @@ def test_first_step_waits_for_its_inputs(monkeypatch, capsys):
 
     monkeypatch.setattr(decode, "DecodeAttention", Late)
     assert run(monkeypatch, capsys, "--steps", "5")["status"] == 0
+
+
+def test_bytes_are_those_of_the_timed_steps(monkeypatch, capsys):
+    """Ten steps before the timed ones, and every step, make the cache a token longer."""
+    got = run(monkeypatch, capsys, "--steps", "7")
+    keys = sum(100 + 10 + i for i in range(7)) / 7
+    assert got["cache_bytes"] == 2 * 2 * keys * 2 * 64 * 2
