@@ -1391,8 +1391,14 @@ int l2d_attn_plan_create(const l2d_kv_cache *cache, const l2d_attn_desc *desc, l
     const size_t arrived = size_t(d.max_batch) * cache->heads * m_tiles * 4;
     void *memory = nullptr;
     L2D_CUDA_TRY(cudaMalloc(&memory, part + ml + arrived + 4));
-    cudaError_t e = cudaMemset(memory, 0, part + ml + arrived + 4);
-    if (e == cudaSuccess) e = cudaDeviceSynchronize();
+    // The counters are set on a stream of their own, so that nothing else on the device is waited for.
+    cudaStream_t own = nullptr;
+    cudaError_t e = cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking);
+    if (e == cudaSuccess) {
+        e = cudaMemsetAsync(static_cast<char *>(memory) + part + ml, 0, arrived + 4, own);
+        if (e == cudaSuccess) e = cudaStreamSynchronize(own);
+        cudaStreamDestroy(own);
+    }
     if (e != cudaSuccess) {
         cudaFree(memory);
         return set_error(L2D_ERR_CUDA, "attention scratch: %s", cudaGetErrorString(e));
