@@ -316,20 +316,14 @@ __device__ __forceinline__ uint32_t pack2(T lo, T hi) {
     return static_cast<uint32_t>(a) | static_cast<uint32_t>(b) << 16;
 }
 
-// What is added to the largest score before exponents are taken relative to it: weights of 2^-24 and less leave sums of
-// 2^24 of the largest values inside the range.  Values of fp16 need no such room.
-template <typename T>
-constexpr float kRoom = 24.0f;
-template <>
-constexpr float kRoom<__half> = 0.0f;
-
 // A running softmax's maximum, and what exponents are taken relative to: never -inf.
 __device__ __forceinline__ float finite_base(float m) { return m == -INFINITY ? 0.0f : m; }
 
-// Weights as numbers of the cache's type: bf16 has the exponents of fp32, but fp16 ends at
-// 2^-24, so there they, 1 for the largest score, are taken 2^15 times as large (and sums of values too, until they leave the registers).
+// What the weights, 1 for the largest score, are multiplied by before they meet the values, and the sums of values with
+// them until they are divided by the sum of weights: fp16 ends at 2^-24, so there small weights need it; bf16 and fp32
+// values may be so large that only sums of fractions of them stay in the range.
 template <typename T>
-constexpr float kWeightUnit = 1.0f;
+constexpr float kWeightUnit = 0x1p-24f;
 template <>
 constexpr float kWeightUnit<__half> = 0x1p15f;
 
@@ -354,7 +348,7 @@ struct MmaCore {
     static constexpr int kQueryBytes = kRows * kPitch;
     static constexpr int kWarpBytes = 0;
     static constexpr float kUnit = kWeightUnit<T>;
-    static constexpr float kLow = SPLIT && kUnit != 1.0f ? 0x1p11f : 1.0f;  // of low halves, beyond kUnit
+    static constexpr float kLow = SPLIT && kUnit > 1.0f ? 0x1p11f : 1.0f;  // of low halves, beyond kUnit
     uint32_t qa[kQueryInSmem ? 1 : KS][SPLIT ? 2 : 4];
     float o[2 * KS][4], m[2], l[2];
     uint32_t query;
@@ -411,7 +405,7 @@ struct MmaCore {
     }
 
     // One tile: keys at ks, values at vs (shared memory), bit j of live: key j counts.  scale2 > 0.  Scores are scaled,
-    // and rounded, before the maximum is taken and taken off: the largest is then -kRoom or close to it whatever its size.  With one
+    // and rounded, before the maximum is taken and taken off: the largest is then 0 whatever its size.  With one
     // rounding fewer, by a fused multiply-add on the unscaled ones, it would be what that rounding left: hundreds for
     // scores of 2^31.
     __device__ __forceinline__ void step(const char *ks, const char *vs, uint32_t live, float scale2) {
@@ -454,7 +448,7 @@ struct MmaCore {
             float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const float m2 = fmaxf(m[r], top + kRoom<T>), base = finite_base(m2);
+            const float m2 = fmaxf(m[r], top), base = finite_base(m2);
             if (__any_sync(0xffffffffu, m2 != m[r])) {
                 const float f = exp2_approx(m[r] - base);
                 l[r] *= f;
@@ -508,7 +502,6 @@ struct MmaCore {
             for (int n = 0; n < 2 * KS; ++n) {
                 float2 v = make_float2(o[n][2 * r], o[n][2 * r + 1]);
                 if constexpr (SPLIT) v = make_float2(fmaf(o[n][2], 1.0f / kLow, v.x), fmaf(o[n][3], 1.0f / kLow, v.y));
-                v = make_float2(v.x * (1.0f / kUnit), v.y * (1.0f / kUnit));
                 *reinterpret_cast<float2 *>(so + (g + 8 * r) * kDim + 8 * n + 2 * t) = v;
             }
         }
@@ -591,11 +584,11 @@ struct SimdCore {
             float top = ok ? s[g] : -INFINITY;
 #pragma unroll
             for (int d = 1; d < kKeys; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-            const float m2 = fmaxf(m[g], top + kRoom<float>), base = finite_base(m2), f = exp2_approx(m[g] - base);
+            const float m2 = fmaxf(m[g], top), base = finite_base(m2), f = exp2_approx(m[g] - base);
             const float w = ok ? exp2_approx(s[g] - base) : 0.0f;
             l[g] = fmaf(l[g], f, w);
             m[g] = m2;
-            if (sub == 0) weights[g * kKeys + key] = w;
+            if (sub == 0) weights[g * kKeys + key] = w * kWeightUnit<float>;
 #pragma unroll
             for (int v = 0; v < DV; ++v)
 #pragma unroll
@@ -833,7 +826,7 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
 // Where a head's row of the output and its log-sum-exp go.
 template <typename T>
 __device__ __forceinline__ void store_row4(const AttnArgs &a, int b, int h, int i, int D, float4 x, float base, float sum) {
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / kWeightUnit<T> / sum;
     const float v[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
     T *out = static_cast<T *>(a.out) + b * a.out_token + static_cast<int64_t>(h) * D + i;
 #pragma unroll
