@@ -655,13 +655,17 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
         for (int half = 0; half < halves; ++half) {
             if (!(sums[half * 8 * NT + ((v * PARTS) << kShift)].y < 0.0f)) continue;
             const uint32_t *bits = reinterpret_cast<const uint32_t *>(marks + (half * a.vectors + v) * 16);
-            for (int w = 0; w < 4; ++w) {
-                for (uint32_t left = bits[w]; left; left &= left - 1) {
-                    const int col = (first + half) * kQ4Half + 32 * w + __ffs(left) - 1;
-                    const int64_t i = (r0 + row) * a.lds + group_of(col);
-                    const int q = a.W[(r0 + row) * a.ldw + col / 2] >> (4 * (col & 1)) & 15, z = a.zeros ? a.zeros[i] & 15 : 8;
-                    const float x = dev::load_as_float(a.x, a.dtype_x, v * a.stride_x + col);
-                    sum += dev::load_as_float(a.scales, a.dtype_s, i) * (static_cast<float>(q - z) * x);
+            for (int w = 0; w < 4; ++w) {  // 32 columns, of one group
+                uint32_t left = bits[w];
+                if (!left) continue;
+                const int col = (first + half) * kQ4Half + 32 * w;
+                const int64_t i = (r0 + row) * a.lds + group_of(col);
+                const uint4 q = load_any(a.W + (r0 + row) * a.ldw + col / 2, row_bytes - col / 2, a.W, w_end);
+                const float s = dev::load_as_float(a.scales, a.dtype_s, i), z = a.zeros ? a.zeros[i] & 15 : 8;
+                for (; left; left &= left - 1) {
+                    const int j = __ffs(left) - 1;
+                    const uint32_t eight = j < 16 ? (j < 8 ? q.x : q.y) : j < 24 ? q.z : q.w;
+                    sum += s * ((static_cast<float>(eight >> (4 * (j & 7)) & 15) - z) * dev::load_as_float(a.x, a.dtype_x, v * a.stride_x + col + j));
                 }
             }
         }
