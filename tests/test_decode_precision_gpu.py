@@ -313,3 +313,16 @@ def test_q4_infinities_and_nans_several_vectors(dt, group, vectors):
 @pytest.mark.parametrize("vectors", [1, 2])
 def test_q4_infinities_and_nans(dt, group, vectors):
     infinities_and_nans(dt, group, vectors)
+
+
+@pytest.mark.parametrize("dt,dt_y", [(L.F32, L.F32), (L.F16, L.F16), (L.BF16, L.BF16), (L.F16, L.F32)])
+@pytest.mark.parametrize("group", [32, 64, 128, 384])
+def test_q4_vector_alone_and_in_company(dt, dt_y, group):
+    """A vector by itself and the same one among eight: both within the rounding of the same sums."""
+    M, N = 90, 1152
+    w, s, z = weights(M, N, group, True, seed=13)
+    x = normal(gen(6), dt, 8, N)
+    want, total = q4_exact(w, s, z, x, N, group)
+    close(product(w, s, z, x, N, group, dt, dt_y), want, tolerance(N, total), dt_y)
+    for b in range(8):
+        close(product(w, s, z, x[b:b + 1], N, group, dt, dt_y), want[b:b + 1], tolerance(N, total[b:b + 1]), dt_y)
