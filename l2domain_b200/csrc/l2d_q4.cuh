@@ -563,10 +563,15 @@ __global__ void __launch_bounds__(kQ4Threads, 1) k_q4_gemv(Q4Args a) {
                 // four more of the next 30 bits.  The factor back is short of 2^16, which the end makes good.
                 const uint32_t p = min(283u - (top >> 23), 253u);
                 const float up = __uint_as_float(p << 23), back = __uint_as_float((254u - p) << 23) * 0x1p-16f;
-                const float least = FP32 ? 0x1p-7f : 0x1p10f;  // from here on all bits of a value are there
+                // All bits of a value are there from 2^-7 on (fp32) or 2^10 (16 bits); each that is below is looked at.
                 bool far = false;
+                if constexpr (FP32) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) far = far || (fabsf(f[i] * up) < least && f[i] != 0.0f);
+                    for (int i = 0; i < 8; ++i) far = far || (fabsf(f[i] * up) < 0x1p-7f && f[i] != 0.0f);
+                } else {
+                    const uint32_t m = __vminu2(__vminu2(raw[0] & 0x7fff7fffu, raw[1] & 0x7fff7fffu), __vminu2(raw[2] & 0x7fff7fffu, raw[3] & 0x7fff7fffu));
+                    far = (__float_as_uint(scale_value(min(m & 0xffffu, m >> 16), false, a.dtype_x == L2D_F16)) >> 23) + p < 264;
+                }
                 if (far) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
