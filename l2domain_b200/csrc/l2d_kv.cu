@@ -1357,6 +1357,7 @@ int l2d_attn_plan_create(const l2d_kv_cache *cache, const l2d_attn_desc *desc, l
         return set_error(L2D_ERR_INVALID, "%d query heads for %d key-value heads", d.heads_q, cache->heads);
     if (d.window < 0) return set_error(L2D_ERR_INVALID, "window %d", d.window);
     if (!std::isfinite(d.scale)) return set_error(L2D_ERR_INVALID, "scale is not finite");
+    if (!std::isfinite(d.scale * 1.4426950408889634f)) return set_error(L2D_ERR_INVALID, "scale %g is too large", d.scale);
     if (d.max_batch < 0 || d.max_batch > cache->num_seqs)
         return set_error(L2D_ERR_INVALID, "max_batch %d for a page table of %d sequences", d.max_batch, cache->num_seqs);
     if (!d.max_batch) d.max_batch = cache->num_seqs;

@@ -29,3 +29,12 @@ def test_append_of_other_strides_is_no_refusal(tokens, q_out, desc):
     with pytest.raises(L.L2DError) as e:
         append(tokens, q_out, **desc)
     assert e.value.status == -3  # no device: every check before has passed
+
+
+@pytest.mark.parametrize("scale", [3e38, -2.5e38])
+def test_attention_scale_must_leave_room_for_its_logarithm(scale):
+    """The kernel takes powers of two: a scale whose product with log2(e) is infinite would make 0 * inf of a score of 0."""
+    cache = L.KvCache(k=PTR, v=PTR, dtype=L.BF16, num_pages=8, page_size=16, heads=2, head_dim=64)
+    with pytest.raises(L.L2DError, match="too large") as e:
+        L.PagedAttention(cache, PTR, 4, 4, heads_q=4, scale=scale)
+    assert e.value.status == -1
