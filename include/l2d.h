@@ -378,8 +378,10 @@ enum {
 /* Matrix-vector products with 4-bit weights and group scales.
  *   y[b][i] = sum_j s[i][j / group] * (q[i][j] - z[i][j / group]) * x[b][j]
  * W holds q as rows of packed bytes, column 2j in the low half of byte j.  z is the low four bits of
- * one byte per scale; without zeros every z is 8.  The difference q - z is exact in every dtype_x,
- * products and sums are fp32, y is rounded once. */
+ * one byte per scale; without zeros every z is 8.  The difference q - z is exact, and so is x, but that
+ * the last of the 24 bits of an fp32 x may be lost where there are several vectors or groups of 32 or
+ * 64; sums are fp32, y is rounded once.  An x of less than 2^-19 of the largest among its 128 columns may
+ * take a way of its own: it counts in full, but many of them make a call slow. */
 typedef struct {
     int64_t M, N;
     int64_t ldw;          /* bytes between rows of W (0 = ceil(N / 2)) */
@@ -441,7 +443,9 @@ L2D_API int l2d_kv_append(const l2d_kv_cache *cache, const l2d_append_desc *desc
  * over positions max(0, lens[b] - window) .. lens[b] - 1 (window 0: all), with key-value head
  * h / (heads_q / heads).  A row with no position, or none whose score is above -inf, gives 0 and -inf in
  * lse.  Slots outside those positions are never used, whatever they hold; a position on a bad page
- * counts as absent.  Scores, softmax and sums are fp32. */
+ * counts as absent.  Scores, softmax and sums are fp32; the weights of a 16-bit cache meet the values as
+ * two numbers of its type, which leaves 2^-17 of a weight (bf16), or 2^-23 of it and 2^-40 of the largest
+ * (fp16). */
 typedef struct l2d_attn_plan l2d_attn_plan;
 typedef struct {
     int heads_q;              /* a multiple of the cache's heads */

@@ -199,9 +199,9 @@ __global__ void __launch_bounds__(kAppendThreads) k_append(const __grid_constant
 //
 // Memory bound: each key and value is read once, for all query heads of its group.  A block of
 // eight warps (four for heads of more than 128 elements, whose rings would not fit) works on one
-// key-value head of one sequence at a time; each warp streams its own 16 keys (8 of 32 bits) of every 128
-// through a ring of shared memory of its own (no block-wide barrier in the loop) and keeps a running
-// maximum and sum per query head, so the data is passed over once.  16-bit caches feed matrix
+// key-value head of one sequence at a time; each warp streams its own 16 keys (8 of 32 bits) of every 128 (64 with four
+// warps or 32 bits, 32 with both) through a ring of shared memory of its own (no block-wide barrier in the loop) and
+// keeps a running maximum and sum per query head, so the data is passed over once.  16-bit caches feed matrix
 // instructions with the query heads as the 16 rows; 32-bit caches use fp32 fused multiply-adds.
 //
 // A tile of 16 keys that lies in one page is one box of a tensor map over the cache (elements, heads,
@@ -214,8 +214,8 @@ __global__ void __launch_bounds__(kAppendThreads) k_append(const __grid_constant
 // scratch, and the last piece of that sequence to arrive adds them in piece order, so the result does
 // not depend on which block came last.
 //
-// Measured (32 query and 8 key-value heads of 128, bf16): 64 sequences of 1 to 8192 keys 169-182 us, 6.0-6.4
-// TB/s of keys and values; 64 x 2048 89 us, 6.0 TB/s; one sequence of 17 keys 5.9 us, of which a launch 4.1.
+// Measured (32 query and 8 key-value heads of 128, bf16): 64 sequences of 0 to 8192 keys 170-182 us, 6.0-6.4
+// TB/s of keys and values; 64 x 2048 91 us, 5.9 TB/s; one sequence of 17 keys 5.9 us, of which a launch 4.1.
 // ---------------------------------------------------------------------------------------------
 
 constexpr int kMaxRows = 16;    // query heads a block works on
@@ -1064,8 +1064,8 @@ __global__ void __launch_bounds__(Core::kThreads, 1) k_attn(const __grid_constan
     __syncthreads();
     for (;;) {
         core.begin(query, smem + Sm::kWarp + warp * Core::kWarpBytes, D);
-        // While the first tiles come: what follows, and its queries (with those loaded while the sums meet, heads of 256
-        // elements took 49 us and not 46, ragged 64 x 8192 keys of 128 170 and not 169).
+        // While the first tiles come: what follows, and its queries (with those loaded while the sums meet, 32 x 4096 keys
+        // with 16 heads of 256 elements took 3 us more).
         Piece following = find(p.u0 + p.t0 + p.n);
         const bool more = following.n;
         if (more) stage_query(following, next_query);

@@ -41,8 +41,9 @@ int q4_clusters(int device, const Q4Entry &k, int (&clusters)[4]) {
 }
 
 // Blocks of a cluster and warps of a tile: the choice that gives a warp the least to do, in units of 128 columns
-// of a tile of fp16 products in one n-tile (105 warp instructions).  Measured with every choice forced on nine
-// shapes of 360 x 171 to 28672 x 8192 and 1 to 16 vectors: this picks the fastest of them or one within 10 %.
+// of a tile of fp16 products in one n-tile.  Measured with every choice forced on 14 shapes of 360 x 171 to
+// 28672 x 8192 and 1 to 16 vectors: this picks the fastest of them or one within 3 %, but 9 % for 8 vectors of
+// 28672 x 8192 (46.8 us, and 43.1 in pairs).
 struct Q4Shape {
     int ranks, warps_k, rows;
     int64_t shares;

@@ -15,8 +15,9 @@
 //    taken first, exactly, from 1024 + q and 1024 + z, because sum q x and z sum x may nearly cancel: where the largest
 //    x meets a weight of zero, or a row has few others, their difference has few right bits left.  (A nibble masked
 //    into the low mantissa bits of an fp16 number is exact as it is, and two instructions less for every two weights:
-//    8 vectors 28672 x 8192 on groups of 128 take 42 us so, and 48 with the differences.)  A mask higher up gives 16 (q - z), with
-//    a sixteenth of x.  Each 128 columns of a vector are scaled by a power of two to a largest value just under 2^15.
+//    8 vectors 28672 x 8192 on groups of 128 took 42 us so, and take 47 with the differences.)  A mask higher up
+//    gives 16 (q - z), with a sixteenth of x.  Each 128 columns of a vector are scaled by a power of two to a largest
+//    value just under 2^15.
 //  * fp32 vectors take two columns of fp16, 11 bits each and a sign between them: the last of 24 bits of x may be lost.
 //  * Infinities and NaNs, and values so far below the largest of their 128 columns that the scaled number loses bits of
 //    them, are staged as zeros, and the threads that store a vector's results add their terms at the end.  In fp16 that
@@ -29,14 +30,15 @@
 //    weights, a step of 512 columns ahead, in code without branches.  A product's order of columns is free,
 //    so nibbles are used in the order in which masks deliver them, and x is put into that order when it is
 //    staged.  A request for eight rows occupies the L1 for eight cycles whatever its width, so the scales of
-//    a whole step are loaded as one word per row.
+//    a whole step are loaded as one word per row.  Up to 16 columns of B that fits the 128 registers that 16 warps leave,
+//    but for a few words; with 17 to 32 of them 44 to 440 bytes of a thread go to local memory.
 //  * A block's rows are its even share of M, in tiles of at most 16 rows of nearly equal size, so that
 //    blocks finish together whatever M is; groups of its warps take a tile each, split its columns and
 //    meet in shared memory at its end, in a fixed order.
 //  * Where a block has few rows, or there are many vectors, staging x costs more than multiplying: a cluster
 //    of blocks then takes its rows together, each block a share of the columns, and adds its sums over
-//    distributed shared memory, in rank order (q4_shape() weighs it; 8 vectors of 8192 x 8192: 42 us alone, 31 us
-//    in pairs, 29 us in fours).
+//    distributed shared memory, in rank order (q4_shape() weighs it; 8 vectors of 8192 x 8192 on groups of 32:
+//    37 us alone, 28.5 in pairs, 27.5 in fours).
 #pragma once
 
 #include "l2d_launch.cuh"
