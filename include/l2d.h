@@ -462,6 +462,53 @@ L2D_API int l2d_attn_decode(l2d_attn_plan *plan, const void *q, void *out, float
                             void *stream);
 L2D_API int l2d_attn_plan_destroy(l2d_attn_plan *plan);
 
+/* Other scores: after the scale, s becomes cap * tanh(s / cap) where cap is not 0, then slopes[h] * (p - (lens[b] - 1)) is
+ * added where slopes is given: a bias by the distance from the last position, each head's own. */
+typedef struct {
+    float cap;
+    const float *slopes;      /* [heads_q], on the device, or NULL */
+} l2d_attn_scores;
+/* As l2d_attn_plan_create; scores may be NULL. */
+L2D_API int l2d_attn_plan_create_scored(const l2d_kv_cache *cache, const l2d_attn_desc *desc, const l2d_attn_scores *scores,
+                                        l2d_attn_plan **plan);
+/* As l2d_attn_decode, over positions from starts[b] on: a sequence's earlier documents, which the new token does not see
+ * (NULL: all; negative: 0).  The window counts as well, and pages before both are never looked up. */
+L2D_API int l2d_attn_decode_from(l2d_attn_plan *plan, const void *q, void *out, float *lse, const int32_t *lens, const int32_t *starts,
+                                 int batch, void *stream);
+
+/* A paged cache in 4 bits.  A group of elements of one head is held as s (n - z) with n and z in 0..15, that is:
+ *   s = hi c - lo c, lo = min(0, least), hi = max(0, largest), c = fp32(1/15), each step rounded to fp32, then up to a number
+ *   whose last four bits are zero;  z = min(15, rint(-lo / s)),  n = clamp(rint(x / s) + z, 0, 15);  s = 0 gives zeros.
+ * A group with an infinity or a NaN stands for NaN throughout.  s (n - z) is exact in fp32.
+ * A page: blocks of 16 slots; in each the heads; in each head, for every 32 elements 16 rows (one per slot) of 16
+ * bytes, element 2j in the low half of byte j (places past head_dim: 0), then for every group 16 words (one per slot):
+ * the bits of s, with z in the last four.  k and v may be one buffer or two. */
+typedef struct {
+    void *k, *v;              /* on 16-byte boundaries */
+    int dtype;                /* of new keys and values, queries and outputs */
+    int heads, head_dim;      /* key-value heads; head_dim 1..256 */
+    int page_size;            /* a multiple of 16 */
+    int group;                /* elements that share a scale: 32, 64 or 128 (the last group of a head may be short) */
+    int64_t num_pages;
+    int64_t k_page, v_page;   /* bytes between pages, multiples of 16 (0 = l2d_kv4_page_bytes) */
+    const int32_t *table;     /* as in l2d_kv_cache, to the end */
+    int64_t table_stride;
+    int num_seqs, table_width;
+    uint32_t *status;
+    int device;
+} l2d_kv4_cache;
+/* The bytes of one page of keys, or of values. */
+L2D_API int l2d_kv4_page_bytes(int heads, int head_dim, int page_size, int group, int64_t *bytes);
+/* As l2d_kv_append, with every product and sum of the rotation rounded to fp32 by itself; keys are not rounded to dtype before
+ * they are held.  k_out and v_out (NULL: not wanted) get keys and values as they are held, rounded to dtype and strided as
+ * k and v: what the attention will see, for a prompt's own.  They may be k and v, and must not overlap them otherwise. */
+L2D_API int l2d_kv4_append(const l2d_kv4_cache *cache, const l2d_append_desc *desc, const void *k, const void *v, const void *q, void *q_out,
+                           void *k_out, void *v_out, const int32_t *pos, const int32_t *seq, int64_t tokens, void *stream);
+/* A plan of l2d_attn_decode and l2d_attn_decode_from over a cache in 4 bits; scores may be NULL.  Weights times scales meet
+ * the values as two bf16 numbers (2^-17 of a weight is left), for fp32 queries as three, and so do the queries. */
+L2D_API int l2d_attn_plan_create_kv4(const l2d_kv4_cache *cache, const l2d_attn_desc *desc, const l2d_attn_scores *scores,
+                                     l2d_attn_plan **plan);
+
 /* ---- helpers used by the benchmark and the CLI ---- */
 /* Reference-mode inputs (init_data): A/x from mix32 of the flat index (stream 0 = A, 1 = x). */
 L2D_API int l2d_fill_ref(void *dst, int dtype, uint64_t first, uint64_t n, uint32_t seed, int stream,

@@ -106,6 +106,13 @@ class KvCacheDesc(C.Structure):
                 ("status", C.c_void_p), ("device", C.c_int)]
 
 
+class KvCache4Desc(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int), ("heads", C.c_int), ("head_dim", C.c_int),
+                ("page_size", C.c_int), ("group", C.c_int), ("num_pages", C.c_int64), ("k_page", C.c_int64),
+                ("v_page", C.c_int64), ("table", C.c_void_p), ("table_stride", C.c_int64), ("num_seqs", C.c_int),
+                ("table_width", C.c_int), ("status", C.c_void_p), ("device", C.c_int)]
+
+
 class AppendDesc(C.Structure):
     _fields_ = [("heads_q", C.c_int), ("cos", C.c_void_p), ("sin", C.c_void_p), ("max_pos", C.c_int64),
                 ("rot_dim", C.c_int), ("interleaved", C.c_int), ("k_token", C.c_int64), ("v_token", C.c_int64),
@@ -115,6 +122,10 @@ class AppendDesc(C.Structure):
 class AttnDesc(C.Structure):
     _fields_ = [("heads_q", C.c_int), ("window", C.c_int), ("scale", C.c_float), ("max_batch", C.c_int),
                 ("q_token", C.c_int64), ("out_token", C.c_int64)]
+
+
+class AttnScores(C.Structure):
+    _fields_ = [("cap", C.c_float), ("slopes", C.c_void_p)]
 
 
 # Every symbol include/l2d.h declares, with its ctypes signature.
@@ -179,6 +190,11 @@ SIGNATURES = {
     "l2d_attn_plan_create": (_i, [C.POINTER(KvCacheDesc), C.POINTER(AttnDesc), C.POINTER(_vp)]),
     "l2d_attn_decode": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _vp]),
     "l2d_attn_plan_destroy": (_i, [_vp]),
+    "l2d_attn_plan_create_scored": (_i, [C.POINTER(KvCacheDesc), C.POINTER(AttnDesc), C.POINTER(AttnScores), C.POINTER(_vp)]),
+    "l2d_attn_plan_create_kv4": (_i, [C.POINTER(KvCache4Desc), C.POINTER(AttnDesc), C.POINTER(AttnScores), C.POINTER(_vp)]),
+    "l2d_attn_decode_from": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _vp]),
+    "l2d_kv4_page_bytes": (_i, [_i, _i, _i, _i, C.POINTER(_i64)]),
+    "l2d_kv4_append": (_i, [C.POINTER(KvCache4Desc), C.POINTER(AppendDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
     "l2d_fill_ref": (_i, [_vp, _i, _u64, _u64, _u32, _i, _i, _vp]),
     "l2d_fill_cfg": (_i, [_vp, _i, _u64, _u64, _u64, _u64, _i, C.c_float, C.c_float, _vp]),
     "l2d_l2_flush": (_i, [_i, _vp]),
@@ -629,13 +645,38 @@ class KvCache:
                            status=_ptr(status), **self.fields)
 
 
+class KvCache4:
+    """A paged cache of keys and values in 4 bits, in memory of the caller's: ``k`` and ``v`` hold ``num_pages`` pages of
+    :func:`kv4_page_bytes` bytes each, ``k_page`` / ``v_page`` bytes apart (0 = dense).  ``dtype`` is that of new keys and
+    values, queries and outputs; ``group`` elements (32, 64 or 128) share a scale; ``page_size`` is a multiple of 16.  Takes the
+    place of a :class:`KvCache` in :class:`KvAppend` and :class:`PagedAttention`."""
+
+    def __init__(self, k, v, dtype: int, num_pages: int, page_size: int, heads: int, head_dim: int, group: int = 128,
+                 k_page: int = 0, v_page: int = 0, device: int = 0):
+        self._hold = (k, v)
+        self.fields = dict(k=_ptr(k), v=_ptr(v), dtype=dtype, heads=heads, head_dim=head_dim, page_size=page_size, group=group,
+                           num_pages=num_pages, k_page=k_page, v_page=v_page, device=device)
+
+    def desc(self, table, num_seqs: int, table_width: int, table_stride: int = 0, status=None) -> KvCache4Desc:
+        """The C description of this cache with a page table (int32, on the device)."""
+        return KvCache4Desc(table=_ptr(table), num_seqs=num_seqs, table_width=table_width, table_stride=table_stride,
+                            status=_ptr(status), **self.fields)
+
+
+def kv4_page_bytes(page_size: int, heads: int, head_dim: int, group: int = 128) -> int:
+    """Bytes of one page of keys, or of values, of a :class:`KvCache4`."""
+    n = C.c_int64(0)
+    check(lib().l2d_kv4_page_bytes(heads, head_dim, page_size, group, C.byref(n)))
+    return n.value
+
+
 class KvAppend:
-    """Appends new tokens' keys and values to a :class:`KvCache`, rotating keys (and queries) by their
+    """Appends new tokens' keys and values to a :class:`KvCache` or :class:`KvCache4`, rotating keys (and queries) by their
     positions on the way.  ``cos`` / ``sin``: fp32 [max_pos][rot_dim / 2], see :func:`rotation_tables`;
     ``interleaved`` pairs elements (2i, 2i + 1) instead of (i, i + rot_dim / 2).  ``status``: a uint32 on the device that
     collects KV_BAD_* bits."""
 
-    def __init__(self, cache: KvCache, table, num_seqs: int, table_width: int, heads_q: int = 0, cos=None, sin=None,
+    def __init__(self, cache, table, num_seqs: int, table_width: int, heads_q: int = 0, cos=None, sin=None,
                  max_pos: int = 0, rot_dim: int = 0, interleaved: bool = False, table_stride: int = 0, k_token: int = 0,
                  v_token: int = 0, q_token: int = 0, q_out_token: int = 0, status=None):
         self._hold = (cache, table, cos, sin, status)
@@ -644,33 +685,44 @@ class KvAppend:
                                 interleaved=int(interleaved), k_token=k_token, v_token=v_token, q_token=q_token,
                                 q_out_token=q_out_token)
         self._refs = (C.byref(self._cache), C.byref(self._desc))
-        self._call = lib().l2d_kv_append
+        self._four = isinstance(cache, KvCache4)
+        self._call = lib().l2d_kv4_append if self._four else lib().l2d_kv_append
 
-    def append(self, k, v, pos, tokens: int, seq=None, q=None, q_out=None, stream=None) -> None:
+    def append(self, k, v, pos, tokens: int, seq=None, q=None, q_out=None, stream=None, k_out=None, v_out=None) -> None:
         """``pos`` (int32): each token's position, negative for padding; ``seq`` (int32): its row of the
-        page table (None: token t belongs to row t); ``q_out`` may be ``q``, with q_token and q_out_token alike."""
-        check(self._call(self._refs[0], self._refs[1], _ptr(k), _ptr(v), _ptr(q), _ptr(q_out), _ptr(pos), _ptr(seq),
-                         tokens, _stream_handle(stream)))
+        page table (None: token t belongs to row t); ``q_out`` may be ``q``, with q_token and q_out_token alike.  ``k_out`` /
+        ``v_out`` (a :class:`KvCache4` only): rotated keys, and values, as the cache holds them, strided as k and v."""
+        refs, args = self._refs, (_ptr(k), _ptr(v), _ptr(q), _ptr(q_out))
+        if self._four:
+            args += (_ptr(k_out), _ptr(v_out))
+        elif k_out is not None or v_out is not None:
+            raise ValueError("k_out and v_out belong to a cache in 4 bits")
+        check(self._call(refs[0], refs[1], *args, _ptr(pos), _ptr(seq), tokens, _stream_handle(stream)))
 
 
 class PagedAttention:
-    """Attention of one new token per sequence over a :class:`KvCache`.  The plan owns its scratch; calls
-    of one plan must not overlap on the GPU.  ``scale`` 0 means 1 / sqrt(head_dim), ``window`` 0 all keys."""
+    """Attention of one new token per sequence over a :class:`KvCache` or :class:`KvCache4`.  The plan owns its scratch; calls
+    of one plan must not overlap on the GPU.  ``scale`` 0 means 1 / sqrt(head_dim), ``window`` 0 all keys.  ``cap`` > 0 makes a
+    scaled score s cap * tanh(s / cap); ``slopes`` (fp32 [heads_q], on the device) then adds slopes[h] * (p - (len - 1)) to that
+    of position p (:func:`distance_slopes`)."""
 
-    def __init__(self, cache: KvCache, table, num_seqs: int, table_width: int, heads_q: int, scale: float = 0.0,
+    def __init__(self, cache, table, num_seqs: int, table_width: int, heads_q: int, scale: float = 0.0,
                  window: int = 0, max_batch: int = 0, table_stride: int = 0, q_token: int = 0, out_token: int = 0,
-                 status=None):
+                 status=None, cap: float = 0.0, slopes=None):
         self._plan = C.c_void_p(0)
-        self._hold = (cache, table, status)
+        self._hold = (cache, table, status, slopes)
         cd = cache.desc(table, num_seqs, table_width, table_stride, status)
         ad = AttnDesc(heads_q=heads_q, window=window, scale=scale, max_batch=max_batch, q_token=q_token,
                       out_token=out_token)
-        check(lib().l2d_attn_plan_create(C.byref(cd), C.byref(ad), C.byref(self._plan)))
-        self._call = lib().l2d_attn_decode
+        sc = AttnScores(cap=cap, slopes=_ptr(slopes))
+        create = lib().l2d_attn_plan_create_kv4 if isinstance(cache, KvCache4) else lib().l2d_attn_plan_create_scored
+        check(create(C.byref(cd), C.byref(ad), C.byref(sc), C.byref(self._plan)))
+        self._call = lib().l2d_attn_decode_from
 
-    def decode(self, q, out, lens, batch: int, lse=None, stream=None) -> None:
-        """out[b] = attention of q[b] over the first lens[b] (int32, on the device) positions of row b."""
-        check(self._call(self._plan, _ptr(q), _ptr(out), _ptr(lse), _ptr(lens), batch, _stream_handle(stream)))
+    def decode(self, q, out, lens, batch: int, lse=None, stream=None, starts=None) -> None:
+        """out[b] = attention of q[b] over the first lens[b] (int32, on the device) positions of row b, from starts[b]
+        (int32, on the device; None: 0) on."""
+        check(self._call(self._plan, _ptr(q), _ptr(out), _ptr(lse), _ptr(lens), _ptr(starts), batch, _stream_handle(stream)))
 
     def close(self) -> None:
         if self._plan and self._plan.value:
@@ -682,6 +734,13 @@ class PagedAttention:
             self.close()
         except Exception:
             pass
+
+
+def distance_slopes(heads: int, device=None):
+    """fp32 [heads]: a geometric row of slopes from 2^(-8 / heads) to 2^-8, for :class:`PagedAttention`."""
+    import torch
+
+    return torch.exp2(-8.0 * torch.arange(1, heads + 1, dtype=torch.float64, device=device) / heads).float()
 
 
 def rotation_tables(max_pos: int, rot_dim: int, theta: float = 10000.0, stretch: float = 1.0, device=None):
