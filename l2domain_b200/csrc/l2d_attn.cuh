@@ -5,6 +5,8 @@
 
 #include <cuda.h>
 
+#include <type_traits>
+
 namespace l2d {
 
 struct AttnArgs {
@@ -86,7 +88,7 @@ __device__ __forceinline__ void copy_box(uint32_t dst, const CUtensorMap *map, i
 __device__ __forceinline__ void copy_run(uint32_t dst, const void *src, int bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
-__device__ __forceinline__ void barrier_init(uint32_t bar) { asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void barrier_init(uint32_t bar, int arrivals) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(arrivals) : "memory"); }
 __device__ __forceinline__ void barrier_expect(uint32_t bar, int bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
@@ -552,9 +554,8 @@ struct Stream {
     // The entry is not looked at before the next tile is started: an instruction that used it here would wait for
     // it, and the products with it.
     __device__ __forceinline__ void lookup() {
-        const bool whole = Core::kPacked || how == kBoxes;
-        const int64_t key = whole ? next : next + (threadIdx.x & 31) / kLanes;
-        wanted = key < len && (whole ? key + Core::kKeys : key + 1) > lo;
+        const int64_t key = how == kBoxes ? next : next + (threadIdx.x & 31) / kLanes;
+        wanted = key < len && (how == kBoxes ? key + Core::kKeys : key + 1) > lo;
         const unsigned i = page_index(c, static_cast<unsigned>(key));
         slot = static_cast<int>(static_cast<unsigned>(key) - i * static_cast<unsigned>(c.page_size));
         if (wanted) page = __ldg(table + i);
@@ -567,7 +568,7 @@ struct Stream {
         const bool real = wanted && page >= 0 && page < c.num_pages;
         if (wanted && !real) report(c.status, L2D_KV_BAD_PAGE);
         char *tile = ring + stage * (Core::kWarps * Sm::kStage);
-        if (Core::kPacked || how == kBoxes) {
+        if (how == kBoxes) {
             uint32_t bits = 0;
             if (real) {
                 bits = kAll;
@@ -578,23 +579,16 @@ struct Stream {
                 live[stage] = bits;
                 if (bits) {
                     const uint32_t bar = bars + 8 * stage, to = smem_addr(tile);
-                    if constexpr (Core::kPacked) {
-                        const int64_t at = (static_cast<int64_t>(slot >> 4) * c.heads + head) * c.tile_bytes;
-                        barrier_expect(bar, 2 * c.tile_bytes);
-                        copy_run(to, c.k + page * c.k_page + at, c.tile_bytes, bar);
-                        copy_run(to + Sm::kTile, c.v + page * c.v_page + at, c.tile_bytes, bar);
-                    } else {
-                        barrier_expect(bar, Sm::kStage);
+                    barrier_expect(bar, Sm::kStage);
 #pragma unroll
-                        for (int b = 0; b < Core::kBoxes; ++b) {
-                            const int x = b * (128 / static_cast<int>(sizeof(T)));
-                            copy_box(to + b * Core::kKeys * 128, &maps.k, x, head, slot, page, bar);
-                            copy_box(to + Sm::kTile + b * Core::kKeys * 128, &maps.v, x, head, slot, page, bar);
-                        }
+                    for (int b = 0; b < Core::kBoxes; ++b) {
+                        const int x = b * (128 / static_cast<int>(sizeof(T)));
+                        copy_box(to + b * Core::kKeys * 128, &maps.k, x, head, slot, page, bar);
+                        copy_box(to + Sm::kTile + b * Core::kKeys * 128, &maps.v, x, head, slot, page, bar);
                     }
                 }
             }
-        } else if constexpr (!Core::kPacked) {
+        } else {
             // Bit kLanes j of the vote to bit j.
             const uint32_t vote = __ballot_sync(0xffffffffu, real);
             const uint32_t bits = __ballot_sync(0xffffffffu, lane < Core::kKeys && (vote >> (lane * kLanes & 31) & 1));
@@ -652,23 +646,96 @@ struct Stream {
     // The live bits of a stage, once its copies are there.  Values of keys that do not count are made zeros, as
     // their weights are: slots that were never written may hold anything.
     __device__ __forceinline__ uint32_t take(int stage) {
-        const bool whole = Core::kPacked || how == kBoxes;
-        if (!whole) copies_wait<STAGES - 2>();
+        if (how != kBoxes) copies_wait<STAGES - 2>();
         __syncwarp();
         const uint32_t bits = live[stage];
-        if (whole && bits) {
+        if (how == kBoxes && bits) {
             if (!barrier_wait(bars + 8 * stage, phases >> stage & 1)) give_up(stage);
             phases ^= 1u << stage;
             if (bits != (1u << Core::kKeys) - 1) {
                 char *values = ring + stage * (Core::kWarps * Sm::kStage) + Sm::kTile;
-                if constexpr (Core::kPacked) {
-                    Core::clear(values, bits, c);
-                } else {
-                    for (int r = 0; r < Core::kKeys; ++r)
-                        if (!(bits >> r & 1))
-                            for (int ch = threadIdx.x & 31; ch < Core::kChunks; ch += 32)
-                                *reinterpret_cast<uint4 *>(values + chunk_at<Core::kKeys>(r, ch)) = make_uint4(0, 0, 0, 0);
+                for (int r = 0; r < Core::kKeys; ++r)
+                    if (!(bits >> r & 1))
+                        for (int ch = threadIdx.x & 31; ch < Core::kChunks; ch += 32)
+                            *reinterpret_cast<uint4 *>(values + chunk_at<Core::kKeys>(r, ch)) = make_uint4(0, 0, 0, 0);
+                before_boxes();
+                __syncwarp();
+            }
+        }
+        return bits;
+    }
+};
+
+// The same over a cache in 4 bits: tiles of two runs of 16 keys, each of them one run of bytes of keys and one of values, and
+// in a page of its own; lanes 0 and 1 look up one each and start its copies.
+template <typename Core, int STAGES>
+struct PackedStream {
+    using Sm = AttnSmem<Core, STAGES>;
+    static_assert(STAGES == 2, "one tile on its way while one is worked on");
+    const Cache &c;
+    const AttnMaps &unused_maps;
+    int unused_how, head;
+    const int32_t *table;
+    char *ring;
+    uint32_t bars;
+    uint32_t *live;
+    uint32_t phases;
+    int64_t next;
+    int lo, len, step;
+    int slot, page;       // of the first key of this lane's run
+    bool wanted;          // one of its keys counts
+    static constexpr uint32_t kLate = 1u << 31;
+
+    __device__ __forceinline__ void lookup() {
+        const int64_t key = next + 16 * (threadIdx.x & 1);
+        wanted = key < len && key + 16 > lo;
+        const unsigned i = page_index(c, static_cast<unsigned>(key));
+        slot = static_cast<int>(static_cast<unsigned>(key) - i * static_cast<unsigned>(c.page_size));
+        if (wanted) page = __ldg(table + i);
+    }
+
+    __device__ __forceinline__ void issue(int stage) {
+        const int lane = threadIdx.x & 31;
+        const bool real = wanted && page >= 0 && page < c.num_pages;
+        if (wanted && !real && lane < 2) report(c.status, L2D_KV_BAD_PAGE);
+        uint32_t bits = 0;
+        if (real) {
+            const int64_t key = next + 16 * (lane & 1);
+            bits = 0xffffu;
+            if (key < lo) bits &= 0xffffu << (lo - static_cast<int>(key));
+            if (key + 16 > len) bits &= 0xffffu >> (static_cast<int>(key) + 16 - len);
+        }
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, bits, 1), all = lane & 1 ? other | bits << 16 : bits | other << 16;
+        if (lane < 2) {
+            if (lane == 0) live[stage] = all;
+            if (all) {  // both lanes arrive
+                const uint32_t bar = bars + 8 * stage;
+                barrier_expect(bar, bits ? 2 * c.tile_bytes : 0);
+                if (bits) {
+                    const uint32_t to = smem_addr(ring) + stage * (Core::kWarps * Sm::kStage) + lane * Core::kRunBytes;
+                    const int64_t at = static_cast<int64_t>((slot >> 4) * c.heads + head) * c.tile_bytes;
+                    copy_run(to, c.k + page * c.k_page + at, c.tile_bytes, bar);
+                    copy_run(to + Sm::kTile, c.v + page * c.v_page + at, c.tile_bytes, bar);
                 }
+            }
+        }
+        next += step;
+        lookup();
+    }
+
+    __device__ __forceinline__ uint32_t take(int stage) {
+        __syncwarp();
+        const uint32_t bits = live[stage];
+        if (bits) {
+            if (!barrier_wait(bars + 8 * stage, phases >> stage & 1)) {  // no more are started, and none is on its way
+                report(c.status, L2D_KV_TIMEOUT);
+                phases |= kLate;
+                len = 0;
+                wanted = false;
+            }
+            phases ^= 1u << stage;
+            if (bits != 0xffffffffu) {
+                Core::clear(ring + stage * (Core::kWarps * Sm::kStage) + Sm::kTile, bits, c);
                 before_boxes();
                 __syncwarp();
             }
@@ -825,7 +892,7 @@ __global__ void __launch_bounds__(Core::kThreads, Core::kBlocks) k_attn(const __
     // What needs nothing of the kernels before: the maps' way to the copy unit, and the barriers.
     const uint32_t bars = smem_addr(smem + Sm::kBars) + warp * STAGES * 8;
     if (how == kBoxes && tid < 2) asm volatile("prefetch.tensormap [%0];" ::"l"(tid ? &maps.v : &maps.k) : "memory");
-    if (lane < STAGES) barrier_init(bars + 8 * lane);
+    if (lane < STAGES) barrier_init(bars + 8 * lane, Core::kPacked ? 2 : 1);
     before_boxes();
     dev::wait_for_previous();
 
@@ -872,7 +939,7 @@ __global__ void __launch_bounds__(Core::kThreads, Core::kBlocks) k_attn(const __
     // A negative scale turns the queries' signs, or is part of the scores.
     const float scale = (kSigned ? a.scale : fabsf(a.scale)) * Core::kScale;
     Scoring scoring = {scale * 1.4426950408889634f, scale, a.cap, a.cap != 0.0f ? 1.0f / a.cap : 0.0f, nullptr, 0};
-    Stream<Core, STAGES> in{a.c, maps, how};
+    typename std::conditional<Core::kPacked, PackedStream<Core, STAGES>, Stream<Core, STAGES>>::type in{a.c, maps, how};
     in.ring = smem + warp * Sm::kStage;
     in.bars = bars;
     in.live = reinterpret_cast<uint32_t *>(smem + Sm::kLive) + warp * STAGES;
@@ -1071,6 +1138,7 @@ AttnKernel pick_dense(int dtype, int D, int G) {
 }
 
 AttnKernel pick_attn_scored(int dtype, int D, int G);
-AttnKernel pick_attn_kv4(int dtype, int D, int G);
+// For a cache in 4 bits (l2d_kv4.cu).
+AttnKernel pick_attn_kv4(int dtype, int D, int group, int G);
 
 }  // namespace l2d

@@ -244,8 +244,7 @@ namespace l2d {
 AttnKernel pick_attn(int dtype, int D, int G) { return pick_dense<false>(dtype, D, G); }
 
 // A plan over a checked cache, without its way of copying.
-int make_plan(const Cache &c, int dtype, int device, const l2d_attn_desc *desc, const l2d_attn_scores *scores, AttnKernel (*pick)(int, int, int),
-              l2d_attn_plan **plan) {
+int make_plan(const Cache &c, int dtype, int device, const l2d_attn_desc *desc, const l2d_attn_scores *scores, l2d_attn_plan **plan) {
     if (!desc) return set_error(L2D_ERR_INVALID, "null descriptor");
     l2d_attn_desc d = *desc;
     if (d.heads_q < 1 || d.heads_q > 65535 || d.heads_q % c.heads)
@@ -273,7 +272,8 @@ int make_plan(const Cache &c, int dtype, int device, const l2d_attn_desc *desc, 
     OnDevice on(device);
     L2D_CUDA_TRY(on.err);
     const int G = d.heads_q / c.heads;
-    const AttnKernel k = pick(dtype, c.head_dim, G);
+    const bool scored = s.cap != 0.0f || s.slopes;
+    const AttnKernel k = c.group ? pick_attn_kv4(dtype, c.head_dim, c.group, G) : scored ? pick_attn_scored(dtype, c.head_dim, G) : pick_attn(dtype, c.head_dim, G);
     if (!std::isfinite(d.scale * 1.4426950408889634f * k.scale)) return set_error(L2D_ERR_INVALID, "scale %g is too large", d.scale);
     const int m_tiles = (G + k.rows - 1) / k.rows;
     int blocks = 0;
@@ -369,8 +369,8 @@ int l2d_attn_plan_create_scored(const l2d_kv_cache *cache, const l2d_attn_desc *
     Cache c;
     int st = check_cache(cache, &c);
     if (st != L2D_OK) return st;
-    const bool scored = scores && (scores->cap != 0.0f || scores->slopes);
-    st = make_plan(c, cache->dtype, cache->device, desc, scores, scored ? pick_attn_scored : pick_attn, plan);
+    c.group = 0;
+    st = make_plan(c, cache->dtype, cache->device, desc, scores, plan);
     if (st != L2D_OK) return st;
     l2d_attn_plan *p = *plan;
     // 16-byte copies need rows of whole 16-byte words on 16-byte boundaries; boxes also pages of whole tiles.
@@ -391,7 +391,7 @@ int l2d_attn_plan_create_kv4(const l2d_kv4_cache *cache, const l2d_attn_desc *de
     Cache c;
     const int st = check_cache4(cache, &c);
     if (st != L2D_OK) return st;
-    return make_plan(c, cache->dtype, cache->device, desc, scores, pick_attn_kv4, plan);
+    return make_plan(c, cache->dtype, cache->device, desc, scores, plan);
 }
 
 int l2d_attn_decode(l2d_attn_plan *p, const void *q, void *out, float *lse, const int32_t *lens, int batch, void *stream) {

@@ -1,22 +1,9 @@
-// The paged cache in 4 bits: appending to it (l2d_kv4_append), and how the attention works on it.
-//
-// A page is cut into blocks of 16 slots; a block holds, head by head, a tile: for every 32 elements of the head 16 rows of
-// 16 bytes (one per slot; element 2j in the low half of byte j), then for every group of elements 16 words.  So the
-// attention's tile of 16 keys of one head is one run of bytes, which one bulk copy brings, already in the order in which
-// eight rows of 16 bytes meet all banks.  A word is the bits of the group's scale with the zero point in the last
-// four: scales have 20 significant bits, and a scale times a difference of two 4-bit numbers is exact in fp32.
-#include "l2d_attn.cuh"
+// The paged cache in 4 bits: appending to it (l2d_kv4_append), and its checks.
+#include "l2d_kv4.cuh"
 
 #include <algorithm>
-#include <cfloat>
-#include <type_traits>
 
 namespace l2d {
-
-constexpr int kBlockSlots = 16;
-constexpr int kChunk = 32;                           // elements of a row of 16 bytes
-constexpr int kChunkBytes = kBlockSlots * 16;
-constexpr int kGroupBytes = kBlockSlots * 4;
 
 // ---------------------------------------------------------------------------------------------
 // Appending.
@@ -192,372 +179,9 @@ __global__ void __launch_bounds__(kAppend4Threads) k_append4(const __grid_consta
     }
 }
 
-// ---------------------------------------------------------------------------------------------
-// Attention: one warp's part of one head group, in the kernel that l2d_attn.cuh describes.
-//
-// Per 16 keys of 128 elements a warp reads 2 x 1088 bytes, which an SM's share of the memory brings in about 100 cycles,
-// the issue of 400 instructions; so the conversion of 4096 nibbles is what has to be cheap.  A word of eight nibbles gives
-// four registers of two 16-bit numbers each, by one mask that also sets the exponent of 2^10 (fp16) or 2^7 (bf16), and one
-// subtraction that takes off this and the zero point together; the differences n - z are exact.  Scales stay outside
-// the products: the scores of a group's elements are multiplied by its key's scale as fp32 sums, and weights by the
-// value's scale before they are cut into 16-bit parts.
-//
-// Keys: a matrix of ldmatrix (8 keys x 16 bytes) gives a lane word t of key g, elements 8t .. 8t + 7 of the 32; queries are
-// staged in the order in which two instructions meet them.  Values: the transposed load gives a lane the same four elements
-// of keys 2t and 2t + 1 side by side, which is what a B operand needs of two neighbouring rows, nibble by nibble.
-//
-// Queries of 32 bits are three bf16 numbers that add up to them, and weights three; of 16 bits, weights two (2^-17 of
-// a weight is left).
-// ---------------------------------------------------------------------------------------------
-
-__device__ __forceinline__ uint32_t sub2_half(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
-// a / 16 + b
-__device__ __forceinline__ uint32_t sixteenth_plus(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(0x2c002c00u), "r"(b));
-    return r;
-}
-__device__ __forceinline__ uint32_t sub2_bf16(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(b), "r"(0xbf80bf80u), "r"(a));
-    return r;
-}
-// (w & mask) | bits
-__device__ __forceinline__ uint32_t masked_or(uint32_t w, uint32_t mask, uint32_t bits) {
-    uint32_t r;
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(bits));
-    return r;
-}
-
-// Nibbles i of both halves of a word, i = 0..3, less their zero points.  T = bf16: zero holds 128 + z twice.
-__device__ __forceinline__ void differences_bf16(uint32_t (&r)[4], uint32_t w, uint32_t zero) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = sub2_bf16(masked_or(w >> (4 * i), 0x000f000fu, 0x43004300u), zero);
-}
-// fp16: zero holds 1024 + z twice, and high -(64 + z): nibbles in the second place count 16-fold there.
-__device__ __forceinline__ void differences_half(uint32_t (&r)[4], uint32_t w, uint32_t zero, uint32_t high) {
-#pragma unroll
-    for (int i = 0; i < 4; i += 2) {
-        const uint32_t u = w >> (4 * i);
-        r[i] = sub2_half(masked_or(u, 0x000f000fu, 0x64006400u), zero);
-        r[i + 1] = sixteenth_plus(masked_or(u, 0x00f000f0u, 0x64006400u), high);
-    }
-}
-
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-__device__ __forceinline__ float low_of(uint32_t w) { return __uint_as_float(w << 16); }
-__device__ __forceinline__ float high_of(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
-
-// IO: queries and outputs; C: 32s of elements of a head, rounded up; SPLIT: groups of up to eight heads, whose other eight
-// rows are the weights' second parts.
-template <typename IO, int C, bool SPLIT>
-struct NibbleCore {
-    using Elem = IO;
-    static constexpr bool kPacked = true, kScored = false;  // other scores are a branch here
-    static constexpr int kWholeTiles = 6, kSwitch = 4;
-    static constexpr bool kThree = sizeof(IO) == 4;         // parts of queries and weights
-    static constexpr bool kHalf = std::is_same<IO, __half>::value;
-    using Q = typename std::conditional<kHalf, __half, __nv_bfloat16>::type;
-    static constexpr int kParts = kThree ? 3 : 1;
-    static constexpr int kKeys = 16;
-    static constexpr int kWarps = SPLIT || C <= 4 ? 8 : 4;  // whose sums fit an SM
-    static constexpr int kBlocks = 1;
-    static constexpr bool kWholeRows = true;
-    static constexpr int kThreads = kWarps * 32;
-    static constexpr int kRows = SPLIT ? 8 : 16;
-    static constexpr int kDim = C * kChunk;
-    static constexpr int kBoxes = 0, kChunks = 0;
-    static constexpr int kTileBytes = C * (kChunkBytes + kGroupBytes);
-    static constexpr int kPitch = (C * 4 + 1) * 16;         // of queries: an odd number of 16-byte chunks
-    static constexpr bool kQueryInSmem = kThree || (!SPLIT && C > 4);
-    static constexpr int kPartBytes = kRows * kPitch;
-    static constexpr int kQueryBytes = kParts * kPartBytes;
-    static constexpr int kWarpBytes = 0;
-    static constexpr float kUnit = 0x1p-24f;                // weights and their parts are bf16 whatever IO is
-    // Queries of the range of fp32 are taken 2^12 times smaller: 256 products with numbers up to 15, whose scale is yet to
-    // come, then stay in it.
-    static constexpr float kQuery = kHalf ? 1.0f : 0x1p-12f, kScale = 1.0f / kQuery;
-    uint32_t qa[kQueryInSmem ? 1 : 2 * C][SPLIT ? 2 : 4];
-    float o[4 * C][4], m[2], l[2], slope[2];
-    uint32_t query;
-    int words, group_shift, groups;
-
-    // Word w of a row's 32 elements holds two, this one and the fourth after it: word t, or 4 + t, of an instruction's eight is
-    // what the lanes of column t multiply with their first, or second, register.
-    static __device__ __forceinline__ int element(int w) { return 8 * (w % 4) + 2 * (w / 8) + w % 8 / 4; }
-
-    static __device__ __forceinline__ void stage_query(const IO *q, int heads, int D, bool, bool, char *smem_q) {
-        for (int e = threadIdx.x; e < kRows * kDim / 2; e += kThreads) {
-            const int r = e / (kDim / 2), w = e - r * (kDim / 2), i = w / 16 * kChunk + element(w % 16);
-            uint32_t *to = reinterpret_cast<uint32_t *>(smem_q + r * kPitch) + w;
-            float x[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) x[h] = r < heads && i + 4 * h < D ? dev::widen(q[r * D + i + 4 * h]) * kQuery : 0.0f;
-            if constexpr (kThree) {
-                // Cut off, not rounded, so that the parts' sum is exact; a number that is not finite is its first part.
-                uint32_t bits[2][3];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const bool finite = fabsf(x[h]) <= FLT_MAX;
-#pragma unroll
-                    for (int part = 0; part < 3; ++part) {
-                        bits[h][part] = __float_as_uint(x[h]);
-                        x[h] = finite ? x[h] - __uint_as_float(bits[h][part] & 0xffff0000u) : 0.0f;
-                    }
-                    if (!finite && (bits[h][0] & 0xffffu)) bits[h][0] |= 0x400000u;  // a NaN stays one
-                }
-#pragma unroll
-                for (int part = 0; part < 3; ++part) to[part * (kPartBytes / 4)] = bits[0][part] >> 16 | (bits[1][part] & 0xffff0000u);
-            } else {
-                *to = pack2(dev::narrow<IO>(x[0]), dev::narrow<IO>(x[1]));
-            }
-        }
-    }
-
-    __device__ __forceinline__ void begin(char *smem_q, char *, const AttnArgs &a, const Scoring &sc) {
-        const int lane = threadIdx.x & 31;
-        query = smem_addr(smem_q);
-        words = (a.c.head_dim + kChunk - 1) / kChunk * kChunkBytes;
-        group_shift = __ffs(a.c.group / kChunk) - 1;
-        groups = (a.c.head_dim + a.c.group - 1) / a.c.group;
-        for (int r = 0; r < (SPLIT ? 1 : 2); ++r) slope[r] = slope_of(sc, (lane >> 2) + 8 * r);
-        if constexpr (!kQueryInSmem) {
-#pragma unroll
-            for (int c = 0; c < C; ++c) load_query(qa[2 * c], qa[2 * c + 1], c, 0);
-        }
-#pragma unroll
-        for (int n = 0; n < 4 * C; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[n][e] = 0.0f;
-        m[0] = m[1] = -INFINITY;
-        l[0] = l[1] = 0.0f;
-    }
-
-    // The queries of one 32 of elements, for its two instructions.
-    template <int N>
-    __device__ __forceinline__ void load_query(uint32_t (&x)[N], uint32_t (&y)[N], int c, int part) const {
-        const int lane = threadIdx.x & 31;
-        uint32_t r[4];
-        if constexpr (SPLIT) {  // matrices of 8 heads x 8 elements
-            ldmatrix4(r, query + part * kPartBytes + (lane & 7) * kPitch + (4 * c + (lane >> 3)) * 16);
-            x[0] = r[0], x[1] = r[1], y[0] = r[2], y[1] = r[3];
-        } else {
-            const uint32_t at = query + part * kPartBytes + (((lane >> 3) & 1) * 8 + (lane & 7)) * kPitch + (lane >> 4) * 16 + c * 64;
-            ldmatrix4(r, at);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = r[e];
-            ldmatrix4(r, at + 32);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = r[e];
-        }
-    }
-    template <typename T, int N>
-    static __device__ __forceinline__ void multiply(float (&c)[4], const uint32_t (&a)[N], uint32_t b0, uint32_t b1) {
-        if constexpr (N == 2) {
-            const uint32_t a4[4] = {a[0], 0, a[1], 0};
-            mma16816<T>(c, a4, b0, b1);
-        } else {
-            mma16816<T>(c, a, b0, b1);
-        }
-    }
-
-    // Makes the words of values that do not count zeros: their weights are, and the words may hold anything.
-    static __device__ __forceinline__ void clear(char *values, uint32_t live, const Cache &c) {
-        const int lane = threadIdx.x & 31;
-        if (lane < kKeys && !(live >> lane & 1))
-            for (int at = (c.head_dim + kChunk - 1) / kChunk * kChunkBytes; at < c.tile_bytes; at += kGroupBytes)
-                *reinterpret_cast<uint32_t *>(values + at + 4 * lane) = 0;
-    }
-
-    __device__ __forceinline__ void step(const char *ks, const char *vs, uint32_t live, const Scoring &sc, int first) {
-        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-        const uint32_t ka = smem_addr(ks) + lane * 16, va = smem_addr(vs) + lane * 16;
-        const int last = groups - 1;
-        // Scores: of each group, then their sum over the groups, scaled.
-        float s[2][4] = {}, part[2][4] = {};
-        uint32_t b[4], zero[2], high[2];
-        float2 scale[2];
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            if (c == 0 || (c & ((1 << group_shift) - 1)) == 0) {
-                const char *w = ks + words + min(c >> group_shift, last) * kGroupBytes;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint32_t z = *reinterpret_cast<const uint32_t *>(w + (8 * h + g) * 4) & 15u;
-                    zero[h] = (kHalf ? 0x64006400u : 0x43004300u) + z * 0x10001u;
-                    high[h] = 0xd400d400u + z * 0x100010u;
-                    const uint2 two = *reinterpret_cast<const uint2 *>(w + (8 * h + 2 * t) * 4);
-                    scale[h] = make_float2(__uint_as_float(two.x & ~15u), __uint_as_float(two.y & ~15u));
-                }
-            }
-            if (c % 2 == 0) ldmatrix4(b, ka + c * kChunkBytes - (c + 1 == C ? (lane >> 4) * kChunkBytes : 0));
-            uint32_t n[2][4];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                if constexpr (kHalf) differences_half(n[h], b[2 * (c % 2) + h], zero[h], high[h]);
-                else differences_bf16(n[h], b[2 * (c % 2) + h], zero[h]);
-            }
-#pragma unroll
-            for (int p = 0; p < kParts; ++p) {
-                uint32_t x[SPLIT ? 2 : 4], y[SPLIT ? 2 : 4];
-                if constexpr (kQueryInSmem) {
-                    load_query(x, y, c, p);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < (SPLIT ? 2 : 4); ++e) x[e] = qa[2 * c][e], y[e] = qa[2 * c + 1][e];
-                }
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    multiply<Q>(part[h], x, n[h][0], n[h][1]);
-                    multiply<Q>(part[h], y, n[h][2], n[h][3]);
-                }
-            }
-            if (c + 1 == C || ((c + 1) & ((1 << group_shift) - 1)) == 0) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int e = 0; e < (SPLIT ? 2 : 4); ++e) {
-                        s[h][e] = fmaf(part[h][e], e & 1 ? scale[h].y : scale[h].x, s[h][e]);
-                        part[h][e] = 0.0f;
-                    }
-            }
-        }
-        if (sc.cap != 0.0f || sc.slopes) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int e = 0; e < (SPLIT ? 2 : 4); ++e) s[h][e] = score_of(sc, s[h][e], slope[e >> 1], first + h * 8 + 2 * t + (e & 1));
-        } else {
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int e = 0; e < (SPLIT ? 2 : 4); ++e) s[h][e] *= sc.scale2;
-        }
-        if (live != (1u << kKeys) - 1) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int e = 0; e < (SPLIT ? 2 : 4); ++e)
-                    if (!(live >> (h * 8 + 2 * t + (e & 1)) & 1)) s[h][e] = -INFINITY;
-        }
-        // Weights, relative to the largest score so far.
-#pragma unroll
-        for (int r = 0; r < (SPLIT ? 1 : 2); ++r) {
-            float top = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const float m2 = fmaxf(m[r], top), base = finite_base(m2);
-            if (__any_sync(0xffffffffu, m2 != m[r])) {
-                const float f = exp2_approx(m[r] - base);
-                l[r] *= f;
-#pragma unroll
-                for (int n = 0; n < 4 * C; ++n) {
-                    o[n][2 * r] *= f;
-                    o[n][2 * r + 1] *= f;
-                    if constexpr (SPLIT) {
-                        o[n][2] *= f;
-                        o[n][3] *= f;
-                    }
-                }
-                m[r] = m2;
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int e = 2 * r; e < 2 * r + 2; ++e) s[h][e] = exp2_approx(s[h][e] - base);
-            l[r] += (s[0][2 * r] + s[0][2 * r + 1]) + (s[1][2 * r] + s[1][2 * r + 1]);
-        }
-        // Values: weights with a group's scales, in parts, times the differences of its elements.
-        uint32_t p[kThree ? 3 : 2][4], zeros[2];
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            if (c == 0 || (c & ((1 << group_shift) - 1)) == 0) {
-                const char *w = vs + words + min(c >> group_shift, last) * kGroupBytes;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint2 two = *reinterpret_cast<const uint2 *>(w + (8 * h + 2 * t) * 4);
-                    zeros[h] = 0x43004300u + (two.x & 15u) + ((two.y & 15u) << 16);
-                    const float sx = __uint_as_float(two.x & ~15u) * kUnit, sy = __uint_as_float(two.y & ~15u) * kUnit;
-#pragma unroll
-                    for (int r = 0; r < (SPLIT ? 1 : 2); ++r) {
-                        float x = s[h][2 * r] * sx, y = s[h][2 * r + 1] * sy;
-#pragma unroll
-                        for (int k = 0; k < (kThree ? 3 : 2); ++k) {
-                            const uint32_t two16 = pack_bf16(x, y);
-                            x -= low_of(two16);
-                            y -= high_of(two16);
-                            // SPLIT: the first two parts in one instruction, a third in one of its own.
-                            if (!SPLIT) p[k][r + 2 * h] = two16;
-                            else if (k < 2) p[0][k + 2 * h] = two16;
-                            else p[1][2 * h] = two16, p[1][1 + 2 * h] = 0;
-                        }
-                    }
-                }
-            }
-            if (c % 2 == 0) ldmatrix4_trans(b, va + c * kChunkBytes - (c + 1 == C ? (lane >> 4) * kChunkBytes : 0));
-            uint32_t n[2][4];
-            differences_bf16(n[0], b[2 * (c % 2)], zeros[0]);
-            differences_bf16(n[1], b[2 * (c % 2) + 1], zeros[1]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int k = 0; k < (SPLIT ? (kThree ? 2 : 1) : (kThree ? 3 : 2)); ++k)
-                    mma16816<__nv_bfloat16>(o[4 * c + i], p[k], n[0][i], n[1][i]);
-        }
-    }
-
-    // This warp's sums [kRows][kDim], maxima and sums of weights [kRows] to shared memory.
-    __device__ __forceinline__ void end(float *so, float *sm, float *sl) {
-        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-#pragma unroll
-        for (int r = 0; r < (SPLIT ? 1 : 2); ++r) {
-            float sum = l[r] + __shfl_xor_sync(0xffffffffu, l[r], 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            if (t == 0) {
-                sm[g + 8 * r] = m[r];
-                sl[g + 8 * r] = sum;
-            }
-#pragma unroll
-            for (int c = 0; c < C; ++c)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {  // columns 2t + e: elements 4 (2t + e) .. + 3 of the 32
-                    float v[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) v[i] = o[4 * c + i][2 * r + e] + (SPLIT ? o[4 * c + i][2 + e] : 0.0f);
-                    *reinterpret_cast<float4 *>(so + (g + 8 * r) * kDim + c * kChunk + 4 * (2 * t + e)) = make_float4(v[0], v[1], v[2], v[3]);
-                }
-        }
-    }
-};
-
-template <typename IO, int C, bool SPLIT>
-AttnKernel nibble_kernel() {
-    constexpr int kStages = 4;
-    static_assert(AttnSmem<NibbleCore<IO, C, SPLIT>, kStages>::kBytes <= 227 * 1024, "fits an SM");
-    return attn_kernel<NibbleCore<IO, C, SPLIT>, kStages>();
-}
-
-template <typename IO, bool SPLIT>
-AttnKernel pick_nibbles(int D) {
-    if (D <= 64) return nibble_kernel<IO, 2, SPLIT>();
-    if (D <= 96) return nibble_kernel<IO, 3, SPLIT>();
-    if (D <= 128) return nibble_kernel<IO, 4, SPLIT>();
-    if (D <= 192) return nibble_kernel<IO, 6, SPLIT>();
-    return nibble_kernel<IO, 8, SPLIT>();
-}
-
-AttnKernel pick_attn_kv4(int dtype, int D, int G) {
-    if (dtype == L2D_F16) return G <= 8 ? pick_nibbles<__half, true>(D) : pick_nibbles<__half, false>(D);
-    if (dtype == L2D_BF16) return G <= 8 ? pick_nibbles<__nv_bfloat16, true>(D) : pick_nibbles<__nv_bfloat16, false>(D);
-    return G <= 8 ? pick_nibbles<float, true>(D) : pick_nibbles<float, false>(D);
+AttnKernel pick_attn_kv4(int dtype, int D, int group, int G) {
+    if (dtype == L2D_F16) return pick_kv4_half(D, group, G);
+    return dtype == L2D_BF16 ? pick_kv4_bf16(D, group, G) : pick_kv4_float(D, group, G);
 }
 
 int check_cache4(const l2d_kv4_cache *cache, Cache *c) {
