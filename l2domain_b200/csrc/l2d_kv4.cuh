@@ -24,10 +24,9 @@ constexpr int kGroupBytes = kBlockSlots * 4;
 //
 // Per 16 keys of 128 elements a warp reads 2 x 1088 bytes, which an SM's share of the memory brings in about 100 cycles,
 // the issue of 400 instructions; so the conversion of 4096 nibbles is what has to be cheap.  A word of eight nibbles gives
-// four registers of two 16-bit numbers each, by one mask that also sets the exponent of 2^10 (fp16) or 2^7 (bf16), and one
-// subtraction that takes off this and the zero point together; the differences n - z are exact.  Scales stay outside
-// the products: the scores of a group's elements are multiplied by its key's scale as fp32 sums, and weights by the
-// value's scale before they are cut into 16-bit parts.
+// four registers of two 16-bit numbers each: a mask and a multiply-add that takes off the zero point, and one shift for the
+// upper two; the differences n - z are exact.  Scales stay outside the products: the scores of a group's elements are
+// multiplied by its key's scale as fp32 sums, and weights by the value's scale before they are cut into 16-bit parts.
 //
 // Keys are the rows of a product with the queries of eight heads as columns: a matrix of ldmatrix (8 keys x 16 bytes) gives a
 // lane word t of key g, elements 8t .. 8t + 7 of the 32, and queries are staged in the order in which two instructions meet
@@ -40,42 +39,38 @@ constexpr int kGroupBytes = kBlockSlots * 4;
 // a weight is left).
 // ---------------------------------------------------------------------------------------------
 
-__device__ __forceinline__ uint32_t sub2_half(uint32_t a, uint32_t b) {
+// a b + c of two pairs
+template <typename T>
+__device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
     uint32_t r;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
-// a / 16 + b
-__device__ __forceinline__ uint32_t sixteenth_plus(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(0x2c002c00u), "r"(b));
-    return r;
-}
-__device__ __forceinline__ uint32_t sub2_bf16(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(b), "r"(0xbf80bf80u), "r"(a));
-    return r;
-}
-// (w & mask) | bits
-__device__ __forceinline__ uint32_t masked_or(uint32_t w, uint32_t mask, uint32_t bits) {
-    uint32_t r;
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(bits));
+    if constexpr (std::is_same<T, __half>::value) asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    else asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
     return r;
 }
 
-// Nibbles i of both halves of a word, i = 0..3, less their zero points.  T = bf16: zero holds 128 + z twice.
-__device__ __forceinline__ void differences_bf16(uint32_t (&r)[4], uint32_t w, uint32_t zero) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = sub2_bf16(masked_or(w >> (4 * i), 0x000f000fu, 0x43004300u), zero);
-}
-// fp16: zero holds 1024 + z twice, and high -(64 + z): nibbles in the second place count 16-fold there.
-__device__ __forceinline__ void differences_half(uint32_t (&r)[4], uint32_t w, uint32_t zero, uint32_t high) {
+// Nibbles i of both halves of a word, i = 0..3, less their zero points, times kStep<T>.  The lowest bits of a 16-bit number are a
+// count of 2^-24 (fp16, eleven bits) or 2^-133 (bf16, eight): the subnormal numbers and the first normal ones.  So a nibble
+// in the first place, or in the second 16-fold, is one without more than a mask.
+template <typename T>
+constexpr float kStep = 0x1p-6f;
+template <>
+constexpr float kStep<__half> = 0x1p-9f;
+template <typename T>
+__device__ __forceinline__ void differences(uint32_t (&r)[4], uint32_t w, uint32_t minus_zero) {
+    constexpr bool kHalf = std::is_same<T, __half>::value;
+    constexpr uint32_t kFirst = kHalf ? 0x78007800u : 0x7f007f00u, kSecond = kHalf ? 0x68006800u : 0x7d007d00u;  // 2^15 and 2^11, 2^127 and 2^123
 #pragma unroll
     for (int i = 0; i < 4; i += 2) {
         const uint32_t u = w >> (4 * i);
-        r[i] = sub2_half(masked_or(u, 0x000f000fu, 0x64006400u), zero);
-        r[i + 1] = sixteenth_plus(masked_or(u, 0x00f000f0u, 0x64006400u), high);
+        r[i] = fma2<T>(u & 0x000f000fu, kFirst, minus_zero);
+        r[i + 1] = fma2<T>(u & 0x00f000f0u, kSecond, minus_zero);
     }
+}
+// Of two zero points, in the halves of z: -z kStep<T>, by way of 1024 + z or 128 + z.
+template <typename T>
+__device__ __forceinline__ uint32_t minus_zeros(uint32_t z) {
+    if constexpr (std::is_same<T, __half>::value) return fma2<T>(0x64006400u + z, 0x98009800u, 0x40004000u);
+    else return fma2<T>(0x43004300u + z, 0xbc80bc80u, 0x40004000u);
 }
 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
@@ -122,7 +117,7 @@ struct NibbleCore {
     // Queries of the range of fp32 are taken 2^12 times smaller: 256 products with numbers up to 15, whose scale is yet to
     // come, then stay in it.
     static constexpr float kRoom = 8.0f;
-    static constexpr float kQuery = kHalf ? 1.0f : 0x1p-12f, kScale = 1.0f / kQuery;
+    static constexpr float kQuery = kHalf ? 1.0f : 0x1p-12f, kScale = 1.0f / kQuery / kStep<Q>;
     // Columns are heads 8 j + 2 t + e, for which a lane keeps maximum and sum.
     uint32_t qb[kQueryInSmem ? 1 : C][N][4];
     float o[2 * C][N][4], m[N][2], l[N][2], slope[N][2];
@@ -208,7 +203,7 @@ struct NibbleCore {
         const int lane = threadIdx.x & 31, g = lane >> 2;
         const uint32_t ka = smem_addr(ks) + lane * 16;
         float part[N][4] = {};
-        uint32_t b[4], zero[2], high[2];
+        uint32_t b[4], zero[2];
         float scale[2];
 #pragma unroll
         for (int j = 0; j < N; ++j)
@@ -220,19 +215,15 @@ struct NibbleCore {
                 const char *w = ks + words + min(c / G, last) * kGroupBytes + 4 * g;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const uint32_t word = *reinterpret_cast<const uint32_t *>(w + 32 * h), z = word & 15u;
-                    zero[h] = (kHalf ? 0x64006400u : 0x43004300u) + z * 0x10001u;
-                    high[h] = 0xd400d400u + z * 0x100010u;
+                    const uint32_t word = *reinterpret_cast<const uint32_t *>(w + 32 * h);
+                    zero[h] = minus_zeros<Q>((word & 15u) * 0x10001u);
                     scale[h] = __uint_as_float(word & ~15u);
                 }
             }
             if (c % 2 == 0) ldmatrix4(b, ka + c * kChunkBytes - (c + 1 == C ? (lane >> 4) * kChunkBytes : 0));
             uint32_t n[2][4];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                if constexpr (kHalf) differences_half(n[h], b[2 * (c % 2) + h], zero[h], high[h]);
-                else differences_bf16(n[h], b[2 * (c % 2) + h], zero[h]);
-            }
+            for (int h = 0; h < 2; ++h) differences<Q>(n[h], b[2 * (c % 2) + h], zero[h]);
             const uint32_t a0[4] = {n[0][0], n[1][0], n[0][1], n[1][1]}, a1[4] = {n[0][2], n[1][2], n[0][3], n[1][3]};
 #pragma unroll
             for (int j = 0; j < N; ++j)
@@ -272,8 +263,8 @@ struct NibbleCore {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const uint2 two = *reinterpret_cast<const uint2 *>(w + (8 * h + 2 * t) * 4);
-                    zeros[h] = 0x43004300u + (two.x & 15u) + ((two.y & 15u) << 16);
-                    const float by = __uint_as_float(*reinterpret_cast<const uint32_t *>(w + (8 * h + g) * 4) & ~15u) * kUnit;
+                    zeros[h] = minus_zeros<__nv_bfloat16>((two.x & 15u) + ((two.y & 15u) << 16));
+                    const float by = __uint_as_float(*reinterpret_cast<const uint32_t *>(w + (8 * h + g) * 4) & ~15u) * (kUnit / kStep<__nv_bfloat16>);
 #pragma unroll
                     for (int j = 0; j < N; ++j) {
                         float x = s[j][2 * h] * by, y = s[j][2 * h + 1] * by;
@@ -289,8 +280,8 @@ struct NibbleCore {
             }
             if (c % 2 == 0) ldmatrix4_trans(b, va + c * kChunkBytes - (c + 1 == C ? (lane >> 4) * kChunkBytes : 0));
             uint32_t n[2][4];
-            differences_bf16(n[0], b[2 * (c % 2)], zeros[0]);
-            differences_bf16(n[1], b[2 * (c % 2) + 1], zeros[1]);
+            differences<__nv_bfloat16>(n[0], b[2 * (c % 2)], zeros[0]);
+            differences<__nv_bfloat16>(n[1], b[2 * (c % 2) + 1], zeros[1]);
             const uint32_t a0[4] = {n[0][0], n[0][1], n[1][0], n[1][1]}, a1[4] = {n[0][2], n[0][3], n[1][2], n[1][3]};
 #pragma unroll
             for (int j = 0; j < N; ++j)
