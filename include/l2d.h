@@ -509,6 +509,34 @@ L2D_API int l2d_kv4_append(const l2d_kv4_cache *cache, const l2d_append_desc *de
 L2D_API int l2d_attn_plan_create_kv4(const l2d_kv4_cache *cache, const l2d_attn_desc *desc, const l2d_attn_scores *scores,
                                      l2d_attn_plan **plan);
 
+/* A mixture-of-experts layer for a few tokens:
+ *   y[t] = sum_k w_k down_e (silu(gate_e x[t]) * (up_e x[t])),  e = ids[t][k]
+ * The experts are the `top` largest of router x[t], in falling order and of equal ones the lower first (a NaN counts as the
+ * least); w is their softmax over all experts and, where normalize is set, divided by the chosen ones' sum.  Router sums
+ * are fp64, so that no order of addition chooses; the others fp32.  silu(..) * .. meets down as two numbers of dtype (fp32: as it
+ * is): 2^-16 of it is left (bf16), or 2^-22 of it and 2^-39 of the token's largest with this expert (fp16). */
+typedef struct l2d_moe_plan l2d_moe_plan;
+typedef struct {
+    int64_t hidden, inner;               /* elements of a token, and of an expert's inner vector */
+    int experts, top;                    /* experts 1..512, top 1..32 */
+    int max_tokens;                      /* 1..65535 */
+    int dtype;                           /* of x, y and all weights */
+    int normalize;
+    const void *router;                  /* [experts][hidden] */
+    const void *gate, *up;               /* [experts][inner][hidden]; one buffer or two */
+    const void *down;                    /* [experts][hidden][inner] */
+    int64_t router_row, gate_row, up_row, down_row;    /* elements between rows (0 = dense) */
+    int64_t gate_expert, up_expert, down_expert;       /* elements between experts (0 = one after the other) */
+    int64_t x_token, y_token;            /* elements between tokens (0 = hidden) */
+    int device;
+} l2d_moe_desc;
+/* The plan owns its device scratch (allocated here, never during l2d_moe_forward); calls of one plan must not overlap on the GPU. */
+L2D_API int l2d_moe_plan_create(const l2d_moe_desc *desc, l2d_moe_plan **plan);
+/* ids (int32) and weights (fp32), both [tokens][top], receive the choice; either may be NULL.  y must not overlap x or the weights.
+ * Rows on 16-byte boundaries are read fastest; any are read. */
+L2D_API int l2d_moe_forward(l2d_moe_plan *plan, const void *x, void *y, int32_t *ids, float *weights, int tokens, void *stream);
+L2D_API int l2d_moe_plan_destroy(l2d_moe_plan *plan);
+
 /* ---- helpers used by the benchmark and the CLI ---- */
 /* Reference-mode inputs (init_data): A/x from mix32 of the flat index (stream 0 = A, 1 = x). */
 L2D_API int l2d_fill_ref(void *dst, int dtype, uint64_t first, uint64_t n, uint32_t seed, int stream,

@@ -128,6 +128,14 @@ class AttnScores(C.Structure):
     _fields_ = [("cap", C.c_float), ("slopes", C.c_void_p)]
 
 
+class MoeDesc(C.Structure):
+    _fields_ = [("hidden", C.c_int64), ("inner", C.c_int64), ("experts", C.c_int), ("top", C.c_int), ("max_tokens", C.c_int),
+                ("dtype", C.c_int), ("normalize", C.c_int), ("router", C.c_void_p), ("gate", C.c_void_p), ("up", C.c_void_p),
+                ("down", C.c_void_p), ("router_row", C.c_int64), ("gate_row", C.c_int64), ("up_row", C.c_int64),
+                ("down_row", C.c_int64), ("gate_expert", C.c_int64), ("up_expert", C.c_int64), ("down_expert", C.c_int64),
+                ("x_token", C.c_int64), ("y_token", C.c_int64), ("device", C.c_int)]
+
+
 # Every symbol include/l2d.h declares, with its ctypes signature.
 _vp, _i, _u32, _u64, _i64, _sz = C.c_void_p, C.c_int, C.c_uint32, C.c_uint64, C.c_int64, C.c_size_t
 _pi, _pu32, _pu64, _psz = C.POINTER(C.c_int), C.POINTER(C.c_uint32), C.POINTER(C.c_uint64), C.POINTER(C.c_size_t)
@@ -195,6 +203,9 @@ SIGNATURES = {
     "l2d_attn_decode_from": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _vp]),
     "l2d_kv4_page_bytes": (_i, [_i, _i, _i, _i, C.POINTER(_i64)]),
     "l2d_kv4_append": (_i, [C.POINTER(KvCache4Desc), C.POINTER(AppendDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "l2d_moe_plan_create": (_i, [C.POINTER(MoeDesc), C.POINTER(_vp)]),
+    "l2d_moe_forward": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _vp]),
+    "l2d_moe_plan_destroy": (_i, [_vp]),
     "l2d_fill_ref": (_i, [_vp, _i, _u64, _u64, _u32, _i, _i, _vp]),
     "l2d_fill_cfg": (_i, [_vp, _i, _u64, _u64, _u64, _u64, _i, C.c_float, C.c_float, _vp]),
     "l2d_l2_flush": (_i, [_i, _vp]),
@@ -741,6 +752,41 @@ def distance_slopes(heads: int, device=None):
     import torch
 
     return torch.exp2(-8.0 * torch.arange(1, heads + 1, dtype=torch.float64, device=device) / heads).float()
+
+
+class MoeLayer:
+    """A mixture-of-experts layer for up to ``max_tokens`` tokens: ``router`` [experts][hidden], ``gate`` and ``up``
+    [experts][inner][hidden], ``down`` [experts][hidden][inner], all of ``dtype``; y = sum of w_k down_k (silu(gate_k x) * (up_k x))
+    over the ``top`` best experts, whose weights are softmax over all experts, divided by their sum where ``normalize``.
+    ``*_row`` / ``*_expert`` / ``*_token``: elements between rows, experts, tokens (0 = dense).  The plan owns its scratch;
+    calls of one plan must not overlap on the GPU."""
+
+    def __init__(self, router, gate, up, down, hidden: int, inner: int, experts: int, top: int, max_tokens: int, dtype: int = BF16,
+                 normalize: bool = True, router_row: int = 0, gate_row: int = 0, up_row: int = 0, down_row: int = 0,
+                 gate_expert: int = 0, up_expert: int = 0, down_expert: int = 0, x_token: int = 0, y_token: int = 0, device: int = 0):
+        self._plan = C.c_void_p(0)
+        self._hold = (router, gate, up, down)
+        d = MoeDesc(hidden=hidden, inner=inner, experts=experts, top=top, max_tokens=max_tokens, dtype=dtype, normalize=int(normalize),
+                    router=_ptr(router), gate=_ptr(gate), up=_ptr(up), down=_ptr(down), router_row=router_row, gate_row=gate_row,
+                    up_row=up_row, down_row=down_row, gate_expert=gate_expert, up_expert=up_expert, down_expert=down_expert,
+                    x_token=x_token, y_token=y_token, device=device)
+        check(lib().l2d_moe_plan_create(C.byref(d), C.byref(self._plan)))
+        self._call = lib().l2d_moe_forward
+
+    def forward(self, x, y, tokens: int, ids=None, weights=None, stream=None) -> None:
+        """y[t] of x[t]; ``ids`` (int32) and ``weights`` (fp32), [tokens][top], receive the choice where given."""
+        check(self._call(self._plan, _ptr(x), _ptr(y), _ptr(ids), _ptr(weights), tokens, _stream_handle(stream)))
+
+    def close(self) -> None:
+        if self._plan and self._plan.value:
+            check(lib().l2d_moe_plan_destroy(self._plan))
+            self._plan = C.c_void_p(0)
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 def rotation_tables(max_pos: int, rot_dim: int, theta: float = 10000.0, stretch: float = 1.0, device=None):

@@ -1,0 +1,919 @@
+// A mixture-of-experts layer for a few tokens (l2d_moe_*): the router, the chosen experts' products, their weighted sum.
+//
+// Memory bound: the weights of every chosen expert are read once and meet one token or a few.  Four launches, each of which
+// waits for the one before on the device and not on the host:
+//   k_route    a router row and up to eight tokens per block; the last block of eight tokens chooses their experts, the last of
+//              all sorts (token, choice) pairs ("slots") into entries: an expert and up to so many slots as one pass takes
+//   k_experts  gate and up: silu(gate x) * (up x) of every slot, to scratch
+//   k_experts  down: of every slot, to scratch
+//   k_combine  the weighted sum over a token's slots, in their order
+// Nothing depends on the order in which blocks come: a slot's sums are its own.
+#include "l2d_launch.cuh"
+
+#include <algorithm>
+#include <cfloat>
+#include <climits>
+#include <cmath>
+#include <cstring>
+#include <new>
+#include <type_traits>
+
+namespace l2d {
+
+constexpr int kMaxExperts = 512;
+constexpr int kMoeThreads = 256, kMoeWarps = kMoeThreads / 32;
+constexpr int kRouteTokens = kMoeWarps;  // of a block of the router: a warp each chooses
+
+struct MoeArgs {
+    const void *x, *router, *gate, *up, *down;
+    void *y;
+    int32_t *ids_out;
+    float *weights_out;
+    int64_t x_token, y_token, router_row, gate_row, up_row, down_row, gate_expert, up_expert, down_expert;
+    int tokens, hidden, inner, experts, top, normalize, per_entry;
+    // The plan's scratch.
+    double *logits;       // [tokens][experts]
+    int *ids;             // [slots], slot = token * top + choice
+    float *weights;       // [slots]
+    uint32_t *largest;    // [slots] bits of the largest |silu(gate x) (up x)| (fp16)
+    int *sorted;          // [slots], by expert
+    int4 *entries;        // expert, first place in sorted, slots
+    int *num_entries;
+    unsigned *arrived;    // [token tiles + 1], zero between calls
+    uint32_t *inner_out;  // [slots][inner_row] fp32, or two bf16 numbers that add up to one
+    float *part;          // [slots][hidden]
+    int64_t inner_row;
+};
+
+// ---------------------------------------------------------------------------------------------
+// Router.  Its sums are 64-bit ones: they choose, and two experts whose scores differ by less than a 32-bit sum is off would be
+// chosen by the order of addition.  A router row's numbers are made 64-bit ones once for up to eight tokens.
+// ---------------------------------------------------------------------------------------------
+
+template <typename T>
+struct Eight {
+    T v[8];
+};
+template <typename T>
+__device__ __forceinline__ Eight<T> load_eight(const T *p) {
+    Eight<T> r;
+    const uint4 *from = reinterpret_cast<const uint4 *>(p);
+    uint4 *to = reinterpret_cast<uint4 *>(&r);
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) to[i] = from[i];
+    return r;
+}
+
+// Chooses the experts of one token: a warp, `top` rounds over up to kMaxExperts / 32 scores a lane.
+__device__ __forceinline__ void choose(const MoeArgs &a, int token) {
+    constexpr int kEach = kMaxExperts / 32;
+    const int lane = threadIdx.x & 31;
+    const double *logits = a.logits + static_cast<int64_t>(token) * a.experts;
+    double v[kEach];
+    uint32_t open = 0;  // this lane's experts that are not chosen yet
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        const int e = lane + 32 * i;
+        v[i] = 0.0;
+        if (e < a.experts) {
+            v[i] = __ldcg(logits + e);
+            open |= 1u << i;
+        }
+    }
+    int mine = 0;
+    double score = 0.0, first = 0.0;  // of the choice that this lane keeps, and of the first
+    for (int k = 0; k < a.top; ++k) {
+        double best = -INFINITY;
+        int at = INT_MAX;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const double x = v[i] == v[i] ? v[i] : -INFINITY;  // what is no number comes last
+            if ((open >> i & 1) && (x > best || at == INT_MAX)) best = x, at = lane + 32 * i;
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) {
+            const double x = __shfl_xor_sync(0xffffffffu, best, d);
+            const int i = __shfl_xor_sync(0xffffffffu, at, d);
+            if (i != INT_MAX && (at == INT_MAX || x > best || (x == best && i < at))) best = x, at = i;
+        }
+        double given = 0.0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            if (at == lane + 32 * i) {
+                open &= ~(1u << i);
+                given = v[i];
+            }
+        given = __shfl_sync(0xffffffffu, given, at & 31);
+        if (k == 0) first = given;
+        if (k % 32 == lane) mine = at, score = given;
+    }
+    double sum = 0.0;
+    if (a.normalize) {
+        if (lane < a.top) sum = exp(score - first);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            if (lane + 32 * i < a.experts) sum += exp(v[i] - first);
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if (lane < a.top) {
+        const int64_t slot = static_cast<int64_t>(token) * a.top + lane;
+        const float w = static_cast<float>(exp(score - first) / sum);
+        a.ids[slot] = mine;
+        a.weights[slot] = w;
+        a.largest[slot] = 0;
+        if (a.ids_out) a.ids_out[slot] = mine;
+        if (a.weights_out) a.weights_out[slot] = w;
+    }
+}
+
+// Sorts the slots by expert, and cuts each expert's into entries.
+__device__ __forceinline__ void sort_slots(const MoeArgs &a) {
+    __shared__ int count[kMaxExperts], place[kMaxExperts], entry[kMaxExperts];
+    const int tid = threadIdx.x, slots = a.tokens * a.top;
+    for (int e = tid; e < kMaxExperts; e += kMoeThreads) count[e] = 0;
+    __syncthreads();
+    for (int s = tid; s < slots; s += kMoeThreads) atomicAdd(&count[__ldcg(a.ids + s)], 1);
+    __syncthreads();
+    if (tid < 32) {  // places and entries before each expert's: 16 experts a lane
+        constexpr int kEach = kMaxExperts / 32;
+        int here = 0, entries = 0;
+        for (int i = 0; i < kEach; ++i) {
+            const int n = count[tid * kEach + i];
+            here += n;
+            entries += (n + a.per_entry - 1) / a.per_entry;
+        }
+        int upto = here, upto_entries = entries;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, upto, d), y = __shfl_up_sync(0xffffffffu, upto_entries, d);
+            if (tid >= d) upto += x, upto_entries += y;
+        }
+        if (tid == 31) *a.num_entries = upto_entries;
+        upto -= here;
+        upto_entries -= entries;
+        for (int i = 0; i < kEach; ++i) {
+            const int n = count[tid * kEach + i];
+            place[tid * kEach + i] = upto;
+            entry[tid * kEach + i] = upto_entries;
+            upto += n;
+            upto_entries += (n + a.per_entry - 1) / a.per_entry;
+        }
+    }
+    __syncthreads();
+    for (int e = tid; e < a.experts; e += kMoeThreads)
+        for (int done = 0, i = entry[e]; done < count[e]; done += a.per_entry, ++i)
+            a.entries[i] = make_int4(e, place[e] + done, min(count[e] - done, a.per_entry), 0);
+    __syncthreads();
+    for (int s = tid; s < slots; s += kMoeThreads) a.sorted[atomicAdd(&place[__ldcg(a.ids + s)], 1)] = s;
+}
+
+// Whether this block is the last of `n` to come here; what the others wrote before is then visible.
+__device__ __forceinline__ bool last_of(unsigned *arrived, unsigned n) {
+    __shared__ bool last;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        last = atomicAdd(arrived, 1u) == n - 1;
+        if (last) *arrived = 0;
+    }
+    __syncthreads();
+    if (last) __threadfence();
+    return last;
+}
+
+template <typename T, bool WORDS>
+__global__ void __launch_bounds__(kMoeThreads) k_route(const __grid_constant__ MoeArgs a) {
+    dev::wait_for_previous();
+    __shared__ double sums[kMoeWarps][kRouteTokens];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, e = blockIdx.x, t0 = blockIdx.y * kRouteTokens, n = min(a.tokens - t0, kRouteTokens);
+    const T *w = static_cast<const T *>(a.router) + e * a.router_row, *x = static_cast<const T *>(a.x) + t0 * a.x_token;
+    double acc[kRouteTokens] = {};
+    if constexpr (WORDS) {
+        for (int k = 8 * tid; k < a.hidden; k += 8 * kMoeThreads) {
+            const Eight<T> r = load_eight(w + k);
+            double wide[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) wide[i] = dev::widen(r.v[i]);
+#pragma unroll
+            for (int t = 0; t < kRouteTokens; ++t) {
+                if (t >= n) break;
+                const Eight<T> v = load_eight(x + t * a.x_token + k);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) acc[t] = fma(wide[i], static_cast<double>(dev::widen(v.v[i])), acc[t]);
+            }
+        }
+    } else {
+        for (int k = tid; k < a.hidden; k += kMoeThreads) {
+            const double r = dev::widen(w[k]);
+#pragma unroll
+            for (int t = 0; t < kRouteTokens; ++t)
+                if (t < n) acc[t] = fma(r, static_cast<double>(dev::widen(x[t * a.x_token + k])), acc[t]);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < kRouteTokens; ++t) {
+        if (t >= n) break;
+#pragma unroll
+        for (int d = 16; d; d >>= 1) acc[t] += __shfl_xor_sync(0xffffffffu, acc[t], d);
+        if (lane == 0) sums[warp][t] = acc[t];
+    }
+    __syncthreads();
+    if (tid < n) {
+        double s = 0.0;
+#pragma unroll
+        for (int i = 0; i < kMoeWarps; ++i) s += sums[i][tid];
+        a.logits[static_cast<int64_t>(t0 + tid) * a.experts + e] = s;
+    }
+    if (!last_of(a.arrived + 1 + blockIdx.y, gridDim.x)) return;
+    if (warp < n) choose(a, t0 + warp);
+    if (!last_of(a.arrived, gridDim.y)) return;
+    sort_slots(a);
+}
+
+// ---------------------------------------------------------------------------------------------
+// The experts' products.
+//
+// 16 bits: a warp works on 16 rows of a matrix (eight of gate and the same eight of up, or 16 of down) and the slots of an
+// entry, the columns of m16n8k16.  A lane brings 16 bytes of rows g and g + 8 at a time, elements 8t .. 8t + 7 of 32: any order
+// of the sum's terms will do as long as both sides have it, and so no lane needs what another one brought.  Rows go through a
+// ring of shared memory of the lane's own (asynchronous copies, no barrier), which keeps kDepth steps on their way across
+// the ends of items; columns are read from L1 or L2 a step ahead.  Where there are few items, their rows are cut into S
+// parts for as many warps of a block.
+//
+// silu(gate x) (up x) is held to more than 16 bits: for bf16 as two numbers, for fp16 in fp32 and cut into two on the way to
+// the down product, relative to the slot's largest, which only the whole first product knows.
+//
+// 32 bits: a warp works on four rows (two of gate and of up) with the lanes along them, by fused multiply-adds.
+// ---------------------------------------------------------------------------------------------
+
+constexpr int kDepth = 8;                 // steps on their way
+constexpr int kStepBytes = 1024;          // of 16 rows of 64 bytes
+enum { kBy16 = 0, kBy4 = 1, kByElement = 2 };  // how rows come: 16 bytes at a time, 4, or one element
+
+__device__ __forceinline__ uint32_t smem_at(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// 16 bytes of a row, of which `n` elements are real.
+template <typename T, int COPY>
+__device__ __forceinline__ void bring(char *to, const T *from, int n) {
+    constexpr int kEach = 16 / sizeof(T);
+    if constexpr (COPY == kBy16) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_at(to)), "l"(from), "r"(n * static_cast<int>(sizeof(T))) : "memory");
+    } else if constexpr (COPY == kBy4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int have = min(max(n * static_cast<int>(sizeof(T)) - 4 * i, 0), 4);
+            const char *p = have ? reinterpret_cast<const char *>(from) + 4 * i : reinterpret_cast<const char *>(from);
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_at(to + 4 * i)), "l"(p), "r"(have) : "memory");
+        }
+    } else {
+        T v[kEach];
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) v[i] = i < n ? from[i] : dev::narrow<T>(0.0f);
+        memcpy(to, v, 16);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same<T, __half>::value)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The items of a launch, and this group of warps' share of them: entry by entry for gate and up, whose columns are the same for
+// all rows of an entry; tile of rows by tile for down.
+struct Items {
+    int tiles, entries, first, stop;
+    __device__ __forceinline__ void split(int item, bool by_entry, int &entry, int &tile) const {
+        entry = by_entry ? item / tiles : item % entries;
+        tile = by_entry ? item - entry * tiles : item / entries;
+    }
+};
+__device__ __forceinline__ Items items_of(const MoeArgs &a, int tiles, int groups, int group) {
+    Items r;
+    r.tiles = tiles;
+    r.entries = *a.num_entries;
+    const int64_t total = static_cast<int64_t>(tiles) * r.entries;
+    // Even shares to within one item.
+    r.first = static_cast<int>(total * group / groups);
+    r.stop = static_cast<int>(total * (group + 1) / groups);
+    return r;
+}
+
+__device__ __forceinline__ float silu_times(float gate, float up) { return gate / (1.0f + expf(-gate)) * up; }
+
+// The first of two bf16 numbers that add up to a number, in the low half, the second in the upper.  An infinity or a NaN is its
+// first, and no finite number's first is one.
+__device__ __forceinline__ uint32_t two_bf16(float x) {
+    const uint32_t bits = __float_as_uint(x);
+    const bool finite = fabsf(x) <= FLT_MAX;
+    const uint32_t hi = finite ? bits >> 16 : bits >> 16 | ((bits & 0x7fffffu) ? 0x40u : 0u);
+    const __nv_bfloat16 lo = __float2bfloat16_rn(finite ? x - __uint_as_float(bits & 0xffff0000u) : 0.0f);
+    uint16_t low;
+    memcpy(&low, &lo, 2);
+    return hi | static_cast<uint32_t>(low) << 16;
+}
+
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    uint32_t r;
+    memcpy(&r, &h, 4);
+    return r;
+}
+
+// What a slot's numbers are multiplied by before they become fp16: the largest then lies in 2^14 .. 2^15.
+__device__ __forceinline__ float to_half_range(uint32_t largest_bits) {
+    const int exponent = static_cast<int>(largest_bits >> 23);  // 255: not finite
+    if (exponent == 255 || exponent == 0) return exponent ? 1.0f : 0x1p100f;
+    return __uint_as_float(static_cast<uint32_t>(min(127 + 14 - (exponent - 127), 254)) << 23);
+}
+
+// N: eights of columns; DOWN: the second product.  S: warps that share an item.
+template <typename T, int N, bool DOWN, int COPY>
+__global__ void __launch_bounds__(kMoeThreads, 2) k_experts(const __grid_constant__ MoeArgs a, int S) {
+    extern __shared__ __align__(128) char smem[];
+    dev::wait_for_previous();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int K = DOWN ? a.inner : a.hidden, rows = DOWN ? a.hidden : a.inner, per_tile = DOWN ? 16 : 8;
+    const int part = warp % S, groups = kMoeWarps / S, group = warp / S;
+    const Items items = items_of(a, (rows + per_tile - 1) / per_tile, gridDim.x * groups, blockIdx.x * groups + group);
+    // This warp's part of K, in steps of 32.
+    const int steps = (K + 31) / 32, each = (steps + S - 1) / S, k_first = min(part * each, steps) * 32, k_stop = min((part + 1) * each, steps) * 32;
+    char *ring = smem + warp * kDepth * kStepBytes + lane * 16;
+    float *meet = reinterpret_cast<float *>(smem + kMoeWarps * kDepth * kStepBytes);  // [warp][4 N][lane]
+
+    // What is brought next.
+    int item = items.first, k = k_first;
+    const T *p0 = nullptr, *p1 = nullptr;
+    bool in0 = false, in1 = false;
+    auto point = [&] {
+        int at, tile;
+        items.split(item, !DOWN, at, tile);
+        const int expert = a.entries[at].x;
+        if constexpr (DOWN) {
+            const int r0 = tile * 16 + g;
+            in0 = r0 < rows;
+            in1 = r0 + 8 < rows;
+            const T *w = static_cast<const T *>(a.down) + expert * a.down_expert;
+            p0 = in0 ? w + r0 * a.down_row : w;
+            p1 = in1 ? w + (r0 + 8) * a.down_row : w;
+        } else {
+            const int r = tile * 8 + g;
+            in0 = in1 = r < rows;
+            p0 = static_cast<const T *>(a.gate) + expert * a.gate_expert + (in0 ? r * a.gate_row : 0);
+            p1 = static_cast<const T *>(a.up) + expert * a.up_expert + (in1 ? r * a.up_row : 0);
+        }
+    };
+    int stage_in = 0;
+    auto bring_step = [&] {
+        if (item < items.stop && k_first < k_stop) {
+            const int at = k + 8 * t, n = min(max(K - at, 0), 8);
+            char *to = ring + stage_in * kStepBytes;
+            bring<T, COPY>(to, p0 + (in0 && n ? at : 0), in0 ? n : 0);
+            bring<T, COPY>(to + 512, p1 + (in1 && n ? at : 0), in1 ? n : 0);
+            k += 32;
+            if (k >= k_stop) {
+                k = k_first;
+                ++item;
+                if (item < items.stop) point();
+            }
+        }
+        copy_commit();
+        stage_in = stage_in + 1 == kDepth ? 0 : stage_in + 1;
+    };
+    if (item < items.stop) point();
+#pragma unroll 1
+    for (int i = 0; i < kDepth - 1; ++i) bring_step();
+
+    int stage = 0;
+#pragma unroll 1
+    for (int now = items.first; now < items.stop; ++now) {
+        int at, tile;
+        items.split(now, !DOWN, at, tile);
+        const int4 entry = a.entries[at];
+        // This lane's columns of B, and what makes them fp16.
+        const void *column[N];
+        float factor[N];
+        uint32_t low_mask[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            column[j] = nullptr;
+            factor[j] = 1.0f;
+            low_mask[j] = 0xffffffffu;
+            if (8 * j + g < entry.z) {
+                const int slot = a.sorted[entry.y + 8 * j + g];
+                if constexpr (DOWN) {
+                    column[j] = a.inner_out + slot * a.inner_row;
+                    if constexpr (std::is_same<T, __half>::value) {
+                        const uint32_t bits = a.largest[slot];
+                        factor[j] = to_half_range(bits);
+                        if (bits >= 0x7f800000u) low_mask[j] = 0;
+                    }
+                } else {
+                    column[j] = static_cast<const T *>(a.x) + slot / a.top * a.x_token;
+                }
+            }
+        }
+        float acc[N][4] = {};
+#pragma unroll 2
+        for (int kk = k_first; kk < k_stop; kk += 32) {
+            copy_wait<kDepth - 2>();
+            const char *from = ring + stage * kStepBytes;
+            const uint4 r0 = *reinterpret_cast<const uint4 *>(from), r1 = *reinterpret_cast<const uint4 *>(from + 512);
+            bring_step();  // into the stage before, which this lane read in the step before
+            stage = stage + 1 == kDepth ? 0 : stage + 1;
+            const int at_k = kk + 8 * t;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                if (8 * j >= entry.z) break;
+                if constexpr (!DOWN) {
+                    uint4 c = make_uint4(0, 0, 0, 0);
+                    if (column[j]) {
+                        const T *p = static_cast<const T *>(column[j]) + at_k;
+                        if constexpr (COPY == kBy16) {
+                            if (at_k < K) c = *reinterpret_cast<const uint4 *>(p);
+                        } else {
+                            T v[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) v[i] = at_k + i < K ? p[i] : dev::narrow<T>(0.0f);
+                            memcpy(&c, v, 16);
+                        }
+                    }
+                    mma<T>(acc[j], r0.x, r1.x, r0.y, r1.y, c.x, c.y);
+                    mma<T>(acc[j], r0.z, r1.z, r0.w, r1.w, c.z, c.w);
+                } else {
+                    uint4 u = make_uint4(0, 0, 0, 0), v = u;
+                    if (column[j]) {
+                        const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const uint32_t *>(column[j]) + at_k);
+                        u = p[0];
+                        v = p[1];
+                    }
+                    uint32_t hi[4], lo[4];
+                    if constexpr (std::is_same<T, __half>::value) {
+                        const uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float x = __uint_as_float(w[2 * i]) * factor[j], y = __uint_as_float(w[2 * i + 1]) * factor[j];
+                            hi[i] = pack_half(x, y);
+                            __half2 h;
+                            memcpy(&h, &hi[i], 4);
+                            lo[i] = pack_half(x - __low2float(h), y - __high2float(h)) & low_mask[j];
+                        }
+                    } else {
+                        const uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            hi[i] = __byte_perm(w[2 * i], w[2 * i + 1], 0x5410);
+                            lo[i] = __byte_perm(w[2 * i], w[2 * i + 1], 0x7632);
+                        }
+                    }
+                    mma<T>(acc[j], r0.x, r1.x, r0.y, r1.y, hi[0], hi[1]);
+                    mma<T>(acc[j], r0.z, r1.z, r0.w, r1.w, hi[2], hi[3]);
+                    mma<T>(acc[j], r0.x, r1.x, r0.y, r1.y, lo[0], lo[1]);
+                    mma<T>(acc[j], r0.z, r1.z, r0.w, r1.w, lo[2], lo[3]);
+                }
+            }
+        }
+        // The parts' sums meet, in their order, in the group's first warp.
+        if (S > 1) {
+            const int bar = 1 + group;
+            asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(32 * S) : "memory");  // the item before is done with
+            if (part) {
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) meet[(warp * 4 * N + 4 * j + e) * 32 + lane] = acc[j][e];
+            }
+            asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(32 * S) : "memory");
+            if (part) continue;
+            for (int p = 1; p < S; ++p)
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[j][e] += meet[((warp + p) * 4 * N + 4 * j + e) * 32 + lane];
+        }
+        // Columns 2 t and 2 t + 1 of rows g and g + 8.
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            if (8 * j >= entry.z) break;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int c = 8 * j + 2 * t + e;
+                const int slot = c < entry.z ? a.sorted[entry.y + c] : 0;
+                if constexpr (DOWN) {
+                    float back = 1.0f;
+                    if constexpr (std::is_same<T, __half>::value) back = 1.0f / to_half_range(a.largest[slot]);
+                    float *to = a.part + static_cast<int64_t>(slot) * a.hidden + tile * 16 + g;
+                    if (c < entry.z && tile * 16 + g < rows) to[0] = acc[j][e] * back;
+                    if (c < entry.z && tile * 16 + g + 8 < rows) to[8] = acc[j][2 + e] * back;
+                } else {
+                    const int r = tile * 8 + g;
+                    const bool real = c < entry.z && r < rows;
+                    const float h = real ? silu_times(acc[j][e], acc[j][2 + e]) : 0.0f;
+                    if constexpr (std::is_same<T, __half>::value) {
+                        uint32_t top = __float_as_uint(h) & 0x7fffffffu;
+#pragma unroll
+                        for (int d = 4; d < 32; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+                        if (g == 0 && c < entry.z && top) atomicMax(a.largest + slot, top);
+                        if (real) a.inner_out[slot * a.inner_row + r] = __float_as_uint(h);
+                    } else {
+                        if (real) a.inner_out[slot * a.inner_row + r] = two_bf16(h);
+                    }
+                }
+            }
+        }
+    }
+}
+
+// The same of 32 bits: rows 0 and 1 of gate and 2 and 3 of up, or four of down, up to eight columns.
+template <bool DOWN, int COPY>
+__global__ void __launch_bounds__(kMoeThreads, 2) k_experts32(const __grid_constant__ MoeArgs a, int S) {
+    extern __shared__ __align__(128) char smem[];
+    dev::wait_for_previous();
+    constexpr int kDepth32 = kDepth / 2, kBytes = 2 * kStepBytes;  // of four rows of 512 bytes
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int K = DOWN ? a.inner : a.hidden, rows = DOWN ? a.hidden : a.inner, per_tile = DOWN ? 4 : 2;
+    const int part = warp % S, groups = kMoeWarps / S, group = warp / S;
+    const Items items = items_of(a, (rows + per_tile - 1) / per_tile, gridDim.x * groups, blockIdx.x * groups + group);
+    const int steps = (K + 127) / 128, each = (steps + S - 1) / S, k_first = min(part * each, steps) * 128, k_stop = min((part + 1) * each, steps) * 128;
+    char *ring = smem + warp * kDepth32 * kBytes + lane * 16;
+    float *meet = reinterpret_cast<float *>(smem + kMoeWarps * kDepth32 * kBytes);  // [warp][lane]
+
+    int item = items.first, k = k_first;
+    const float *p[4] = {};
+    uint32_t in = 0;
+    auto point = [&] {
+        int at, tile;
+        items.split(item, !DOWN, at, tile);
+        const int expert = a.entries[at].x;
+        in = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = tile * per_tile + (DOWN ? i : i & 1);
+            const float *w = DOWN ? static_cast<const float *>(a.down) + expert * a.down_expert
+                             : i < 2 ? static_cast<const float *>(a.gate) + expert * a.gate_expert : static_cast<const float *>(a.up) + expert * a.up_expert;
+            const int64_t row = DOWN ? a.down_row : i < 2 ? a.gate_row : a.up_row;
+            p[i] = w;
+            if (r < rows) {
+                p[i] += r * row;
+                in |= 1u << i;
+            }
+        }
+    };
+    int stage_in = 0;
+    auto bring_step = [&] {
+        if (item < items.stop && k_first < k_stop) {
+            const int at = k + 4 * lane, n = min(max(K - at, 0), 4);
+            char *to = ring + stage_in * kBytes;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bool real = (in >> i & 1) && n;
+                bring<float, COPY>(to + 512 * i, p[i] + (real ? at : 0), real ? n : 0);
+            }
+            k += 128;
+            if (k >= k_stop) {
+                k = k_first;
+                ++item;
+                if (item < items.stop) point();
+            }
+        }
+        copy_commit();
+        stage_in = stage_in + 1 == kDepth32 ? 0 : stage_in + 1;
+    };
+    if (item < items.stop) point();
+#pragma unroll 1
+    for (int i = 0; i < kDepth32 - 1; ++i) bring_step();
+
+    int stage = 0;
+#pragma unroll 1
+    for (int now = items.first; now < items.stop; ++now) {
+        int at, tile;
+        items.split(now, !DOWN, at, tile);
+        const int4 entry = a.entries[at];
+        const float *column[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            const int slot = a.sorted[entry.y + min(c, entry.z - 1)];
+            column[c] = DOWN ? reinterpret_cast<const float *>(a.inner_out) + slot * a.inner_row : static_cast<const float *>(a.x) + slot / a.top * a.x_token;
+        }
+        float acc[32] = {};  // [row][column]
+#pragma unroll 1
+        for (int kk = k_first; kk < k_stop; kk += 128) {
+            copy_wait<kDepth32 - 2>();
+            const char *from = ring + stage * kBytes;
+            float4 w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const float4 *>(from + 512 * i);
+            bring_step();
+            stage = stage + 1 == kDepth32 ? 0 : stage + 1;
+            const int at_k = kk + 4 * lane;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                if (c >= entry.z) break;
+                float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                const float *q = column[c] + at_k;
+                if constexpr (DOWN || COPY == kBy16) {  // rows of the scratch are padded with zeros
+                    if (at_k < K) x = *reinterpret_cast<const float4 *>(q);
+                } else {
+                    if (at_k < K) x.x = q[0];
+                    if (at_k + 1 < K) x.y = q[1];
+                    if (at_k + 2 < K) x.z = q[2];
+                    if (at_k + 3 < K) x.w = q[3];
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float s = acc[8 * i + c];
+                    s = fmaf(w[i].x, x.x, s);
+                    s = fmaf(w[i].y, x.y, s);
+                    s = fmaf(w[i].z, x.z, s);
+                    acc[8 * i + c] = fmaf(w[i].w, x.w, s);
+                }
+            }
+        }
+        // Lane l gets the sum of row l / 8 and column l % 8: halves exchanged until one is left.
+#pragma unroll
+        for (int d = 16; d; d >>= 1) {
+            const bool upper = lane & d;
+#pragma unroll
+            for (int i = 0; i < d; ++i) {
+                const float give = upper ? acc[i] : acc[i + d], keep = upper ? acc[i + d] : acc[i];
+                acc[i] = keep + __shfl_xor_sync(0xffffffffu, give, d);
+            }
+        }
+        float s = acc[0];
+        if (S > 1) {
+            const int bar = 1 + group;
+            asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(32 * S) : "memory");
+            if (part) meet[warp * 32 + lane] = s;
+            asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(32 * S) : "memory");
+            if (part) continue;
+            for (int i = 1; i < S; ++i) s += meet[(warp + i) * 32 + lane];
+        }
+        const int c = lane % 8, row = lane / 8;
+        if constexpr (DOWN) {
+            if (c < entry.z && tile * 4 + row < rows) a.part[static_cast<int64_t>(a.sorted[entry.y + c]) * a.hidden + tile * 4 + row] = s;
+        } else {
+            const float up = __shfl_down_sync(0xffffffffu, s, 16);
+            if (row < 2 && c < entry.z && tile * 2 + row < rows)
+                a.inner_out[a.sorted[entry.y + c] * a.inner_row + tile * 2 + row] = __float_as_uint(silu_times(s, up));
+        }
+    }
+}
+
+// The sum over a token's slots.
+template <typename T>
+__global__ void __launch_bounds__(kMoeThreads) k_combine(const __grid_constant__ MoeArgs a) {
+    dev::wait_for_previous();
+    const int h = blockIdx.x * kMoeThreads + threadIdx.x, t = blockIdx.y;
+    if (h >= a.hidden) return;
+    const float *part = a.part + static_cast<int64_t>(t) * a.top * a.hidden + h, *w = a.weights + t * a.top;
+    float y = 0.0f;
+    for (int k0 = 0; k0 < a.top; k0 += 4) {
+        float v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = k0 + k < a.top ? part[static_cast<int64_t>(k0 + k) * a.hidden] : 0.0f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (k0 + k < a.top) y = fmaf(w[k0 + k], v[k], y);
+    }
+    static_cast<T *>(a.y)[t * a.y_token + h] = dev::narrow<T>(y);
+}
+
+struct MoeKernels {
+    void (*route)(MoeArgs);
+    void (*gate_up)(MoeArgs, int);
+    void (*down)(MoeArgs, int);
+    void (*combine)(MoeArgs);
+    int smem;
+};
+
+template <typename T, int N>
+int experts_smem() {
+    return kMoeWarps * (kDepth * kStepBytes + (sizeof(T) == 4 ? 128 : 4 * N * 128));
+}
+
+template <typename T, int N, int COPY>
+void (*pick_experts(bool down))(MoeArgs, int) {
+    if constexpr (sizeof(T) == 4) return down ? k_experts32<true, COPY> : k_experts32<false, COPY>;
+    else return down ? k_experts<T, N, true, COPY> : k_experts<T, N, false, COPY>;
+}
+
+template <typename T, int N>
+void (*pick_copy(bool down, int copy))(MoeArgs, int) {
+    if (copy == kBy16) return pick_experts<T, N, kBy16>(down);
+    if (copy == kBy4 || sizeof(T) == 4) return pick_experts<T, N, kBy4>(down);
+    return pick_experts<T, N, sizeof(T) == 4 ? kBy4 : kByElement>(down);
+}
+
+template <typename T, int N>
+MoeKernels moe_kernels(bool route_words, int copy_up, int copy_down) {
+    return {route_words ? k_route<T, true> : k_route<T, false>, pick_copy<T, N>(false, copy_up), pick_copy<T, N>(true, copy_down), k_combine<T>,
+            experts_smem<T, N>()};
+}
+
+template <typename T>
+MoeKernels pick_moe(int eights, bool route_words, int copy_up, int copy_down) {
+    if constexpr (sizeof(T) == 4) return moe_kernels<T, 1>(route_words, copy_up, copy_down);
+    else
+        return eights == 1   ? moe_kernels<T, 1>(route_words, copy_up, copy_down)
+               : eights == 2 ? moe_kernels<T, 2>(route_words, copy_up, copy_down)
+                             : moe_kernels<T, 4>(route_words, copy_up, copy_down);
+}
+
+}  // namespace l2d
+
+using namespace l2d;
+
+struct l2d_moe_plan {
+    l2d_moe_desc desc;
+    int sms;
+    MoeArgs args;
+    void *memory;
+    void (*allowed[2])(MoeArgs, int);  // the kernels whose shared memory limit was raised last
+};
+
+namespace l2d {
+
+// How rows of a matrix can be brought: by what they and their strides are aligned to.
+int copy_of(const void *p, int64_t row, int64_t expert, int eb) {
+    const uintptr_t any = reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(row * eb) | static_cast<uintptr_t>(expert * eb);
+    return any % 16 == 0 ? kBy16 : any % 4 == 0 ? kBy4 : kByElement;
+}
+
+// Warps that share an item: as few as leave every warp of the GPU one.
+int parts_of(int64_t items, int warps, int steps) {
+    int s = 1;
+    while (s < kMoeWarps && items * s < warps && steps >= 4 * s) s *= 2;
+    return s;
+}
+
+}  // namespace l2d
+
+extern "C" {
+
+int l2d_moe_plan_create(const l2d_moe_desc *desc, l2d_moe_plan **plan) {
+    if (!plan) return set_error(L2D_ERR_INVALID, "null plan pointer");
+    *plan = nullptr;
+    if (!desc) return set_error(L2D_ERR_INVALID, "null descriptor");
+    l2d_moe_desc d = *desc;
+    if (!valid_dtype(d.dtype)) return set_error(L2D_ERR_INVALID, "bad dtype %d", d.dtype);
+    constexpr int64_t kMost = 1 << 24;
+    if (d.hidden < 1 || d.hidden > kMost || d.inner < 1 || d.inner > kMost)
+        return set_error(L2D_ERR_INVALID, "hidden %lld and inner %lld: 1 to 2^24 are supported", static_cast<long long>(d.hidden), static_cast<long long>(d.inner));
+    if (d.experts < 1 || d.experts > kMaxExperts) return set_error(L2D_ERR_UNSUPPORTED, "%d experts: 1 to %d are supported", d.experts, kMaxExperts);
+    if (d.top < 1 || d.top > d.experts || d.top > 32) return set_error(L2D_ERR_UNSUPPORTED, "top %d of %d experts: 1 to 32 are supported", d.top, d.experts);
+    if (d.max_tokens < 1 || d.max_tokens > 65535) return set_error(L2D_ERR_INVALID, "max_tokens %d: 1 to 65535 are supported", d.max_tokens);
+    if (!d.x_token) d.x_token = d.hidden;
+    if (!d.y_token) d.y_token = d.hidden;
+    if (!d.router_row) d.router_row = d.hidden;
+    if (!d.gate_row) d.gate_row = d.hidden;
+    if (!d.up_row) d.up_row = d.hidden;
+    if (!d.down_row) d.down_row = d.inner;
+    const int64_t least = std::min({d.x_token, d.y_token, d.router_row, d.gate_row, d.up_row});
+    if (least < d.hidden || d.down_row < d.inner) return set_error(L2D_ERR_INVALID, "a stride is shorter than its row");
+    if (std::max({d.x_token, d.y_token, d.router_row, d.gate_row, d.up_row, d.down_row}) > (int64_t(1) << 32)) return set_error(L2D_ERR_INVALID, "strides too large");
+    if (!d.gate_expert) d.gate_expert = d.gate_row * d.inner;
+    if (!d.up_expert) d.up_expert = d.up_row * d.inner;
+    if (!d.down_expert) d.down_expert = d.down_row * d.hidden;
+    // Experts of one matrix after the other, or row by row beside another's: no row may lie in two.
+    if (std::min({d.gate_expert, d.up_expert}) < d.hidden || d.down_expert < d.inner)
+        return set_error(L2D_ERR_INVALID, "experts' strides are shorter than a row");
+    if (std::max({d.gate_expert, d.up_expert, d.down_expert}) > (int64_t(1) << 48)) return set_error(L2D_ERR_INVALID, "strides too large");
+    if (!d.router || !d.gate || !d.up || !d.down) return set_error(L2D_ERR_INVALID, "null pointer");
+    const int eb = elem_bytes(d.dtype);
+    if (misaligned(d.router, eb) || misaligned(d.gate, eb) || misaligned(d.up, eb) || misaligned(d.down, eb))
+        return set_error(L2D_ERR_INVALID, "pointers must be aligned to their elements");
+    const int64_t slots = int64_t(d.max_tokens) * d.top, inner_row = (d.inner + 127) / 128 * 128;
+    if (int64_t(std::max(d.hidden, d.inner)) * std::min<int64_t>(slots, d.experts + slots / 8) > INT32_MAX)
+        return set_error(L2D_ERR_INVALID, "rows of all experts' entries must stay below 2^31");
+    int sms = 0;
+    int st = device_sms(d.device, &sms);
+    if (st != L2D_OK) return st;
+    OnDevice on(d.device);
+    L2D_CUDA_TRY(on.err);
+    // Sixteen-byte rows of numbers first.
+    size_t bytes = 0;
+    auto take = [&](size_t n) {
+        const size_t at = bytes;
+        bytes += (n + 255) / 256 * 256;
+        return at;
+    };
+    const size_t tiles = (d.max_tokens + kRouteTokens - 1) / kRouteTokens, entries = d.experts + slots / 8 + 1;
+    const size_t inner_at = take(slots * inner_row * 4), part_at = take(slots * d.hidden * 4), logits_at = take(size_t(d.max_tokens) * d.experts * 8),
+                 ids_at = take(slots * 4), weights_at = take(slots * 4), largest_at = take(slots * 4), sorted_at = take(slots * 4),
+                 entries_at = take(entries * 16), num_at = take(4), arrived_at = take((tiles + 1) * 4);
+    void *memory = nullptr;
+    L2D_CUDA_TRY(cudaMalloc(&memory, bytes));
+    // Counters, and what pads the rows of inner_out, on a stream of their own, so that nothing else on the device is waited for.
+    cudaStream_t own = nullptr;
+    cudaError_t e = cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking);
+    if (e == cudaSuccess) {
+        e = cudaMemsetAsync(memory, 0, bytes, own);
+        if (e == cudaSuccess) e = cudaStreamSynchronize(own);
+        cudaStreamDestroy(own);
+    }
+    l2d_moe_plan *p = e == cudaSuccess ? new (std::nothrow) l2d_moe_plan() : nullptr;
+    if (!p) {
+        cudaFree(memory);
+        return e != cudaSuccess ? set_error(L2D_ERR_CUDA, "experts' scratch: %s", cudaGetErrorString(e)) : set_error(L2D_ERR_INVALID, "out of host memory");
+    }
+    char *base = static_cast<char *>(memory);
+    p->desc = d;
+    p->sms = sms;
+    p->memory = memory;
+    MoeArgs &a = p->args;
+    a.router = d.router;
+    a.gate = d.gate;
+    a.up = d.up;
+    a.down = d.down;
+    a.x_token = d.x_token;
+    a.y_token = d.y_token;
+    a.router_row = d.router_row;
+    a.gate_row = d.gate_row;
+    a.up_row = d.up_row;
+    a.down_row = d.down_row;
+    a.gate_expert = d.gate_expert;
+    a.up_expert = d.up_expert;
+    a.down_expert = d.down_expert;
+    a.hidden = static_cast<int>(d.hidden);
+    a.inner = static_cast<int>(d.inner);
+    a.experts = d.experts;
+    a.top = d.top;
+    a.normalize = d.normalize;
+    a.inner_out = reinterpret_cast<uint32_t *>(base + inner_at);
+    a.part = reinterpret_cast<float *>(base + part_at);
+    a.logits = reinterpret_cast<double *>(base + logits_at);
+    a.ids = reinterpret_cast<int *>(base + ids_at);
+    a.weights = reinterpret_cast<float *>(base + weights_at);
+    a.largest = reinterpret_cast<uint32_t *>(base + largest_at);
+    a.sorted = reinterpret_cast<int *>(base + sorted_at);
+    a.entries = reinterpret_cast<int4 *>(base + entries_at);
+    a.num_entries = reinterpret_cast<int *>(base + num_at);
+    a.arrived = reinterpret_cast<unsigned *>(base + arrived_at);
+    a.inner_row = inner_row;
+    *plan = p;
+    return L2D_OK;
+}
+
+int l2d_moe_forward(l2d_moe_plan *p, const void *x, void *y, int32_t *ids, float *weights, int tokens, void *stream) {
+    if (!p) return set_error(L2D_ERR_INVALID, "null plan");
+    const l2d_moe_desc &d = p->desc;
+    if (tokens < 0 || tokens > d.max_tokens) return set_error(L2D_ERR_INVALID, "%d tokens of at most %d", tokens, d.max_tokens);
+    if (tokens == 0) return L2D_OK;
+    if (!x || !y) return set_error(L2D_ERR_INVALID, "null pointer");
+    const int eb = elem_bytes(d.dtype);
+    if (misaligned(x, eb) || misaligned(y, eb) || misaligned(ids, 4) || misaligned(weights, 4))
+        return set_error(L2D_ERR_INVALID, "pointers must be aligned to their elements");
+    OnDevice on(d.device);
+    L2D_CUDA_TRY(on.err);
+    MoeArgs a = p->args;
+    a.x = x;
+    a.y = y;
+    a.ids_out = ids;
+    a.weights_out = weights;
+    a.tokens = tokens;
+    // An expert has at most `tokens` slots.
+    const int eights = eb == 4 || tokens <= 8 ? 1 : tokens <= 16 ? 2 : 4;
+    a.per_entry = 8 * eights;
+    const int x_copy = copy_of(x, d.x_token, 0, eb), whole = d.hidden % (16 / eb) == 0 ? kBy16 : kBy4;
+    const int copy_up = std::max({copy_of(d.gate, d.gate_row, d.gate_expert, eb), copy_of(d.up, d.up_row, d.up_expert, eb), std::min<int>(std::max(x_copy, whole), kBy4)});
+    const int copy_down = copy_of(d.down, d.down_row, d.down_expert, eb);
+    const bool route_words = x_copy == kBy16 && d.hidden % 8 == 0 && copy_of(d.router, d.router_row, 0, eb) == kBy16;
+    const MoeKernels k = d.dtype == L2D_F32   ? pick_moe<float>(eights, route_words, copy_up, copy_down)
+                         : d.dtype == L2D_F16 ? pick_moe<__half>(eights, route_words, copy_up, copy_down)
+                                              : pick_moe<__nv_bfloat16>(eights, route_words, copy_up, copy_down);
+    L2D_CUDA_TRY(launch(k.route, dim3(d.experts, (tokens + kRouteTokens - 1) / kRouteTokens), kMoeThreads, 0, stream, a));
+    const int up_rows = eb == 4 ? 2 : 8, down_rows = eb == 4 ? 4 : 16, step = eb == 4 ? 128 : 32;
+    const int64_t entries = std::min<int64_t>(int64_t(tokens) * d.top, d.experts);
+    const int blocks = 2 * p->sms, warps = blocks * kMoeWarps;
+    const int s_up = parts_of(entries * ((d.inner + up_rows - 1) / up_rows), warps, static_cast<int>((d.hidden + step - 1) / step));
+    const int s_down = parts_of(entries * ((d.hidden + down_rows - 1) / down_rows), warps, static_cast<int>((d.inner + step - 1) / step));
+    if (p->allowed[0] != k.gate_up) L2D_CUDA_TRY(cudaFuncSetAttribute(k.gate_up, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem));
+    if (p->allowed[1] != k.down) L2D_CUDA_TRY(cudaFuncSetAttribute(k.down, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem));
+    p->allowed[0] = k.gate_up;
+    p->allowed[1] = k.down;
+    L2D_CUDA_TRY(launch(k.gate_up, dim3(blocks), kMoeThreads, k.smem, stream, a, s_up));
+    L2D_CUDA_TRY(launch(k.down, dim3(blocks), kMoeThreads, k.smem, stream, a, s_down));
+    L2D_CUDA_TRY(launch(k.combine, dim3((a.hidden + kMoeThreads - 1) / kMoeThreads, tokens), kMoeThreads, 0, stream, a));
+    return L2D_OK;
+}
+
+int l2d_moe_plan_destroy(l2d_moe_plan *p) {
+    if (!p) return L2D_OK;
+    OnDevice on(p->desc.device);
+    cudaError_t e = cudaFree(p->memory);  // waits for the device
+    delete p;
+    if (e != cudaSuccess) return set_error(L2D_ERR_CUDA, "moe_plan_destroy: %s", cudaGetErrorString(e));
+    return L2D_OK;
+}
+
+}  // extern "C"
