@@ -64,9 +64,9 @@ __device__ __forceinline__ Eight<T> load_eight(const T *p) {
     return r;
 }
 
-// Chooses the experts of one token: a warp, `top` rounds over up to kMaxExperts / 32 scores a lane.
+// Chooses the experts of one token: a warp, `top` rounds over kEach scores a lane.
+template <int kEach>
 __device__ __forceinline__ void choose(const MoeArgs &a, int token) {
-    constexpr int kEach = kMaxExperts / 32;
     const int lane = threadIdx.x & 31;
     const double *logits = a.logits + static_cast<int64_t>(token) * a.experts;
     double v[kEach];
@@ -136,8 +136,8 @@ __device__ __forceinline__ void sort_slots(const MoeArgs &a) {
     __syncthreads();
     for (int s = tid; s < slots; s += kMoeThreads) atomicAdd(&count[__ldcg(a.ids + s)], 1);
     __syncthreads();
-    if (tid < 32) {  // places and entries before each expert's: 16 experts a lane
-        constexpr int kEach = kMaxExperts / 32;
+    if (tid < 32) {  // places and entries before each expert's: as many experts a lane
+        const int kEach = (a.experts + 31) / 32;
         int here = 0, entries = 0;
         for (int i = 0; i < kEach; ++i) {
             const int n = count[tid * kEach + i];
@@ -227,8 +227,16 @@ __global__ void __launch_bounds__(kMoeThreads) k_route(const __grid_constant__ M
         a.logits[static_cast<int64_t>(t0 + tid) * a.experts + e] = s;
     }
     if (!last_of(a.arrived + 1 + blockIdx.y, gridDim.x)) return;
-    if (warp < n) choose(a, t0 + warp);
-    if (!last_of(a.arrived, gridDim.y)) return;
+    if (warp < n) {
+        if (a.experts <= 32) choose<1>(a, t0 + warp);
+        else if (a.experts <= 128) choose<4>(a, t0 + warp);
+        else choose<kMaxExperts / 32>(a, t0 + warp);
+    }
+    if (gridDim.y > 1) {
+        if (!last_of(a.arrived, gridDim.y)) return;
+    } else {
+        __syncthreads();
+    }
     sort_slots(a);
 }
 
@@ -248,8 +256,9 @@ __global__ void __launch_bounds__(kMoeThreads) k_route(const __grid_constant__ M
 // 32 bits: a warp works on four rows (two of gate and of up) with the lanes along them, by fused multiply-adds.
 // ---------------------------------------------------------------------------------------------
 
-constexpr int kDepth = 8;                 // steps on their way
-constexpr int kStepBytes = 1024;          // of 16 rows of 64 bytes
+constexpr int kDepth = 4;                 // steps in a ring, all but one of them on their way
+constexpr int kStepBytes = 2048;          // of 16 rows of 128 bytes, or four of 512
+constexpr int kCached = 128, kCachedSlots = 1024;  // entries and slots that a block keeps in shared memory
 enum { kBy16 = 0, kBy4 = 1, kByElement = 2 };  // how rows come: 16 bytes at a time, 4, or one element
 
 __device__ __forceinline__ uint32_t smem_at(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -337,150 +346,221 @@ __device__ __forceinline__ float to_half_range(uint32_t largest_bits) {
     return __uint_as_float(static_cast<uint32_t>(min(127 + 14 - (exponent - 127), 254)) << 23);
 }
 
+// The entries and the slots behind them: a block's own copy where they are few.
+struct Lists {
+    const int4 *entries;
+    const int *sorted;
+};
+__device__ __forceinline__ Lists lists_of(const MoeArgs &a, int entries) {
+    __shared__ int4 kept_entries[kCached];
+    __shared__ int kept_sorted[kCachedSlots];
+    const int slots = a.tokens * a.top;
+    if (entries > kCached || slots > kCachedSlots) return {a.entries, a.sorted};
+    for (int i = threadIdx.x; i < entries; i += kMoeThreads) kept_entries[i] = a.entries[i];
+    for (int i = threadIdx.x; i < slots; i += kMoeThreads) kept_sorted[i] = a.sorted[i];
+    __syncthreads();
+    return {kept_entries, kept_sorted};
+}
+
 // N: eights of columns; DOWN: the second product.  S: warps that share an item.
 template <typename T, int N, bool DOWN, int COPY>
 __global__ void __launch_bounds__(kMoeThreads, 2) k_experts(const __grid_constant__ MoeArgs a, int S) {
+    constexpr bool kHalf = std::is_same<T, __half>::value;
+    constexpr bool kAhead = DOWN ? N == 1 : N <= 2;  // columns are read a step ahead where registers hold them
+    constexpr int kK = 64;                           // elements of a step: two runs of 32
     extern __shared__ __align__(128) char smem[];
     dev::wait_for_previous();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int K = DOWN ? a.inner : a.hidden, rows = DOWN ? a.hidden : a.inner, per_tile = DOWN ? 16 : 8;
     const int part = warp % S, groups = kMoeWarps / S, group = warp / S;
     const Items items = items_of(a, (rows + per_tile - 1) / per_tile, gridDim.x * groups, blockIdx.x * groups + group);
-    // This warp's part of K, in steps of 32.
-    const int steps = (K + 31) / 32, each = (steps + S - 1) / S, k_first = min(part * each, steps) * 32, k_stop = min((part + 1) * each, steps) * 32;
+    const Lists lists = lists_of(a, items.entries);
+    // This warp's part of K.  Only the last step of all may be short.
+    const int all = (K + kK - 1) / kK, each = (all + S - 1) / S, begin = min(part * each, all), steps = min(begin + each, all) - begin;
+    const bool short_end = begin + steps == all && K % kK;
+    const int n_end[2] = {min(max(K - (all - 1) * kK - 8 * t, 0), 8), min(max(K - (all - 1) * kK - 32 - 8 * t, 0), 8)};
+    const int first_k = begin * kK + 8 * t;
     char *ring = smem + warp * kDepth * kStepBytes + lane * 16;
     float *meet = reinterpret_cast<float *>(smem + kMoeWarps * kDepth * kStepBytes);  // [warp][4 N][lane]
 
-    // What is brought next.
-    int item = items.first, k = k_first;
+    // What is brought next: rows g and g + 8 from p0 and p1 on, `left` steps of them.
+    int item = items.first, left = 0, in_at = 0;
     const T *p0 = nullptr, *p1 = nullptr;
     bool in0 = false, in1 = false;
     auto point = [&] {
         int at, tile;
         items.split(item, !DOWN, at, tile);
-        const int expert = a.entries[at].x;
+        const int expert = lists.entries[at].x;
         if constexpr (DOWN) {
             const int r0 = tile * 16 + g;
             in0 = r0 < rows;
             in1 = r0 + 8 < rows;
             const T *w = static_cast<const T *>(a.down) + expert * a.down_expert;
-            p0 = in0 ? w + r0 * a.down_row : w;
-            p1 = in1 ? w + (r0 + 8) * a.down_row : w;
+            p0 = w + (in0 ? r0 * a.down_row + first_k : 0);
+            p1 = w + (in1 ? (r0 + 8) * a.down_row + first_k : 0);
         } else {
             const int r = tile * 8 + g;
             in0 = in1 = r < rows;
-            p0 = static_cast<const T *>(a.gate) + expert * a.gate_expert + (in0 ? r * a.gate_row : 0);
-            p1 = static_cast<const T *>(a.up) + expert * a.up_expert + (in1 ? r * a.up_row : 0);
+            p0 = static_cast<const T *>(a.gate) + expert * a.gate_expert + (in0 ? r * a.gate_row + first_k : 0);
+            p1 = static_cast<const T *>(a.up) + expert * a.up_expert + (in1 ? r * a.up_row + first_k : 0);
         }
+        left = steps;
     };
-    int stage_in = 0;
     auto bring_step = [&] {
-        if (item < items.stop && k_first < k_stop) {
-            const int at = k + 8 * t, n = min(max(K - at, 0), 8);
-            char *to = ring + stage_in * kStepBytes;
-            bring<T, COPY>(to, p0 + (in0 && n ? at : 0), in0 ? n : 0);
-            bring<T, COPY>(to + 512, p1 + (in1 && n ? at : 0), in1 ? n : 0);
-            k += 32;
-            if (k >= k_stop) {
-                k = k_first;
-                ++item;
-                if (item < items.stop) point();
+        if (left) {
+            char *to = ring + in_at;
+            const bool end = short_end && left == 1;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int n = end ? n_end[h] : 8, n0 = in0 ? n : 0, n1 = in1 ? n : 0;
+                bring<T, COPY>(to + 1024 * h, n0 ? p0 + 32 * h : p0, n0);
+                bring<T, COPY>(to + 1024 * h + 512, n1 ? p1 + 32 * h : p1, n1);
             }
+            if (in0) p0 += kK;
+            if (in1) p1 += kK;
+            if (--left == 0 && ++item < items.stop) point();
         }
         copy_commit();
-        stage_in = stage_in + 1 == kDepth ? 0 : stage_in + 1;
+        in_at = in_at + kStepBytes == kDepth * kStepBytes ? 0 : in_at + kStepBytes;
     };
-    if (item < items.stop) point();
+    if (item < items.stop && steps) point();
 #pragma unroll 1
     for (int i = 0; i < kDepth - 1; ++i) bring_step();
 
-    int stage = 0;
-#pragma unroll 1
-    for (int now = items.first; now < items.stop; ++now) {
-        int at, tile;
-        items.split(now, !DOWN, at, tile);
-        const int4 entry = a.entries[at];
-        // This lane's columns of B, and what makes them fp16.
-        const void *column[N];
-        float factor[N];
+    // The columns of an item: entry.z of them, the others are the last one's and never looked at.
+    struct Columns {
+        int4 entry;
+        int tile;
+        const char *from[N];   // this lane's of each eight, at its first element
+        float factor[N];       // what makes them fp16
         uint32_t low_mask[N];
+    };
+    auto columns_of = [&](Columns &c, int now) {
+        int at;
+        items.split(now, !DOWN, at, c.tile);
+        c.entry = lists.entries[at];
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            column[j] = nullptr;
-            factor[j] = 1.0f;
-            low_mask[j] = 0xffffffffu;
-            if (8 * j + g < entry.z) {
-                const int slot = a.sorted[entry.y + 8 * j + g];
-                if constexpr (DOWN) {
-                    column[j] = a.inner_out + slot * a.inner_row;
-                    if constexpr (std::is_same<T, __half>::value) {
-                        const uint32_t bits = a.largest[slot];
-                        factor[j] = to_half_range(bits);
-                        if (bits >= 0x7f800000u) low_mask[j] = 0;
-                    }
+            const int slot = lists.sorted[c.entry.y + min(8 * j + g, c.entry.z - 1)];
+            if constexpr (DOWN) {
+                c.from[j] = reinterpret_cast<const char *>(a.inner_out + slot * a.inner_row + first_k);
+                if constexpr (kHalf) {
+                    const uint32_t bits = a.largest[slot];
+                    c.factor[j] = to_half_range(bits);
+                    c.low_mask[j] = bits >= 0x7f800000u ? 0 : 0xffffffffu;
+                }
+            } else {
+                c.from[j] = reinterpret_cast<const char *>(static_cast<const T *>(a.x) + slot / a.top * a.x_token + first_k);
+            }
+        }
+    };
+    // Their elements of one step: eight of each run, of T or of four bytes.
+    struct Elements {
+        uint4 v[2][DOWN ? 2 : 1];
+    };
+    auto elements_of = [&](Elements &x, const char *from, int step) {
+        if constexpr (DOWN) {  // rows of the scratch are padded with zeros
+            const uint4 *p = reinterpret_cast<const uint4 *>(from + step * (kK * 4));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) x.v[h][0] = p[8 * h], x.v[h][1] = p[8 * h + 1];
+        } else if constexpr (COPY == kBy16) {
+            const uint4 *p = reinterpret_cast<const uint4 *>(from + step * (kK * 2));
+            const bool end = short_end && step + 1 == steps;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                x.v[h][0] = make_uint4(0, 0, 0, 0);
+                if (!end || n_end[h]) x.v[h][0] = p[4 * h];
+            }
+        } else {
+            const T *p = reinterpret_cast<const T *>(from) + step * kK;
+            const bool end = short_end && step + 1 == steps;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                T e[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) e[i] = !end || i < n_end[h] ? p[32 * h + i] : dev::narrow<T>(0.0f);
+                memcpy(&x.v[h][0], e, 16);
+            }
+        }
+    };
+    Columns cols;
+    Elements x[N];
+    if (items.first < items.stop) {
+        columns_of(cols, items.first);
+        if (kAhead && steps) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) elements_of(x[j], cols.from[j], 0);
+        }
+    }
+    int out_at = 0;
+#pragma unroll 1
+    for (int now = items.first; now < items.stop; ++now) {
+        const int4 entry = cols.entry;
+        const int tile = cols.tile;
+        float acc[N][4] = {};
+#pragma unroll 1
+        for (int step = 0; step < steps; ++step) {
+            copy_wait<kDepth - 2>();
+            const char *from = ring + out_at;
+            uint4 r[2][2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) r[h][i] = *reinterpret_cast<const uint4 *>(from + 1024 * h + 512 * i);
+            bring_step();  // into the stage before, which this lane read in the step before
+            out_at = out_at + kStepBytes == kDepth * kStepBytes ? 0 : out_at + kStepBytes;
+            Elements use[N];
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                if (j && 8 * j >= entry.z) break;
+                if constexpr (kAhead) {
+                    use[j] = x[j];
+                    if (step + 1 < steps) elements_of(x[j], cols.from[j], step + 1);
                 } else {
-                    column[j] = static_cast<const T *>(a.x) + slot / a.top * a.x_token;
+                    elements_of(use[j], cols.from[j], step);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                if (j && 8 * j >= entry.z) break;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint4 &r0 = r[h][0], &r1 = r[h][1];
+                    if constexpr (!DOWN) {
+                        const uint4 &c = use[j].v[h][0];
+                        mma<T>(acc[j], r0.x, r1.x, r0.y, r1.y, c.x, c.y);
+                        mma<T>(acc[j], r0.z, r1.z, r0.w, r1.w, c.z, c.w);
+                    } else {
+                        const uint4 &u = use[j].v[h][0], &v = use[j].v[h][DOWN ? 1 : 0];
+                        const uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if constexpr (kHalf) {
+                                const float one = __uint_as_float(w[2 * i]) * cols.factor[j], two = __uint_as_float(w[2 * i + 1]) * cols.factor[j];
+                                hi[i] = pack_half(one, two);
+                                __half2 halves;
+                                memcpy(&halves, &hi[i], 4);
+                                lo[i] = pack_half(one - __low2float(halves), two - __high2float(halves)) & cols.low_mask[j];
+                            } else {
+                                hi[i] = __byte_perm(w[2 * i], w[2 * i + 1], 0x5410);
+                                lo[i] = __byte_perm(w[2 * i], w[2 * i + 1], 0x7632);
+                            }
+                        }
+                        mma<T>(acc[j], r0.x, r1.x, r0.y, r1.y, hi[0], hi[1]);
+                        mma<T>(acc[j], r0.z, r1.z, r0.w, r1.w, hi[2], hi[3]);
+                        mma<T>(acc[j], r0.x, r1.x, r0.y, r1.y, lo[0], lo[1]);
+                        mma<T>(acc[j], r0.z, r1.z, r0.w, r1.w, lo[2], lo[3]);
+                    }
                 }
             }
         }
-        float acc[N][4] = {};
-#pragma unroll 2
-        for (int kk = k_first; kk < k_stop; kk += 32) {
-            copy_wait<kDepth - 2>();
-            const char *from = ring + stage * kStepBytes;
-            const uint4 r0 = *reinterpret_cast<const uint4 *>(from), r1 = *reinterpret_cast<const uint4 *>(from + 512);
-            bring_step();  // into the stage before, which this lane read in the step before
-            stage = stage + 1 == kDepth ? 0 : stage + 1;
-            const int at_k = kk + 8 * t;
+        // The next item's columns, on their way while this one's sums meet.
+        if (now + 1 < items.stop) {
+            columns_of(cols, now + 1);
+            if (kAhead && steps) {
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-                if (8 * j >= entry.z) break;
-                if constexpr (!DOWN) {
-                    uint4 c = make_uint4(0, 0, 0, 0);
-                    if (column[j]) {
-                        const T *p = static_cast<const T *>(column[j]) + at_k;
-                        if constexpr (COPY == kBy16) {
-                            if (at_k < K) c = *reinterpret_cast<const uint4 *>(p);
-                        } else {
-                            T v[8];
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) v[i] = at_k + i < K ? p[i] : dev::narrow<T>(0.0f);
-                            memcpy(&c, v, 16);
-                        }
-                    }
-                    mma<T>(acc[j], r0.x, r1.x, r0.y, r1.y, c.x, c.y);
-                    mma<T>(acc[j], r0.z, r1.z, r0.w, r1.w, c.z, c.w);
-                } else {
-                    uint4 u = make_uint4(0, 0, 0, 0), v = u;
-                    if (column[j]) {
-                        const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const uint32_t *>(column[j]) + at_k);
-                        u = p[0];
-                        v = p[1];
-                    }
-                    uint32_t hi[4], lo[4];
-                    if constexpr (std::is_same<T, __half>::value) {
-                        const uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float x = __uint_as_float(w[2 * i]) * factor[j], y = __uint_as_float(w[2 * i + 1]) * factor[j];
-                            hi[i] = pack_half(x, y);
-                            __half2 h;
-                            memcpy(&h, &hi[i], 4);
-                            lo[i] = pack_half(x - __low2float(h), y - __high2float(h)) & low_mask[j];
-                        }
-                    } else {
-                        const uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            hi[i] = __byte_perm(w[2 * i], w[2 * i + 1], 0x5410);
-                            lo[i] = __byte_perm(w[2 * i], w[2 * i + 1], 0x7632);
-                        }
-                    }
-                    mma<T>(acc[j], r0.x, r1.x, r0.y, r1.y, hi[0], hi[1]);
-                    mma<T>(acc[j], r0.z, r1.z, r0.w, r1.w, hi[2], hi[3]);
-                    mma<T>(acc[j], r0.x, r1.x, r0.y, r1.y, lo[0], lo[1]);
-                    mma<T>(acc[j], r0.z, r1.z, r0.w, r1.w, lo[2], lo[3]);
-                }
+                for (int j = 0; j < N; ++j) elements_of(x[j], cols.from[j], 0);
             }
         }
         // The parts' sums meet, in their order, in the group's first warp.
@@ -508,25 +588,25 @@ __global__ void __launch_bounds__(kMoeThreads, 2) k_experts(const __grid_constan
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int c = 8 * j + 2 * t + e;
-                const int slot = c < entry.z ? a.sorted[entry.y + c] : 0;
+                const int slot = lists.sorted[entry.y + min(c, entry.z - 1)];
                 if constexpr (DOWN) {
                     float back = 1.0f;
-                    if constexpr (std::is_same<T, __half>::value) back = 1.0f / to_half_range(a.largest[slot]);
+                    if constexpr (kHalf) back = 1.0f / to_half_range(a.largest[slot]);
                     float *to = a.part + static_cast<int64_t>(slot) * a.hidden + tile * 16 + g;
                     if (c < entry.z && tile * 16 + g < rows) to[0] = acc[j][e] * back;
                     if (c < entry.z && tile * 16 + g + 8 < rows) to[8] = acc[j][2 + e] * back;
                 } else {
-                    const int r = tile * 8 + g;
-                    const bool real = c < entry.z && r < rows;
+                    const int row = tile * 8 + g;
+                    const bool real = c < entry.z && row < rows;
                     const float h = real ? silu_times(acc[j][e], acc[j][2 + e]) : 0.0f;
-                    if constexpr (std::is_same<T, __half>::value) {
+                    if constexpr (kHalf) {
                         uint32_t top = __float_as_uint(h) & 0x7fffffffu;
 #pragma unroll
                         for (int d = 4; d < 32; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
                         if (g == 0 && c < entry.z && top) atomicMax(a.largest + slot, top);
-                        if (real) a.inner_out[slot * a.inner_row + r] = __float_as_uint(h);
+                        if (real) a.inner_out[slot * a.inner_row + row] = __float_as_uint(h);
                     } else {
-                        if (real) a.inner_out[slot * a.inner_row + r] = two_bf16(h);
+                        if (real) a.inner_out[slot * a.inner_row + row] = two_bf16(h);
                     }
                 }
             }
@@ -534,27 +614,30 @@ __global__ void __launch_bounds__(kMoeThreads, 2) k_experts(const __grid_constan
     }
 }
 
-// The same of 32 bits: rows 0 and 1 of gate and 2 and 3 of up, or four of down, up to eight columns.
+// The same of 32 bits: rows 0 and 1 of gate and 2 and 3 of up, or four of down, up to eight columns.  Elements of a step that
+// a lane has: four side by side, or every 32nd where they come one by one.
 template <bool DOWN, int COPY>
 __global__ void __launch_bounds__(kMoeThreads, 2) k_experts32(const __grid_constant__ MoeArgs a, int S) {
+    constexpr int kK = 128, kOne = COPY == kBy16 ? 1 : 32;  // elements of a step, and between two of a lane's
     extern __shared__ __align__(128) char smem[];
     dev::wait_for_previous();
-    constexpr int kDepth32 = kDepth / 2, kBytes = 2 * kStepBytes;  // of four rows of 512 bytes
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int K = DOWN ? a.inner : a.hidden, rows = DOWN ? a.hidden : a.inner, per_tile = DOWN ? 4 : 2;
     const int part = warp % S, groups = kMoeWarps / S, group = warp / S;
     const Items items = items_of(a, (rows + per_tile - 1) / per_tile, gridDim.x * groups, blockIdx.x * groups + group);
-    const int steps = (K + 127) / 128, each = (steps + S - 1) / S, k_first = min(part * each, steps) * 128, k_stop = min((part + 1) * each, steps) * 128;
-    char *ring = smem + warp * kDepth32 * kBytes + lane * 16;
-    float *meet = reinterpret_cast<float *>(smem + kMoeWarps * kDepth32 * kBytes);  // [warp][lane]
+    const Lists lists = lists_of(a, items.entries);
+    const int all = (K + kK - 1) / kK, each = (all + S - 1) / S, begin = min(part * each, all), steps = min(begin + each, all) - begin;
+    const int first_k = begin * kK + (COPY == kBy16 ? 4 * lane : lane);
+    char *ring = smem + warp * kDepth * kStepBytes + lane * 16;
+    float *meet = reinterpret_cast<float *>(smem + kMoeWarps * kDepth * kStepBytes);  // [warp][lane]
 
-    int item = items.first, k = k_first;
+    int item = items.first, left = 0, in_at = 0, in_k = first_k;
     const float *p[4] = {};
     uint32_t in = 0;
     auto point = [&] {
         int at, tile;
         items.split(item, !DOWN, at, tile);
-        const int expert = a.entries[at].x;
+        const int expert = lists.entries[at].x;
         in = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -568,74 +651,84 @@ __global__ void __launch_bounds__(kMoeThreads, 2) k_experts32(const __grid_const
                 in |= 1u << i;
             }
         }
+        left = steps;
+        in_k = first_k;
     };
-    int stage_in = 0;
     auto bring_step = [&] {
-        if (item < items.stop && k_first < k_stop) {
-            const int at = k + 4 * lane, n = min(max(K - at, 0), 4);
-            char *to = ring + stage_in * kBytes;
+        if (left) {
+            char *to = ring + in_at;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const bool real = (in >> i & 1) && n;
-                bring<float, COPY>(to + 512 * i, p[i] + (real ? at : 0), real ? n : 0);
+                if constexpr (COPY == kBy16) {
+                    const int n = in >> i & 1 ? min(max(K - in_k, 0), 4) : 0;
+                    bring<float, kBy16>(to + 512 * i, p[i] + (n ? in_k : 0), n);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const bool real = (in >> i & 1) && in_k + 32 * e < K;
+                        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_at(to + 512 * i + 4 * e)), "l"(real ? p[i] + in_k + 32 * e : p[i]),
+                                     "r"(real ? 4 : 0) : "memory");
+                    }
+                }
             }
-            k += 128;
-            if (k >= k_stop) {
-                k = k_first;
-                ++item;
-                if (item < items.stop) point();
-            }
+            in_k += kK;
+            if (--left == 0 && ++item < items.stop) point();
         }
         copy_commit();
-        stage_in = stage_in + 1 == kDepth32 ? 0 : stage_in + 1;
+        in_at = in_at + kStepBytes == kDepth * kStepBytes ? 0 : in_at + kStepBytes;
     };
-    if (item < items.stop) point();
+    if (item < items.stop && steps) point();
 #pragma unroll 1
-    for (int i = 0; i < kDepth32 - 1; ++i) bring_step();
+    for (int i = 0; i < kDepth - 1; ++i) bring_step();
 
-    int stage = 0;
+    int out_at = 0;
 #pragma unroll 1
     for (int now = items.first; now < items.stop; ++now) {
         int at, tile;
         items.split(now, !DOWN, at, tile);
-        const int4 entry = a.entries[at];
+        const int4 entry = lists.entries[at];
         const float *column[8];
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
-            const int slot = a.sorted[entry.y + min(c, entry.z - 1)];
+            const int slot = lists.sorted[entry.y + min(c, entry.z - 1)];
             column[c] = DOWN ? reinterpret_cast<const float *>(a.inner_out) + slot * a.inner_row : static_cast<const float *>(a.x) + slot / a.top * a.x_token;
         }
         float acc[32] = {};  // [row][column]
+        int k = first_k;
 #pragma unroll 1
-        for (int kk = k_first; kk < k_stop; kk += 128) {
-            copy_wait<kDepth32 - 2>();
-            const char *from = ring + stage * kBytes;
+        for (int step = 0; step < steps; ++step, k += kK) {
+            float4 x[8];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                x[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (c >= entry.z) break;
+                const float *q = column[c] + k;
+                if constexpr (COPY == kBy16) {  // whole words: of K, or of the scratch's rows, which are padded with zeros
+                    if (k < K) x[c] = *reinterpret_cast<const float4 *>(q);
+                } else {
+                    if (k < K) x[c].x = q[0];
+                    if (k + kOne < K) x[c].y = q[kOne];
+                    if (k + 2 * kOne < K) x[c].z = q[2 * kOne];
+                    if (k + 3 * kOne < K) x[c].w = q[3 * kOne];
+                }
+            }
+            copy_wait<kDepth - 2>();
+            const char *from = ring + out_at;
             float4 w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const float4 *>(from + 512 * i);
             bring_step();
-            stage = stage + 1 == kDepth32 ? 0 : stage + 1;
-            const int at_k = kk + 4 * lane;
+            out_at = out_at + kStepBytes == kDepth * kStepBytes ? 0 : out_at + kStepBytes;
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
                 if (c >= entry.z) break;
-                float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                const float *q = column[c] + at_k;
-                if constexpr (DOWN || COPY == kBy16) {  // rows of the scratch are padded with zeros
-                    if (at_k < K) x = *reinterpret_cast<const float4 *>(q);
-                } else {
-                    if (at_k < K) x.x = q[0];
-                    if (at_k + 1 < K) x.y = q[1];
-                    if (at_k + 2 < K) x.z = q[2];
-                    if (at_k + 3 < K) x.w = q[3];
-                }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     float s = acc[8 * i + c];
-                    s = fmaf(w[i].x, x.x, s);
-                    s = fmaf(w[i].y, x.y, s);
-                    s = fmaf(w[i].z, x.z, s);
-                    acc[8 * i + c] = fmaf(w[i].w, x.w, s);
+                    s = fmaf(w[i].x, x[c].x, s);
+                    s = fmaf(w[i].y, x[c].y, s);
+                    s = fmaf(w[i].z, x[c].z, s);
+                    acc[8 * i + c] = fmaf(w[i].w, x[c].w, s);
                 }
             }
         }
@@ -660,11 +753,11 @@ __global__ void __launch_bounds__(kMoeThreads, 2) k_experts32(const __grid_const
         }
         const int c = lane % 8, row = lane / 8;
         if constexpr (DOWN) {
-            if (c < entry.z && tile * 4 + row < rows) a.part[static_cast<int64_t>(a.sorted[entry.y + c]) * a.hidden + tile * 4 + row] = s;
+            if (c < entry.z && tile * 4 + row < rows) a.part[static_cast<int64_t>(lists.sorted[entry.y + c]) * a.hidden + tile * 4 + row] = s;
         } else {
             const float up = __shfl_down_sync(0xffffffffu, s, 16);
             if (row < 2 && c < entry.z && tile * 2 + row < rows)
-                a.inner_out[a.sorted[entry.y + c] * a.inner_row + tile * 2 + row] = __float_as_uint(silu_times(s, up));
+                a.inner_out[lists.sorted[entry.y + c] * a.inner_row + tile * 2 + row] = __float_as_uint(silu_times(s, up));
         }
     }
 }
@@ -749,10 +842,10 @@ int copy_of(const void *p, int64_t row, int64_t expert, int eb) {
     return any % 16 == 0 ? kBy16 : any % 4 == 0 ? kBy4 : kByElement;
 }
 
-// Warps that share an item: as few as leave every warp of the GPU one.
+// Warps that share an item: so many that every warp of the GPU has two, as long as each has a few steps of it.
 int parts_of(int64_t items, int warps, int steps) {
     int s = 1;
-    while (s < kMoeWarps && items * s < warps && steps >= 4 * s) s *= 2;
+    while (s < kMoeWarps && items * s < 2 * warps && steps >= 8 * s) s *= 2;
     return s;
 }
 
@@ -881,8 +974,9 @@ int l2d_moe_forward(l2d_moe_plan *p, const void *x, void *y, int32_t *ids, float
     a.ids_out = ids;
     a.weights_out = weights;
     a.tokens = tokens;
-    // An expert has at most `tokens` slots.
-    const int eights = eb == 4 || tokens <= 8 ? 1 : tokens <= 16 ? 2 : 4;
+    // An expert with more slots than an entry takes is read again for the next one, mostly from L2.
+    const int64_t likely = int64_t(tokens) * d.top / d.experts;
+    const int eights = eb == 4 || tokens <= 8 || likely <= 3 ? 1 : tokens <= 16 || likely <= 8 ? 2 : 4;
     a.per_entry = 8 * eights;
     const int x_copy = copy_of(x, d.x_token, 0, eb), whole = d.hidden % (16 / eb) == 0 ? kBy16 : kBy4;
     const int copy_up = std::max({copy_of(d.gate, d.gate_row, d.gate_expert, eb), copy_of(d.up, d.up_row, d.up_expert, eb), std::min<int>(std::max(x_copy, whole), kBy4)});
@@ -892,7 +986,7 @@ int l2d_moe_forward(l2d_moe_plan *p, const void *x, void *y, int32_t *ids, float
                          : d.dtype == L2D_F16 ? pick_moe<__half>(eights, route_words, copy_up, copy_down)
                                               : pick_moe<__nv_bfloat16>(eights, route_words, copy_up, copy_down);
     L2D_CUDA_TRY(launch(k.route, dim3(d.experts, (tokens + kRouteTokens - 1) / kRouteTokens), kMoeThreads, 0, stream, a));
-    const int up_rows = eb == 4 ? 2 : 8, down_rows = eb == 4 ? 4 : 16, step = eb == 4 ? 128 : 32;
+    const int up_rows = eb == 4 ? 2 : 8, down_rows = eb == 4 ? 4 : 16, step = eb == 4 ? 128 : 64;
     const int64_t entries = std::min<int64_t>(int64_t(tokens) * d.top, d.experts);
     const int blocks = 2 * p->sms, warps = blocks * kMoeWarps;
     const int s_up = parts_of(entries * ((d.inner + up_rows - 1) / up_rows), warps, static_cast<int>((d.hidden + step - 1) / step));
