@@ -256,8 +256,8 @@ __global__ void __launch_bounds__(kMoeThreads) k_route(const __grid_constant__ M
 // 32 bits: a warp works on four rows (two of gate and of up) with the lanes along them, by fused multiply-adds.
 // ---------------------------------------------------------------------------------------------
 
-constexpr int kDepth = 4;                 // steps in a ring, all but one of them on their way
-constexpr int kStepBytes = 2048;          // of 16 rows of 128 bytes, or four of 512
+constexpr int kDepth32 = 4;               // steps in a ring, all but one of them on their way
+constexpr int kRowBytes = 2048;           // of a step: 16 rows of 128 bytes, or four of 512
 constexpr int kCached = 128, kCachedSlots = 1024;  // entries and slots that a block keeps in shared memory
 enum { kBy16 = 0, kBy4 = 1, kByElement = 2 };  // how rows come: 16 bytes at a time, 4, or one element
 
@@ -270,7 +270,7 @@ __device__ __forceinline__ void copy_wait() {
 // 16 bytes of a row, of which `n` elements are real.
 template <typename T, int COPY>
 __device__ __forceinline__ void bring(char *to, const T *from, int n) {
-    constexpr int kEach = 16 / sizeof(T);
+    constexpr int kEach = 16 / static_cast<int>(sizeof(T));
     if constexpr (COPY == kBy16) {
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_at(to)), "l"(from), "r"(n * static_cast<int>(sizeof(T))) : "memory");
     } else if constexpr (COPY == kBy4) {
@@ -286,6 +286,17 @@ __device__ __forceinline__ void bring(char *to, const T *from, int n) {
         for (int i = 0; i < kEach; ++i) v[i] = i < n ? from[i] : dev::narrow<T>(0.0f);
         memcpy(to, v, 16);
     }
+}
+
+template <typename T, int COPY>
+__device__ __forceinline__ void bring_all(char *to, const T *from) {
+    if constexpr (COPY == kBy16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_at(to)), "l"(from) : "memory");
+    else bring<T, COPY>(to, from, 16 / static_cast<int>(sizeof(T)));
+}
+
+// Sixteen bytes by way of L1, for what all warps of an SM read: of rows, which are read once, L1 keeps nothing.
+__device__ __forceinline__ void bring_shared(char *to, const void *from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(smem_at(to)), "l"(from) : "memory");
 }
 
 template <typename T>
@@ -362,12 +373,23 @@ __device__ __forceinline__ Lists lists_of(const MoeArgs &a, int entries) {
     return {kept_entries, kept_sorted};
 }
 
+// A warp's ring: a step's rows, then its columns (16 bytes a lane of each eight and run, of four-byte elements twice), as deep as
+// sixteen warps an SM leave room for (eight of many columns).
+template <int N, bool DOWN>
+struct ExpertsRing {
+    static constexpr int kStep = kRowBytes + N * (DOWN ? 2048 : 1024);
+    static constexpr int kBlocks = N == 4 ? 1 : 2;
+    static constexpr int kDepth = 12 * 1024 * (3 - kBlocks) / kStep;
+    static constexpr int kBytes = kDepth * kStep;
+    static_assert(kDepth >= 2, "one step on its way");
+};
+
 // N: eights of columns; DOWN: the second product.  S: warps that share an item.
 template <typename T, int N, bool DOWN, int COPY>
-__global__ void __launch_bounds__(kMoeThreads, 2) k_experts(const __grid_constant__ MoeArgs a, int S) {
+__global__ void __launch_bounds__(kMoeThreads, ExpertsRing<N, DOWN>::kBlocks) k_experts(const __grid_constant__ MoeArgs a, int S) {
     constexpr bool kHalf = std::is_same<T, __half>::value;
-    constexpr bool kAhead = DOWN ? N == 1 : N <= 2;  // columns are read a step ahead where registers hold them
     constexpr int kK = 64;                           // elements of a step: two runs of 32
+    using Ring = ExpertsRing<N, DOWN>;
     extern __shared__ __align__(128) char smem[];
     dev::wait_for_previous();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -380,168 +402,139 @@ __global__ void __launch_bounds__(kMoeThreads, 2) k_experts(const __grid_constan
     const bool short_end = begin + steps == all && K % kK;
     const int n_end[2] = {min(max(K - (all - 1) * kK - 8 * t, 0), 8), min(max(K - (all - 1) * kK - 32 - 8 * t, 0), 8)};
     const int first_k = begin * kK + 8 * t;
-    char *ring = smem + warp * kDepth * kStepBytes + lane * 16;
-    float *meet = reinterpret_cast<float *>(smem + kMoeWarps * kDepth * kStepBytes);  // [warp][4 N][lane]
+    char *ring = smem + warp * Ring::kBytes + lane * 16;
+    float *meet = reinterpret_cast<float *>(smem + kMoeWarps * Ring::kBytes);  // [warp][4 N][lane]
 
-    // What is brought next: rows g and g + 8 from p0 and p1 on, `left` steps of them.
-    int item = items.first, left = 0, in_at = 0;
+    // What is brought next: rows g and g + 8 from p0 and p1 on, and column g of each eight, `left` steps of them.
+    using X = typename std::conditional<DOWN, uint32_t, T>::type;
+    constexpr int kRun = DOWN ? 2 : 1;  // 16-byte words of eight elements of a column
+    int item = items.first, left = 0, in_at = 0, in_count = 0;
     const T *p0 = nullptr, *p1 = nullptr;
-    bool in0 = false, in1 = false;
-    auto point = [&] {
+    const X *column[N] = {};
+    auto point = [&] {  // rows past the last are the last one's, and so are columns: their sums go nowhere
         int at, tile;
         items.split(item, !DOWN, at, tile);
-        const int expert = lists.entries[at].x;
+        const int4 entry = lists.entries[at];
+        const int expert = entry.x;
+        in_count = entry.z;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int slot = lists.sorted[entry.y + min(8 * j + g, entry.z - 1)];
+            if constexpr (DOWN) column[j] = a.inner_out + slot * a.inner_row + first_k;
+            else column[j] = static_cast<const T *>(a.x) + slot / a.top * a.x_token + first_k;
+        }
         if constexpr (DOWN) {
-            const int r0 = tile * 16 + g;
-            in0 = r0 < rows;
-            in1 = r0 + 8 < rows;
-            const T *w = static_cast<const T *>(a.down) + expert * a.down_expert;
-            p0 = w + (in0 ? r0 * a.down_row + first_k : 0);
-            p1 = w + (in1 ? (r0 + 8) * a.down_row + first_k : 0);
+            const T *w = static_cast<const T *>(a.down) + expert * a.down_expert + first_k;
+            p0 = w + min(tile * 16 + g, rows - 1) * a.down_row;
+            p1 = w + min(tile * 16 + g + 8, rows - 1) * a.down_row;
         } else {
-            const int r = tile * 8 + g;
-            in0 = in1 = r < rows;
-            p0 = static_cast<const T *>(a.gate) + expert * a.gate_expert + (in0 ? r * a.gate_row + first_k : 0);
-            p1 = static_cast<const T *>(a.up) + expert * a.up_expert + (in1 ? r * a.up_row + first_k : 0);
+            const int r = min(tile * 8 + g, rows - 1);
+            p0 = static_cast<const T *>(a.gate) + expert * a.gate_expert + r * a.gate_row + first_k;
+            p1 = static_cast<const T *>(a.up) + expert * a.up_expert + r * a.up_row + first_k;
         }
         left = steps;
     };
     auto bring_step = [&] {
         if (left) {
             char *to = ring + in_at;
-            const bool end = short_end && left == 1;
+            if (short_end && left == 1) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int n = end ? n_end[h] : 8, n0 = in0 ? n : 0, n1 = in1 ? n : 0;
-                bring<T, COPY>(to + 1024 * h, n0 ? p0 + 32 * h : p0, n0);
-                bring<T, COPY>(to + 1024 * h + 512, n1 ? p1 + 32 * h : p1, n1);
+                for (int h = 0; h < 2; ++h) {  // nothing is read of a run without elements, whose first may lie anywhere
+                    const T *none = static_cast<const T *>(a.down);
+                    bring<T, COPY>(to + 1024 * h, n_end[h] ? p0 + 32 * h : none, n_end[h]);
+                    bring<T, COPY>(to + 1024 * h + 512, n_end[h] ? p1 + 32 * h : none, n_end[h]);
+                    if constexpr (!DOWN) {
+#pragma unroll
+                        for (int j = 0; j < N; ++j)
+                            if (j == 0 || 8 * j < in_count) bring<T, COPY>(to + kRowBytes + 1024 * j + 512 * h, n_end[h] ? column[j] + 32 * h : none, n_end[h]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    bring_all<T, COPY>(to + 1024 * h, p0 + 32 * h);
+                    bring_all<T, COPY>(to + 1024 * h + 512, p1 + 32 * h);
+                    if constexpr (!DOWN) {
+#pragma unroll
+                        for (int j = 0; j < N; ++j)
+                            if (j == 0 || 8 * j < in_count) {
+                                char *x = to + kRowBytes + 1024 * j + 512 * h;
+                                if constexpr (COPY == kBy16) bring_shared(x, column[j] + 32 * h);
+                                else bring_all<T, COPY>(x, column[j] + 32 * h);
+                            }
+                    }
+                }
             }
-            if (in0) p0 += kK;
-            if (in1) p1 += kK;
+            if constexpr (DOWN) {  // rows of the scratch are padded with zeros, and aligned
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+                    if (j == 0 || 8 * j < in_count)
+#pragma unroll
+                        for (int h = 0; h < 4; ++h)
+                            bring_shared(to + kRowBytes + 2048 * j + 512 * h, column[j] + 32 * (h / 2) + 4 * (h % 2));
+            }
+            p0 += kK;
+            p1 += kK;
+#pragma unroll
+            for (int j = 0; j < N; ++j) column[j] += kK;
             if (--left == 0 && ++item < items.stop) point();
         }
         copy_commit();
-        in_at = in_at + kStepBytes == kDepth * kStepBytes ? 0 : in_at + kStepBytes;
+        in_at = in_at + Ring::kStep == Ring::kBytes ? 0 : in_at + Ring::kStep;
     };
     if (item < items.stop && steps) point();
 #pragma unroll 1
-    for (int i = 0; i < kDepth - 1; ++i) bring_step();
+    for (int i = 0; i < Ring::kDepth - 1; ++i) bring_step();
 
-    // The columns of an item: entry.z of them, the others are the last one's and never looked at.
-    struct Columns {
-        int4 entry;
-        int tile;
-        const char *from[N];   // this lane's of each eight, at its first element
-        float factor[N];       // what makes them fp16
-        uint32_t low_mask[N];
-    };
-    auto columns_of = [&](Columns &c, int now) {
-        int at;
-        items.split(now, !DOWN, at, c.tile);
-        c.entry = lists.entries[at];
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int slot = lists.sorted[c.entry.y + min(8 * j + g, c.entry.z - 1)];
-            if constexpr (DOWN) {
-                c.from[j] = reinterpret_cast<const char *>(a.inner_out + slot * a.inner_row + first_k);
-                if constexpr (kHalf) {
-                    const uint32_t bits = a.largest[slot];
-                    c.factor[j] = to_half_range(bits);
-                    c.low_mask[j] = bits >= 0x7f800000u ? 0 : 0xffffffffu;
-                }
-            } else {
-                c.from[j] = reinterpret_cast<const char *>(static_cast<const T *>(a.x) + slot / a.top * a.x_token + first_k);
-            }
-        }
-    };
-    // Their elements of one step: eight of each run, of T or of four bytes.
-    struct Elements {
-        uint4 v[2][DOWN ? 2 : 1];
-    };
-    auto elements_of = [&](Elements &x, const char *from, int step) {
-        if constexpr (DOWN) {  // rows of the scratch are padded with zeros
-            const uint4 *p = reinterpret_cast<const uint4 *>(from + step * (kK * 4));
-#pragma unroll
-            for (int h = 0; h < 2; ++h) x.v[h][0] = p[8 * h], x.v[h][1] = p[8 * h + 1];
-        } else if constexpr (COPY == kBy16) {
-            const uint4 *p = reinterpret_cast<const uint4 *>(from + step * (kK * 2));
-            const bool end = short_end && step + 1 == steps;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                x.v[h][0] = make_uint4(0, 0, 0, 0);
-                if (!end || n_end[h]) x.v[h][0] = p[4 * h];
-            }
-        } else {
-            const T *p = reinterpret_cast<const T *>(from) + step * kK;
-            const bool end = short_end && step + 1 == steps;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                T e[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) e[i] = !end || i < n_end[h] ? p[32 * h + i] : dev::narrow<T>(0.0f);
-                memcpy(&x.v[h][0], e, 16);
-            }
-        }
-    };
-    Columns cols;
-    Elements x[N];
-    if (items.first < items.stop) {
-        columns_of(cols, items.first);
-        if (kAhead && steps) {
-#pragma unroll
-            for (int j = 0; j < N; ++j) elements_of(x[j], cols.from[j], 0);
-        }
-    }
     int out_at = 0;
 #pragma unroll 1
     for (int now = items.first; now < items.stop; ++now) {
-        const int4 entry = cols.entry;
-        const int tile = cols.tile;
+        int at, tile;
+        items.split(now, !DOWN, at, tile);
+        const int4 entry = lists.entries[at];
+        float factor[N];  // what makes this lane's columns fp16
+        uint32_t low_mask[N];
+        if constexpr (DOWN && kHalf) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const uint32_t bits = a.largest[lists.sorted[entry.y + min(8 * j + g, entry.z - 1)]];
+                factor[j] = to_half_range(bits);
+                low_mask[j] = bits >= 0x7f800000u ? 0 : 0xffffffffu;
+            }
+        }
         float acc[N][4] = {};
 #pragma unroll 1
         for (int step = 0; step < steps; ++step) {
-            copy_wait<kDepth - 2>();
+            copy_wait<Ring::kDepth - 2>();
             const char *from = ring + out_at;
             uint4 r[2][2];
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) r[h][i] = *reinterpret_cast<const uint4 *>(from + 1024 * h + 512 * i);
-            bring_step();  // into the stage before, which this lane read in the step before
-            out_at = out_at + kStepBytes == kDepth * kStepBytes ? 0 : out_at + kStepBytes;
-            Elements use[N];
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                if (j && 8 * j >= entry.z) break;
-                if constexpr (kAhead) {
-                    use[j] = x[j];
-                    if (step + 1 < steps) elements_of(x[j], cols.from[j], step + 1);
-                } else {
-                    elements_of(use[j], cols.from[j], step);
-                }
-            }
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 if (j && 8 * j >= entry.z) break;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const uint4 &r0 = r[h][0], &r1 = r[h][1];
+                    const uint4 *x = reinterpret_cast<const uint4 *>(from + kRowBytes + 1024 * kRun * j + 512 * kRun * h);
+                    const uint4 u = x[0];
                     if constexpr (!DOWN) {
-                        const uint4 &c = use[j].v[h][0];
-                        mma<T>(acc[j], r0.x, r1.x, r0.y, r1.y, c.x, c.y);
-                        mma<T>(acc[j], r0.z, r1.z, r0.w, r1.w, c.z, c.w);
+                        mma<T>(acc[j], r0.x, r1.x, r0.y, r1.y, u.x, u.y);
+                        mma<T>(acc[j], r0.z, r1.z, r0.w, r1.w, u.z, u.w);
                     } else {
-                        const uint4 &u = use[j].v[h][0], &v = use[j].v[h][DOWN ? 1 : 0];
+                        const uint4 v = x[32];
                         const uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
                         uint32_t hi[4], lo[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             if constexpr (kHalf) {
-                                const float one = __uint_as_float(w[2 * i]) * cols.factor[j], two = __uint_as_float(w[2 * i + 1]) * cols.factor[j];
+                                const float one = __uint_as_float(w[2 * i]) * factor[j], two = __uint_as_float(w[2 * i + 1]) * factor[j];
                                 hi[i] = pack_half(one, two);
                                 __half2 halves;
                                 memcpy(&halves, &hi[i], 4);
-                                lo[i] = pack_half(one - __low2float(halves), two - __high2float(halves)) & cols.low_mask[j];
+                                lo[i] = pack_half(one - __low2float(halves), two - __high2float(halves)) & low_mask[j];
                             } else {
                                 hi[i] = __byte_perm(w[2 * i], w[2 * i + 1], 0x5410);
                                 lo[i] = __byte_perm(w[2 * i], w[2 * i + 1], 0x7632);
@@ -554,14 +547,8 @@ __global__ void __launch_bounds__(kMoeThreads, 2) k_experts(const __grid_constan
                     }
                 }
             }
-        }
-        // The next item's columns, on their way while this one's sums meet.
-        if (now + 1 < items.stop) {
-            columns_of(cols, now + 1);
-            if (kAhead && steps) {
-#pragma unroll
-                for (int j = 0; j < N; ++j) elements_of(x[j], cols.from[j], 0);
-            }
+            bring_step();  // into the step before's place, which this lane has read
+            out_at = out_at + Ring::kStep == Ring::kBytes ? 0 : out_at + Ring::kStep;
         }
         // The parts' sums meet, in their order, in the group's first warp.
         if (S > 1) {
@@ -628,8 +615,8 @@ __global__ void __launch_bounds__(kMoeThreads, 2) k_experts32(const __grid_const
     const Lists lists = lists_of(a, items.entries);
     const int all = (K + kK - 1) / kK, each = (all + S - 1) / S, begin = min(part * each, all), steps = min(begin + each, all) - begin;
     const int first_k = begin * kK + (COPY == kBy16 ? 4 * lane : lane);
-    char *ring = smem + warp * kDepth * kStepBytes + lane * 16;
-    float *meet = reinterpret_cast<float *>(smem + kMoeWarps * kDepth * kStepBytes);  // [warp][lane]
+    char *ring = smem + warp * kDepth32 * kRowBytes + lane * 16;
+    float *meet = reinterpret_cast<float *>(smem + kMoeWarps * kDepth32 * kRowBytes);  // [warp][lane]
 
     int item = items.first, left = 0, in_at = 0, in_k = first_k;
     const float *p[4] = {};
@@ -675,11 +662,11 @@ __global__ void __launch_bounds__(kMoeThreads, 2) k_experts32(const __grid_const
             if (--left == 0 && ++item < items.stop) point();
         }
         copy_commit();
-        in_at = in_at + kStepBytes == kDepth * kStepBytes ? 0 : in_at + kStepBytes;
+        in_at = in_at + kRowBytes == kDepth32 * kRowBytes ? 0 : in_at + kRowBytes;
     };
     if (item < items.stop && steps) point();
 #pragma unroll 1
-    for (int i = 0; i < kDepth - 1; ++i) bring_step();
+    for (int i = 0; i < kDepth32 - 1; ++i) bring_step();
 
     int out_at = 0;
 #pragma unroll 1
@@ -712,13 +699,13 @@ __global__ void __launch_bounds__(kMoeThreads, 2) k_experts32(const __grid_const
                     if (k + 3 * kOne < K) x[c].w = q[3 * kOne];
                 }
             }
-            copy_wait<kDepth - 2>();
+            copy_wait<kDepth32 - 2>();
             const char *from = ring + out_at;
             float4 w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const float4 *>(from + 512 * i);
             bring_step();
-            out_at = out_at + kStepBytes == kDepth * kStepBytes ? 0 : out_at + kStepBytes;
+            out_at = out_at + kRowBytes == kDepth32 * kRowBytes ? 0 : out_at + kRowBytes;
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
                 if (c >= entry.z) break;
@@ -786,12 +773,12 @@ struct MoeKernels {
     void (*gate_up)(MoeArgs, int);
     void (*down)(MoeArgs, int);
     void (*combine)(MoeArgs);
-    int smem;
+    int smem[2], blocks[2];  // of gate and up, and of down: bytes of a block, blocks an SM
 };
 
-template <typename T, int N>
-int experts_smem() {
-    return kMoeWarps * (kDepth * kStepBytes + (sizeof(T) == 4 ? 128 : 4 * N * 128));
+template <typename T, int N, bool DOWN>
+constexpr int experts_smem() {
+    return kMoeWarps * (sizeof(T) == 4 ? kDepth32 * kRowBytes + 128 : ExpertsRing<N, DOWN>::kBytes + 4 * N * 128);
 }
 
 template <typename T, int N, int COPY>
@@ -810,7 +797,8 @@ void (*pick_copy(bool down, int copy))(MoeArgs, int) {
 template <typename T, int N>
 MoeKernels moe_kernels(bool route_words, int copy_up, int copy_down) {
     return {route_words ? k_route<T, true> : k_route<T, false>, pick_copy<T, N>(false, copy_up), pick_copy<T, N>(true, copy_down), k_combine<T>,
-            experts_smem<T, N>()};
+            {experts_smem<T, N, false>(), experts_smem<T, N, true>()},
+            {sizeof(T) == 4 ? 2 : ExpertsRing<N, false>::kBlocks, sizeof(T) == 4 ? 2 : ExpertsRing<N, true>::kBlocks}};
 }
 
 template <typename T>
@@ -978,8 +966,8 @@ int l2d_moe_forward(l2d_moe_plan *p, const void *x, void *y, int32_t *ids, float
     const int64_t likely = int64_t(tokens) * d.top / d.experts;
     const int eights = eb == 4 || tokens <= 8 || likely <= 3 ? 1 : tokens <= 16 || likely <= 8 ? 2 : 4;
     a.per_entry = 8 * eights;
-    const int x_copy = copy_of(x, d.x_token, 0, eb), whole = d.hidden % (16 / eb) == 0 ? kBy16 : kBy4;
-    const int copy_up = std::max({copy_of(d.gate, d.gate_row, d.gate_expert, eb), copy_of(d.up, d.up_row, d.up_expert, eb), std::min<int>(std::max(x_copy, whole), kBy4)});
+    const int x_copy = copy_of(x, d.x_token, 0, eb), whole = eb == 4 && d.hidden % 4 ? kBy4 : kBy16;
+    const int copy_up = std::max({copy_of(d.gate, d.gate_row, d.gate_expert, eb), copy_of(d.up, d.up_row, d.up_expert, eb), x_copy, whole});
     const int copy_down = copy_of(d.down, d.down_row, d.down_expert, eb);
     const bool route_words = x_copy == kBy16 && d.hidden % 8 == 0 && copy_of(d.router, d.router_row, 0, eb) == kBy16;
     const MoeKernels k = d.dtype == L2D_F32   ? pick_moe<float>(eights, route_words, copy_up, copy_down)
@@ -988,15 +976,15 @@ int l2d_moe_forward(l2d_moe_plan *p, const void *x, void *y, int32_t *ids, float
     L2D_CUDA_TRY(launch(k.route, dim3(d.experts, (tokens + kRouteTokens - 1) / kRouteTokens), kMoeThreads, 0, stream, a));
     const int up_rows = eb == 4 ? 2 : 8, down_rows = eb == 4 ? 4 : 16, step = eb == 4 ? 128 : 64;
     const int64_t entries = std::min<int64_t>(int64_t(tokens) * d.top, d.experts);
-    const int blocks = 2 * p->sms, warps = blocks * kMoeWarps;
-    const int s_up = parts_of(entries * ((d.inner + up_rows - 1) / up_rows), warps, static_cast<int>((d.hidden + step - 1) / step));
-    const int s_down = parts_of(entries * ((d.hidden + down_rows - 1) / down_rows), warps, static_cast<int>((d.inner + step - 1) / step));
-    if (p->allowed[0] != k.gate_up) L2D_CUDA_TRY(cudaFuncSetAttribute(k.gate_up, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem));
-    if (p->allowed[1] != k.down) L2D_CUDA_TRY(cudaFuncSetAttribute(k.down, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem));
+    const int grid_up = k.blocks[0] * p->sms, grid_down = k.blocks[1] * p->sms;
+    const int s_up = parts_of(entries * ((d.inner + up_rows - 1) / up_rows), grid_up * kMoeWarps, static_cast<int>((d.hidden + step - 1) / step));
+    const int s_down = parts_of(entries * ((d.hidden + down_rows - 1) / down_rows), grid_down * kMoeWarps, static_cast<int>((d.inner + step - 1) / step));
+    if (p->allowed[0] != k.gate_up) L2D_CUDA_TRY(cudaFuncSetAttribute(k.gate_up, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem[0]));
+    if (p->allowed[1] != k.down) L2D_CUDA_TRY(cudaFuncSetAttribute(k.down, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem[1]));
     p->allowed[0] = k.gate_up;
     p->allowed[1] = k.down;
-    L2D_CUDA_TRY(launch(k.gate_up, dim3(blocks), kMoeThreads, k.smem, stream, a, s_up));
-    L2D_CUDA_TRY(launch(k.down, dim3(blocks), kMoeThreads, k.smem, stream, a, s_down));
+    L2D_CUDA_TRY(launch(k.gate_up, dim3(grid_up), kMoeThreads, k.smem[0], stream, a, s_up));
+    L2D_CUDA_TRY(launch(k.down, dim3(grid_down), kMoeThreads, k.smem[1], stream, a, s_down));
     L2D_CUDA_TRY(launch(k.combine, dim3((a.hidden + kMoeThreads - 1) / kMoeThreads, tokens), kMoeThreads, 0, stream, a));
     return L2D_OK;
 }
