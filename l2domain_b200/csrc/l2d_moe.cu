@@ -2,7 +2,7 @@
 //
 // Memory bound: the weights of every chosen expert are read once and meet one token or a few.  Four launches, each of which
 // waits for the one before on the device and not on the host:
-//   k_route    a router row and up to eight tokens per block; the last block of eight tokens chooses their experts, the last of
+//   k_route    a router row and up to four tokens per block; the last block of these tokens chooses their experts, the last of
 //              all sorts (token, choice) pairs ("slots") into entries: an expert and up to so many slots as one pass takes
 //   k_experts  gate and up: silu(gate x) * (up x) of every slot, to scratch
 //   k_experts  down: of every slot, to scratch
@@ -22,7 +22,7 @@ namespace l2d {
 
 constexpr int kMaxExperts = 512;
 constexpr int kMoeThreads = 256, kMoeWarps = kMoeThreads / 32;
-constexpr int kRouteTokens = kMoeWarps;  // of a block of the router: a warp each chooses
+constexpr int kRouteTokens = 4;  // of a block of the router
 
 struct MoeArgs {
     const void *x, *router, *gate, *up, *down;
@@ -47,7 +47,7 @@ struct MoeArgs {
 
 // ---------------------------------------------------------------------------------------------
 // Router.  Its sums are 64-bit ones: they choose, and two experts whose scores differ by less than a 32-bit sum is off would be
-// chosen by the order of addition.  A router row's numbers are made 64-bit ones once for up to eight tokens.
+// chosen by the order of addition.  A router row's numbers are made 64-bit ones once for up to four tokens.
 // ---------------------------------------------------------------------------------------------
 
 template <typename T>
@@ -132,9 +132,10 @@ __device__ __forceinline__ void choose(const MoeArgs &a, int token) {
 __device__ __forceinline__ void sort_slots(const MoeArgs &a) {
     __shared__ int count[kMaxExperts], place[kMaxExperts], entry[kMaxExperts];
     const int tid = threadIdx.x, slots = a.tokens * a.top;
+    const int mine = tid < slots ? __ldcg(a.ids + tid) : 0;
     for (int e = tid; e < kMaxExperts; e += kMoeThreads) count[e] = 0;
     __syncthreads();
-    for (int s = tid; s < slots; s += kMoeThreads) atomicAdd(&count[__ldcg(a.ids + s)], 1);
+    for (int s = tid; s < slots; s += kMoeThreads) atomicAdd(&count[s == tid ? mine : __ldcg(a.ids + s)], 1);
     __syncthreads();
     if (tid < 32) {  // places and entries before each expert's: as many experts a lane
         const int kEach = (a.experts + 31) / 32;
@@ -166,20 +167,20 @@ __device__ __forceinline__ void sort_slots(const MoeArgs &a) {
         for (int done = 0, i = entry[e]; done < count[e]; done += a.per_entry, ++i)
             a.entries[i] = make_int4(e, place[e] + done, min(count[e] - done, a.per_entry), 0);
     __syncthreads();
-    for (int s = tid; s < slots; s += kMoeThreads) a.sorted[atomicAdd(&place[__ldcg(a.ids + s)], 1)] = s;
+    for (int s = tid; s < slots; s += kMoeThreads) a.sorted[atomicAdd(&place[s == tid ? mine : __ldcg(a.ids + s)], 1)] = s;
 }
 
 // Whether this block is the last of `n` to come here; what the others wrote before is then visible.
 __device__ __forceinline__ bool last_of(unsigned *arrived, unsigned n) {
     __shared__ bool last;
-    __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) {
+        __threadfence();  // after the barrier, for the whole block
         last = atomicAdd(arrived, 1u) == n - 1;
         if (last) *arrived = 0;
+        __threadfence();
     }
     __syncthreads();
-    if (last) __threadfence();
     return last;
 }
 
