@@ -7,6 +7,9 @@
 //   k_experts  gate and up: silu(gate x) * (up x) of every slot, to scratch
 //   k_experts  down: of every slot, to scratch
 //   k_combine  the weighted sum over a token's slots, in their order
+// (Measured and dropped for a token or a few: choosing in every block of gate and up, which saves a meeting of blocks, 8 us
+// there for 6.6 here; summing in the blocks of down, which saves a launch, with whole tiles of rows to a block: 20.6 us for
+// 17 + 5 at 4096 x 1536, and 45 for 30 in all at 1001 x 333.)
 // Nothing depends on the order in which blocks come: a slot's sums are its own.
 #include "l2d_launch.cuh"
 
@@ -64,68 +67,81 @@ __device__ __forceinline__ Eight<T> load_eight(const T *p) {
     return r;
 }
 
-// Chooses the experts of one token: a warp, `top` rounds over kEach scores a lane.
+// exp of a difference of two scores, to two roundings of fp32: the part that fp32 has not room for comes on top.
+__device__ __forceinline__ float exp_of(double d) {
+    const float hi = static_cast<float>(d), lo = static_cast<float>(d - hi), e = expf(hi);
+    return fabsf(hi) < 100.0f ? fmaf(e, lo, e) : e;
+}
+
+// Chooses the experts of one token: a warp, `top` rounds over kEach scores a lane, as numbers whose order is that of whole
+// numbers (fp64 comparisons took ten times as long).  What is no number comes last.
 template <int kEach>
-__device__ __forceinline__ void choose(const MoeArgs &a, int token) {
+__device__ __forceinline__ void choose_of(const MoeArgs &a, int token) {
     const int lane = threadIdx.x & 31;
     const double *logits = a.logits + static_cast<int64_t>(token) * a.experts;
     double v[kEach];
+    uint32_t high[kEach], low[kEach];
     uint32_t open = 0;  // this lane's experts that are not chosen yet
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
         const int e = lane + 32 * i;
         v[i] = 0.0;
         if (e < a.experts) {
-            v[i] = __ldcg(logits + e);
+            v[i] = __ldcg(logits + e) + 0.0;  // one zero
             open |= 1u << i;
         }
+        const uint64_t bits = static_cast<uint64_t>(__double_as_longlong(v[i])), order = bits >> 63 ? ~bits : bits | 1ull << 63;
+        const bool number = (bits & 0x7fffffffffffffffull) <= 0x7ff0000000000000ull;
+        high[i] = number ? static_cast<uint32_t>(order >> 32) : 0;
+        low[i] = number ? static_cast<uint32_t>(order) : 0;
     }
     int mine = 0;
     double score = 0.0, first = 0.0;  // of the choice that this lane keeps, and of the first
     for (int k = 0; k < a.top; ++k) {
-        double best = -INFINITY;
+        uint32_t h = 0, l = 0;
         int at = INT_MAX;
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const double x = v[i] == v[i] ? v[i] : -INFINITY;  // what is no number comes last
-            if ((open >> i & 1) && (x > best || at == INT_MAX)) best = x, at = lane + 32 * i;
-        }
-#pragma unroll
-        for (int d = 16; d; d >>= 1) {
-            const double x = __shfl_xor_sync(0xffffffffu, best, d);
-            const int i = __shfl_xor_sync(0xffffffffu, at, d);
-            if (i != INT_MAX && (at == INT_MAX || x > best || (x == best && i < at))) best = x, at = i;
-        }
+        for (int i = 0; i < kEach; ++i)
+            if ((open >> i & 1) && (at == INT_MAX || high[i] > h || (high[i] == h && low[i] > l))) h = high[i], l = low[i], at = lane + 32 * i;
+        const uint32_t top_high = __reduce_max_sync(0xffffffffu, h);
+        const bool with_high = at != INT_MAX && h == top_high;
+        const uint32_t top_low = __reduce_max_sync(0xffffffffu, with_high ? l : 0);
+        const int won = static_cast<int>(__reduce_min_sync(0xffffffffu, with_high && l == top_low ? static_cast<uint32_t>(at) : static_cast<uint32_t>(INT_MAX)));
         double given = 0.0;
 #pragma unroll
         for (int i = 0; i < kEach; ++i)
-            if (at == lane + 32 * i) {
+            if (won == lane + 32 * i) {
                 open &= ~(1u << i);
                 given = v[i];
             }
-        given = __shfl_sync(0xffffffffu, given, at & 31);
+        given = __shfl_sync(0xffffffffu, given, won & 31);
         if (k == 0) first = given;
-        if (k % 32 == lane) mine = at, score = given;
+        if (k == lane) mine = won, score = given;
     }
-    double sum = 0.0;
+    const float e = lane < a.top ? exp_of(score - first) : 0.0f;
+    float sum = 0.0f;
     if (a.normalize) {
-        if (lane < a.top) sum = exp(score - first);
+        sum = e;
     } else {
 #pragma unroll
         for (int i = 0; i < kEach; ++i)
-            if (lane + 32 * i < a.experts) sum += exp(v[i] - first);
+            if (lane + 32 * i < a.experts) sum += exp_of(v[i] - first);
     }
 #pragma unroll
     for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     if (lane < a.top) {
         const int64_t slot = static_cast<int64_t>(token) * a.top + lane;
-        const float w = static_cast<float>(exp(score - first) / sum);
+        const float w = e / sum;
         a.ids[slot] = mine;
         a.weights[slot] = w;
-        a.largest[slot] = 0;
         if (a.ids_out) a.ids_out[slot] = mine;
         if (a.weights_out) a.weights_out[slot] = w;
     }
+}
+__device__ __forceinline__ void choose(const MoeArgs &a, int token) {
+    if (a.experts <= 32) choose_of<1>(a, token);
+    else if (a.experts <= 128) choose_of<4>(a, token);
+    else choose_of<kMaxExperts / 32>(a, token);
 }
 
 // Sorts the slots by expert, and cuts each expert's into entries.
@@ -227,12 +243,10 @@ __global__ void __launch_bounds__(kMoeThreads) k_route(const __grid_constant__ M
         for (int i = 0; i < kMoeWarps; ++i) s += sums[i][tid];
         a.logits[static_cast<int64_t>(t0 + tid) * a.experts + e] = s;
     }
+    if (e == 0)
+        for (int i = tid; i < n * a.top; i += kMoeThreads) a.largest[static_cast<int64_t>(t0) * a.top + i] = 0;
     if (!last_of(a.arrived + 1 + blockIdx.y, gridDim.x)) return;
-    if (warp < n) {
-        if (a.experts <= 32) choose<1>(a, t0 + warp);
-        else if (a.experts <= 128) choose<4>(a, t0 + warp);
-        else choose<kMaxExperts / 32>(a, t0 + warp);
-    }
+    if (warp < n) choose(a, t0 + warp);
     if (gridDim.y > 1) {
         if (!last_of(a.arrived, gridDim.y)) return;
     } else {
@@ -319,15 +333,10 @@ struct Items {
         tile = by_entry ? item - entry * tiles : item / entries;
     }
 };
-__device__ __forceinline__ Items items_of(const MoeArgs &a, int tiles, int groups, int group) {
-    Items r;
-    r.tiles = tiles;
-    r.entries = *a.num_entries;
-    const int64_t total = static_cast<int64_t>(tiles) * r.entries;
-    // Even shares to within one item.
-    r.first = static_cast<int>(total * group / groups);
-    r.stop = static_cast<int>(total * (group + 1) / groups);
-    return r;
+// Even shares to within one item.
+__device__ __forceinline__ Items items_of(int entries, int tiles, int groups, int group) {
+    const int64_t total = static_cast<int64_t>(tiles) * entries;
+    return {tiles, entries, static_cast<int>(total * group / groups), static_cast<int>(total * (group + 1) / groups)};
 }
 
 __device__ __forceinline__ float silu_times(float gate, float up) { return gate / (1.0f + expf(-gate)) * up; }
@@ -362,16 +371,18 @@ __device__ __forceinline__ float to_half_range(uint32_t largest_bits) {
 struct Lists {
     const int4 *entries;
     const int *sorted;
+    int num;
 };
-__device__ __forceinline__ Lists lists_of(const MoeArgs &a, int entries) {
+__device__ __forceinline__ Lists lists_of(const MoeArgs &a) {
     __shared__ int4 kept_entries[kCached];
     __shared__ int kept_sorted[kCachedSlots];
     const int slots = a.tokens * a.top;
-    if (entries > kCached || slots > kCachedSlots) return {a.entries, a.sorted};
-    for (int i = threadIdx.x; i < entries; i += kMoeThreads) kept_entries[i] = a.entries[i];
+    const int num = *a.num_entries;
+    if (num > kCached || slots > kCachedSlots) return {a.entries, a.sorted, num};
+    for (int i = threadIdx.x; i < num; i += kMoeThreads) kept_entries[i] = a.entries[i];
     for (int i = threadIdx.x; i < slots; i += kMoeThreads) kept_sorted[i] = a.sorted[i];
     __syncthreads();
-    return {kept_entries, kept_sorted};
+    return {kept_entries, kept_sorted, num};
 }
 
 // A warp's ring: a step's rows, then its columns (16 bytes a lane of each eight and run, of four-byte elements twice), as deep as
@@ -396,8 +407,8 @@ __global__ void __launch_bounds__(kMoeThreads, ExpertsRing<N, DOWN>::kBlocks) k_
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int K = DOWN ? a.inner : a.hidden, rows = DOWN ? a.hidden : a.inner, per_tile = DOWN ? 16 : 8;
     const int part = warp % S, groups = kMoeWarps / S, group = warp / S;
-    const Items items = items_of(a, (rows + per_tile - 1) / per_tile, gridDim.x * groups, blockIdx.x * groups + group);
-    const Lists lists = lists_of(a, items.entries);
+    const Lists lists = lists_of(a);
+    const Items items = items_of(lists.num, (rows + per_tile - 1) / per_tile, gridDim.x * groups, blockIdx.x * groups + group);
     // This warp's part of K.  Only the last step of all may be short.
     const int all = (K + kK - 1) / kK, each = (all + S - 1) / S, begin = min(part * each, all), steps = min(begin + each, all) - begin;
     const bool short_end = begin + steps == all && K % kK;
@@ -612,8 +623,8 @@ __global__ void __launch_bounds__(kMoeThreads, 2) k_experts32(const __grid_const
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int K = DOWN ? a.inner : a.hidden, rows = DOWN ? a.hidden : a.inner, per_tile = DOWN ? 4 : 2;
     const int part = warp % S, groups = kMoeWarps / S, group = warp / S;
-    const Items items = items_of(a, (rows + per_tile - 1) / per_tile, gridDim.x * groups, blockIdx.x * groups + group);
-    const Lists lists = lists_of(a, items.entries);
+    const Lists lists = lists_of(a);
+    const Items items = items_of(lists.num, (rows + per_tile - 1) / per_tile, gridDim.x * groups, blockIdx.x * groups + group);
     const int all = (K + kK - 1) / kK, each = (all + S - 1) / S, begin = min(part * each, all), steps = min(begin + each, all) - begin;
     const int first_k = begin * kK + (COPY == kBy16 ? 4 * lane : lane);
     char *ring = smem + warp * kDepth32 * kRowBytes + lane * 16;
@@ -974,12 +985,13 @@ int l2d_moe_forward(l2d_moe_plan *p, const void *x, void *y, int32_t *ids, float
     const MoeKernels k = d.dtype == L2D_F32   ? pick_moe<float>(eights, route_words, copy_up, copy_down)
                          : d.dtype == L2D_F16 ? pick_moe<__half>(eights, route_words, copy_up, copy_down)
                                               : pick_moe<__nv_bfloat16>(eights, route_words, copy_up, copy_down);
-    L2D_CUDA_TRY(launch(k.route, dim3(d.experts, (tokens + kRouteTokens - 1) / kRouteTokens), kMoeThreads, 0, stream, a));
     const int up_rows = eb == 4 ? 2 : 8, down_rows = eb == 4 ? 4 : 16, step = eb == 4 ? 128 : 64;
+    const int64_t tiles_up = (d.inner + up_rows - 1) / up_rows, tiles_down = (d.hidden + down_rows - 1) / down_rows;
+    L2D_CUDA_TRY(launch(k.route, dim3(d.experts, (tokens + kRouteTokens - 1) / kRouteTokens), kMoeThreads, 0, stream, a));
     const int64_t entries = std::min<int64_t>(int64_t(tokens) * d.top, d.experts);
     const int grid_up = k.blocks[0] * p->sms, grid_down = k.blocks[1] * p->sms;
-    const int s_up = parts_of(entries * ((d.inner + up_rows - 1) / up_rows), grid_up * kMoeWarps, static_cast<int>((d.hidden + step - 1) / step));
-    const int s_down = parts_of(entries * ((d.hidden + down_rows - 1) / down_rows), grid_down * kMoeWarps, static_cast<int>((d.inner + step - 1) / step));
+    const int s_up = parts_of(entries * tiles_up, grid_up * kMoeWarps, static_cast<int>((d.hidden + step - 1) / step));
+    const int s_down = parts_of(entries * tiles_down, grid_down * kMoeWarps, static_cast<int>((d.inner + step - 1) / step));
     if (p->allowed[0] != k.gate_up) L2D_CUDA_TRY(cudaFuncSetAttribute(k.gate_up, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem[0]));
     if (p->allowed[1] != k.down) L2D_CUDA_TRY(cudaFuncSetAttribute(k.down, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem[1]));
     p->allowed[0] = k.gate_up;
