@@ -499,8 +499,8 @@ typedef struct {
 } l2d_kv4_cache;
 /* The bytes of one page of keys, or of values. */
 L2D_API int l2d_kv4_page_bytes(int heads, int head_dim, int page_size, int group, int64_t *bytes);
-/* As l2d_kv_append, with every product and sum of the rotation rounded to fp32 by itself; keys are not rounded to dtype before
- * they are held.  k_out and v_out (NULL: not wanted) get keys and values as they are held, rounded to dtype and strided as
+/* As l2d_kv_append, with every product and sum of the keys' rotation rounded to fp32 by itself; keys are not rounded to dtype
+ * before they are held.  k_out and v_out (NULL: not wanted) get keys and values as they are held, rounded to dtype and strided as
  * k and v: what the attention will see, for a prompt's own.  They may be k and v, and must not overlap them otherwise. */
 L2D_API int l2d_kv4_append(const l2d_kv4_cache *cache, const l2d_append_desc *desc, const void *k, const void *v, const void *q, void *q_out,
                            void *k_out, void *v_out, const int32_t *pos, const int32_t *seq, int64_t tokens, void *stream);

@@ -9,100 +9,10 @@
 
 namespace l2d {
 
-// ---------------------------------------------------------------------------------------------
-// Appending.
-//
-// A copy with a few multiplications: every element is read once and written once.  A head is cut into units
-// of VEC pairs (the rotated part: for the half layout VEC elements and their VEC partners, for the interleaved
-// one 2 VEC elements side by side) and of 2 VEC elements (the rest, and values), so that a thread moves 32 bytes
-// of 16-bit elements.  A thread keeps its unit's cosines and sines for as many heads of its token as the grid
-// leaves it: heads are split over blocks only while there are too few tokens to fill the GPU.
-// ---------------------------------------------------------------------------------------------
-
-constexpr int kAppendThreads = 256;
-
-// units: rotated units of a head (rot_units), then plain ones.  A thread's unit is fixed; the threads of a token
-// for which `rows` are left take every rows-th of its heads.
 template <typename T, int VEC, bool INTERLEAVED>
 __global__ void __launch_bounds__(kAppendThreads) k_append(const __grid_constant__ AppendArgs a, int units, int rot_units, int rows) {
     dev::wait_for_previous();
-    const int D = a.c.head_dim, half = a.rot_dim / 2, hk = a.c.heads, heads = a.heads_q + 2 * hk;
-    const int64_t thread = static_cast<int64_t>(blockIdx.x) * kAppendThreads + threadIdx.x;
-    const int64_t t = thread / (units * rows);
-    if (t >= a.tokens) return;
-    const int rest = static_cast<int>(thread - t * (units * rows)), row = rest / units, unit = rest - row * units;
-    const int p = a.pos[t];
-    if (p < 0) return;
-    if (a.rot_dim && p >= a.max_pos) {
-        if (rest == 0) report(a.c.status, L2D_KV_BAD_POSITION);
-        return;
-    }
-    const int64_t page = page_of(a.c, a.seq ? a.seq[t] : t, p);
-    if (page < 0) {
-        if (rest == 0) report(a.c.status, L2D_KV_BAD_PAGE);
-        return;
-    }
-    const int slot = p - static_cast<int>(page_index(a.c, p)) * a.c.page_size;
-    const T *k = static_cast<const T *>(a.k) + t * a.k_token, *v = static_cast<const T *>(a.v) + t * a.v_token;
-    const T *q = static_cast<const T *>(a.q) + t * a.q_token;
-    T *q_out = static_cast<T *>(a.q_out) + t * a.q_out_token;
-    T *kc = reinterpret_cast<T *>(a.c.k) + page * a.c.k_page + slot * a.c.k_slot;
-    T *vc = reinterpret_cast<T *>(a.c.v) + page * a.c.v_page + slot * a.c.v_slot;
-
-    // Where the unit's two halves are, and its angles.
-    const bool rotated = unit < rot_units;
-    const int pair = unit * VEC;  // first pair of a rotated unit
-    const int first = !rotated ? a.rot_dim + (unit - rot_units) * 2 * VEC : INTERLEAVED ? 2 * pair : pair;
-    const int second = rotated && !INTERLEAVED ? pair + half : first + VEC;
-    const bool both = rotated || second < D;  // the plain part may end with one half
-    float c[VEC], s[VEC];
-    if (rotated) {
-        const Pack<float, VEC> cc = load_pack<float, VEC>(a.cos + static_cast<int64_t>(p) * half + pair);
-        const Pack<float, VEC> ss = load_pack<float, VEC>(a.sin + static_cast<int64_t>(p) * half + pair);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) c[i] = cc.v[i], s[i] = ss.v[i];
-    }
-    // Heads in order: queries, keys, values; a few at a time, loads first.
-    auto at = [&](int h, const T *&src, T *&dst) {
-        const int g = h - a.heads_q, w = g - hk;
-        if (g < 0) src = q + static_cast<int64_t>(h) * D, dst = q_out + static_cast<int64_t>(h) * D;
-        else if (w < 0) src = k + static_cast<int64_t>(g) * D, dst = kc + g * a.c.k_head;
-        else src = v + static_cast<int64_t>(w) * D, dst = vc + w * a.c.v_head;
-    };
-    constexpr int kHeads = 4;
-    for (int h0 = row; h0 < heads; h0 += kHeads * rows) {
-        Pack<T, VEC> x[kHeads], y[kHeads];
-        T *dst[kHeads];
-#pragma unroll
-        for (int j = 0; j < kHeads; ++j) {
-            const T *src = nullptr;
-            dst[j] = nullptr;
-            if (h0 + j * rows >= heads) continue;
-            at(h0 + j * rows, src, dst[j]);
-            x[j] = load_pack<T, VEC>(src + first);
-            if (both) y[j] = load_pack<T, VEC>(src + second);
-        }
-#pragma unroll
-        for (int j = 0; j < kHeads; ++j) {
-            if (h0 + j * rows >= heads) continue;
-            if (rotated && h0 + j * rows < a.heads_q + hk) {
-                float u[2 * VEC];
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) u[i] = dev::widen(x[j].v[i]), u[VEC + i] = dev::widen(y[j].v[i]);
-                T r[2 * VEC];
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    const int lo = INTERLEAVED ? 2 * i : i, hi = INTERLEAVED ? 2 * i + 1 : VEC + i;
-                    r[lo] = dev::narrow<T>(fmaf(u[lo], c[i], -(u[hi] * s[i])));
-                    r[hi] = dev::narrow<T>(fmaf(u[hi], c[i], u[lo] * s[i]));
-                }
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) x[j].v[i] = r[i], y[j].v[i] = r[VEC + i];
-            }
-            store_pack<T, VEC>(dst[j] + first, x[j]);
-            if (both) store_pack<T, VEC>(dst[j] + second, y[j]);
-        }
-    }
+    append_heads<T, VEC, INTERLEAVED>(a, blockIdx.x, units, rot_units, rows, a.heads_q + 2 * a.c.heads);
 }
 
 // Checks a cache description and fills in its strides.
@@ -341,7 +251,7 @@ int l2d_kv_append(const l2d_kv_cache *cache, const l2d_append_desc *desc, const 
     if (d.heads_q) all |= a.q_token | a.q_out_token;
     const bool words = all % vec == 0 && !misaligned(k, 16) && !misaligned(v, 16) && !misaligned(q, 16) && !misaligned(q_out, 16) &&
                        !misaligned(a.c.k, 16) && !misaligned(a.c.v, 16) && !misaligned(d.cos, 16) && !misaligned(d.sin, 16);
-    const int each = words ? vec : 1, rot_units = half / each, units = rot_units + (D - d.rot_dim + 2 * each - 1) / (2 * each);
+    const auto [units, rot_units] = append_units(words, eb, D, d.rot_dim);
     // Heads of a token in one thread: all of them, or as few as it takes for two blocks a SM.
     const int heads = d.heads_q + 2 * cache->heads;
     const int64_t want = int64_t(sms) * 2 * kAppendThreads, have = tokens * units;

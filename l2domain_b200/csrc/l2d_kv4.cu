@@ -8,14 +8,40 @@ namespace l2d {
 // ---------------------------------------------------------------------------------------------
 // Appending.
 //
-// The same copy as to a cache of 16 or 32 bits, with a maximum and a minimum per group in between.  A thread has eight
+// Queries are rotated as beside a cache of 16 or 32 bits.  Keys and values: a copy with a maximum and a minimum per group in
+// between.  A thread has eight
 // elements of a row (one word of nibbles), the threads of a row, a power of two of them, are neighbours in a warp and
 // meet by shuffles; a thread keeps its angles for as many heads of its token as the grid leaves it.  Products,
 // sums and quotients are rounded one by one to fp32, so that what is stored follows from the inputs and not from how an
 // expression was compiled.
 // ---------------------------------------------------------------------------------------------
 
-constexpr int kAppend4Threads = 256;
+// Two numbers at a time, each rounded as by itself.
+__device__ __forceinline__ unsigned long long bits_of(float2 v) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
+    return r;
+}
+__device__ __forceinline__ float2 two_of(unsigned long long b) {
+    float2 v;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(b));
+    return v;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits_of(a)), "l"(bits_of(b)));
+    return two_of(r);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits_of(a)), "l"(bits_of(b)));
+    return two_of(r);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits_of(a)), "l"(bits_of(b)), "l"(bits_of(c)));
+    return two_of(r);
+}
 
 struct Append4Args {
     AppendArgs a;
@@ -24,17 +50,14 @@ struct Append4Args {
 
 // Eight elements from p on, of which those at d, d + 1, .. below D are real; by 16-byte words where WORDS.
 template <typename T, bool WORDS>
-__device__ __forceinline__ void load8(float (&x)[8], const T *p, int d, int D) {
+__device__ __forceinline__ Pack<T, 8> load8(const T *p, int d, int D) {
+    Pack<T, 8> r;
     if constexpr (WORDS) {
-        if (d < D) {
-            const Pack<T, 8> r = load_pack<T, 8>(p);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = dev::widen(r.v[i]);
-            return;
-        }
+        if (d < D) return load_pack<T, 8>(p);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = d + i < D ? dev::widen(p[i]) : 0.0f;
+    for (int i = 0; i < 8; ++i) r.v[i] = d + i < D ? p[i] : dev::narrow<T>(0.0f);
+    return r;
 }
 template <typename T, bool WORDS>
 __device__ __forceinline__ void store8(T *p, const float (&x)[8], int d, int D) {
@@ -53,12 +76,11 @@ __device__ __forceinline__ void store8(T *p, const float (&x)[8], int d, int D) 
 // lanes: threads of a row; the lanes * rows threads of a token take every rows-th of its heads.  WORDS: every row, and the
 // second halves of rotated ones, on 16-byte boundaries, and angles too.
 template <typename T, bool WORDS, bool INTERLEAVED>
-__global__ void __launch_bounds__(kAppend4Threads) k_append4(const __grid_constant__ Append4Args args, int lanes, int rows) {
-    dev::wait_for_previous();
+__device__ __forceinline__ void append4(const Append4Args &args, unsigned block_at, int lanes, int rows) {
     const AppendArgs &a = args.a;
-    const int D = a.c.head_dim, half = a.rot_dim / 2, hk = a.c.heads, heads = a.heads_q + 2 * hk;
-    const int64_t thread = static_cast<int64_t>(blockIdx.x) * kAppend4Threads + threadIdx.x;
-    const int64_t t = thread / (lanes * rows);
+    const int D = a.c.head_dim, half = a.rot_dim / 2, hk = a.c.heads;
+    const int64_t thread = static_cast<int64_t>(block_at) * kAppendThreads + threadIdx.x;
+    const int64_t t = quotient(thread, lanes * rows);
     if (t >= a.tokens) return;
     const int rest = static_cast<int>(thread - t * (lanes * rows)), row = rest / lanes, unit = rest - row * lanes, lane = threadIdx.x & 31;
     const unsigned mine = lanes == 32 ? 0xffffffffu : ((1u << lanes) - 1) << (lane & ~(lanes - 1));  // the threads of this row
@@ -75,23 +97,20 @@ __global__ void __launch_bounds__(kAppend4Threads) k_append4(const __grid_consta
     }
     const int slot = p - static_cast<int>(page_index(a.c, p)) * a.c.page_size, inside = slot % kBlockSlots;
     const int chunks = (D + kChunk - 1) / kChunk, meet = min(a.c.group / 8, lanes), d = 8 * unit;
-    const int64_t block = static_cast<int64_t>(slot / kBlockSlots) * hk * a.c.tile_bytes;
-    const T *k = static_cast<const T *>(a.k) + t * a.k_token, *v = static_cast<const T *>(a.v) + t * a.v_token;
-    const T *q = static_cast<const T *>(a.q) + t * a.q_token;
-    T *q_out = static_cast<T *>(a.q_out) + t * a.q_out_token;
 
     // The angles of this thread's elements, and where the other elements of their pairs are: the second halves' angles
     // turn the other way.
+    const bool rotated = d < a.rot_dim;
     float cs[8], sn[8];
-    int other = 0;
-    if (d < a.rot_dim) {
+    int other[WORDS ? 1 : 8] = {};
+    if (rotated) {
         const float *cos = a.cos + static_cast<int64_t>(p) * half, *sin = a.sin + static_cast<int64_t>(p) * half;
         if constexpr (WORDS && !INTERLEAVED) {
             const bool second = d >= half;
             const Pack<float, 8> c8 = load_pack<float, 8>(cos + (second ? d - half : d)), s8 = load_pack<float, 8>(sin + (second ? d - half : d));
 #pragma unroll
             for (int i = 0; i < 8; ++i) cs[i] = c8.v[i], sn[i] = second ? s8.v[i] : -s8.v[i];
-            other = second ? -half : half;
+            other[0] = second ? -half : half;
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -100,83 +119,147 @@ __global__ void __launch_bounds__(kAppend4Threads) k_append4(const __grid_consta
                 const int pair = INTERLEAVED ? e / 2 : second ? e - half : e;
                 cs[i] = in ? cos[pair] : 1.0f;
                 sn[i] = in ? (second ? sin[pair] : -sin[pair]) : 0.0f;
+                if constexpr (!WORDS) other[i] = !in ? 0 : second ? -half : half;
             }
         }
     }
-    auto rotate = [&](float (&x)[8], const T *src) {  // src: this thread's elements
-        float y[8];
-        if constexpr (INTERLEAVED) {
+    // This thread's elements of a head at src, and the others of their pairs.
+    auto load = [&](Pack<T, 8> &own, Pack<T, 8> &pair, const T *src, bool turn) {
+        own = load8<T, WORDS>(src, d, D);
+        if constexpr (!INTERLEAVED) {
+            if (!turn || !rotated) return;
+            if constexpr (WORDS) {
+                pair = load_pack<T, 8>(src + other[0]);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
-        } else if constexpr (WORDS) {
-            load8<T, true>(y, src + other, 0, 8);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int e = d + i;
-                y[i] = e < a.rot_dim ? dev::widen(src[i + (e >= half ? -half : half)]) : 0.0f;
+                for (int i = 0; i < 8; ++i) pair.v[i] = d + i < D ? src[i + other[i]] : dev::narrow<T>(0.0f);
             }
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (d + i < a.rot_dim) x[i] = __fadd_rn(__fmul_rn(x[i], cs[i]), __fmul_rn(y[i], sn[i]));
     };
-    // Heads in order: queries, keys, values; a few at a time, loads first.
-    constexpr int kHeads = 2;
-    for (int h0 = row; h0 < heads; h0 += kHeads * rows) {
-        float x[kHeads][8];
+    auto rotate = [&](float (&x)[8], const Pack<T, 8> &own, const Pack<T, 8> &pair) {
 #pragma unroll
-        for (int j = 0; j < kHeads; ++j) {
-            const int h = h0 + j * rows, g = h - a.heads_q, w = g - hk;
-            if (h >= heads) continue;
-            const T *src = (g < 0 ? q + static_cast<int64_t>(h) * D : w < 0 ? k + static_cast<int64_t>(g) * D : v + static_cast<int64_t>(w) * D) + d;
-            load8<T, WORDS>(x[j], src, d, D);
-            if (w < 0 && d < a.rot_dim) rotate(x[j], src);
+        for (int i = 0; i < 8; i += 2) {
+            float2 u = make_float2(dev::widen(own.v[i]), dev::widen(own.v[i + 1]));
+            if (rotated) {
+                const float2 y = INTERLEAVED ? make_float2(u.y, u.x) : make_float2(dev::widen(pair.v[i]), dev::widen(pair.v[i + 1]));
+                // (The sum of two products taken as one multiply-add would be rounded once.)
+                const float2 one = mul2(u, make_float2(cs[i], cs[i + 1])), two = mul2(y, make_float2(sn[i], sn[i + 1]));
+                const float2 turned = make_float2(__fadd_rn(one.x, two.x), __fadd_rn(one.y, two.y));
+                if (WORDS || d + i < a.rot_dim) u.x = turned.x;
+                if (WORDS || d + i + 1 < a.rot_dim) u.y = turned.y;
+            }
+            x[i] = u.x;
+            x[i + 1] = u.y;
         }
-        __syncwarp(mine);  // outputs may be the inputs
+    };
+    // Holds a head's elements x in the tile, and leaves in x what they stand for.
+    auto hold = [&](float (&x)[8], char *tile) {
+        float lo = 0.0f, hi = 0.0f;
+        float2 odd = make_float2(0.0f, 0.0f);  // 0 times an infinity or a NaN is one
 #pragma unroll
-        for (int j = 0; j < kHeads; ++j) {
-            const int h = h0 + j * rows, g = h - a.heads_q, w = g - hk;
-            if (h >= heads) continue;
-            if (g < 0) {
-                store8<T, WORDS>(q_out + static_cast<int64_t>(h) * D + d, x[j], d, D);
-                continue;
-            }
-            float lo = 0.0f, hi = 0.0f;
-            bool bad = false;
+        for (int i = 0; i < 8; i += 2) {
+            lo = fminf(lo, fminf(x[i], x[i + 1]));
+            hi = fmaxf(hi, fmaxf(x[i], x[i + 1]));
+            odd = fma2(make_float2(x[i], x[i + 1]), make_float2(0.0f, 0.0f), odd);
+        }
+        if (!(odd.x + odd.y == 0.0f)) hi = INFINITY;
+        for (int m = 1; m < meet; m <<= 1) {
+            lo = fminf(lo, __shfl_xor_sync(mine, lo, m));
+            hi = fmaxf(hi, __shfl_xor_sync(mine, hi, m));
+        }
+        constexpr float kFifteenth = 1.0f / 15.0f;
+        uint32_t word = (__float_as_uint(__fsub_rn(__fmul_rn(hi, kFifteenth), __fmul_rn(lo, kFifteenth))) + 15u) & ~15u;
+        const bool bad = hi == INFINITY;
+        const float by = word == 0 ? 1.0f : __uint_as_float(word), inverse = 1.0f / by;
+        float z = fminf(rintf(__fdiv_rn(-lo, by)), 15.0f), s = __uint_as_float(word);
+        // x / s rounded to a whole number.  By the reciprocal it is off by less than 2^-20; where that may decide, and where
+        // the reciprocal is no number, the quotient itself is taken.  Adding 1.5 * 2^23 rounds to whole numbers.
+        constexpr float kWhole = 12582912.0f;
+        float2 near[4];
+        float far = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                lo = fminf(lo, x[j][i]);
-                hi = fmaxf(hi, x[j][i]);
-                bad |= !(fabsf(x[j][i]) <= FLT_MAX);
-            }
-            if (bad) hi = INFINITY;
-            for (int m = 1; m < meet; m <<= 1) {
-                lo = fminf(lo, __shfl_xor_sync(mine, lo, m));
-                hi = fmaxf(hi, __shfl_xor_sync(mine, hi, m));
-            }
-            constexpr float kFifteenth = 1.0f / 15.0f;
-            uint32_t word = (__float_as_uint(__fsub_rn(__fmul_rn(hi, kFifteenth), __fmul_rn(lo, kFifteenth))) + 15u) & ~15u;
-            if (hi == INFINITY) word = 0x7fc00000u;
-            const float s = __uint_as_float(word), by = word == 0 ? 1.0f : s;
-            const float z = hi == INFINITY ? 0.0f : fminf(rintf(__fdiv_rn(-lo, by)), 15.0f);
-            uint32_t nibbles = 0;
+        for (int i = 0; i < 4; ++i) {
+            const float2 r = mul2(make_float2(x[2 * i], x[2 * i + 1]), make_float2(inverse, inverse));
+            near[i] = add2(add2(r, make_float2(kWhole, kWhole)), make_float2(-kWhole, -kWhole));
+            const float2 off = fma2(near[i], make_float2(-1.0f, -1.0f), r);
+            far = fmaxf(far, fmaxf(fabsf(off.x), fabsf(off.y)));
+        }
+        if (!(far < 0.5f - 0x1p-17f) || !(inverse <= FLT_MAX)) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                // Of a group that is not a number every difference is 0.
-                const float n = hi == INFINITY ? 0.0f : fminf(fmaxf(rintf(__fdiv_rn(x[j][i], by)) + z, 0.0f), 15.0f);
-                if (d + i < D) nibbles |= static_cast<uint32_t>(n) << (4 * i);
-                x[j][i] = s * (n - z);
+            for (int i = 0; i < 4; ++i) near[i] = make_float2(rintf(__fdiv_rn(x[2 * i], by)), rintf(__fdiv_rn(x[2 * i + 1], by)));
+        }
+        if (bad) {  // every number is 0, and stands for NaN
+            word = 0x7fc00000u;
+            s = __uint_as_float(word);
+            z = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) near[i] = make_float2(0.0f, 0.0f);
+        }
+        // Four numbers of 0..15 are one below 2^16.
+        float four[2] = {};
+#pragma unroll
+        for (int i = 3; i >= 0; --i) {
+            float2 n = add2(near[i], make_float2(z, z));
+            n = make_float2(fminf(fmaxf(n.x, 0.0f), 15.0f), fminf(fmaxf(n.y, 0.0f), 15.0f));
+            if (!WORDS) n = make_float2(d + 2 * i < D ? n.x : 0.0f, d + 2 * i + 1 < D ? n.y : 0.0f);
+            four[i / 2] = fmaf(four[i / 2], 16.0f, n.y);
+            four[i / 2] = fmaf(four[i / 2], 16.0f, n.x);
+            const float2 stands = mul2(make_float2(s, s), add2(n, make_float2(-z, -z)));
+            x[2 * i] = stands.x;
+            x[2 * i + 1] = stands.y;
+        }
+        const uint32_t nibbles = __byte_perm(__float_as_uint(four[0] + kWhole), __float_as_uint(four[1] + kWhole), 0x5410);
+        if (unit < 4 * chunks) *reinterpret_cast<uint32_t *>(tile + (unit / 4) * kChunkBytes + inside * 16 + (unit % 4) * 4) = d < D ? nibbles : 0;
+        if (d < D && d % a.c.group == 0)
+            *reinterpret_cast<uint32_t *>(tile + chunks * kChunkBytes + d / a.c.group * kGroupBytes + inside * 4) = word | static_cast<uint32_t>(z);
+    };
+    // Every rows-th head is this thread's, a few at a time and loads first.  The barriers: outputs may be the inputs.
+    constexpr int kHeads = WORDS ? 2 : 1;
+    const int64_t block = static_cast<int64_t>(slot / kBlockSlots) * hk * a.c.tile_bytes;
+#pragma unroll 1
+    for (int which = 0; which < 2; ++which) {  // keys, then values
+        const int64_t at = t * (which ? a.v_token : a.k_token) + d;
+        const T *from = static_cast<const T *>(which ? a.v : a.k) + at;
+        T *out = static_cast<T *>(which ? args.v_out : args.k_out);
+        const bool tell = out;
+        out += at;
+        char *tiles = (which ? a.c.v + page * a.c.v_page : a.c.k + page * a.c.k_page) + block;
+#pragma unroll 1
+        for (int h0 = row; h0 < hk; h0 += kHeads * rows) {
+            Pack<T, 8> own[kHeads], pair[kHeads];
+#pragma unroll
+            for (int j = 0; j < kHeads; ++j)
+                if (h0 + j * rows < hk) load(own[j], pair[j], from + (h0 + j * rows) * D, !which);
+            __syncwarp(mine);
+#pragma unroll
+            for (int j = 0; j < kHeads; ++j) {
+                const int h = h0 + j * rows;
+                if (h >= hk) continue;
+                float x[8];
+                if (!which) {
+                    rotate(x, own[j], pair[j]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[i] = dev::widen(own[j].v[i]);
+                }
+                hold(x, tiles + h * a.c.tile_bytes);
+                if (tell) store8<T, WORDS>(out + h * D, x, d, D);
             }
-            char *tile = w < 0 ? a.c.k + page * a.c.k_page + block + static_cast<int64_t>(g) * a.c.tile_bytes
-                               : a.c.v + page * a.c.v_page + block + static_cast<int64_t>(w) * a.c.tile_bytes;
-            if (unit < 4 * chunks) *reinterpret_cast<uint32_t *>(tile + (unit / 4) * kChunkBytes + inside * 16 + (unit % 4) * 4) = nibbles;
-            if (d < D && d % a.c.group == 0)
-                *reinterpret_cast<uint32_t *>(tile + chunks * kChunkBytes + d / a.c.group * kGroupBytes + inside * 4) = word | static_cast<uint32_t>(z);
-            T *out = static_cast<T *>(w < 0 ? args.k_out : args.v_out);
-            if (out) store8<T, WORDS>(out + (w < 0 ? t * a.k_token + static_cast<int64_t>(g) * D : t * a.v_token + static_cast<int64_t>(w) * D) + d, x[j], d, D);
         }
     }
+}
+
+// Queries, as a cache of 16 or 32 bits has them, in the first `query.blocks` blocks; keys and values.
+struct QueryBlocks {
+    unsigned blocks;
+    int units, rot_units, rows;
+};
+template <typename T, bool WORDS, bool INTERLEAVED, bool QUERY_WORDS>
+__global__ void __launch_bounds__(kAppendThreads, 3) k_append4(const __grid_constant__ Append4Args args, QueryBlocks query, int lanes, int rows) {
+    dev::wait_for_previous();
+    constexpr int kVec = QUERY_WORDS ? 16 / static_cast<int>(sizeof(T)) : 1;
+    if (blockIdx.x < query.blocks) append_heads<T, kVec, INTERLEAVED>(args.a, blockIdx.x, query.units, query.rot_units, query.rows, args.a.heads_q);
+    else append4<T, WORDS, INTERLEAVED>(args, blockIdx.x - query.blocks, lanes, rows);
 }
 
 AttnKernel pick_attn_kv4(int dtype, int D, int group, int G) {
@@ -254,27 +337,42 @@ int l2d_kv4_append(const l2d_kv4_cache *cache, const l2d_append_desc *desc, cons
     L2D_CUDA_TRY(on.err);
     args.k_out = k_out;
     args.v_out = v_out;
-    // Eight elements of 16 bits, or half as many of 32, are a word; halves of heads are whole runs of eight or interleaved.
-    const int64_t each = 8, in_words = 16 / eb;
-    const bool words = D % each == 0 && a.rot_dim % each == 0 && (desc->interleaved || half % each == 0) && a.k_token % in_words == 0 &&
-                       a.v_token % in_words == 0 && a.q_token % in_words == 0 && a.q_out_token % in_words == 0 && !misaligned(k, 16) &&
-                       !misaligned(v, 16) && !misaligned(q, 16) && !misaligned(q_out, 16) && !misaligned(k_out, 16) && !misaligned(v_out, 16) &&
-                       (desc->interleaved || (!misaligned(a.cos, 16) && !misaligned(a.sin, 16)));
+    // Runs of eight elements, in whole words.
+    const int in_words = 16 / eb;
+    const bool words = D % 8 == 0 && a.rot_dim % 8 == 0 && (desc->interleaved || half % 8 == 0) && a.k_token % in_words == 0 &&
+                       a.v_token % in_words == 0 && !misaligned(k, 16) && !misaligned(v, 16) && !misaligned(k_out, 16) && !misaligned(v_out, 16) &&
+                       !misaligned(a.cos, 16) && !misaligned(a.sin, 16);
+    const bool query_words = desc->heads_q && (D | half | a.q_token | a.q_out_token) % in_words == 0 && !misaligned(q, 16) && !misaligned(q_out, 16) &&
+                             !misaligned(a.cos, 16) && !misaligned(a.sin, 16);
     int lanes = 4;  // of a row, so that its groups meet by shuffles
     while (lanes * 8 < D) lanes *= 2;
-    // Heads of a token in one thread: all of them, or as few as it takes for four blocks a SM.
-    const int heads = desc->heads_q + 2 * cache->heads;
-    const int64_t want = int64_t(sms) * 4 * kAppend4Threads, have = tokens * lanes;
-    const int rows = static_cast<int>(std::min<int64_t>(heads, std::max<int64_t>(1, (want + have - 1) / have)));
-    const int64_t blocks = (have * rows + kAppend4Threads - 1) / kAppend4Threads;
+    // Heads of a token in one thread: all of them, or as few as it takes for eight blocks a SM (two of queries).
+    auto rows_of = [&](int heads, int64_t threads, int per_sm) {
+        return static_cast<int>(std::min<int64_t>(heads, std::max<int64_t>(1, (int64_t(sms) * per_sm * kAppendThreads + threads - 1) / threads)));
+    };
+    const int rows = rows_of(cache->heads, tokens * lanes, 8);
+    int64_t blocks = (tokens * lanes * rows + kAppendThreads - 1) / kAppendThreads;
+    QueryBlocks query = {};
+    if (desc->heads_q) {
+        const AppendUnits u = append_units(query_words, eb, D, a.rot_dim);
+        query.units = u.units;
+        query.rot_units = u.rot_units;
+        query.rows = rows_of(desc->heads_q, tokens * u.units, 2);
+        const int64_t n = (tokens * u.units * query.rows + kAppendThreads - 1) / kAppendThreads;
+        blocks += n;
+        query.blocks = static_cast<unsigned>(std::min<int64_t>(n, INT32_MAX));
+    }
     if (blocks > INT32_MAX) return set_error(L2D_ERR_INVALID, "%lld tokens are too many", static_cast<long long>(tokens));
-    auto pick = [&](auto type) {
+    auto pick_query = [&](auto type, auto in_runs, auto interleaved) {
         using T = decltype(type);
-        if (words) return desc->interleaved ? k_append4<T, true, true> : k_append4<T, true, false>;
-        return desc->interleaved ? k_append4<T, false, true> : k_append4<T, false, false>;
+        return query_words ? k_append4<T, decltype(in_runs)::value, decltype(interleaved)::value, true> : k_append4<T, decltype(in_runs)::value, decltype(interleaved)::value, false>;
+    };
+    auto pick = [&](auto type) {
+        if (words) return desc->interleaved ? pick_query(type, std::true_type(), std::true_type()) : pick_query(type, std::true_type(), std::false_type());
+        return desc->interleaved ? pick_query(type, std::false_type(), std::true_type()) : pick_query(type, std::false_type(), std::false_type());
     };
     auto kernel = cache->dtype == L2D_F32 ? pick(float()) : cache->dtype == L2D_F16 ? pick(__half()) : pick(__nv_bfloat16());
-    L2D_CUDA_TRY(launch(kernel, dim3(static_cast<unsigned>(blocks)), kAppend4Threads, 0, stream, args, lanes, rows));
+    L2D_CUDA_TRY(launch(kernel, dim3(static_cast<unsigned>(blocks)), kAppendThreads, 0, stream, args, query, lanes, rows));
     return L2D_OK;
 }
 
