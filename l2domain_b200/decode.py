@@ -1,10 +1,11 @@
-"""The attention part of a decoding step, from this package's operators: 4-bit projections, the append to the
-paged cache with its rotation, attention over the cache, and the 4-bit output projection.
+"""A layer's decoding step, from this package's operators: 4-bit projections, the append to the paged cache with its
+rotation, attention over the cache, the 4-bit output projection, and a mixture of experts.
 
     python -m l2domain_b200.decode --batch 8 --length 4096 [--hidden 4096 --heads 32 --kv-heads 8 --head-dim 128]
+                                   [--cache-bits 4 --cap 50 --slopes] [--experts 64 --top 4 --inner 1024]
 
 runs steps of that shape on synthetic weights and an already filled cache, as one captured graph, and prints the
-mean time of a step with the bytes it cannot do without.
+mean time of a step with the bytes it cannot do without.  Without --experts a step is the attention part alone.
 """
 from __future__ import annotations
 
@@ -55,10 +56,12 @@ class DecodeAttention:
     """One layer's attention for ``batch`` sequences of up to ``max_len`` tokens, in bf16 with 4-bit weights.
 
     ``w_qkv`` [(heads + 2 kv_heads) * head_dim][hidden] and ``w_out`` [hidden][heads * head_dim] are packed once.
+    ``cache_bits`` is 16, or 4 with a scale per ``cache_group`` elements; ``cap`` and ``slopes`` as in :class:`PagedAttention`.
     :meth:`step` takes one new token per sequence; it allocates nothing and may be captured into a graph."""
 
     def __init__(self, w_qkv, w_out, heads: int, kv_heads: int, head_dim: int, batch: int, max_len: int, group: int = 128,
-                 page_size: int = 16, theta: float = 10000.0, device: int = 0):
+                 page_size: int = 16, theta: float = 10000.0, device: int = 0, cache_bits: int = 16, cache_group: int = 128,
+                 cap: float = 0.0, slopes=None):
         import torch
 
         self.heads, self.kv_heads, self.head_dim, self.batch = heads, kv_heads, head_dim, batch
@@ -72,31 +75,70 @@ class DecodeAttention:
 
         self.qkv_matrix, self.out_matrix = matrix(w_qkv), matrix(w_out)
         width = -(-max_len // page_size)
-        shape = (batch * width, page_size, kv_heads, head_dim)
-        self.k, self.v = (torch.zeros(shape, dtype=torch.bfloat16, device=dev) for _ in range(2))
+        pages = batch * width
+        if cache_bits == 4:
+            shape, kind = (pages, L.kv4_page_bytes(page_size, kv_heads, head_dim, cache_group)), torch.uint8
+            self.key_bytes = (head_dim + 1) // 2 + 4 * -(-head_dim // cache_group)  # of one key or value of one head
+        elif cache_bits == 16:
+            shape, kind = (pages, page_size, kv_heads, head_dim), torch.bfloat16
+            self.key_bytes = 2 * head_dim
+        else:
+            raise ValueError(f"a cache of {cache_bits} bits: 16 or 4")
+        self.k, self.v = (torch.zeros(shape, dtype=kind, device=dev) for _ in range(2))
         # Pages in the order sequences get them, one after the other; any other order does as well.
         self.table = torch.arange(batch * width, dtype=torch.int32, device=dev).view(width, batch).t().contiguous()
         self.status = torch.zeros(1, dtype=torch.int32, device=dev)
-        cache = L.KvCache(self.k, self.v, L.BF16, shape[0], page_size, kv_heads, head_dim, device=device)
+        if cache_bits == 4:
+            cache = L.KvCache4(self.k, self.v, L.BF16, pages, page_size, kv_heads, head_dim, cache_group, device=device)
+        else:
+            cache = L.KvCache(self.k, self.v, L.BF16, pages, page_size, kv_heads, head_dim, device=device)
         row = (heads + 2 * kv_heads) * head_dim
         self.cos, self.sin = L.rotation_tables(max_len, head_dim, theta, device=dev)
         self.append = L.KvAppend(cache, self.table, batch, width, heads_q=heads, cos=self.cos, sin=self.sin, max_pos=max_len,
                                  rot_dim=head_dim, k_token=row, v_token=row, q_token=row, q_out_token=row, status=self.status)
-        self.attention = L.PagedAttention(cache, self.table, batch, width, heads, q_token=row, status=self.status)
+        self.attention = L.PagedAttention(cache, self.table, batch, width, heads, q_token=row, status=self.status, cap=cap, slopes=slopes)
         self.qkv = torch.zeros(batch, row, dtype=torch.bfloat16, device=dev)
         self.mixed = torch.zeros(batch, heads * head_dim, dtype=torch.bfloat16, device=dev)
         self.hidden = hidden
 
-    def step(self, x, pos, lens, out, stream=None) -> None:
-        """out[b] = W_out . attention of the token x[b] at position pos[b] over itself and the lens[b] - 1 before it
-        (pos and lens int32 on the device; lens = pos + 1)."""
+    def prompt(self, qkv, pos, seq, tokens: int, k_out=None, v_out=None, stream=None) -> None:
+        """Appends ``tokens`` tokens of prompts, rows of ``qkv`` [tokens][(heads + 2 kv_heads) * head_dim] at positions pos
+        of sequences seq (int32), and rotates their queries in place.  ``k_out`` and ``v_out`` (a cache of 4 bits; strided as
+        qkv): keys and values as the cache holds them, for the prompt's own attention."""
+        hd = self.heads * self.head_dim
+        self.append.append(qkv[:, hd:], qkv[:, hd + self.kv_heads * self.head_dim:], pos, tokens, seq=seq, q=qkv, q_out=qkv, k_out=k_out,
+                           v_out=v_out, stream=stream)
+
+    def step(self, x, pos, lens, out, stream=None, starts=None) -> None:
+        """out[b] = W_out . attention of the token x[b] at position pos[b] over itself and the lens[b] - 1 before it, those from
+        starts[b] on where given (pos, lens and starts int32 on the device; lens = pos + 1)."""
         n, hd = self.batch, self.heads * self.head_dim
         self.qkv_matrix.gemv(x, self.qkv, vectors=n, stream=stream)
         keys = self.qkv[:, hd:]
         values = self.qkv[:, hd + self.kv_heads * self.head_dim:]
         self.append.append(keys, values, pos, n, q=self.qkv, q_out=self.qkv, stream=stream)
-        self.attention.decode(self.qkv, self.mixed, lens, n, stream=stream)
+        self.attention.decode(self.qkv, self.mixed, lens, n, stream=stream, starts=starts)
         self.out_matrix.gemv(self.mixed, out, vectors=n, stream=stream)
+
+
+class DecodeExperts:
+    """One layer's experts for up to ``batch`` tokens: ``router`` [experts][hidden], ``gate`` and ``up`` [experts][inner][hidden],
+    ``down`` [experts][hidden][inner], of one type (see :class:`MoeLayer`).  :meth:`step` allocates nothing and may be captured."""
+
+    def __init__(self, router, gate, up, down, top: int, batch: int, normalize: bool = True, device: int = 0):
+        import torch
+
+        experts, inner, hidden = gate.shape
+        kind = {torch.float32: L.F32, torch.float16: L.F16, torch.bfloat16: L.BF16}[gate.dtype]
+        self.layer = L.MoeLayer(router, gate, up, down, hidden, inner, experts, top, batch, kind, normalize, router_row=router.stride(0),
+                                gate_row=gate.stride(1), up_row=up.stride(1), down_row=down.stride(1), gate_expert=gate.stride(0),
+                                up_expert=up.stride(0), down_expert=down.stride(0), device=device)
+        self.batch = batch
+        self.ids = torch.zeros(batch, top, dtype=torch.int32, device=gate.device)
+
+    def step(self, x, out, stream=None) -> None:
+        """out[b] of the token x[b]; ``ids`` holds the experts that it chose."""
+        self.layer.forward(x, out, self.batch, ids=self.ids, stream=stream)
 
 
 def main() -> int:
@@ -107,6 +149,12 @@ def main() -> int:
     ap.add_argument("--heads", type=int, default=32)
     ap.add_argument("--kv-heads", type=int, default=8)
     ap.add_argument("--head-dim", type=int, default=128)
+    ap.add_argument("--cache-bits", type=int, default=16, choices=(16, 4))
+    ap.add_argument("--cap", type=float, default=0.0, help="of scores, by a tanh (0: none)")
+    ap.add_argument("--slopes", action="store_true", help="a bias by distance")
+    ap.add_argument("--experts", type=int, default=0)
+    ap.add_argument("--top", type=int, default=4)
+    ap.add_argument("--inner", type=int, default=1024)
     ap.add_argument("--steps", type=int, default=200)
     args = ap.parse_args()
 
@@ -120,20 +168,40 @@ def main() -> int:
         return (torch.empty(shape, device="cuda").normal_(generator=g) * scale).to(torch.bfloat16)
 
     layer = DecodeAttention(normal(row, args.hidden, scale=0.02), normal(args.hidden, args.heads * args.head_dim, scale=0.02),
-                            args.heads, args.kv_heads, args.head_dim, args.batch, args.length + args.steps + 16)
-    layer.k.normal_(generator=g)
-    layer.v.normal_(generator=g)
+                            args.heads, args.kv_heads, args.head_dim, args.batch, args.length + args.steps + 16, cache_bits=args.cache_bits,
+                            cap=args.cap, slopes=L.distance_slopes(args.heads, device="cuda") if args.slopes else None)
+    if args.cache_bits == 16:
+        layer.k.normal_(generator=g)
+        layer.v.normal_(generator=g)
+    else:  # as a prompt of every sequence, some tokens at a time
+        for first in range(0, args.length, 256):
+            n = min(256, args.length - first)
+            at = torch.arange(first, first + n, dtype=torch.int32, device="cuda").repeat(args.batch)
+            of = torch.arange(args.batch, dtype=torch.int32, device="cuda").repeat_interleave(n)
+            layer.prompt(normal(args.batch * n, row), at, of, args.batch * n, stream=torch.cuda.current_stream())
+    experts = None
+    if args.experts:
+        e, f, h = args.experts, args.inner, args.hidden
+        experts = DecodeExperts(normal(e, h, scale=h ** -0.5), normal(e, f, h, scale=h ** -0.5), normal(e, f, h, scale=h ** -0.5),
+                                normal(e, h, f, scale=f ** -0.5), args.top, args.batch)
     x, out = normal(args.batch, args.hidden), torch.empty(args.batch, args.hidden, dtype=torch.bfloat16, device="cuda")
     pos = torch.full((args.batch,), args.length - 1, dtype=torch.int32, device="cuda")
     lens = pos + 1
+    after = torch.empty_like(out)
+
+    def step(stream):
+        layer.step(x, pos, lens, out, stream=stream)
+        if experts:
+            experts.step(out, after, stream=stream)
+
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())  # which fills the cache, x, pos and lens
     with torch.cuda.stream(side):
-        layer.step(x, pos, lens, out, stream=side)
+        step(side)
     side.synchronize()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        layer.step(x, pos, lens, out, stream=torch.cuda.current_stream())
+        step(torch.cuda.current_stream())
         pos.add_(1)
         lens.add_(1)
     before = 10  # steps, each of which leaves the cache a token longer
@@ -147,8 +215,10 @@ def main() -> int:
     end.synchronize()
     us = start.elapsed_time(end) / args.steps * 1e3
     keys = args.length + before + (args.steps - 1) / 2  # of a sequence in the timed steps, on average
-    cache = int(2 * args.batch * keys * args.kv_heads * args.head_dim * 2)
+    cache = int(2 * args.batch * keys * args.kv_heads * layer.key_bytes)
     weights = (row * args.hidden + args.hidden * args.heads * args.head_dim) * (0.5 + 2 / 128)
+    if experts:  # those that the last step chose
+        weights += 2 * (experts.ids.unique().numel() * 3 * args.inner + args.experts) * args.hidden
     print(json.dumps({"us_per_step": round(us, 2), "cache_bytes": cache, "weight_bytes": int(weights),
                       "gb_per_s": round((cache + weights) / us / 1e3, 1), "status": int(layer.status.item())}))
     return 0
