@@ -364,7 +364,7 @@ L2D_API int l2d_pool_release(int device);
 
 /* ---- decoding operators (no counterpart in the reference): what one new token of a language model
  *      reads around the GEMV -- 4-bit weights, and the paged cache of earlier keys and values ----
- * All three are stream-ordered, allocate nothing when called and may be captured into a graph.
+ * All are stream-ordered, allocate nothing when called and may be captured into a graph.
  * Arguments the host can see are checked before anything is launched; what only the device can see
  * (lengths, positions, page numbers) is checked by the kernels, which leave the access out and set a
  * bit of *status, a device word of the caller's that only ever gains bits (NULL: not reported). */

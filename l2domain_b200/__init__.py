@@ -11,7 +11,8 @@ Python mirror of the reference's probe/GEMV interface over the C ABI of ``lib/li
 * :class:`GemvPlan`                  -- build_side_info + the kernel launches (:73-103, :163-231, :301-334)
 
 The operators of a decoding step beside the GEMV (no counterpart in the reference): :class:`Q4Matrix`
-(products with 4-bit weights), :class:`KvCache` with :class:`KvAppend` and :class:`PagedAttention`.
+(products with 4-bit weights), :class:`KvCache` or :class:`KvCache4` (the cache in 4 bits) with :class:`KvAppend` and
+:class:`PagedAttention`, and :class:`MoeLayer` (a mixture of experts for a few tokens).
 
 Errors raise :class:`L2DError` (the reference aborts the process instead).  There is no CPU
 fallback: importing this package without the built library raises immediately.
@@ -608,7 +609,7 @@ class PeerShard:
 
 
 # --------------------------------------------------------------------------------------------
-# Decoding operators: 4-bit weights, the paged cache, attention over it
+# Decoding operators: 4-bit weights, the paged cache, attention over it, experts
 # --------------------------------------------------------------------------------------------
 
 KV_BAD_PAGE, KV_BAD_POSITION, KV_TIMEOUT = 1, 2, 4

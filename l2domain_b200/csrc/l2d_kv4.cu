@@ -350,6 +350,7 @@ int l2d_kv4_append(const l2d_kv4_cache *cache, const l2d_append_desc *desc, cons
     auto rows_of = [&](int heads, int64_t threads, int per_sm) {
         return static_cast<int>(std::min<int64_t>(heads, std::max<int64_t>(1, (int64_t(sms) * per_sm * kAppendThreads + threads - 1) / threads)));
     };
+    if (tokens > INT32_MAX) return set_error(L2D_ERR_INVALID, "%lld tokens are too many", static_cast<long long>(tokens));
     const int rows = rows_of(cache->heads, tokens * lanes, 8);
     int64_t blocks = (tokens * lanes * rows + kAppendThreads - 1) / kAppendThreads;
     QueryBlocks query = {};

@@ -905,12 +905,18 @@ int l2d_moe_plan_create(const l2d_moe_desc *desc, l2d_moe_plan **plan) {
                  ids_at = take(slots * 4), weights_at = take(slots * 4), largest_at = take(slots * 4), sorted_at = take(slots * 4),
                  entries_at = take(entries * 16), num_at = take(4), arrived_at = take((tiles + 1) * 4);
     void *memory = nullptr;
-    L2D_CUDA_TRY(cudaMalloc(&memory, bytes));
+    cudaError_t e = cudaMalloc(&memory, bytes);
+    if (e != cudaSuccess) {
+        cudaGetLastError();  // not the next caller's error
+        return set_error(L2D_ERR_CUDA, "experts' scratch of %zu bytes: %s", bytes, cudaGetErrorString(e));
+    }
     // Counters, and what pads the rows of inner_out, on a stream of their own, so that nothing else on the device is waited for.
     cudaStream_t own = nullptr;
-    cudaError_t e = cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking);
+    e = cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking);
     if (e == cudaSuccess) {
-        e = cudaMemsetAsync(memory, 0, bytes, own);
+        if (inner_row > d.inner)
+            e = cudaMemset2DAsync(static_cast<char *>(memory) + inner_at + d.inner * 4, inner_row * 4, 0, (inner_row - d.inner) * 4, slots, own);
+        if (e == cudaSuccess) e = cudaMemsetAsync(static_cast<char *>(memory) + arrived_at, 0, (tiles + 1) * 4, own);
         if (e == cudaSuccess) e = cudaStreamSynchronize(own);
         cudaStreamDestroy(own);
     }
