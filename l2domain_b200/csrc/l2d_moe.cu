@@ -287,7 +287,7 @@ template <typename T, int COPY>
 __device__ __forceinline__ void bring(char *to, const T *from, int n) {
     constexpr int kEach = 16 / static_cast<int>(sizeof(T));
     if constexpr (COPY == kBy16) {
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_at(to)), "l"(from), "r"(n * static_cast<int>(sizeof(T))) : "memory");
+        asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(smem_at(to)), "l"(from), "r"(n * static_cast<int>(sizeof(T))) : "memory");
     } else if constexpr (COPY == kBy4) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -305,7 +305,7 @@ __device__ __forceinline__ void bring(char *to, const T *from, int n) {
 
 template <typename T, int COPY>
 __device__ __forceinline__ void bring_all(char *to, const T *from) {
-    if constexpr (COPY == kBy16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_at(to)), "l"(from) : "memory");
+    if constexpr (COPY == kBy16) asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(smem_at(to)), "l"(from) : "memory");
     else bring<T, COPY>(to, from, 16 / static_cast<int>(sizeof(T)));
 }
 
