@@ -26,6 +26,7 @@ namespace l2d {
 constexpr int kMaxExperts = 512;
 constexpr int kMoeThreads = 256, kMoeWarps = kMoeThreads / 32;
 constexpr int kRouteTokens = 4;  // of a block of the router
+constexpr int kRouteExperts = 2; // where there are tokens for blocks enough
 
 struct MoeArgs {
     const void *x, *router, *gate, *up, *down;
@@ -200,48 +201,63 @@ __device__ __forceinline__ bool last_of(unsigned *arrived, unsigned n) {
     return last;
 }
 
-template <typename T, bool WORDS>
+// EXPERTS: router rows of a block.  More of them read the tokens, and make them 64-bit numbers, less often.
+template <typename T, bool WORDS, int EXPERTS>
 __global__ void __launch_bounds__(kMoeThreads) k_route(const __grid_constant__ MoeArgs a) {
     dev::wait_for_previous();
-    __shared__ double sums[kMoeWarps][kRouteTokens];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, e = blockIdx.x, t0 = blockIdx.y * kRouteTokens, n = min(a.tokens - t0, kRouteTokens);
+    __shared__ double sums[kMoeWarps][EXPERTS * kRouteTokens];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, e = blockIdx.x * EXPERTS, t0 = blockIdx.y * kRouteTokens;
+    const int n = min(a.tokens - t0, kRouteTokens), experts = min(a.experts - e, EXPERTS);
     const T *w = static_cast<const T *>(a.router) + e * a.router_row, *x = static_cast<const T *>(a.x) + t0 * a.x_token;
-    double acc[kRouteTokens] = {};
-    if constexpr (WORDS) {
-        for (int k = 8 * tid; k < a.hidden; k += 8 * kMoeThreads) {
-            const Eight<T> r = load_eight(w + k);
-            double wide[8];
+    double acc[EXPERTS][kRouteTokens] = {};
+    constexpr int kEach = WORDS ? 8 : 1;
+    for (int k = kEach * tid; k < a.hidden; k += kEach * kMoeThreads) {
+        double wide[EXPERTS][kEach];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) wide[i] = dev::widen(r.v[i]);
+        for (int j = 0; j < EXPERTS; ++j) {
+            const T *row = w + min(j, experts - 1) * a.router_row + k;  // past the last: nobody's sum
+            if constexpr (WORDS) {
+                const Eight<T> r = load_eight(row);
 #pragma unroll
-            for (int t = 0; t < kRouteTokens; ++t) {
-                if (t >= n) break;
-                const Eight<T> v = load_eight(x + t * a.x_token + k);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) acc[t] = fma(wide[i], static_cast<double>(dev::widen(v.v[i])), acc[t]);
+                for (int i = 0; i < 8; ++i) wide[j][i] = dev::widen(r.v[i]);
+            } else {
+                wide[j][0] = dev::widen(*row);
             }
         }
-    } else {
-        for (int k = tid; k < a.hidden; k += kMoeThreads) {
-            const double r = dev::widen(w[k]);
 #pragma unroll
-            for (int t = 0; t < kRouteTokens; ++t)
-                if (t < n) acc[t] = fma(r, static_cast<double>(dev::widen(x[t * a.x_token + k])), acc[t]);
+        for (int t = 0; t < kRouteTokens; ++t) {
+            if (t >= n) break;
+            T v[kEach];
+            if constexpr (WORDS) {
+                const Eight<T> r = load_eight(x + t * a.x_token + k);
+                memcpy(v, &r, sizeof r);
+            } else {
+                v[0] = x[t * a.x_token + k];
+            }
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                const double y = dev::widen(v[i]);
+#pragma unroll
+                for (int j = 0; j < EXPERTS; ++j) acc[j][t] = fma(wide[j][i], y, acc[j][t]);
+            }
         }
     }
 #pragma unroll
     for (int t = 0; t < kRouteTokens; ++t) {
         if (t >= n) break;
 #pragma unroll
-        for (int d = 16; d; d >>= 1) acc[t] += __shfl_xor_sync(0xffffffffu, acc[t], d);
-        if (lane == 0) sums[warp][t] = acc[t];
+        for (int j = 0; j < EXPERTS; ++j) {
+#pragma unroll
+            for (int d = 16; d; d >>= 1) acc[j][t] += __shfl_xor_sync(0xffffffffu, acc[j][t], d);
+            if (lane == 0) sums[warp][j * kRouteTokens + t] = acc[j][t];
+        }
     }
     __syncthreads();
-    if (tid < n) {
+    if (const int j = tid / kRouteTokens, t = tid % kRouteTokens; j < experts && t < n) {
         double s = 0.0;
 #pragma unroll
         for (int i = 0; i < kMoeWarps; ++i) s += sums[i][tid];
-        a.logits[static_cast<int64_t>(t0 + tid) * a.experts + e] = s;
+        a.logits[static_cast<int64_t>(t0 + t) * a.experts + e + j] = s;
     }
     if (e == 0)
         for (int i = tid; i < n * a.top; i += kMoeThreads) a.largest[static_cast<int64_t>(t0) * a.top + i] = 0;
@@ -807,19 +823,21 @@ void (*pick_copy(bool down, int copy))(MoeArgs, int) {
 }
 
 template <typename T, int N>
-MoeKernels moe_kernels(bool route_words, int copy_up, int copy_down) {
-    return {route_words ? k_route<T, true> : k_route<T, false>, pick_copy<T, N>(false, copy_up), pick_copy<T, N>(true, copy_down), k_combine<T>,
+MoeKernels moe_kernels(int tokens, bool route_words, int copy_up, int copy_down) {
+    auto route = tokens >= 16 ? (route_words ? k_route<T, true, kRouteExperts> : k_route<T, false, kRouteExperts>)
+                              : (route_words ? k_route<T, true, 1> : k_route<T, false, 1>);
+    return {route, pick_copy<T, N>(false, copy_up), pick_copy<T, N>(true, copy_down), k_combine<T>,
             {experts_smem<T, N, false>(), experts_smem<T, N, true>()},
             {sizeof(T) == 4 ? 2 : ExpertsRing<N, false>::kBlocks, sizeof(T) == 4 ? 2 : ExpertsRing<N, true>::kBlocks}};
 }
 
 template <typename T>
-MoeKernels pick_moe(int eights, bool route_words, int copy_up, int copy_down) {
-    if constexpr (sizeof(T) == 4) return moe_kernels<T, 1>(route_words, copy_up, copy_down);
+MoeKernels pick_moe(int eights, int tokens, bool route_words, int copy_up, int copy_down) {
+    if constexpr (sizeof(T) == 4) return moe_kernels<T, 1>(tokens, route_words, copy_up, copy_down);
     else
-        return eights == 1   ? moe_kernels<T, 1>(route_words, copy_up, copy_down)
-               : eights == 2 ? moe_kernels<T, 2>(route_words, copy_up, copy_down)
-                             : moe_kernels<T, 4>(route_words, copy_up, copy_down);
+        return eights == 1   ? moe_kernels<T, 1>(tokens, route_words, copy_up, copy_down)
+               : eights == 2 ? moe_kernels<T, 2>(tokens, route_words, copy_up, copy_down)
+                             : moe_kernels<T, 4>(tokens, route_words, copy_up, copy_down);
 }
 
 }  // namespace l2d
@@ -988,12 +1006,12 @@ int l2d_moe_forward(l2d_moe_plan *p, const void *x, void *y, int32_t *ids, float
     const int copy_up = std::max({copy_of(d.gate, d.gate_row, d.gate_expert, eb), copy_of(d.up, d.up_row, d.up_expert, eb), x_copy, whole});
     const int copy_down = copy_of(d.down, d.down_row, d.down_expert, eb);
     const bool route_words = x_copy == kBy16 && d.hidden % 8 == 0 && copy_of(d.router, d.router_row, 0, eb) == kBy16;
-    const MoeKernels k = d.dtype == L2D_F32   ? pick_moe<float>(eights, route_words, copy_up, copy_down)
-                         : d.dtype == L2D_F16 ? pick_moe<__half>(eights, route_words, copy_up, copy_down)
-                                              : pick_moe<__nv_bfloat16>(eights, route_words, copy_up, copy_down);
+    const MoeKernels k = d.dtype == L2D_F32   ? pick_moe<float>(eights, tokens, route_words, copy_up, copy_down)
+                         : d.dtype == L2D_F16 ? pick_moe<__half>(eights, tokens, route_words, copy_up, copy_down)
+                                              : pick_moe<__nv_bfloat16>(eights, tokens, route_words, copy_up, copy_down);
     const int up_rows = eb == 4 ? 2 : 8, down_rows = eb == 4 ? 4 : 16, step = eb == 4 ? 128 : 64;
     const int64_t tiles_up = (d.inner + up_rows - 1) / up_rows, tiles_down = (d.hidden + down_rows - 1) / down_rows;
-    L2D_CUDA_TRY(launch(k.route, dim3(d.experts, (tokens + kRouteTokens - 1) / kRouteTokens), kMoeThreads, 0, stream, a));
+    L2D_CUDA_TRY(launch(k.route, dim3(tokens >= 16 ? (d.experts + kRouteExperts - 1) / kRouteExperts : d.experts, (tokens + kRouteTokens - 1) / kRouteTokens), kMoeThreads, 0, stream, a));
     const int64_t entries = std::min<int64_t>(int64_t(tokens) * d.top, d.experts);
     const int grid_up = k.blocks[0] * p->sms, grid_down = k.blocks[1] * p->sms;
     const int s_up = parts_of(entries * tiles_up, grid_up * kMoeWarps, static_cast<int>((d.hidden + step - 1) / step));
