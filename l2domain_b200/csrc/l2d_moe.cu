@@ -290,7 +290,8 @@ __global__ void __launch_bounds__(kMoeThreads) k_route(const __grid_constant__ M
 constexpr int kDepth32 = 4;               // steps in a ring, all but one of them on their way
 constexpr int kRowBytes = 2048;           // of a step: 16 rows of 128 bytes, or four of 512
 constexpr int kCached = 128, kCachedSlots = 1024;  // entries and slots that a block keeps in shared memory
-enum { kBy16 = 0, kBy4 = 1, kByElement = 2 };  // how rows come: 16 bytes at a time, 4, or one element
+// How rows come: 16 bytes at a time; 4; 4, of rows of 16-bit elements that may begin in the middle of a word; one element.
+enum { kBy16 = 0, kBy4 = 1, kByHalves = 2, kByElement = 3 };
 
 __device__ __forceinline__ uint32_t smem_at(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -317,6 +318,29 @@ __device__ __forceinline__ void bring(char *to, const T *from, int n) {
         for (int i = 0; i < kEach; ++i) v[i] = i < n ? from[i] : dev::narrow<T>(0.0f);
         memcpy(to, v, 16);
     }
+}
+
+// Eight 16-bit elements, of which `n` are real, as the four words that they lie in, and the fifth where they begin in the middle
+// of one: what is before them in their first word is the row before's last element.
+template <typename T>
+__device__ __forceinline__ void bring_halves(char *to, char *fifth, const T *from, int n, const T *none) {
+    const int skip = static_cast<int>(reinterpret_cast<uintptr_t>(from) & 2);
+    const char *p = n ? reinterpret_cast<const char *>(from) - skip : reinterpret_cast<const char *>(none);  // nothing is read there
+#pragma unroll
+    for (int i = 0; i < 5; ++i) {
+        if (i == 4 && !skip) break;
+        const int have = n ? min(max(skip + 2 * n - 4 * i, 0), 4) : 0;
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_at(i < 4 ? to + 4 * i : fifth)), "l"(have ? p + 4 * i : p), "r"(have) : "memory");
+    }
+}
+// The elements of such words.
+__device__ __forceinline__ uint4 from_halves(const char *at, const char *fifth, bool skip) {
+    uint4 w = *reinterpret_cast<const uint4 *>(at);
+    if (skip) {
+        const uint32_t last = *reinterpret_cast<const uint32_t *>(fifth);
+        w = make_uint4(w.x >> 16 | w.y << 16, w.y >> 16 | w.z << 16, w.z >> 16 | w.w << 16, w.w >> 16 | last << 16);
+    }
+    return w;
 }
 
 template <typename T, int COPY>
@@ -403,10 +427,11 @@ __device__ __forceinline__ Lists lists_of(const MoeArgs &a) {
 
 // A warp's ring: a step's rows, then its columns (16 bytes a lane of each eight and run, of four-byte elements twice), as deep as
 // sixteen warps an SM leave room for (eight of many columns).
-template <int N, bool DOWN>
+template <int N, bool DOWN, bool HALVES>
 struct ExpertsRing {
-    static constexpr int kStep = kRowBytes + N * (DOWN ? 2048 : 1024);
-    static constexpr int kBlocks = N == 4 ? 1 : 2;
+    static constexpr int kWords = kRowBytes + N * (DOWN ? 2048 : 1024);
+    static constexpr int kStep = kWords + (HALVES ? 128 * (4 + (DOWN ? 0 : 2 * N)) : 0);  // and fifth words, four bytes a lane
+    static constexpr int kBlocks = N == 4 || (N == 2 && HALVES) ? 1 : 2;
     static constexpr int kDepth = 12 * 1024 * (3 - kBlocks) / kStep;
     static constexpr int kBytes = kDepth * kStep;
     static_assert(kDepth >= 2, "one step on its way");
@@ -414,10 +439,10 @@ struct ExpertsRing {
 
 // N: eights of columns; DOWN: the second product.  S: warps that share an item.
 template <typename T, int N, bool DOWN, int COPY>
-__global__ void __launch_bounds__(kMoeThreads, ExpertsRing<N, DOWN>::kBlocks) k_experts(const __grid_constant__ MoeArgs a, int S) {
+__global__ void __launch_bounds__(kMoeThreads, ExpertsRing<N, DOWN, COPY == kByHalves>::kBlocks) k_experts(const __grid_constant__ MoeArgs a, int S) {
     constexpr bool kHalf = std::is_same<T, __half>::value;
     constexpr int kK = 64;                           // elements of a step: two runs of 32
-    using Ring = ExpertsRing<N, DOWN>;
+    using Ring = ExpertsRing<N, DOWN, COPY == kByHalves>;
     extern __shared__ __align__(128) char smem[];
     dev::wait_for_previous();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -431,6 +456,7 @@ __global__ void __launch_bounds__(kMoeThreads, ExpertsRing<N, DOWN>::kBlocks) k_
     const int n_end[2] = {min(max(K - (all - 1) * kK - 8 * t, 0), 8), min(max(K - (all - 1) * kK - 32 - 8 * t, 0), 8)};
     const int first_k = begin * kK + 8 * t;
     char *ring = smem + warp * Ring::kBytes + lane * 16;
+    const int fifths = Ring::kWords - lane * 12;  // of a step's words, where this lane's fifth words begin
     float *meet = reinterpret_cast<float *>(smem + kMoeWarps * Ring::kBytes);  // [warp][4 N][lane]
 
     // What is brought next: rows g and g + 8 from p0 and p1 on, and column g of each eight, `left` steps of them.
@@ -465,7 +491,22 @@ __global__ void __launch_bounds__(kMoeThreads, ExpertsRing<N, DOWN>::kBlocks) k_
     auto bring_step = [&] {
         if (left) {
             char *to = ring + in_at;
-            if (short_end && left == 1) {
+            const bool end = short_end && left == 1;
+            if constexpr (COPY == kByHalves) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int n = end ? n_end[h] : 8;
+                    const T *none = static_cast<const T *>(a.down);
+                    bring_halves(to + 1024 * h, to + fifths + 256 * h, p0 + 32 * h, n, none);
+                    bring_halves(to + 1024 * h + 512, to + fifths + 256 * h + 128, p1 + 32 * h, n, none);
+                    if constexpr (!DOWN) {
+#pragma unroll
+                        for (int j = 0; j < N; ++j)
+                            if (j == 0 || 8 * j < in_count)
+                                bring_halves(to + kRowBytes + 1024 * j + 512 * h, to + fifths + 512 + 256 * j + 128 * h, column[j] + 32 * h, n, none);
+                    }
+                }
+            } else if (end) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {  // nothing is read of a run without elements, whose first may lie anywhere
                     const T *none = static_cast<const T *>(a.down);
@@ -530,6 +571,16 @@ __global__ void __launch_bounds__(kMoeThreads, ExpertsRing<N, DOWN>::kBlocks) k_
                 low_mask[j] = bits >= 0x7f800000u ? 0 : 0xffffffffu;
             }
         }
+        // Which rows and columns begin in the middle of a word: the products' matrices begin at one.
+        bool skip[2] = {}, skip_x[N] = {};
+        if constexpr (COPY == kByHalves) {
+            const int r0 = DOWN ? min(tile * 16 + g, rows - 1) : min(tile * 8 + g, rows - 1), r1 = DOWN ? min(tile * 16 + g + 8, rows - 1) : r0;
+            skip[0] = (entry.x * (DOWN ? a.down_expert : a.gate_expert) + r0 * (DOWN ? a.down_row : a.gate_row)) & 1;
+            skip[1] = (entry.x * (DOWN ? a.down_expert : a.up_expert) + r1 * (DOWN ? a.down_row : a.up_row)) & 1;
+            if constexpr (!DOWN)
+#pragma unroll
+                for (int j = 0; j < N; ++j) skip_x[j] = (lists.sorted[entry.y + min(8 * j + g, entry.z - 1)] / a.top * a.x_token) & 1;
+        }
         float acc[N][4] = {};
 #pragma unroll 1
         for (int step = 0; step < steps; ++step) {
@@ -539,7 +590,10 @@ __global__ void __launch_bounds__(kMoeThreads, ExpertsRing<N, DOWN>::kBlocks) k_
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) r[h][i] = *reinterpret_cast<const uint4 *>(from + 1024 * h + 512 * i);
+                for (int i = 0; i < 2; ++i) {
+                    if constexpr (COPY == kByHalves) r[h][i] = from_halves(from + 1024 * h + 512 * i, from + fifths + 256 * h + 128 * i, skip[i]);
+                    else r[h][i] = *reinterpret_cast<const uint4 *>(from + 1024 * h + 512 * i);
+                }
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 if (j && 8 * j >= entry.z) break;
@@ -547,7 +601,9 @@ __global__ void __launch_bounds__(kMoeThreads, ExpertsRing<N, DOWN>::kBlocks) k_
                 for (int h = 0; h < 2; ++h) {
                     const uint4 &r0 = r[h][0], &r1 = r[h][1];
                     const uint4 *x = reinterpret_cast<const uint4 *>(from + kRowBytes + 1024 * kRun * j + 512 * kRun * h);
-                    const uint4 u = x[0];
+                    uint4 u;
+                    if constexpr (!DOWN && COPY == kByHalves) u = from_halves(reinterpret_cast<const char *>(x), from + fifths + 512 + 256 * j + 128 * h, skip_x[j]);
+                    else u = x[0];
                     if constexpr (!DOWN) {
                         mma<T>(acc[j], r0.x, r1.x, r0.y, r1.y, u.x, u.y);
                         mma<T>(acc[j], r0.z, r1.z, r0.w, r1.w, u.z, u.w);
@@ -805,8 +861,13 @@ struct MoeKernels {
 };
 
 template <typename T, int N, bool DOWN>
-constexpr int experts_smem() {
-    return kMoeWarps * (sizeof(T) == 4 ? kDepth32 * kRowBytes + 128 : ExpertsRing<N, DOWN>::kBytes + 4 * N * 128);
+int experts_smem(int copy) {
+    return kMoeWarps * (sizeof(T) == 4 ? kDepth32 * kRowBytes + 128 : (copy == kByHalves ? ExpertsRing<N, DOWN, true>::kBytes : ExpertsRing<N, DOWN, false>::kBytes) + 4 * N * 128);
+}
+
+template <typename T, int N>
+int experts_blocks(int copy) {
+    return sizeof(T) == 4 ? 2 : copy == kByHalves ? ExpertsRing<N, false, true>::kBlocks : ExpertsRing<N, false, false>::kBlocks;
 }
 
 template <typename T, int N, int COPY>
@@ -819,7 +880,8 @@ template <typename T, int N>
 void (*pick_copy(bool down, int copy))(MoeArgs, int) {
     if (copy == kBy16) return pick_experts<T, N, kBy16>(down);
     if (copy == kBy4 || sizeof(T) == 4) return pick_experts<T, N, kBy4>(down);
-    return pick_experts<T, N, sizeof(T) == 4 ? kBy4 : kByElement>(down);
+    if constexpr (sizeof(T) == 2) return copy == kByHalves ? pick_experts<T, N, kByHalves>(down) : pick_experts<T, N, kByElement>(down);
+    else return nullptr;
 }
 
 template <typename T, int N>
@@ -827,8 +889,8 @@ MoeKernels moe_kernels(int tokens, bool route_words, int copy_up, int copy_down)
     auto route = tokens >= 16 ? (route_words ? k_route<T, true, kRouteExperts> : k_route<T, false, kRouteExperts>)
                               : (route_words ? k_route<T, true, 1> : k_route<T, false, 1>);
     return {route, pick_copy<T, N>(false, copy_up), pick_copy<T, N>(true, copy_down), k_combine<T>,
-            {experts_smem<T, N, false>(), experts_smem<T, N, true>()},
-            {sizeof(T) == 4 ? 2 : ExpertsRing<N, false>::kBlocks, sizeof(T) == 4 ? 2 : ExpertsRing<N, true>::kBlocks}};
+            {experts_smem<T, N, false>(copy_up), experts_smem<T, N, true>(copy_down)},
+            {experts_blocks<T, N>(copy_up), experts_blocks<T, N>(copy_down)}};
 }
 
 template <typename T>
@@ -857,7 +919,7 @@ namespace l2d {
 // How rows of a matrix can be brought: by what they and their strides are aligned to.
 int copy_of(const void *p, int64_t row, int64_t expert, int eb) {
     const uintptr_t any = reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(row * eb) | static_cast<uintptr_t>(expert * eb);
-    return any % 16 == 0 ? kBy16 : any % 4 == 0 ? kBy4 : kByElement;
+    return any % 16 == 0 ? kBy16 : any % 4 == 0 ? kBy4 : misaligned(p, 4) ? kByElement : kByHalves;
 }
 
 // Warps that share an item: so many that every warp of the GPU has two, as long as each has a few steps of it.
