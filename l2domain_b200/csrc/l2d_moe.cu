@@ -387,15 +387,18 @@ __device__ __forceinline__ Items items_of(int entries, int tiles, int groups, in
 __device__ __forceinline__ float silu_times(float gate, float up) { return gate / (1.0f + expf(-gate)) * up; }
 
 // The first of two bf16 numbers that add up to a number, in the low half, the second in the upper.  An infinity or a NaN is its
-// first, and no finite number's first is one.
+// first alone; a finite number's first is none, so the largest ones' is cut off and not rounded.
 __device__ __forceinline__ uint32_t two_bf16(float x) {
-    const uint32_t bits = __float_as_uint(x);
-    const bool finite = fabsf(x) <= FLT_MAX;
-    const uint32_t hi = finite ? bits >> 16 : bits >> 16 | ((bits & 0x7fffffu) ? 0x40u : 0u);
-    const __nv_bfloat16 lo = __float2bfloat16_rn(finite ? x - __uint_as_float(bits & 0xffff0000u) : 0.0f);
-    uint16_t low;
-    memcpy(&low, &lo, 2);
-    return hi | static_cast<uint32_t>(low) << 16;
+    auto bits_of = [](float v) {
+        const __nv_bfloat16 b = __float2bfloat16_rn(v);
+        uint16_t r;
+        memcpy(&r, &b, 2);
+        return static_cast<uint32_t>(r);
+    };
+    uint32_t hi = bits_of(x);
+    if (!(fabsf(x) <= FLT_MAX)) return hi;
+    if ((hi & 0x7fffu) == 0x7f80u) hi = __float_as_uint(x) >> 16;
+    return hi | bits_of(x - __uint_as_float(hi << 16)) << 16;
 }
 
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
