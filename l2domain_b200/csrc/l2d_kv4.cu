@@ -217,8 +217,8 @@ __device__ __forceinline__ void append4(const Append4Args &args, unsigned block_
         if (d < D && d % a.c.group == 0)
             *reinterpret_cast<uint32_t *>(tile + chunks * kChunkBytes + d / a.c.group * kGroupBytes + inside * 4) = word | static_cast<uint32_t>(z);
     };
-    // Every rows-th head is this thread's, a few at a time and loads first.  The barriers: outputs may be the inputs.
-    constexpr int kHeads = WORDS ? 2 : 1;
+    // Every rows-th head is this thread's, one at a time (two, loads first, took registers that a block more makes better use of).
+    // The barrier: outputs may be the inputs.
     const int64_t block = static_cast<int64_t>(slot / kBlockSlots) * hk * a.c.tile_bytes;
 #pragma unroll 1
     for (int which = 0; which < 2; ++which) {  // keys, then values
@@ -229,26 +229,19 @@ __device__ __forceinline__ void append4(const Append4Args &args, unsigned block_
         out += at;
         char *tiles = (which ? a.c.v + page * a.c.v_page : a.c.k + page * a.c.k_page) + block;
 #pragma unroll 1
-        for (int h0 = row; h0 < hk; h0 += kHeads * rows) {
-            Pack<T, 8> own[kHeads], pair[kHeads];
-#pragma unroll
-            for (int j = 0; j < kHeads; ++j)
-                if (h0 + j * rows < hk) load(own[j], pair[j], from + (h0 + j * rows) * D, !which);
+        for (int h = row; h < hk; h += rows) {
+            Pack<T, 8> own, pair;
+            load(own, pair, from + h * D, !which);
             __syncwarp(mine);
+            float x[8];
+            if (!which) {
+                rotate(x, own, pair);
+            } else {
 #pragma unroll
-            for (int j = 0; j < kHeads; ++j) {
-                const int h = h0 + j * rows;
-                if (h >= hk) continue;
-                float x[8];
-                if (!which) {
-                    rotate(x, own[j], pair[j]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) x[i] = dev::widen(own[j].v[i]);
-                }
-                hold(x, tiles + h * a.c.tile_bytes);
-                if (tell) store8<T, WORDS>(out + h * D, x, d, D);
+                for (int i = 0; i < 8; ++i) x[i] = dev::widen(own.v[i]);
             }
+            hold(x, tiles + h * a.c.tile_bytes);
+            if (tell) store8<T, WORDS>(out + h * D, x, d, D);
         }
     }
 }
@@ -355,7 +348,8 @@ int l2d_kv4_append(const l2d_kv4_cache *cache, const l2d_append_desc *desc, cons
         return static_cast<int>(std::min<int64_t>(heads, std::max<int64_t>(1, (int64_t(sms) * per_sm * kAppendThreads + threads - 1) / threads)));
     };
     if (tokens > INT32_MAX) return set_error(L2D_ERR_INVALID, "%lld tokens are too many", static_cast<long long>(tokens));
-    const int rows = rows_of(cache->heads, tokens * lanes, 8);
+    int rows = rows_of(cache->heads, tokens * lanes, 8);
+    while (cache->heads % rows) ++rows;  // so that neighbours in a warp have as many heads
     int64_t blocks = (tokens * lanes * rows + kAppendThreads - 1) / kAppendThreads;
     QueryBlocks query = {};
     if (desc->heads_q) {
