@@ -15,9 +15,9 @@ namespace l2d {
 // sums and quotients are rounded one by one to fp32, so that what is stored follows from the inputs and not from how an
 // expression was compiled.
 //
-// Measured (32 query and 8 key-value heads of 128): 8192 tokens of fp16 in groups of 32, with what is held written out, 75 us,
-// 2.9 TB/s, for 34 us of bytes: some 460 warp instructions per 256 elements fill half of the issue slots; 32 tokens 5.6-6.0 us, of
-// which a launch 4.1.  Three blocks a SM: 82 us with two, 81 with four.
+// Measured (32 query and 8 key-value heads of 128): 8192 tokens of fp16 in groups of 32, with what is held written out, 65 us,
+// 3.3 TB/s, for 34 us of bytes: some 400 warp instructions per 256 elements; 32 tokens 6 us, of which a launch 4.1.  Three blocks a
+// SM: 67 us with four.
 // ---------------------------------------------------------------------------------------------
 
 // Two numbers at a time, each rounded as by itself.
