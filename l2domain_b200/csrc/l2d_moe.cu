@@ -12,8 +12,9 @@
 // 17 + 5 at 4096 x 1536, and 45 for 30 in all at 1001 x 333.)
 // Nothing depends on the order in which blocks come: a slot's sums are its own.
 //
-// Measured (bf16): 32 tokens, 4 of 64 experts of 4096 x 1024, 233 us, 6.0 TB/s, for 220 us of bytes at a copy's rate; one token, 4 of
-// 32 of 4096 x 1536, 43 us for 24: the chain of launches and, in each, some microseconds until its rows come.
+// Measured (bf16): 32 tokens, 4 of 64 experts of 4096 x 1024, 233 to 256 us (short runs, and seconds under the
+// power cap), 6.0 to 5.5 TB/s, for 220 us of bytes at a copy's rate; one token, 4 of 32 of 4096 x 1536, 43 us for
+// 24: the chain of launches and, in each, some microseconds until its rows come.
 #include "l2d_launch.cuh"
 
 #include <algorithm>
