@@ -497,6 +497,9 @@ __global__ void __launch_bounds__(kMoeThreads, ExpertsRing<N, DOWN, COPY == kByH
         }
         left = steps;
     };
+    // Where a copy of no elements points: its address has to be aligned as any other's, so it is one of a matrix that the width
+    // of the copies was chosen by.
+    const T *none = static_cast<const T *>(DOWN ? a.down : a.gate);
     auto bring_step = [&] {
         if (left) {
             char *to = ring + in_at;
@@ -505,7 +508,6 @@ __global__ void __launch_bounds__(kMoeThreads, ExpertsRing<N, DOWN, COPY == kByH
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int n = end ? n_end[h] : 8;
-                    const T *none = static_cast<const T *>(a.down);
                     bring_halves(to + 1024 * h, to + fifths + 256 * h, p0 + 32 * h, n, none);
                     bring_halves(to + 1024 * h + 512, to + fifths + 256 * h + 128, p1 + 32 * h, n, none);
                     if constexpr (!DOWN) {
@@ -518,7 +520,6 @@ __global__ void __launch_bounds__(kMoeThreads, ExpertsRing<N, DOWN, COPY == kByH
             } else if (end) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {  // nothing is read of a run without elements, whose first may lie anywhere
-                    const T *none = static_cast<const T *>(a.down);
                     bring<T, COPY>(to + 1024 * h, n_end[h] ? p0 + 32 * h : none, n_end[h]);
                     bring<T, COPY>(to + 1024 * h + 512, n_end[h] ? p1 + 32 * h : none, n_end[h]);
                     if constexpr (!DOWN) {

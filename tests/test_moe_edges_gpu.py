@@ -1,0 +1,43 @@
+"""The mixture-of-experts layer on the GPU where memory, ranges and precision end (tolerances: test_moe_gpu.py, unless a test
+derives its own)."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+import l2domain_b200 as L  # noqa: E402
+from test_decode_ops_gpu import TORCH, close, gpu, offset_view  # noqa: E402,F401
+from test_moe_gpu import Layer, check  # noqa: E402
+
+
+@pytest.mark.parametrize("dt", [L.F32, L.F16, L.BF16])
+@pytest.mark.parametrize("name", ["router", "gate", "up", "down"])
+@pytest.mark.parametrize("shift", [1, 2, 4])
+def test_one_matrix_alone_off_its_boundary(dt, name, shift):
+    """Every other matrix is on 16 bytes, and the last step of each product is short: by runs without an element too."""
+    for H, F in ((72, 40), (32, 104), (1000, 88)):
+        layer = Layer(dt, H, F, 4, 2, seed=H)
+        moved = offset_view(getattr(layer, name + "_raw"), shift)
+        setattr(layer, name + "_raw", moved)
+        setattr(layer, name, moved)
+        for T in (1, 20):
+            check(layer, T)
+
+
+@pytest.mark.parametrize("dt", [L.F16, L.BF16])
+@pytest.mark.parametrize("H", [72, 73])
+def test_odd_rows_beside_even_ones(dt, H):
+    """Rows of each matrix in turn begin in the middle of a word, `down` also off every boundary."""
+    for pads in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 1, 0)):
+        layer = Layer(dt, H, 72, 3, 2, seed=H)
+        for name, pad in zip(("gate", "up", "down"), pads):
+            m = getattr(layer, name)
+            wide = torch.zeros(*m.shape[:-1], m.shape[-1] + pad, dtype=m.dtype, device="cuda")
+            wide[..., : m.shape[-1]] = m
+            if name == "down":
+                wide = offset_view(wide, 1)
+            setattr(layer, name + "_raw", wide)
+            setattr(layer, name, wide[..., : m.shape[-1]])
+        check(layer, 5)
