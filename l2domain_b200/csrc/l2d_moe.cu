@@ -409,10 +409,11 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
     return r;
 }
 
-// What a slot's numbers are multiplied by before they become fp16: the largest then lies in 2^14 .. 2^15.
+// What a slot's numbers are multiplied by before they become fp16: the largest then lies in 2^14 .. 2^15.  Beside an infinity
+// or a NaN the finite ones only have to stay finite, whatever they are: every output is that one's.
 __device__ __forceinline__ float to_half_range(uint32_t largest_bits) {
     const int exponent = static_cast<int>(largest_bits >> 23);  // 255: not finite
-    if (exponent == 255 || exponent == 0) return exponent ? 1.0f : 0x1p100f;
+    if (exponent == 255 || exponent == 0) return exponent ? 0x1p-113f : 0x1p100f;
     return __uint_as_float(static_cast<uint32_t>(min(127 + 14 - (exponent - 127), 254)) << 23);
 }
 

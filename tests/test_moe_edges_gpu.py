@@ -41,3 +41,22 @@ def test_odd_rows_beside_even_ones(dt, H):
             setattr(layer, name + "_raw", wide)
             setattr(layer, name, wide[..., : m.shape[-1]])
         check(layer, 5)
+
+
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_an_infinite_inner_value_keeps_the_sign_of_its_outputs(sign):
+    """fp16: one inner value is infinite and others are beyond 65504 and pull the other way: the outputs are infinite still."""
+    H, F = 16, 24
+    layer = Layer(L.F16, H, F, 1, 1, seed=11)
+    layer.gate[:], layer.up[:] = 0.0, 0.0
+    layer.gate[0, :, 0] = 1.0     # gates of 500
+    layer.up[0, :, 1] = 500.0     # ups of 2000, so inner values of 10^6 ..
+    layer.up[0, 3, 2] = math.inf  # .. and row 3's is infinite
+    layer.down[:] = -sign
+    layer.down[0, :, 3] = sign
+    x = torch.zeros(1, H, dtype=torch.float16, device="cuda")
+    x[0, 0], x[0, 1], x[0, 2] = 500.0, 4.0, 1.0
+    y = torch.zeros_like(x)
+    layer.plan(1).forward(x, y, 1)
+    torch.cuda.synchronize()
+    assert (y == sign * math.inf).all()
