@@ -60,3 +60,22 @@ def test_an_infinite_inner_value_keeps_the_sign_of_its_outputs(sign):
     layer.plan(1).forward(x, y, 1)
     torch.cuda.synchronize()
     assert (y == sign * math.inf).all()
+
+
+@pytest.mark.parametrize("dt", [L.F32, L.F16, L.BF16])
+@pytest.mark.parametrize("E,top", [(1, 1), (8, 2), (32, 32), (100, 5), (512, 16)])
+@pytest.mark.parametrize("normalize", [False, True])
+@pytest.mark.parametrize("spread", [0.05, 1.0, 8.0])
+def test_routing_weights_are_rounded_once(dt, E, top, normalize, spread):
+    """Weights are taken in 64 bits, of sums in 64 bits, and rounded to fp32: half a unit in the last place is 2^-24 of a
+    weight; the sums of 64 products, some 80 in all at the largest spread, are off by 64 * 80 * 2^-53 at most on either side, which
+    with exp and the quotient is less than 2^-38 of a weight.  Below 2^-126 a unit is 2^-149."""
+    layer = Layer(dt, 64, 8, E, top, seed=E)
+    layer.router[:] = (layer.router.float() * spread).to(TORCH[dt])
+    x = layer.tokens(40)
+    y = torch.empty_like(x)
+    w = torch.full((40, top), math.nan, device="cuda")
+    layer.plan(40, normalize).forward(x, y, 40, weights=w)
+    torch.cuda.synchronize()
+    _, _, _, want = layer.exact(x, normalize)
+    assert ((w.double() - want).abs() <= (2.0 ** -24 + 2.0 ** -38) * want + 2.0 ** -149).all()
