@@ -123,16 +123,36 @@ class DecodeAttention:
 
 class DecodeExperts:
     """One layer's experts for up to ``batch`` tokens: ``router`` [experts][hidden], ``gate`` and ``up`` [experts][inner][hidden],
-    ``down`` [experts][hidden][inner], of one type (see :class:`MoeLayer`).  :meth:`step` allocates nothing and may be captured."""
+    ``down`` [experts][hidden][inner], of one type on one device (see :class:`MoeLayer`); rows and experts may be strided.
+    :meth:`step` allocates nothing and may be captured."""
 
     def __init__(self, router, gate, up, down, top: int, batch: int, normalize: bool = True, device: int = 0):
         import torch
 
+        kind = {torch.float32: L.F32, torch.float16: L.F16, torch.bfloat16: L.BF16}.get(gate.dtype)
+        if kind is None or gate.dim() != 3:
+            raise ValueError(f"gate is {gate.dtype} {list(gate.shape)}: [experts][inner][hidden] of 32 or 16 bits")
         experts, inner, hidden = gate.shape
-        kind = {torch.float32: L.F32, torch.float16: L.F16, torch.bfloat16: L.BF16}[gate.dtype]
-        self.layer = L.MoeLayer(router, gate, up, down, hidden, inner, experts, top, batch, kind, normalize, router_row=router.stride(0),
-                                gate_row=gate.stride(1), up_row=up.stride(1), down_row=down.stride(1), gate_expert=gate.stride(0),
-                                up_expert=up.stride(0), down_expert=down.stride(0), device=device)
+        for name, t, shape in (("router", router, (experts, hidden)), ("gate", gate, (experts, inner, hidden)), ("up", up, (experts, inner, hidden)),
+                               ("down", down, (experts, hidden, inner))):
+            if t.dtype != gate.dtype:
+                raise ValueError(f"{name} is {t.dtype}, gate {gate.dtype}: all of one type")
+            if tuple(t.shape) != shape:
+                raise ValueError(f"{name} has the shape {list(t.shape)}, not {list(shape)}")
+            if t.shape[-1] > 1 and t.stride(-1) != 1:
+                raise ValueError(f"{name}: the elements of a row must be next to each other (transposed?)")
+            if any(n > 1 and step == 0 for n, step in zip(t.shape, t.stride())):
+                raise ValueError(f"{name} is expanded: every row must be in memory")
+        for name, t in (("router", router), ("gate", gate), ("up", up), ("down", down)):
+            if t.device != torch.device("cuda", device):
+                raise ValueError(f"{name} is on {t.device}, not on cuda:{device}")
+
+        def step(t, dim):  # 0 (dense) where there is one, whose stride says nothing
+            return t.stride(dim) if t.shape[dim] > 1 else 0
+
+        self.layer = L.MoeLayer(router, gate, up, down, hidden, inner, experts, top, batch, kind, normalize, router_row=step(router, 0),
+                                gate_row=step(gate, 1), up_row=step(up, 1), down_row=step(down, 1), gate_expert=step(gate, 0),
+                                up_expert=step(up, 0), down_expert=step(down, 0), device=device)
         self.batch = batch
         self.ids = torch.zeros(batch, top, dtype=torch.int32, device=gate.device)
 

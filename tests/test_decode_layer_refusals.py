@@ -1,0 +1,33 @@
+"""What the decoding layer's classes refuse of the tensors they are given: before any device is touched, so these run without a GPU."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import l2domain_b200 as L  # noqa: E402
+from l2domain_b200 import decode  # noqa: E402
+
+
+def experts(dtype=torch.bfloat16, **kw):
+    E, F, H = 4, 8, 16
+    w = dict(router=torch.zeros(E, H, dtype=dtype), gate=torch.zeros(E, F, H, dtype=dtype), up=torch.zeros(E, F, H, dtype=dtype),
+             down=torch.zeros(E, H, F, dtype=dtype))
+    w.update(kw)
+    return decode.DecodeExperts(**w, top=2, batch=3)
+
+
+@pytest.mark.parametrize("bad,word", [
+    (dict(router=torch.zeros(4, 16)), "router is torch.float32"), (dict(up=torch.zeros(4, 8, 16)), "up is torch.float32"),
+    (dict(down=torch.zeros(4, 16, 8, dtype=torch.float16)), "down is torch.float16"), (dict(gate=torch.zeros(4, 8, 16, dtype=torch.float64)), "gate is"),
+    (dict(gate=torch.zeros(8, 16, dtype=torch.bfloat16)), "gate is"), (dict(gate=torch.zeros(4, 8, 16)), "router is torch.bfloat16"),
+    (dict(router=torch.zeros(3, 16, dtype=torch.bfloat16)), "router has the shape"), (dict(router=torch.zeros(16, 4, dtype=torch.bfloat16)), "router has the shape"),
+    (dict(up=torch.zeros(4, 16, 8, dtype=torch.bfloat16)), "up has the shape"), (dict(down=torch.zeros(4, 8, 16, dtype=torch.bfloat16)), "down has the shape"),
+    (dict(router=torch.zeros(16, 4, dtype=torch.bfloat16).t()), "router: the elements"), (dict(gate=torch.zeros(4, 16, 8, dtype=torch.bfloat16).mT), "gate: the elements"),
+    (dict(down=torch.zeros(4, 8, 16, dtype=torch.bfloat16).mT), "down: the elements"),
+    (dict(gate=torch.zeros(1, 8, 16, dtype=torch.bfloat16).expand(4, 8, 16)), "gate is expanded"),
+    (dict(up=torch.zeros(4, 1, 16, dtype=torch.bfloat16).expand(4, 8, 16)), "up is expanded"),
+    (dict(router=torch.zeros(1, 16, dtype=torch.bfloat16).expand(4, 16)), "router is expanded"),
+    ({}, "on cpu"),
+])
+def test_experts_of_other_tensors_are_refused(bad, word):
+    with pytest.raises(ValueError, match=word):
+        experts(**bad)

@@ -8,6 +8,7 @@ torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 import l2domain_b200 as L  # noqa: E402
+from l2domain_b200 import decode  # noqa: E402
 from test_decode_ops_gpu import TORCH, close, gpu, offset_view  # noqa: E402,F401
 from test_moe_gpu import Layer, check  # noqa: E402
 
@@ -79,3 +80,22 @@ def test_routing_weights_are_rounded_once(dt, E, top, normalize, spread):
     torch.cuda.synchronize()
     _, _, _, want = layer.exact(x, normalize)
     assert ((w.double() - want).abs() <= (2.0 ** -24 + 2.0 ** -38) * want + 2.0 ** -149).all()
+
+
+def test_experts_of_the_decoding_layer_may_be_strided():
+    """Rows and experts of views, and sizes of one whose strides say nothing."""
+    for E, F, H, top in ((3, 24, 40, 2), (1, 8, 16, 1), (2, 1, 8, 1), (2, 8, 1, 2)):
+        layer = Layer(L.BF16, H, F, E, top, seed=F)
+        wide = torch.zeros(E, F, 2, H + 3, dtype=torch.bfloat16, device="cuda")
+        wide[:, :, 0, :H], wide[:, :, 1, :H] = layer.gate, layer.up
+        router = torch.zeros(E, 2 * H, dtype=torch.bfloat16, device="cuda")[:, H:]
+        router.copy_(layer.router)
+        down = layer.down.as_strided((E, H, F), tuple(s if n > 1 else 5 for n, s in zip((E, H, F), layer.down.stride())))
+        moe = decode.DecodeExperts(router, wide[:, :, 0, :H], wide[:, :, 1, :H], down, top, 4)
+        x = layer.tokens(4)
+        y = torch.empty_like(x)
+        moe.step(x, y)
+        torch.cuda.synchronize()
+        want, slack, ids, _ = layer.exact(x, True)
+        assert torch.equal(moe.ids.long(), ids)
+        close(y, want, slack, L.BF16)
