@@ -722,6 +722,15 @@ class PagedAttention:
                  window: int = 0, max_batch: int = 0, table_stride: int = 0, q_token: int = 0, out_token: int = 0,
                  status=None, cap: float = 0.0, slopes=None):
         self._plan = C.c_void_p(0)
+        if hasattr(slopes, "data_ptr"):  # a tensor, and not an address
+            if str(slopes.dtype) != "torch.float32":
+                raise ValueError(f"slopes are {slopes.dtype}, not float32")
+            if tuple(slopes.shape) != (heads_q,):
+                raise ValueError(f"slopes have the shape {list(slopes.shape)}, for {heads_q} query heads")
+            if heads_q > 1 and slopes.stride(0) != 1:
+                raise ValueError("slopes must be next to each other")
+            if slopes.device.type != "cuda" or slopes.device.index != cache.fields["device"]:
+                raise ValueError(f"slopes are on {slopes.device}, the cache on cuda:{cache.fields['device']}")
         self._hold = (cache, table, status, slopes)
         cd = cache.desc(table, num_seqs, table_width, table_stride, status)
         ad = AttnDesc(heads_q=heads_q, window=window, scale=scale, max_batch=max_batch, q_token=q_token,
@@ -749,7 +758,8 @@ class PagedAttention:
 
 
 def distance_slopes(heads: int, device=None):
-    """fp32 [heads]: a geometric row of slopes from 2^(-8 / heads) to 2^-8, for :class:`PagedAttention`."""
+    """fp32 [heads]: a geometric row of slopes from 2^(-8 / heads) to 2^-8, for :class:`PagedAttention`, which takes them on its
+    device (None: torch's default, the host)."""
     import torch
 
     return torch.exp2(-8.0 * torch.arange(1, heads + 1, dtype=torch.float64, device=device) / heads).float()

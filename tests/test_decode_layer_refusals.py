@@ -31,3 +31,16 @@ def experts(dtype=torch.bfloat16, **kw):
 def test_experts_of_other_tensors_are_refused(bad, word):
     with pytest.raises(ValueError, match=word):
         experts(**bad)
+
+
+@pytest.mark.parametrize("bad,word", [
+    (torch.zeros(4), "on cpu"), (torch.zeros(4, dtype=torch.bfloat16), "float32"), (torch.zeros(4, dtype=torch.float64), "float32"),
+    (torch.zeros(3), "4 query heads"), (torch.zeros(8)[::2], "next to each other"), (torch.zeros(1).expand(4), "next to each other"),
+    (L.distance_slopes(4), "on cpu"),
+])
+@pytest.mark.parametrize("four", [False, True])
+def test_slopes_of_other_tensors_are_refused(four, bad, word):
+    """distance_slopes() gives a tensor of the host unless it is told a device."""
+    c = dict(k=0x10000000, v=0x10000000, dtype=L.BF16, num_pages=8, page_size=16, heads=2, head_dim=64)
+    with pytest.raises(ValueError, match=word):
+        L.PagedAttention((L.KvCache4 if four else L.KvCache)(**c), 0x10000000, 4, 4, 4, slopes=bad)
