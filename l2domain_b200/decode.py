@@ -103,11 +103,27 @@ class DecodeAttention:
 
     def prompt(self, qkv, pos, seq, tokens: int, k_out=None, v_out=None, stream=None) -> None:
         """Appends ``tokens`` tokens of prompts, rows of ``qkv`` [tokens][(heads + 2 kv_heads) * head_dim] at positions pos
-        of sequences seq (int32), and rotates their queries in place.  ``k_out`` and ``v_out`` (a cache of 4 bits; strided as
+        of sequences seq (int32), and rotates their queries in place.  ``k_out`` and ``v_out`` (a cache of 4 bits; bf16, strided as
         qkv): keys and values as the cache holds them, for the prompt's own attention."""
-        hd = self.heads * self.head_dim
-        self.append.append(qkv[:, hd:], qkv[:, hd + self.kv_heads * self.head_dim:], pos, tokens, seq=seq, q=qkv, q_out=qkv, k_out=k_out,
-                           v_out=v_out, stream=stream)
+        import torch
+
+        hd, kv = self.heads * self.head_dim, self.kv_heads * self.head_dim
+        row, dev = hd + 2 * kv, self.status.device
+
+        def rows_of(name, t, least):
+            if t.dtype != torch.bfloat16 or t.dim() != 2 or t.shape[0] < tokens or t.shape[1] < least or t.device != dev or (
+                    t.stride(1) != 1 or (tokens > 1 and t.stride(0) != row)):
+                raise ValueError(f"{name} is {t.dtype} {list(t.shape)} strided {t.stride()} on {t.device}: bfloat16, {tokens} rows of "
+                                 f"{least} elements and more, strided ({row}, 1), on {dev}")
+
+        rows_of("qkv", qkv, row)
+        for name, t in (("k_out", k_out), ("v_out", v_out)):
+            if t is not None:
+                rows_of(name, t, kv)
+        for name, t in (("pos", pos), ("seq", seq)):
+            if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] < tokens or not t.is_contiguous() or t.device != dev:
+                raise ValueError(f"{name} is {t.dtype} {list(t.shape)} on {t.device}: int32, {tokens} or more in a row, on {dev}")
+        self.append.append(qkv[:, hd:], qkv[:, hd + kv:], pos, tokens, seq=seq, q=qkv, q_out=qkv, k_out=k_out, v_out=v_out, stream=stream)
 
     def step(self, x, pos, lens, out, stream=None, starts=None) -> None:
         """out[b] = W_out . attention of the token x[b] at position pos[b] over itself and the lens[b] - 1 before it, those from

@@ -44,3 +44,27 @@ def test_slopes_of_other_tensors_are_refused(four, bad, word):
     c = dict(k=0x10000000, v=0x10000000, dtype=L.BF16, num_pages=8, page_size=16, heads=2, head_dim=64)
     with pytest.raises(ValueError, match=word):
         L.PagedAttention((L.KvCache4 if four else L.KvCache)(**c), 0x10000000, 4, 4, 4, slopes=bad)
+
+
+def layer():
+    """A DecodeAttention's sizes alone: 4 + 2 * 2 heads of 16."""
+    it = object.__new__(decode.DecodeAttention)
+    it.heads, it.kv_heads, it.head_dim = 4, 2, 16
+    it.status = torch.zeros(1)
+    return it
+
+
+@pytest.mark.parametrize("bad,word", [
+    (dict(qkv=torch.zeros(5, 128)), "qkv is"), (dict(qkv=torch.zeros(5, 130, dtype=torch.bfloat16)[:, :128]), "qkv is"),
+    (dict(qkv=torch.zeros(4, 128, dtype=torch.bfloat16)), "qkv is"), (dict(qkv=torch.zeros(5, 96, dtype=torch.bfloat16)), "qkv is"),
+    (dict(k_out=torch.zeros(5, 32, dtype=torch.bfloat16)), "k_out is"), (dict(v_out=torch.zeros(5, 32, dtype=torch.bfloat16)), "v_out is"),
+    (dict(k_out=torch.zeros(5, 128)), "k_out is"), (dict(v_out=torch.zeros(4, 128, dtype=torch.bfloat16)), "v_out is"),
+    (dict(k_out=torch.zeros(5, 128, dtype=torch.bfloat16)[:, :16]), "k_out is"),
+    (dict(pos=torch.zeros(5, dtype=torch.int64)), "pos is"), (dict(seq=torch.zeros(5, dtype=torch.int64)), "seq is"), (dict(pos=torch.zeros(4, dtype=torch.int32)), "pos is"),
+])
+def test_prompts_of_other_tensors_are_refused(bad, word):
+    """Keys and values as held are strided as qkv: rows of their own would be written past their end."""
+    a = dict(qkv=torch.zeros(5, 128, dtype=torch.bfloat16), pos=torch.zeros(5, dtype=torch.int32), seq=torch.zeros(5, dtype=torch.int32))
+    a.update(bad)
+    with pytest.raises(ValueError, match=word):
+        layer().prompt(a["qkv"], a["pos"], a["seq"], 5, k_out=a.get("k_out"), v_out=a.get("v_out"))
