@@ -513,8 +513,8 @@ L2D_API int l2d_attn_plan_create_kv4(const l2d_kv4_cache *cache, const l2d_attn_
  *   y[t] = sum_k w_k down_e (silu(gate_e x[t]) * (up_e x[t])),  e = ids[t][k]
  * The experts are the `top` largest of router x[t], in falling order and of equal ones the lower first (a NaN counts as the
  * least); w is their softmax over all experts and, where normalize is set, divided by the chosen ones' sum.  Router sums
- * are fp64, so that no order of addition chooses; the others fp32.  silu(..) * .. meets down as two numbers of dtype (fp32: as it
- * is): 2^-16 of it is left (bf16), or 2^-22 of it and 2^-39 of the token's largest with this expert (fp16). */
+ * are fp64, so that no order of addition chooses; the others fp32.  silu(..) * .. meets down as it is (fp32),
+ * as three bf16 numbers that add up to it, or as two fp16 ones: 2^-22 of it and 2^-39 of the token's largest with this expert are left. */
 typedef struct l2d_moe_plan l2d_moe_plan;
 typedef struct {
     int64_t hidden, inner;               /* elements of a token, and of an expert's inner vector */

@@ -43,12 +43,12 @@ struct MoeArgs {
     double *logits;       // [tokens][experts]
     int *ids;             // [slots], slot = token * top + choice
     float *weights;       // [slots]
-    uint32_t *largest;    // [slots] bits of the largest |silu(gate x) (up x)| (fp16)
+    uint32_t *largest;    // [slots] bits of the largest |silu(gate x) (up x)| (fp16; bf16: of one that is not finite, or 0)
     int *sorted;          // [slots], by expert
     int4 *entries;        // expert, first place in sorted, slots
-    int *num_entries;
+    int *num_entries;     // and whether an inner value is not finite (bf16)
     unsigned *arrived;    // [token tiles + 1], zero between calls
-    uint32_t *inner_out;  // [slots][inner_row] fp32, or two bf16 numbers that add up to one
+    float *inner_out;     // [slots][inner_row]
     float *part;          // [slots][hidden]
     int64_t inner_row;
 };
@@ -167,7 +167,7 @@ __device__ __forceinline__ void sort_slots(const MoeArgs &a) {
             const int x = __shfl_up_sync(0xffffffffu, upto, d), y = __shfl_up_sync(0xffffffffu, upto_entries, d);
             if (tid >= d) upto += x, upto_entries += y;
         }
-        if (tid == 31) *a.num_entries = upto_entries;
+        if (tid == 31) a.num_entries[0] = upto_entries, a.num_entries[1] = 0;
         upto -= here;
         upto_entries -= entries;
         for (int i = 0; i < kEach; ++i) {
@@ -280,8 +280,11 @@ __global__ void __launch_bounds__(kMoeThreads) k_route(const __grid_constant__ M
 // the ends of items; columns are read from L1 or L2 a step ahead.  Where there are few items, their rows are cut into S
 // parts for as many warps of a block.
 //
-// silu(gate x) (up x) is held to more than 16 bits: for bf16 as two numbers, for fp16 in fp32 and cut into two on the way to
-// the down product, relative to the slot's largest, which only the whole first product knows.
+// silu(gate x) (up x) is held in fp32 and cut on the way to the down product: for bf16 into three numbers that add up to it, for fp16
+// into two, relative to the slot's largest, which only the whole first product knows.
+//
+// The products of a step are added to the sum in fp32: the instruction cuts them off at its sum's last place, which over a long row
+// takes off as much as two numbers for an inner value would.
 //
 // 32 bits: a warp works on four rows (two of gate and of up) with the lanes along them, by fused multiply-adds.
 // ---------------------------------------------------------------------------------------------
@@ -382,21 +385,6 @@ __device__ __forceinline__ Items items_of(int entries, int tiles, int groups, in
 
 __device__ __forceinline__ float silu_times(float gate, float up) { return gate / (1.0f + expf(-gate)) * up; }
 
-// The first of two bf16 numbers that add up to a number, in the low half, the second in the upper.  An infinity or a NaN is its
-// first alone; a finite number's first is none, so the largest ones' is cut off and not rounded.
-__device__ __forceinline__ uint32_t two_bf16(float x) {
-    auto bits_of = [](float v) {
-        const __nv_bfloat16 b = __float2bfloat16_rn(v);
-        uint16_t r;
-        memcpy(&r, &b, 2);
-        return static_cast<uint32_t>(r);
-    };
-    uint32_t hi = bits_of(x);
-    if (!(fabsf(x) <= FLT_MAX)) return hi;
-    if ((hi & 0x7fffu) == 0x7f80u) hi = __float_as_uint(x) >> 16;
-    return hi | bits_of(x - __uint_as_float(hi << 16)) << 16;
-}
-
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     uint32_t r;
@@ -417,17 +405,19 @@ struct Lists {
     const int4 *entries;
     const int *sorted;
     int num;
+    bool odd;  // an inner value is not finite
 };
 __device__ __forceinline__ Lists lists_of(const MoeArgs &a) {
     __shared__ int4 kept_entries[kCached];
     __shared__ int kept_sorted[kCachedSlots];
     const int slots = a.tokens * a.top;
-    const int num = *a.num_entries;
-    if (num > kCached || slots > kCachedSlots) return {a.entries, a.sorted, num};
+    const int2 two = *reinterpret_cast<const int2 *>(a.num_entries);
+    const int num = two.x;
+    if (num > kCached || slots > kCachedSlots) return {a.entries, a.sorted, num, two.y != 0};
     for (int i = threadIdx.x; i < num; i += kMoeThreads) kept_entries[i] = a.entries[i];
     for (int i = threadIdx.x; i < slots; i += kMoeThreads) kept_sorted[i] = a.sorted[i];
     __syncthreads();
-    return {kept_entries, kept_sorted, num};
+    return {kept_entries, kept_sorted, num, two.y != 0};
 }
 
 // A warp's ring: a step's rows, then its columns (16 bytes a lane of each eight and run, of four-byte elements twice), as deep as
@@ -447,6 +437,7 @@ template <typename T, int N, bool DOWN, int COPY>
 __global__ void __launch_bounds__(kMoeThreads, ExpertsRing<N, DOWN, COPY == kByHalves>::kBlocks) k_experts(const __grid_constant__ MoeArgs a, int S) {
     constexpr bool kHalf = std::is_same<T, __half>::value;
     constexpr int kK = 64;                           // elements of a step: two runs of 32
+    constexpr int kCuts = kHalf ? 2 : 3;             // 16-bit numbers of an inner value
     using Ring = ExpertsRing<N, DOWN, COPY == kByHalves>;
     extern __shared__ __align__(128) char smem[];
     dev::wait_for_previous();
@@ -465,7 +456,7 @@ __global__ void __launch_bounds__(kMoeThreads, ExpertsRing<N, DOWN, COPY == kByH
     float *meet = reinterpret_cast<float *>(smem + kMoeWarps * Ring::kBytes);  // [warp][4 N][lane]
 
     // What is brought next: rows g and g + 8 from p0 and p1 on, and column g of each eight, `left` steps of them.
-    using X = typename std::conditional<DOWN, uint32_t, T>::type;
+    using X = typename std::conditional<DOWN, float, T>::type;
     constexpr int kRun = DOWN ? 2 : 1;  // 16-byte words of eight elements of a column
     int item = items.first, left = 0, in_at = 0, in_count = 0;
     const T *p0 = nullptr, *p1 = nullptr;
@@ -569,12 +560,12 @@ __global__ void __launch_bounds__(kMoeThreads, ExpertsRing<N, DOWN, COPY == kByH
         const int4 entry = lists.entries[at];
         float factor[N];  // what makes this lane's columns fp16
         uint32_t low_mask[N];
-        if constexpr (DOWN && kHalf) {
+        if constexpr (DOWN) {
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                const uint32_t bits = a.largest[lists.sorted[entry.y + min(8 * j + g, entry.z - 1)]];
-                factor[j] = to_half_range(bits);
-                low_mask[j] = bits >= 0x7f800000u ? 0 : 0xffffffffu;
+                const uint32_t bits = kHalf || lists.odd ? a.largest[lists.sorted[entry.y + min(8 * j + g, entry.z - 1)]] : 0;
+                if constexpr (kHalf) factor[j] = to_half_range(bits);
+                low_mask[j] = bits >= 0x7f800000u ? 0 : 0xffffffffu;  // beside an infinity or a NaN first numbers alone
             }
         }
         // Which rows and columns begin in the middle of a word: the products' matrices begin at one.
@@ -603,6 +594,7 @@ __global__ void __launch_bounds__(kMoeThreads, ExpertsRing<N, DOWN, COPY == kByH
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 if (j && 8 * j >= entry.z) break;
+                float sum[4] = {};
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const uint4 &r0 = r[h][0], &r1 = r[h][1];
@@ -611,31 +603,44 @@ __global__ void __launch_bounds__(kMoeThreads, ExpertsRing<N, DOWN, COPY == kByH
                     if constexpr (!DOWN && COPY == kByHalves) u = from_halves(reinterpret_cast<const char *>(x), from + fifths + 512 + 256 * j + 128 * h, skip_x[j]);
                     else u = x[0];
                     if constexpr (!DOWN) {
-                        mma<T>(acc[j], r0.x, r1.x, r0.y, r1.y, u.x, u.y);
-                        mma<T>(acc[j], r0.z, r1.z, r0.w, r1.w, u.z, u.w);
+                        mma<T>(sum, r0.x, r1.x, r0.y, r1.y, u.x, u.y);
+                        mma<T>(sum, r0.z, r1.z, r0.w, r1.w, u.z, u.w);
                     } else {
                         const uint4 v = x[32];
                         const uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-                        uint32_t hi[4], lo[4];
+                        uint32_t cut[kCuts][4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
+                            float one = __uint_as_float(w[2 * i]), two = __uint_as_float(w[2 * i + 1]);
                             if constexpr (kHalf) {
-                                const float one = __uint_as_float(w[2 * i]) * factor[j], two = __uint_as_float(w[2 * i + 1]) * factor[j];
-                                hi[i] = pack_half(one, two);
+                                one *= factor[j], two *= factor[j];
+                                cut[0][i] = pack_half(one, two);
                                 __half2 halves;
-                                memcpy(&halves, &hi[i], 4);
-                                lo[i] = pack_half(one - __low2float(halves), two - __high2float(halves)) & low_mask[j];
-                            } else {
-                                hi[i] = __byte_perm(w[2 * i], w[2 * i + 1], 0x5410);
-                                lo[i] = __byte_perm(w[2 * i], w[2 * i + 1], 0x7632);
+                                memcpy(&halves, &cut[0][i], 4);
+                                cut[1][i] = pack_half(one - __low2float(halves), two - __high2float(halves)) & low_mask[j];
+                            } else {  // cut off, not rounded: what is left is exact, and the largest number's first part finite
+#pragma unroll
+                                for (int part = 0; part < kCuts; ++part) {
+                                    const uint32_t low = __float_as_uint(one), high = __float_as_uint(two);
+                                    cut[part][i] = __byte_perm(low, high, 0x7632);
+                                    one -= __uint_as_float(low & 0xffff0000u);
+                                    two -= __uint_as_float(high & 0xffff0000u);
+                                }
                             }
                         }
-                        mma<T>(acc[j], r0.x, r1.x, r0.y, r1.y, hi[0], hi[1]);
-                        mma<T>(acc[j], r0.z, r1.z, r0.w, r1.w, hi[2], hi[3]);
-                        mma<T>(acc[j], r0.x, r1.x, r0.y, r1.y, lo[0], lo[1]);
-                        mma<T>(acc[j], r0.z, r1.z, r0.w, r1.w, lo[2], lo[3]);
+#pragma unroll
+                        for (int part = 0; part < kCuts; ++part) {
+                            if (!kHalf && part && lists.odd) {
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) cut[part][i] &= low_mask[j];
+                            }
+                            mma<T>(sum, r0.x, r1.x, r0.y, r1.y, cut[part][0], cut[part][1]);
+                            mma<T>(sum, r0.z, r1.z, r0.w, r1.w, cut[part][2], cut[part][3]);
+                        }
                     }
                 }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[j][e] += sum[e];
             }
             bring_step();  // into the step before's place, which this lane has read
             out_at = out_at + Ring::kStep == Ring::kBytes ? 0 : out_at + Ring::kStep;
@@ -676,14 +681,15 @@ __global__ void __launch_bounds__(kMoeThreads, ExpertsRing<N, DOWN, COPY == kByH
                     const int row = tile * 8 + g;
                     const bool real = c < entry.z && row < rows;
                     const float h = real ? silu_times(acc[j][e], acc[j][2 + e]) : 0.0f;
+                    if (real) a.inner_out[slot * a.inner_row + row] = h;
                     if constexpr (kHalf) {
                         uint32_t top = __float_as_uint(h) & 0x7fffffffu;
 #pragma unroll
                         for (int d = 4; d < 32; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
                         if (g == 0 && c < entry.z && top) atomicMax(a.largest + slot, top);
-                        if (real) a.inner_out[slot * a.inner_row + row] = __float_as_uint(h);
-                    } else {
-                        if (real) a.inner_out[slot * a.inner_row + row] = two_bf16(h);
+                    } else if (!(fabsf(h) <= FLT_MAX)) {  // not of a row or column that is not real: those are 0
+                        atomicMax(a.largest + slot, __float_as_uint(h) & 0x7fffffffu);
+                        a.num_entries[1] = 1;
                     }
                 }
             }
@@ -768,7 +774,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) k_experts32(const __grid_const
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
             const int slot = lists.sorted[entry.y + min(c, entry.z - 1)];
-            column[c] = DOWN ? reinterpret_cast<const float *>(a.inner_out) + slot * a.inner_row : static_cast<const float *>(a.x) + slot / a.top * a.x_token;
+            column[c] = DOWN ? a.inner_out + slot * a.inner_row : static_cast<const float *>(a.x) + slot / a.top * a.x_token;
         }
         float acc[32] = {};  // [row][column]
         int k = first_k;
@@ -834,7 +840,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) k_experts32(const __grid_const
         } else {
             const float up = __shfl_down_sync(0xffffffffu, s, 16);
             if (row < 2 && c < entry.z && tile * 2 + row < rows)
-                a.inner_out[lists.sorted[entry.y + c] * a.inner_row + tile * 2 + row] = __float_as_uint(silu_times(s, up));
+                a.inner_out[lists.sorted[entry.y + c] * a.inner_row + tile * 2 + row] = silu_times(s, up);
         }
     }
 }
@@ -989,7 +995,7 @@ int l2d_moe_plan_create(const l2d_moe_desc *desc, l2d_moe_plan **plan) {
     const size_t tiles = (d.max_tokens + kRouteTokens - 1) / kRouteTokens, entries = d.experts + slots / 8 + 1;
     const size_t inner_at = take(slots * inner_row * 4), part_at = take(slots * d.hidden * 4), logits_at = take(size_t(d.max_tokens) * d.experts * 8),
                  ids_at = take(slots * 4), weights_at = take(slots * 4), largest_at = take(slots * 4), sorted_at = take(slots * 4),
-                 entries_at = take(entries * 16), num_at = take(4), arrived_at = take((tiles + 1) * 4);
+                 entries_at = take(entries * 16), num_at = take(8), arrived_at = take((tiles + 1) * 4);
     void *memory = nullptr;
     cudaError_t e = cudaMalloc(&memory, bytes);
     if (e != cudaSuccess) {
@@ -1034,7 +1040,7 @@ int l2d_moe_plan_create(const l2d_moe_desc *desc, l2d_moe_plan **plan) {
     a.experts = d.experts;
     a.top = d.top;
     a.normalize = d.normalize;
-    a.inner_out = reinterpret_cast<uint32_t *>(base + inner_at);
+    a.inner_out = reinterpret_cast<float *>(base + inner_at);
     a.part = reinterpret_cast<float *>(base + part_at);
     a.logits = reinterpret_cast<double *>(base + logits_at);
     a.ids = reinterpret_cast<int *>(base + ids_at);

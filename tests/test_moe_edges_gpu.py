@@ -99,3 +99,44 @@ def test_experts_of_the_decoding_layer_may_be_strided():
         want, slack, ids, _ = layer.exact(x, True)
         assert torch.equal(moe.ids.long(), ids)
         close(y, want, slack, L.BF16)
+
+
+def test_inner_values_of_bf16_keep_what_fp32_holds():
+    """Outputs that are differences of two nearly equal inner values.  Their sums are one exact product each; exp is off by two
+    units (2^-22), the three operations after it by 2^-24 each: 14 * 2^-24 of the larger for two.  The difference: three parts of each,
+    in six instructions at most, that cut two operands off at the last place of the largest (2^-23): 24 * 2^-24."""
+    H, F = 2048, 4096
+    layer = Layer(L.BF16, H, F, 1, 1, seed=12)
+    g = layer.g
+    layer.gate[:], layer.up[:], layer.down[:] = 0.0, 0.0, 0.0
+    layer.gate[0, :, 0] = torch.empty(F, device="cuda").uniform_(1.0, 2.0, generator=g).bfloat16()
+    layer.up[0, :, 1] = torch.empty(F, device="cuda").uniform_(1.0, 2.0, generator=g).bfloat16()
+    x = torch.zeros(1, H, dtype=torch.bfloat16, device="cuda")
+    x[0, 0], x[0, 1] = 1.171875, 1.3203125
+    a, b = (m[0].double() @ x[0].double() for m in (layer.gate, layer.up))
+    h = a * torch.sigmoid(a) * b
+    order = torch.sort(h)[1].view(H, 2)
+    rows = torch.arange(H, device="cuda")
+    layer.down[0, rows, order[:, 1]], layer.down[0, rows, order[:, 0]] = 1.0, -1.0
+    y = torch.empty_like(x)
+    layer.plan(1).forward(x, y, 1)
+    torch.cuda.synchronize()
+    want = h[order[:, 1]] - h[order[:, 0]]
+    assert want.abs().mean() < 2.0 ** -9 * h.mean()
+    close(y[0], want, 38 * 2.0 ** -24 * h[order].amax(1), L.BF16)
+
+
+@pytest.mark.parametrize("dt", [L.F16, L.BF16])
+def test_an_odd_inner_value_is_its_slots_alone(dt):
+    """A token whose inner values are not finite beside others of the same expert, in one call and in the next."""
+    layer = Layer(dt, 64, 72, 2, 1, seed=13)
+    x = layer.tokens(20)
+    clean = check(layer, 20, x=x)[0]
+    plan, bad = layer.plan(20), x.clone()
+    bad[3], bad[11] = math.inf, math.nan
+    y = torch.empty_like(x)
+    plan.forward(bad, y, 20)
+    torch.cuda.synchronize()
+    rest = [t for t in range(20) if t not in (3, 11)]
+    assert torch.equal(y[rest], clean[rest]) and not torch.isfinite(y[[3, 11]]).any()
+    assert torch.equal(check(layer, 20, x=x, plan=plan)[0], clean)
