@@ -108,3 +108,12 @@ def test_without_a_gpu_the_operators_report_no_device():
         with pytest.raises(L.L2DError) as e:
             call(op)
         assert e.value.status == NO_DEVICE
+
+
+@pytest.mark.parametrize("op", OPS)
+@pytest.mark.parametrize("side", ["k_page", "v_page"])
+@pytest.mark.parametrize("bytes_apart", [(1 << 31) + 16, 3_000_000_000 // 16 * 16])
+def test_pages_more_than_2_31_bytes_apart_are_refused(op, side, bytes_apart):
+    with pytest.raises(L.L2DError, match="too large") as e:
+        call(op, {side: bytes_apart})
+    assert e.value.status == INVALID

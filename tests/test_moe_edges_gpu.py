@@ -140,3 +140,27 @@ def test_an_odd_inner_value_is_its_slots_alone(dt):
     rest = [t for t in range(20) if t not in (3, 11)]
     assert torch.equal(y[rest], clean[rest]) and not torch.isfinite(y[[3, 11]]).any()
     assert torch.equal(check(layer, 20, x=x, plan=plan)[0], clean)
+
+
+def test_small_inner_values_of_fp16_beside_a_large_one():
+    """Inner values are cut into two fp16 numbers relative to the largest, M = 2^14 .. 2^15 then: the second is off by 2^-25 where
+    it is subnormal, 2^-39 of M.  Beside that an output is off by silu's seven roundings of 2^-24 (an exp of two units and three
+    operations; sums are one exact product each), down times."""
+    H, F = 64, 256
+    layer = Layer(L.F16, H, F, 1, 1, seed=14)
+    layer.gate[:], layer.up[:], layer.down[:] = 0.0, 0.0, 0.0
+    layer.gate[0, :, 0] = torch.empty(F, device="cuda").uniform_(1.0, 2.0, generator=layer.g).half()
+    layer.up[0, :, 1] = torch.exp2(-torch.empty(F, device="cuda").uniform_(0.0, 14.0, generator=layer.g)).half()
+    layer.up[0, 0, 1], layer.up[0, 0, 2] = 0.0, 32768.0  # the largest
+    layer.down[0, :, :H] = 0.0
+    rows, at = torch.arange(H, device="cuda"), torch.arange(1, H + 1, device="cuda") * 3
+    layer.down[0, rows, at] = 32768.0
+    x = torch.zeros(1, H, dtype=torch.float16, device="cuda")
+    x[0, 0], x[0, 1], x[0, 2] = 1.0, 2.0 ** -13, 1.0
+    y = torch.empty_like(x)
+    layer.plan(1).forward(x, y, 1)
+    torch.cuda.synchronize()
+    a, b = (m[0].double() @ x[0].double() for m in (layer.gate, layer.up))
+    h = a * torch.sigmoid(a) * b
+    assert (h[1:] < 2.0 ** -27 * h[0]).all() and (h[at] < 2.0 ** -30 * h[0]).any()
+    close(y[0], 32768.0 * h[at], 32768.0 * (2.0 ** -39 * h[0] + (2.0 ** -22 + 7 * 2.0 ** -24) * h[at]), L.F16)
