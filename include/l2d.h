@@ -505,7 +505,8 @@ L2D_API int l2d_kv4_page_bytes(int heads, int head_dim, int page_size, int group
 L2D_API int l2d_kv4_append(const l2d_kv4_cache *cache, const l2d_append_desc *desc, const void *k, const void *v, const void *q, void *q_out,
                            void *k_out, void *v_out, const int32_t *pos, const int32_t *seq, int64_t tokens, void *stream);
 /* A plan of l2d_attn_decode and l2d_attn_decode_from over a cache in 4 bits; scores may be NULL.  Weights times scales meet
- * the values as two bf16 numbers (2^-16 of a weight is left), for fp32 queries as three, and so do the queries. */
+ * the values as two bf16 numbers (2^-16 of a weight is left), for fp32 queries as three, and so do the queries; what is below
+ * 2^-104 of a weight times its scale is lost whatever its size. */
 L2D_API int l2d_attn_plan_create_kv4(const l2d_kv4_cache *cache, const l2d_attn_desc *desc, const l2d_attn_scores *scores,
                                      l2d_attn_plan **plan);
 
@@ -533,7 +534,8 @@ typedef struct {
 /* The plan owns its device scratch (allocated here, never during l2d_moe_forward); calls of one plan must not overlap on the GPU. */
 L2D_API int l2d_moe_plan_create(const l2d_moe_desc *desc, l2d_moe_plan **plan);
 /* ids (int32) and weights (fp32), both [tokens][top], receive the choice; either may be NULL.  y must not overlap x or the weights.
- * Rows on 16-byte boundaries are read fastest; any are read. */
+ * Rows on 16-byte boundaries are read fastest; any are read.  A token's result is the same bits in every call of as many tokens,
+ * in whatever order they come; with another number of tokens sums may be cut elsewhere, and y's last bits change. */
 L2D_API int l2d_moe_forward(l2d_moe_plan *plan, const void *x, void *y, int32_t *ids, float *weights, int tokens, void *stream);
 L2D_API int l2d_moe_plan_destroy(l2d_moe_plan *plan);
 

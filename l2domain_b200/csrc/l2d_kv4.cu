@@ -15,9 +15,10 @@ namespace l2d {
 // sums and quotients are rounded one by one to fp32, so that what is stored follows from the inputs and not from how an
 // expression was compiled.
 //
-// Measured (32 query and 8 key-value heads of 128): 8192 tokens of fp16 in groups of 32, with what is held written out, 65 us,
-// 3.3 TB/s, for 34 us of bytes: some 400 warp instructions per 256 elements; 32 tokens 6 us, of which a launch 4.1.  Three blocks a
-// SM: 67 us with four.
+// Measured (32 query and 8 key-value heads of 128): 8192 tokens of fp16 in groups of 32, with what is held written out, 64 us,
+// 3.4 TB/s, for 34 us of bytes; 32 tokens 6 us, of which a launch 4.1.  Some 400 warp instructions per 256 elements use half of the
+// issue slots; what binds is the loads of the next head, which begin after this one is stored.  bf16 takes 98 us: at the 80
+// registers of three blocks a SM its kernels spill 172 bytes and more a thread, those of fp16 16 (67 us with four blocks).
 // ---------------------------------------------------------------------------------------------
 
 // Two numbers at a time, each rounded as by itself.
@@ -176,8 +177,9 @@ __device__ __forceinline__ void append4(const Append4Args &args, unsigned block_
         const bool bad = hi == INFINITY;
         const float by = word == 0 ? 1.0f : __uint_as_float(word), inverse = 1.0f / by;
         float z = fminf(rintf(__fdiv_rn(-lo, by)), 15.0f), s = __uint_as_float(word);
-        // x / s rounded to a whole number.  By the reciprocal it is off by less than 2^-20; where that may decide, and where
-        // the reciprocal is no number, the quotient itself is taken.  Adding 1.5 * 2^23 rounds to whole numbers.
+        // x / s rounded to a whole number.  By the reciprocal it is off by less than 2^-19, two roundings of up to 15, and the
+        // quotient rounded to fp32, which decides, by 2^-20 more: where a half is nearer than 2^-17, and where the reciprocal is no
+        // number, the quotient itself is taken.  Adding 1.5 * 2^23 rounds to whole numbers.
         constexpr float kWhole = 12582912.0f;
         float2 near[4];
         float far = 0.0f;

@@ -35,14 +35,21 @@ constexpr int kGroupBytes = kBlockSlots * 4;
 // nibble; the weights come from the layout of sums to that of a B operand by movmatrix.  (With the heads as rows eight of 16 would
 // be empty for groups of up to eight, or hold second parts, and their sums would take twice the registers.)
 //
-// Queries of 32 bits are three bf16 numbers that add up to them, and weights three; of 16 bits, weights two (2^-16 of
-// a weight is left).  The sums of products with each part of a query stay apart, and so do a run's products with weights of three
-// parts: the instruction cuts a product off at its sum's last place, and apart the small parts lose nothing to a large sum (errors
+// Queries of 32 bits are three bf16 numbers that add up to them, and weights three; of 16 bits, weights two, which leaves 2^-16 of
+// a weight times its scale: of a key's whole part in an output at most a 32nd of what rounding the output to fp16 may take off
+// (2^-11), a 256th for bf16.  (Three for fp16 and their sums apart: 1 x 131072 keys 50.6 us for 43.5, 64 x 8192
+// 117 for 101, and the error against 64 bits is 2.099e-4 with two and with three.)  In 16 bits a piece's sum stays in the instruction,
+// which cuts products off at its last place: with positive values alone, where nothing cancels, outputs over 131072 keys are
+// 6e-6 too small on average, an 80th of fp16's half step.  In 32 bits the sums of products with each part of a query stay apart, and so do a run's products with weights of three
+// parts: apart the small parts lose nothing to a large sum (errors
 // against 64 bits over 120 drawn fp32 cases 2.4e-7 at most, not 1.2e-6; 16 x 8192 keys, 32 / 8 heads of 128, 45 us for 42).
 //
 // Measured (32 query and 8 key-value heads of 128, bf16, one group a head): 64 sequences of 0 to 8192 keys 102 us, 2.8 TB/s, for
-// 45 us of bytes (131 us in groups of 32); one sequence of 17 keys 6.6 us, of which a launch 4.1.  457 warp instructions per 16
-// keys and values, 56 % of issue slots in use by 16 warps a SM, which is what registers leave room for.
+// 45 us of bytes (131 us in groups of 32); one sequence of 17 keys 6.5 us, of which a launch 4.1.  457 warp instructions per 16
+// keys and values would take 53 us if they filled the issue slots; they fill 56 % of them.  What binds is the latency of one chain
+// after the other (scores, their maximum, weights, values) in the 16 warps a SM that registers leave room for; the kernels of heads of
+// 97 to 128 elements spill 40 (one group) to 152 bytes (groups of 32) a thread at their 128, of fp32 queries 84 to 128, and those of
+// fp32 queries with more than eight heads and 129 elements 236 to 400 at 255.
 // ---------------------------------------------------------------------------------------------
 
 // a b + c of two pairs

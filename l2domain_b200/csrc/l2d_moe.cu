@@ -12,9 +12,9 @@
 // 17 + 5 at 4096 x 1536, and 45 for 30 in all at 1001 x 333.)
 // Nothing depends on the order in which blocks come: a slot's sums are its own.
 //
-// Measured (bf16): 32 tokens, 4 of 64 experts of 4096 x 1024, 233 to 256 us (short runs, and seconds under the
-// power cap), 6.0 to 5.5 TB/s, for 220 us of bytes at a copy's rate; one token, 4 of 32 of 4096 x 1536, 43 us for
-// 24: the chain of launches and, in each, some microseconds until its rows come.
+// Measured (bf16): 32 tokens, 4 of 64 experts of 4096 x 1024, 250 to 265 us under the power cap, 5.6 to 5.3 TB/s, for 220 us
+// of bytes at a copy's rate; one token, 4 of 32 of 4096 x 1536, 45 us for 24: the chain of launches and, in each, some
+// microseconds until its rows come.
 #include "l2d_launch.cuh"
 
 #include <algorithm>
@@ -280,11 +280,12 @@ __global__ void __launch_bounds__(kMoeThreads) k_route(const __grid_constant__ M
 // the ends of items; columns are read from L1 or L2 a step ahead.  Where there are few items, their rows are cut into S
 // parts for as many warps of a block.
 //
-// silu(gate x) (up x) is held in fp32 and cut on the way to the down product: for bf16 into three numbers that add up to it, for fp16
-// into two, relative to the slot's largest, which only the whole first product knows.
+// silu(gate x) (up x) is held in fp32 and cut on the way to the down product: for bf16 into three numbers that add up to it (two, made
+// once by the first product, took 1.5 us less for one token and 16 of 253 for 156, and 2^-16 of each), for fp16
+// into two, relative to the slot's largest, which only the whole first product knows: 2^-22 of it is left, 2^-11 of what rounding
+// an output to fp16 may take off.
 //
-// The products of a step are added to the sum in fp32: the instruction cuts them off at its sum's last place, which over a long row
-// takes off as much as two numbers for an inner value would.
+// The products of a step are added to the sum in fp32: the instruction cuts them off at its sum's last place (no change in time).
 //
 // 32 bits: a warp works on four rows (two of gate and of up) with the lanes along them, by fused multiply-adds.
 // ---------------------------------------------------------------------------------------------
