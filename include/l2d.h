@@ -505,8 +505,8 @@ L2D_API int l2d_kv4_page_bytes(int heads, int head_dim, int page_size, int group
 L2D_API int l2d_kv4_append(const l2d_kv4_cache *cache, const l2d_append_desc *desc, const void *k, const void *v, const void *q, void *q_out,
                            void *k_out, void *v_out, const int32_t *pos, const int32_t *seq, int64_t tokens, void *stream);
 /* A plan of l2d_attn_decode and l2d_attn_decode_from over a cache in 4 bits; scores may be NULL.  Weights times scales meet
- * the values as two bf16 numbers (2^-16 of a weight is left), for fp32 queries as three, and so do the queries; what is below
- * 2^-104 of a weight times its scale is lost whatever its size. */
+ * the values as three bf16 numbers that add up to them, for bf16 as two (2^-16 is left), and fp32 queries meet the keys as three; what
+ * is below 2^-104 of a weight times its scale is lost whatever its size. */
 L2D_API int l2d_attn_plan_create_kv4(const l2d_kv4_cache *cache, const l2d_attn_desc *desc, const l2d_attn_scores *scores,
                                      l2d_attn_plan **plan);
 

@@ -35,20 +35,20 @@ constexpr int kGroupBytes = kBlockSlots * 4;
 // nibble; the weights come from the layout of sums to that of a B operand by movmatrix.  (With the heads as rows eight of 16 would
 // be empty for groups of up to eight, or hold second parts, and their sums would take twice the registers.)
 //
-// Queries of 32 bits are three bf16 numbers that add up to them, and weights three; of 16 bits, weights two, which leaves 2^-16 of
-// a weight times its scale: of a key's whole part in an output at most a 32nd of what rounding the output to fp16 may take off
-// (2^-11), a 256th for bf16.  (Three for fp16 and their sums apart: 1 x 131072 keys 50.6 us for 43.5, 64 x 8192
-// 117 for 101, and the error against 64 bits is 2.099e-4 with two and with three.)  In 16 bits a piece's sum stays in the instruction,
-// which cuts products off at its last place: with positive values alone, where nothing cancels, outputs over 131072 keys are
-// 6e-6 too small on average, an 80th of fp16's half step.  In 32 bits the sums of products with each part of a query stay apart, and so do a run's products with weights of three
-// parts: apart the small parts lose nothing to a large sum (errors
-// against 64 bits over 120 drawn fp32 cases 2.4e-7 at most, not 1.2e-6; 16 x 8192 keys, 32 / 8 heads of 128, 45 us for 42).
+// Queries of 32 bits are three bf16 numbers that add up to them.  Weights times scales are three for fp32 and fp16, and two for
+// bf16, which leaves 2^-16 of one, a 256th of what rounding an output to bf16 may take off; with two, one output in a hundred was
+// not the nearest fp16 number (1 x 131072 keys; with three one in five hundred, as of a softmax in fp32; 47.1 us for 43.5, and 64 x
+// 8192 keys 112 for 101).  In 32 bits the sums of products with each part of a query stay apart, and so do a run's products with
+// weights: the instruction cuts a product off at its sum's last place, and apart the small parts lose nothing to a large sum (errors
+// against 64 bits over 120 drawn fp32 cases 2.4e-7 at most, not 1.2e-6; 16 x 8192 keys, 32 / 8 heads of 128, 45 us for 42).  In 16
+// bits they stay in the instruction: where all values are positive and nothing cancels, outputs over 131072 keys are 6e-6 too small
+// on average, an 80th of fp16's half step (apart, 1 x 131072 keys take 50.7 us).
 //
 // Measured (32 query and 8 key-value heads of 128, bf16, one group a head): 64 sequences of 0 to 8192 keys 102 us, 2.8 TB/s, for
 // 45 us of bytes (131 us in groups of 32); one sequence of 17 keys 6.5 us, of which a launch 4.1.  457 warp instructions per 16
 // keys and values would take 53 us if they filled the issue slots; they fill 56 % of them.  What binds is the latency of one chain
 // after the other (scores, their maximum, weights, values) in the 16 warps a SM that registers leave room for; the kernels of heads of
-// 97 to 128 elements spill 40 (one group) to 152 bytes (groups of 32) a thread at their 128, of fp32 queries 84 to 128, and those of
+// 97 to 128 elements spill 40 (one group) to 152 bytes (groups of 32, fp16 168) a thread at their 128, of fp32 queries 84 to 128, and those of
 // fp32 queries with more than eight heads and 129 elements 236 to 400 at 255.
 // ---------------------------------------------------------------------------------------------
 
@@ -108,10 +108,10 @@ struct NibbleCore {
     using Elem = IO;
     static constexpr bool kPacked = true, kScored = false;  // other scores are a branch here
     static constexpr int kWholeTiles = 3, kSwitch = 2;
-    static constexpr bool kThree = sizeof(IO) == 4;         // parts of queries and weights
+    static constexpr bool kThree = sizeof(IO) == 4;         // parts of queries, and sums apart
     static constexpr bool kHalf = std::is_same<IO, __half>::value;
     using Q = typename std::conditional<kHalf, __half, __nv_bfloat16>::type;
-    static constexpr int kParts = kThree ? 3 : 1, kWeightParts = kThree ? 3 : 2;
+    static constexpr int kParts = kThree ? 3 : 1, kWeightParts = kThree || kHalf ? 3 : 2;
     static constexpr int kKeys = 32, kRuns = 2;             // of a tile: two runs share what a tile costs besides its products
     static constexpr int kWarps = N == 1 || C <= 4 ? 8 : 4;  // whose sums fit an SM
     static constexpr int kBlocks = N == 1 && C <= 4 ? 2 : 1;
