@@ -118,10 +118,10 @@ class DecodeAttention:
 
         rows_of("qkv", qkv, row)
         for name, t in (("k_out", k_out), ("v_out", v_out)):
-            if t is not None:
+            if hasattr(t, "dtype"):  # a tensor, and not an address
                 rows_of(name, t, kv)
         for name, t in (("pos", pos), ("seq", seq)):
-            if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] < tokens or not t.is_contiguous() or t.device != dev:
+            if hasattr(t, "dtype") and (t.dtype != torch.int32 or t.numel() < tokens or not t.is_contiguous() or t.device != dev):
                 raise ValueError(f"{name} is {t.dtype} {list(t.shape)} on {t.device}: int32, {tokens} or more in a row, on {dev}")
         self.append.append(qkv[:, hd:], qkv[:, hd + kv:], pos, tokens, seq=seq, q=qkv, q_out=qkv, k_out=k_out, v_out=v_out, stream=stream)
 

@@ -68,3 +68,13 @@ def test_prompts_of_other_tensors_are_refused(bad, word):
     a.update(bad)
     with pytest.raises(ValueError, match=word):
         layer().prompt(a["qkv"], a["pos"], a["seq"], 5, k_out=a.get("k_out"), v_out=a.get("v_out"))
+
+
+def test_prompts_of_addresses_and_of_sequences_in_order_reach_the_append():
+    """What has no type is the caller's: addresses, and no seq where token t belongs to sequence t."""
+    it, got = layer(), []
+    it.append = type("Append", (), {"append": lambda self, *a, **kw: got.append((a, kw))})()
+    qkv = torch.zeros(1, 130, dtype=torch.bfloat16)[:, :128]  # one row, whose stride says nothing
+    it.prompt(qkv, 0x10000000, None, 1, k_out=0x20000000, v_out=0x30000000)
+    (a, kw), = got
+    assert a[2:] == (0x10000000, 1) and kw["seq"] is None and kw["k_out"] == 0x20000000 and kw["q"] is qkv
